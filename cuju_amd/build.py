@@ -9,8 +9,8 @@
   in place of the host build when ``CUJU_AMD_HOST_LIBRARY`` names it, with the sanitizer runtimes
   preloaded into Python (``LD_PRELOAD``).
 
-Every source compiles with IEEE semantics and no contraction of multiply-adds, which the engine's
-bit-exactness needs. ``python -m cuju_amd.build`` runs the same steps.
+Every source of the engine compiles with IEEE semantics and no contraction of multiply-adds, which
+its bit-exactness needs; the policy operators (``csrc/layers``) may contract. ``python -m cuju_amd.build`` runs the same steps.
 """
 
 from __future__ import annotations
@@ -52,6 +52,11 @@ HIP_FLAGS = ['-std=c++17', '-O2', '-fPIC', '-ffp-contract=off', '-fno-fast-math'
              '-mllvm', '-amdgpu-spill-vgpr-to-agpr=0']
 
 
+# The policy operators (layers/) hold no match: contraction and -O3, and the default scheduler.
+LAYER_SOURCES = ['layers/delta_rule.hip', 'layers/delta_rule_backward.hip', 'layers/group_norm.hip']
+LAYER_FLAGS = ['-std=c++17', '-O3', '-fPIC', '-fvisibility=hidden', '-w', f'--offload-arch={ARCH}',
+               '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+
 # The device code is built once per group width (lanes per environment); the first build also
 # holds the geometry choice, the static scratch and the math check kernel.
 GROUP_WIDTHS = (4, 2, 8, 16, 32, 64)
@@ -83,6 +88,8 @@ def build(host=True, product=True, jobs=8):
         for lanes in GROUP_WIDTHS:
             tasks.append([HIPCC, *HIP_FLAGS, *_variant_flags(lanes), '-c', os.path.join(SOURCE, 'hip_device.hip'),
                           '-o', _object(f'hip_device_{lanes}.hip', 'p')])
+        for s in LAYER_SOURCES:
+            tasks.append([HIPCC, *LAYER_FLAGS, '-c', os.path.join(SOURCE, s), '-o', _object(s, 'p')])
     if host:
         for s in HOST_SOURCES + ['host/host_library.cpp']:
             tasks.append([CXX, *COMMON, '-c', os.path.join(SOURCE, s), '-o', _object(s, 'h')])
@@ -91,7 +98,7 @@ def build(host=True, product=True, jobs=8):
             f.result()
     built = []
     if product:
-        objects = [_object(s, 'p') for s in HOST_SOURCES] + [_object(f'hip_device_{lanes}.hip', 'p') for lanes in GROUP_WIDTHS]
+        objects = [_object(s, 'p') for s in HOST_SOURCES + LAYER_SOURCES] + [_object(f'hip_device_{lanes}.hip', 'p') for lanes in GROUP_WIDTHS]
         _run([HIPCC, f'--offload-arch={ARCH}', '-shared', '-fPIC', '-o', PRODUCT, *objects])
         built.append(PRODUCT)
     if host:

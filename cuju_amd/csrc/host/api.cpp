@@ -19,6 +19,8 @@ std::unique_ptr<Device> MakeLibraryDevice(int threads, int environments);
 extern const char *const kBackendName;
 // Whether the library's device keeps the batch in host memory (the host debugging build).
 extern const bool kLibraryHostMemory;
+// Keeps `message` as the calling thread's last failure, for entry points outside this file.
+void KeepError(const std::string &message);
 }  // namespace host
 }  // namespace eng
 
@@ -28,7 +30,11 @@ namespace {
 // The calling thread's last failure, and the bytes of the last state it read.
 thread_local std::string lastError;
 thread_local std::string stateBytes;
+}  // namespace
 
+void eng::host::KeepError(const std::string &message) { lastError = message; }
+
+namespace {
 BatchRuntime *Of(void *e) { return static_cast<BatchRuntime *>(e); }
 
 // Runs `body` and turns what it throws into the error convention: the message is kept for

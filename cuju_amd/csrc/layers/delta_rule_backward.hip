@@ -1,0 +1,610 @@
+// The gradients of the gated delta rule over many steps.
+//
+// With the forward pass's chunk (delta_rule.hip), R = (I + A)^-1, P = scale D o Q K^T, the chunk's
+// outputs' gradient dO and the gradient dS of the memory after it:
+//   dU = P^T dO + D_C K dS          dB = R^T dU           dv = beta dB
+//   dP = dO U^T                     dA = -dB U^T
+//   dq = scale G S0 dO + (scale D o dP) K
+//   dk = D_C dS U - beta G S0 dB + (scale D o dP)^T Q + (N + N^T) K,   N = beta D o dA
+//   dbeta_i = dB_i.(v_i - G_i S0^T k_i) + sum_j dA_ij D_ij k_i.k_j
+//   dS0 = G_C dS + scale Q^T (G dO) - K^T (beta G dB)
+// and the log decay of step l, which every product from before l to after it carries, gets
+//   sum_{i>=l} e_i + sum_{j<l<=i} E_ij + sum_{j<l} f_j + G_C <dS, S0>,
+// e_i = q_i.(scale G S0 dO)_i - k_i.(beta G S0 dB)_i, E = dP o P + dA o A, f_j = k_j.(D_C dS U)_j:
+// sums of like terms, with no difference of totals that would cost a strong decay its precision.
+#include "delta_rule.h"
+
+namespace layers {
+namespace {
+
+// One workgroup takes a head backwards through its steps, a segment of two chunks at a time. A
+// wavefront holds 16 columns of the memory. Of a segment, two wavefronts first build a chunk's
+// triangular matrices each; then the first chunk is played forward from the segment's checkpoint, and
+// the chunks are taken in reverse. The products that contract the columns (S0 dO, S0 dB, dS U) go
+// through LDS, each wavefront taking whole tiles of keys.
+template <class T>
+struct BackwardArgs {
+    Rule rule;
+    View<const T> query, key, value, dOutput;
+    Gates gates;
+    void *dQuery, *dKey;  // of T with the key heads, or of float with the heads where `shared`
+    bool shared;
+};
+
+constexpr int kMatrixRow = 20, kMatrix = kChunk * kMatrixRow;  // a 16x16 matrix in LDS
+
+// LDS for keys of up to `KeyTiles` tiles and values of up to `Pairs` pairs of them, in floats.
+template <int KeyTiles, int Pairs, int ElementSize>
+struct BackwardShared {
+    static constexpr int kMemoryRow = Pairs * 32 + 4;  // floats of a row of the memory
+    static constexpr int kRow = Pairs * 32 + 8;        // elements of a step's row of values
+    static constexpr int kMatrices = kSegment / kChunk * kMatrix, kPieceRows = kFloatPieces * kChunk * kRow / 2;
+    static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kCuts = kBetas + kSegment, kInverse = kCuts + 4,
+                         kMixed = kInverse + kMatrices, kProducts = kMixed + kMatrices, kMemory = kProducts + kMatrices,
+                         kU = kMemory + KeyTiles * 16 * kMemoryRow, kB = kU + kPieceRows, kO = kB + kPieceRows,
+                         kTiles = kO + kChunk * kRow * ElementSize / 4, kDots = kTiles + KeyTiles * 256,
+                         kFloats = kDots + 2 * Pairs * 4 * kChunk;
+};
+
+__device__ __forceinline__ F4 RowOrder(const float *matrix, int m, int g) {
+    return *reinterpret_cast<const F4 *>(matrix + m * kMatrixRow + 4 * g);
+}
+__device__ __forceinline__ F4 ColumnOrder(const float *matrix, int m, int g) {
+    F4 x;
+#pragma unroll
+    for (int r = 0; r < 4; r++) x[r] = matrix[(4 * g + r) * kMatrixRow + m];
+    return x;
+}
+template <class T, int KeyTiles, int Pairs, bool Whole>
+__global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))) void BackwardKernel(BackwardArgs<T> a) {
+    using At = BackwardShared<KeyTiles, Pairs, sizeof(T)>;
+    extern __shared__ __align__(16) float shared[];
+    constexpr int P = kPieces<T>;
+    using Args = BackwardArgs<T>;
+    const Rule &rule = a.rule;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    constexpr int ms = At::kMemoryRow, rs = At::kRow;
+    double *reach = reinterpret_cast<double *>(shared + At::kReach);
+    float *betas = shared + At::kBetas, *memory = shared + At::kMemory, *dots = shared + At::kDots;
+    unsigned *cutsOf = reinterpret_cast<unsigned *>(shared + At::kCuts);
+    // Rows of values by step, [piece][step][column].
+    uint16_t *sharedU = reinterpret_cast<uint16_t *>(shared + At::kU), *sharedB = reinterpret_cast<uint16_t *>(shared + At::kB);
+    T *sharedO = reinterpret_cast<T *>(shared + At::kO);
+
+    const unsigned head = Place(blockIdx.x, gridDim.x);
+    const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
+    const int dk = rule.key_size, dv = rule.value_size, time = rule.time;
+    const int column = 16 * wave + m;       // the column of a lane in column order
+    const int column4 = 16 * wave + 4 * g;  // its first of four in row order
+    const int segments = (time + kSegment - 1) / kSegment;
+    const Four eye = Eye(m, g);
+    F4 one;
+#pragma unroll
+    for (int r = 0; r < 4; r++) one[r] = m == 4 * g + r ? 1.f : 0.f;
+
+    const auto loadMemory = [&](const void *memories, long long index, F4(&s)[KeyTiles]) {
+        const int rows = Opaque(dk) - 4 * g, stride = Opaque(dv);
+        const float *from = static_cast<const float *>(memories) + (index * dk + 4 * g) * stride + column;
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                s[t][r] = 0.f;
+                if (memories && 16 * t + r < rows && column < dv) s[t][r] = from[(16 * t + r) * stride];
+            }
+    };
+    // A lane's four elements of each key tile of step m of a chunk.
+    const bool full = Whole && dk == 16 * KeyTiles;
+    const auto loadKeys = [&](const View<const T> &view, int t0, Pack<T, 4>(&x)[KeyTiles]) {
+        const T *p = view.At(b, min(t0 + m, time - 1), kh) + 4 * g;
+        if (full) {
+#pragma unroll
+            for (int i = 0; i < KeyTiles; i++) x[i] = *reinterpret_cast<const Pack<T, 4> *>(p + 16 * i);
+        } else {
+            const int size = Opaque(dk) - 4 * g;
+#pragma unroll
+            for (int i = 0; i < KeyTiles; i++) x[i] = Load<4, Whole>(p + 16 * i, size - 16 * i);
+        }
+    };
+    const auto loadValues = [&](const View<const T> &view, int t0) {
+        return Load<4, Whole>(view.At(b, min(t0 + m, time - 1), h) + column4, dv - column4);
+    };
+
+    // Columns past the last wavefront's stay zero.
+    for (int i = threadIdx.x; i < kChunk * (2 * Pairs - waves) * 16; i += blockDim.x) {
+        const int row = i % kChunk, to = row * rs + 16 * waves + i / kChunk;
+#pragma unroll
+        for (int p = 0; p < kFloatPieces; p++) sharedU[p * kChunk * rs + to] = sharedB[p * kChunk * rs + to] = 0;
+        sharedO[to] = As<T>(0.f);
+        for (int t = 0; t < KeyTiles; t++) memory[(16 * t + row) * ms + 16 * waves + i / kChunk] = 0;
+    }
+
+    F4 dS[KeyTiles];
+    loadMemory(rule.d_last, head, dS);
+
+    for (int segment = segments - 1; segment >= 0; segment--) {
+        const int s0 = segment * kSegment;
+        const int chunks = min(kSegment / kChunk, (time - s0 + kChunk - 1) / kChunk);
+        __syncthreads();
+        // ---- The chunks' matrices, one wavefront a chunk.
+        for (int c = wave; c < chunks; c += waves) {
+            const int t0 = s0 + c * kChunk, count = min(kChunk, time - t0);
+            const StepGates gate = LoadGates(Argument<Args>().gates, b, t0 + m, time, h);
+            const unsigned cuts = (unsigned)(__ballot(gate.reset) & 0xffff);
+            Pack<T, 4> k[KeyTiles], q[KeyTiles];
+            loadKeys(Argument<Args>().key, t0, k), loadKeys(Argument<Args>().query, t0, q);
+            if (g == 0) betas[c * kChunk + m] = gate.beta;
+            if (lane == 0) cutsOf[c] = cuts;
+            for (int low = 0, high; low < count; low = high) {
+                const unsigned later = cuts >> (low + 1);
+                high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;
+                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
+                const double G = RowUpTo(mine && !(starts && m == low) ? gate.decay * kLog2E : 0.0);
+                const float beta = mine ? gate.beta : 0.f;
+                if (mine && g == 0) reach[c * kChunk + m] = G;
+                F4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < KeyTiles / 2; p++) {
+                    B8 kp[P], qp[P];
+                    Pair<T>(Masked(k[2 * p], mine), Masked(k[2 * p + 1], mine), kp);
+                    Pair<T>(Masked(q[2 * p], mine), Masked(q[2 * p + 1], mine), qp);
+                    kk = Mfma32<P, P>(kp, kp, kk);
+                    qk = Mfma32<P, P>(kp, qp, qk);
+                }
+                F4 aA, dA, aP, aKK;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = 4 * g + r;
+                    const double Gj = __shfl(G, j);
+                    const float betaj = __shfl(beta, j);
+                    const float d = Exp2(j <= m ? G - Gj : Gj - G);
+                    aP[r] = j <= m ? rule.scale * d * qk[r] : 0.f;
+                    aKK[r] = j < m ? d * kk[r] : 0.f;
+                    aA[r] = beta * aKK[r];
+                    dA[r] = m < j ? betaj * d * kk[r] : 0.f;
+                }
+                const F4 aT = UnitLowerInverse<false>(aA, dA, m, g).rows;
+                if (mine) {
+                    const int to = c * kMatrix + m * kMatrixRow + 4 * g;
+                    *reinterpret_cast<F4 *>(shared + At::kInverse + to) = aT;
+                    *reinterpret_cast<F4 *>(shared + At::kMixed + to) = aP;
+                    *reinterpret_cast<F4 *>(shared + At::kProducts + to) = aKK;
+                }
+            }
+        }
+        __syncthreads();
+
+        // The values that chunk c writes and their errors, from the memory `s` before it; with `advance`
+        // the memory goes on to the next chunk.
+        const auto play = [&](int c, bool advance, F4(&s)[KeyTiles], F4 &wrote, F4 &errors) {
+            const int t0 = s0 + c * kChunk, count = min(kChunk, time - t0);
+            const unsigned cuts = cutsOf[c];
+            wrote = errors = F4{0, 0, 0, 0};
+            for (int low = 0, high; low < count; low = high) {
+                const unsigned later = cuts >> (low + 1);
+                high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;
+                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
+                Pack<T, 4> k[KeyTiles];
+                loadKeys(Argument<Args>().key, t0, k);
+                Four v[P];
+                Split<T>(Masked(loadValues(Argument<Args>().value, t0), mine), v);
+                if (high - low < kChunk) {
+#pragma unroll
+                    for (int t = 0; t < KeyTiles; t++) k[t] = Masked(k[t], mine);
+                }
+                F4 seen = {0, 0, 0, 0}, error = Turn<P>(v, eye), written;
+                if (!starts) {
+#pragma unroll
+                    for (int p = 0; p < KeyTiles / 2; p++) {
+                        B8 kp[P], sp[kFloatPieces];
+                        Pair<T>(k[2 * p], k[2 * p + 1], kp);
+                        Pair(s[2 * p], s[2 * p + 1], sp);
+                        seen = Mfma32<P, kFloatPieces>(kp, sp, seen);
+                    }
+                }
+                F4 aT = RowOrder(shared + At::kInverse + c * kMatrix, m, g);
+                bool in[4];
+                double Gj[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    in[r] = 4 * g + r >= low && 4 * g + r < high;
+                    Gj[r] = in[r] ? reach[c * kChunk + 4 * g + r] : 0.0;
+                    error[r] = fmaf(-Exp2(Gj[r]), seen[r], error[r]);
+                    written[r] = in[r] ? betas[c * kChunk + 4 * g + r] * error[r] : 0.f;
+                    aT[r] = mine && in[r] ? aT[r] : 0.f;
+                }
+                written = Product(aT, written);
+                const double last = reach[c * kChunk + high - 1];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    wrote[r] = in[r] ? written[r] : wrote[r];
+                    errors[r] = in[r] ? error[r] : errors[r];
+                    written[r] *= in[r] ? Exp2(last - Gj[r]) : 0.f;
+                }
+                if (!advance) continue;
+                Four wp[kFloatPieces];
+                Split(written, wp);
+                const float kept = Exp2(last);
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++) {
+                    Four x[P], turned[P];
+                    Split<T>(k[t], x);
+                    Turn<P>(x, eye, turned);
+                    F4 held = s[t] * kept;
+                    if (starts) held = F4{0, 0, 0, 0};
+                    s[t] = Mfma16(turned, wp, held);
+                }
+            }
+        };
+        const auto checkpoint = [&](F4(&s)[KeyTiles]) {
+            const Args now = Argument<Args>();
+            if (segment > 0) loadMemory(now.rule.checkpoints, (long long)head * (segments - 1) + segment - 1, s);
+            else loadMemory(now.rule.state, head, s);
+        };
+        F4 start[KeyTiles], wroteFirst, errorsFirst;
+        checkpoint(start);
+        if (chunks > 1) play(0, true, start, wroteFirst, errorsFirst);
+
+        for (int c = chunks - 1; c >= 0; c--) {
+            const int t0 = s0 + c * kChunk;
+            const unsigned cuts = cutsOf[c];
+            F4 wroteC, errorC;
+            if (c == 0 && chunks > 1) checkpoint(start), wroteC = wroteFirst, errorC = errorsFirst;
+            else play(c, false, start, wroteC, errorC);
+            for (int high = min(kChunk, time - t0), low; high > 0; high = low) {
+                const unsigned below = cuts & ((1u << high) - 1);
+                low = below ? 31 - __builtin_clz(below) : 0;
+                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
+                Pack<T, 4> k[KeyTiles], q[KeyTiles];
+                loadKeys(Argument<Args>().key, t0, k), loadKeys(Argument<Args>().query, t0, q);
+                const Pack<T, 4> rawO = Masked(loadValues(Argument<Args>().dOutput, t0), mine);
+                if (high - low < kChunk) {
+#pragma unroll
+                    for (int t = 0; t < KeyTiles; t++) k[t] = Masked(k[t], mine), q[t] = Masked(q[t], mine);
+                }
+                const double G = mine ? reach[c * kChunk + m] : 0.0, last = reach[c * kChunk + high - 1];
+                const float beta = mine ? betas[c * kChunk + m] : 0.f;
+                bool in[4];
+                double Gj[4];
+                float betaj[4], afterJ[4], wholeJ[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    in[r] = 4 * g + r >= low && 4 * g + r < high;
+                    Gj[r] = in[r] ? reach[c * kChunk + 4 * g + r] : 0.0;
+                    betaj[r] = in[r] ? betas[c * kChunk + 4 * g + r] : 0.f;
+                    afterJ[r] = in[r] ? Exp2(last - Gj[r]) : 0.f;
+                    wholeJ[r] = in[r] ? Exp2(Gj[r]) : 0.f;
+                }
+
+                // The gradients of the values written, and of the right side they solve.
+                Four op[P];
+                Split<T>(rawO, op);
+                const F4 dO = Turn<P>(op, eye);
+                F4 dU = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < KeyTiles / 2; p++) {
+                    B8 kp[P], sp[kFloatPieces];
+                    Pair<T>(k[2 * p], k[2 * p + 1], kp);
+                    Pair(dS[2 * p], dS[2 * p + 1], sp);
+                    dU = Mfma32<P, kFloatPieces>(kp, sp, dU);
+                }
+                F4 dT = ColumnOrder(shared + At::kInverse + c * kMatrix, m, g);
+                F4 dP = ColumnOrder(shared + At::kMixed + c * kMatrix, m, g), written;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    dU[r] *= afterJ[r];
+                    dT[r] = in[r] && mine ? dT[r] : 0.f;
+                    dP[r] = in[r] && mine ? dP[r] : 0.f;
+                    written[r] = in[r] ? wroteC[r] : 0.f;
+                }
+                dU = Product(dP, dO, dU);
+                const F4 dB = Product(dT, dU), aB = Product(dU, dT), aU = Product(written, one);
+                if (mine) {
+                    Pack<T, 4> x;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x.x[r] = As<T>(beta * aB[r]);
+                    Store<4, Whole>(static_cast<T *>(Argument<Args>().rule.d_value) + (((long long)b * time + t0 + m) * rule.heads + h) * dv + column4,
+                                    x, dv - column4);
+                }
+                Four up[kFloatPieces], bp[kFloatPieces];
+                Split(aU, up), Split(aB, bp);
+                float held = 0;
+                if (!starts) {
+#pragma unroll
+                    for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) held = fmaf(dS[t][r], start[t][r], held);
+                }
+                held = WaveSum(held);
+                F4 wrong;
+#pragma unroll
+                for (int r = 0; r < 4; r++) wrong[r] = RowSum(in[r] ? dB[r] * errorC[r] : 0.f);
+
+                __syncthreads();
+#pragma unroll
+                for (int p = 0; p < kFloatPieces; p++) {
+                    *reinterpret_cast<Four *>(sharedU + (p * kChunk + m) * rs + column4) = up[p];
+                    *reinterpret_cast<Four *>(sharedB + (p * kChunk + m) * rs + column4) = bp[p];
+                }
+                *reinterpret_cast<Pack<T, 4> *>(sharedO + m * rs + column4) = rawO;
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + column] = dS[t][r];
+                if (m == 0) *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kChunk + 4 * g) = wrong;
+                if (lane == 0) dots[(wave * 4 + 3) * kChunk] = held;
+                __syncthreads();
+
+                // The matrices' gradients, and dS U for this wavefront's tiles of keys.
+                const auto rowPieces = [&](const uint16_t *rows, int x, B8(&to)[kFloatPieces]) {
+#pragma unroll
+                    for (int p = 0; p < kFloatPieces; p++) {
+                        const uint16_t *from = rows + (p * kChunk + m) * rs + 32 * x + 4 * g;
+                        to[p] = Eight(*reinterpret_cast<const Four *>(from), *reinterpret_cast<const Four *>(from + 16));
+                    }
+                };
+                const auto memoryPieces = [&](int t, int x, B8(&to)[kFloatPieces]) {
+                    const float *from = memory + (16 * t + m) * ms + 32 * x + 4 * g;
+                    Pair(*reinterpret_cast<const F4 *>(from), *reinterpret_cast<const F4 *>(from + 16), to);
+                };
+                const auto outputPieces = [&](int x, B8(&to)[P]) {
+                    const T *from = sharedO + m * rs + 32 * x + 4 * g;
+                    Pair<T>(*reinterpret_cast<const Pack<T, 4> *>(from), *reinterpret_cast<const Pack<T, 4> *>(from + 16), to);
+                };
+                F4 gP = {0, 0, 0, 0}, gA = {0, 0, 0, 0};
+                for (int x = 0; x < Pairs; x++) {
+                    B8 uw[kFloatPieces], other[kFloatPieces], out[P];
+                    rowPieces(sharedU, x, uw);
+                    outputPieces(x, out);
+                    gP = Mfma32<kFloatPieces, P>(uw, out, gP);
+                    rowPieces(sharedB, x, other);
+                    gA = Mfma32<kFloatPieces, kFloatPieces>(uw, other, gA);
+                }
+                for (int t = wave; t < KeyTiles; t += waves) {
+                    F4 sum = {0, 0, 0, 0};
+                    for (int x = 0; x < Pairs; x++) {
+                        B8 uw[kFloatPieces], sp[kFloatPieces];
+                        rowPieces(sharedU, x, uw);
+                        memoryPieces(t, x, sp);
+                        sum = Mfma32<kFloatPieces, kFloatPieces>(uw, sp, sum);
+                    }
+                    // Read back by the same lane.
+                    *reinterpret_cast<F4 *>(shared + At::kTiles + (t * 64 + lane) * 4) = sum;
+                }
+                const F4 aP = RowOrder(shared + At::kMixed + c * kMatrix, m, g);
+                const F4 aKK = RowOrder(shared + At::kProducts + c * kMatrix, m, g);
+                F4 aM, aN, E;
+                float betaSum = 0;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int j = 4 * g + r;
+                    const bool both = mine && in[r];
+                    const float d = both && j <= m ? Exp2(G - Gj[r]) : 0.f;
+                    aM[r] = rule.scale * d * gP[r];
+                    aN[r] = j < m ? -beta * d * gA[r] : 0.f;
+                    const float part = both && j < m ? -gA[r] * aKK[r] : 0.f;
+                    betaSum += part;
+                    E[r] = (both && j <= m ? gP[r] * aP[r] : 0.f) + beta * part;
+                }
+                Four mp[kFloatPieces], mt[kFloatPieces], np[kFloatPieces];
+                Split(aM, mp), Split(Product(aM, one), mt), Split(aN + Product(aN, one), np);
+
+                // S0 dO and S0 dB, with the memory in the gradient's place.
+                if (!starts) {
+                    __syncthreads();
+#pragma unroll
+                    for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + column] = start[t][r];
+                    __syncthreads();
+                }
+                F4 f = {0, 0, 0, 0}, e = {0, 0, 0, 0};
+                const float kept = Exp2(last);
+                Four dOp[kFloatPieces], dBp[kFloatPieces];
+                {
+                    F4 x, y;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r] = rule.scale * wholeJ[r] * dO[r], y[r] = -betaj[r] * wholeJ[r] * dB[r];
+                    Split(x, dOp), Split(y, dBp);
+                }
+                for (int t = wave; t < KeyTiles; t += waves) {
+                    F4 dQ = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                    if (!starts)
+                        for (int x = 0; x < Pairs; x++) {
+                            B8 sp[kFloatPieces], other[kFloatPieces], out[P];
+                            memoryPieces(t, x, sp);
+                            outputPieces(x, out);
+                            dQ = Mfma32<P, kFloatPieces>(out, sp, dQ);
+                            rowPieces(sharedB, x, other);
+                            y = Mfma32<kFloatPieces, kFloatPieces>(other, sp, y);
+                        }
+                    const Args now = Argument<Args>();
+                    const auto tile = [&](const View<const T> &view) {
+                        const T *p = view.At(b, min(t0 + m, time - 1), kh) + 16 * t + 4 * g;
+                        return Masked(Load<4, Whole>(p, dk - 16 * t - 4 * g), mine);
+                    };
+                    const Pack<T, 4> kt = tile(now.key), qt = tile(now.query);
+                    const F4 dKeys = *reinterpret_cast<const F4 *>(shared + At::kTiles + (t * 64 + lane) * 4);
+                    Four kx[P], qx[P], kTurned[P], qTurned[P];
+                    Split<T>(kt, kx), Split<T>(qt, qx);
+                    Turn<P>(kx, eye, kTurned), Turn<P>(qx, eye, qTurned);
+                    const F4 kf = Turn<P>(kx, eye), qf = Turn<P>(qx, eye);
+                    F4 dK;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        dK[r] = afterJ[r] * dKeys[r];
+                        f[r] = fmaf(dK[r], kf[r], f[r]);
+                        const float fromKey = -betaj[r] * wholeJ[r] * y[r];
+                        dQ[r] *= rule.scale * wholeJ[r];
+                        e[r] = fmaf(qf[r], dQ[r], fmaf(kf[r], fromKey, e[r]));
+                        dK[r] += fromKey;
+                    }
+                    dQ = Mfma16(mp, kTurned, dQ);
+                    dK = Mfma16(mt, qTurned, dK);
+                    dK = Mfma16(np, kTurned, dK);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if (!in[r] || 16 * t + m >= dk) continue;
+                        const long long row = (long long)b * time + t0 + 4 * g + r;
+                        if (now.shared) {
+                            const long long to = (row * rule.heads + h) * dk + 16 * t + m;
+                            static_cast<float *>(now.dQuery)[to] = dQ[r];
+                            static_cast<float *>(now.dKey)[to] = dK[r];
+                        } else {
+                            const long long to = (row * rule.key_heads + kh) * dk + 16 * t + m;
+                            static_cast<T *>(now.dQuery)[to] = As<T>(dQ[r]);
+                            static_cast<T *>(now.dKey)[to] = As<T>(dK[r]);
+                        }
+                    }
+                }
+                F4 eSum, fSum;
+#pragma unroll
+                for (int r = 0; r < 4; r++) eSum[r] = RowSum(e[r]), fSum[r] = RowSum(f[r]);
+                if (m == 0) {
+                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 1) * kChunk + 4 * g) = eSum;
+                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 2) * kChunk + 4 * g) = fSum;
+                }
+
+                // The gradient of the memory before this part.
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++) {
+                    if (starts) {
+                        dS[t] = F4{0, 0, 0, 0};
+                        continue;
+                    }
+                    Four x[P], turned[P];
+                    Split<T>(q[t], x);
+                    Turn<P>(x, eye, turned);
+                    dS[t] = Mfma16(turned, dOp, dS[t] * kept);
+                    Split<T>(k[t], x);
+                    Turn<P>(x, eye, turned);
+                    dS[t] = Mfma16(turned, dBp, dS[t]);
+                }
+                __syncthreads();
+
+                // The gates' gradients, a lane for each step.
+                if (wave == 0) {
+                    float eAll = 0, fAll = 0, bAll = 0, heldAll = 0;
+                    for (int w = 0; w < waves; w++) {
+                        bAll += dots[(w * 4 + 0) * kChunk + m];
+                        eAll += dots[(w * 4 + 1) * kChunk + m];
+                        fAll += dots[(w * 4 + 2) * kChunk + m];
+                        heldAll += dots[(w * 4 + 3) * kChunk];
+                    }
+                    float across = 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float x = RowFrom(E[r]);
+                        across += 4 * g + r < m ? x : 0.f;
+                    }
+                    across += __shfl_xor(across, 16);
+                    across += __shfl_xor(across, 32);
+                    betaSum += __shfl_xor(betaSum, 16);
+                    betaSum += __shfl_xor(betaSum, 32);
+                    const float through = starts ? 0.f : kept * heldAll;
+                    const float decay = RowFrom(eAll) + across + Dpp<kRowShiftRight + 1>(RowUpTo(fAll)) + through;
+                    if (mine && g == 0) {
+                        const long long to = ((long long)b * time + t0 + m) * rule.heads + h;
+                        const Args now = Argument<Args>();
+                        static_cast<float *>(now.rule.d_decay)[to] = starts && m == low ? 0.f : decay;
+                        static_cast<float *>(now.rule.d_beta)[to] = bAll + betaSum;
+                    }
+                }
+            }
+        }
+    }
+    if (rule.d_state) {
+        const int rows = dk - 4 * g;
+        float *to = static_cast<float *>(rule.d_state) + ((long long)head * dk + 4 * g) * dv + column;
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (16 * t + r < rows && column < dv) to[(16 * t + r) * dv] = dS[t][r];
+    }
+}
+
+// The gradients of keys that several heads share: their sum, in the heads' order.
+template <class T>
+__global__ __launch_bounds__(256) void SharedKeysKernel(const float *parts, T *out, int group, int size, long long count) {
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
+        const long long row = i / size;
+        const float *p = parts + row * group * size + (i - row * size);
+        float sum = 0;
+        for (int n = 0; n < group; n++) sum += p[n * size];
+        out[i] = As<T>(sum);
+    }
+}
+
+template <class T, int KeyTiles>
+bool LaunchBackward(const Rule &r, hipStream_t stream) {
+    const int waves = (r.value_size + 15) / 16;
+    const bool shared = r.heads != r.key_heads;
+    const long long steps = (long long)r.batch * r.time, each = steps * r.heads * r.key_size;
+    float *parts = static_cast<float *>(r.workspace);
+    BackwardArgs<T> a{r,
+                      ViewOf<const T>(r.query, r.query_strides, r.key_size),
+                      ViewOf<const T>(r.key, r.key_strides, r.key_size),
+                      ViewOf<const T>(r.value, r.value_strides, r.value_size),
+                      ViewOf<const T>(r.d_output, r.d_output_strides, r.value_size),
+                      GatesOf(r),
+                      shared ? parts : r.d_query,
+                      shared ? parts + each : r.d_key,
+                      shared};
+    const bool whole = a.query.whole && a.key.whole && a.value.whole && a.dOutput.whole && Aligned(4 * sizeof(T), r.d_value);
+    const auto launch = [&](auto kernel, int floats) {
+        const int bytes = floats * sizeof(float);
+        if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+            hipSuccess)
+            return false;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads)), dim3(64 * waves), bytes, stream, a);
+        return true;
+    };
+    bool set;
+    if (!whole) set = launch(BackwardKernel<T, KeyTiles, 4, false>, BackwardShared<KeyTiles, 4, sizeof(T)>::kFloats);
+    else if (waves <= 2) set = launch(BackwardKernel<T, KeyTiles, 1, true>, BackwardShared<KeyTiles, 1, sizeof(T)>::kFloats);
+    else if (waves <= 4) set = launch(BackwardKernel<T, KeyTiles, 2, true>, BackwardShared<KeyTiles, 2, sizeof(T)>::kFloats);
+    else set = launch(BackwardKernel<T, KeyTiles, 4, true>, BackwardShared<KeyTiles, 4, sizeof(T)>::kFloats);
+    if (!set) return false;
+    if (shared && steps > 0) {
+        const long long count = steps * r.key_heads * r.key_size;
+        const unsigned blocks = (unsigned)(count < 256ll * 8192 ? (count + 255) / 256 : 8192);
+        const int group = r.heads / r.key_heads;
+        hipLaunchKernelGGL(SharedKeysKernel<T>, dim3(blocks), dim3(256), 0, stream, parts, static_cast<T *>(r.d_query), group,
+                           r.key_size, count);
+        hipLaunchKernelGGL(SharedKeysKernel<T>, dim3(blocks), dim3(256), 0, stream, parts + each,
+                           static_cast<T *>(r.d_key), group, r.key_size, count);
+    }
+    return true;
+}
+
+}  // namespace
+}  // namespace layers
+
+using namespace layers;
+
+extern "C" __attribute__((visibility("default"))) int cuju_delta_rule_backward(const struct cuju_delta_rule *rule, void *stream) {
+    if (!Fits(rule)) return -1;
+    const Rule &r = *rule;
+    if (r.batch == 0) return 0;
+    if (r.time > 0 && (!r.query || !r.key || !r.value || !r.decay || !r.beta || !r.d_output || !r.d_query || !r.d_key ||
+                       !r.d_value || !r.d_decay || !r.d_beta))
+        return Failed("expected inputs and their gradients");
+    if (r.time > 0 && r.heads != r.key_heads && !r.workspace) return Failed("expected a workspace for shared keys");
+    if (r.time > kSegment && !r.checkpoints) return Failed("expected the forward pass's checkpoints");
+    bool set = true;
+    ForType(r.type, [&](auto x) {
+        using T = decltype(x);
+        const auto s = static_cast<hipStream_t>(stream);
+        if (r.key_size <= 32) set = LaunchBackward<T, 2>(r, s);
+        else if (r.key_size <= 64) set = LaunchBackward<T, 4>(r, s);
+        else if (r.key_size <= 96) set = LaunchBackward<T, 6>(r, s);
+        else set = LaunchBackward<T, 8>(r, s);
+    });
+    if (!set) {
+        (void)hipGetLastError();
+        return Failed("hipFuncSetAttribute: the delta rule's gradients do not fit the shared memory");
+    }
+    return Launched("the delta rule's gradients");
+}

@@ -1,0 +1,391 @@
+"""Operators of a policy that learns from a batch, as hand-written kernels for the MI355X.
+
+* `delta_rule`: the gated delta rule over many steps, a recurrent memory with gradients. Its
+  `resets` take a batch's `done`, so a memory never reaches over the end of an episode.
+* `delta_rule_step`: one step of it for acting, with the memory updated in place.
+* `group_norm`: group norm with an activation over channels-last maps, such as an encoder of super
+  mini-maps makes, with gradients.
+
+All run on the current stream of their tensors' device, wait for nothing, and can be captured in a
+HIP graph. Under `torch.compile` they are the operators `cuju_amd::delta_rule`,
+`cuju_amd::delta_rule_step` and `cuju_amd::group_norm` with their backward operators. Element types
+are float32, bfloat16 and float16; sums, statistics and memories are held in 32 bits whatever the
+type. There is no implementation for another device.
+"""
+
+from __future__ import annotations
+
+import struct
+
+import torch
+
+from .errors import ArgumentError, ChoiceError, from_library
+from .library import load
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2}
+# Key and value sizes, and heads of a batch, that the delta rule's kernels take.
+MOST_SIZE = 128
+MOST_HEADS = (1 << 23) - 1
+# Steps between two memories that the forward pass keeps for the backward pass.
+SEGMENT = 32
+
+# `struct cuju_delta_rule` and `struct cuju_group_norm` (include/cuju_amd.h).
+_RULE = struct.Struct('@7if3P2PP17q4PP3qP3P2PPP')
+_NORM = struct.Struct('@6if3P3P2P2P')
+
+
+def _pointer(tensor) -> int:
+    return 0 if tensor is None else tensor.data_ptr()
+
+
+def _call(function, packed: bytes, device: torch.device) -> None:
+    lib = load()
+    if device.index == torch.cuda.current_device():
+        status = getattr(lib, function)(packed, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib, function)(packed, torch.cuda.current_stream(device).cuda_stream)
+    if status != 0:
+        raise from_library(lib.cuju_last_error().decode())
+
+
+def _shape(name: str, tensor: torch.Tensor, shape: tuple) -> None:
+    if tuple(tensor.shape) != shape:
+        raise ArgumentError(f'expected {name} of the shape {shape}, found {tuple(tensor.shape)}')
+
+
+def _device(first: str, tensor: torch.Tensor, others: dict) -> None:
+    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
+        raise ArgumentError(f'expected {first} on a HIP device')
+    for name, other in others.items():
+        if other is not None and (not isinstance(other, torch.Tensor) or other.device != tensor.device):
+            raise ArgumentError(f'expected {name} on the device of {first}')
+
+
+def _flat(tensor: torch.Tensor) -> torch.Tensor:
+    """`tensor` with neighbouring values of its last axis side by side."""
+    return tensor if tensor.stride(-1) == 1 or tensor.shape[-1] == 1 else tensor.contiguous()
+
+
+# ----------------------------------------------------------------------------------- the delta rule
+
+def _rule(q, k, v, decay, beta, state, resets, scale, output=None, last=None, checkpoints=None, d_output=None, d_last=None,
+          gradients=(None,) * 6, workspace=None) -> bytes:
+    """The arguments of a call; tensors are [batch, time, head, size], packed for the library."""
+    batch, time, key_heads, key_size = q.shape
+    heads, value_size = v.shape[2:]
+    sb, st = resets.stride() if resets is not None else (0, 0)
+    d_strides = d_output.stride()[:3] if d_output is not None else (0, 0, 0)
+    return _RULE.pack(TYPES[q.dtype], batch, time, key_heads, heads, key_size, value_size, scale,
+                      q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), beta.data_ptr(), _pointer(resets),
+                      *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *decay.stride(), *beta.stride(), sb, st,
+                      _pointer(state), _pointer(output), _pointer(last), _pointer(checkpoints),
+                      _pointer(d_output), *d_strides, _pointer(d_last),
+                      *[_pointer(g) for g in gradients], _pointer(workspace))
+
+
+def _check_rule(query, key, value, decay, beta, state, resets, steps):
+    """The checked arguments as the kernels take them; `steps`: whether they have a time axis."""
+    axes = 4 if steps else 3
+    _device('query', query, {'key': key, 'value': value, 'decay': decay, 'beta': beta, 'state': state, 'resets': resets})
+    if query.dtype not in TYPES:
+        raise ArgumentError(f'expected query of float32, bfloat16 or float16, found {query.dtype}')
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ArgumentError(f'expected key and value of {query.dtype}, found {key.dtype} and {value.dtype}')
+    if query.dim() != axes or value.dim() != axes:
+        raise ArgumentError(f'expected query and value of {axes} axes, found {query.dim()} and {value.dim()}')
+    lead = tuple(query.shape[:axes - 2])
+    key_heads, key_size = query.shape[-2:]
+    heads, value_size = value.shape[-2:]
+    _shape('key', key, tuple(query.shape))
+    _shape('value', value, (*lead, heads, value_size))
+    _shape('decay', decay, (*lead, heads))
+    _shape('beta', beta, (*lead, heads))
+    if key_heads < 1 or heads < 1 or heads % key_heads:
+        raise ArgumentError(f'expected heads that are a multiple of the {key_heads} key heads, found {heads}')
+    if not 1 <= key_size <= MOST_SIZE or not 1 <= value_size <= MOST_SIZE:
+        raise ArgumentError(f'expected key and value sizes from 1 to {MOST_SIZE}, found {key_size} and {value_size}')
+    if lead[0] * heads > MOST_HEADS:
+        raise ArgumentError(f'expected at most {MOST_HEADS} heads in the batch, found {lead[0] * heads}')
+    for name, gate in (('decay', decay), ('beta', beta)):
+        if not gate.is_floating_point():
+            raise ArgumentError(f'expected {name} of a floating type, found {gate.dtype}')
+    if state is not None:
+        _shape('state', state, (lead[0], heads, key_size, value_size))
+    if resets is not None:
+        _shape('resets', resets, lead)
+        if resets.dtype == torch.bool:
+            resets = resets.view(torch.uint8)
+        elif resets.dtype != torch.uint8:
+            raise ArgumentError(f'expected resets of bool or uint8, found {resets.dtype}')
+    if decay.dtype != torch.float32:
+        decay = decay.float()
+    if beta.dtype != torch.float32:
+        beta = beta.float()
+    return _flat(query), _flat(key), _flat(value), decay, beta, resets
+
+
+def _rule_forward(q, k, v, decay, beta, state, resets, scale, train):
+    batch, time = q.shape[:2]
+    heads, value_size = v.shape[2:]
+    output = torch.empty((batch, time, heads, value_size), dtype=v.dtype, device=v.device)
+    last = torch.empty((batch, heads, q.shape[3], value_size), dtype=torch.float32, device=v.device)
+    kept = max(time - 1, 0) // SEGMENT if train else 0
+    checkpoints = torch.empty((batch, heads, kept, q.shape[3], value_size), dtype=torch.float32, device=v.device)
+    if batch:
+        _call('cuju_delta_rule_forward', _rule(q, k, v, decay, beta, state, resets, scale, output, last,
+                                               checkpoints if kept else None), v.device)
+    return output, last, checkpoints
+
+
+def _rule_backward(q, k, v, decay, beta, state, resets, scale, checkpoints, d_output, d_last):
+    batch, time, key_heads, key_size = q.shape
+    heads = v.shape[2]
+    dense = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v, decay, beta)]
+    d_state = torch.empty((batch, heads, key_size, v.shape[3]), dtype=torch.float32, device=v.device)
+    workspace = None
+    if heads != key_heads:
+        workspace = torch.empty(2 * batch * time * heads * key_size, dtype=torch.float32, device=v.device)
+    if batch:
+        _call('cuju_delta_rule_backward',
+              _rule(q, k, v, decay, beta, state, resets, scale, checkpoints=checkpoints if checkpoints.numel() else None,
+                    d_output=d_output, d_last=d_last, gradients=(*dense, d_state), workspace=workspace), v.device)
+    return (*dense, d_state)
+
+
+def _rule_step(q, k, v, decay, beta, state, resets, scale):
+    batch, heads, value_size = v.shape
+    output = torch.empty((batch, heads, value_size), dtype=v.dtype, device=v.device)
+    if batch:
+        sb = resets.stride(0) if resets is not None else 0
+        qb, qh = q.stride()[:2]
+        kb, kh = k.stride()[:2]
+        vb, vh = v.stride()[:2]
+        db, dh = decay.stride()
+        bb, bh = beta.stride()
+        _call('cuju_delta_rule_step',
+              _RULE.pack(TYPES[q.dtype], batch, 1, q.shape[1], heads, q.shape[2], value_size, scale,
+                         q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), beta.data_ptr(), _pointer(resets),
+                         qb, 0, qh, kb, 0, kh, vb, 0, vh, db, 0, dh, bb, 0, bh, sb, 0,
+                         state.data_ptr(), output.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), v.device)
+    return output
+
+
+class _DeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, decay, beta, state, resets, scale):
+        run = torch.ops.cuju_amd.delta_rule if torch.compiler.is_compiling() else _rule_forward
+        output, last, checkpoints = run(q, k, v, decay, beta, state, resets, scale, True)
+        ctx.save_for_backward(q, k, v, decay, beta, state, resets, checkpoints)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return output, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_output, d_last):
+        q, k, v, decay, beta, state, resets, checkpoints = ctx.saved_tensors
+        d_output = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if d_output is None else _flat(d_output)
+        d_last = d_last.contiguous() if d_last is not None else None
+        run = torch.ops.cuju_amd.delta_rule_backward if torch.compiler.is_compiling() else _rule_backward
+        *dense, d_state = run(q, k, v, decay, beta, state, resets, ctx.scale, checkpoints, d_output, d_last)
+        return (*dense, d_state if state is not None else None, None, None)
+
+
+def delta_rule(query, key, value, decay, beta, *, state=None, resets=None, scale=None):
+    """The gated delta rule over many steps: `(output, last)`.
+
+    Each head keeps a matrix S [key size, value size], from `state` or zeros. At each step it is
+    cleared where `resets` is true, scaled by `exp(decay)`, and written:
+    `u = beta * (value - S^T key)`, `S += key u^T`; the output is `scale * S^T query`.
+
+    * `query`, `key`: [batch, time, key heads, key size]; `value`: [batch, time, heads, value size], all
+      of one type. Head h reads the key head `h // (heads / key heads)`. Keys are taken as they are:
+      the rule is stable for `beta * |key|^2` up to 2, as with keys of unit length and beta up to 1.
+    * `decay` (the logarithm of the factor, so at most 0 in use; -inf keeps nothing) and `beta`:
+      [batch, time, heads], of any floating type, held in 32 bits.
+    * `state`: [batch, heads, key size, value size], in 32 bits.
+    * `resets`: [batch, time], bool or uint8: true where an episode starts. Nothing before such a step,
+      not even an infinity, reaches its outputs, the later ones or their gradients.
+    * `scale`: by default 1 / sqrt(key size).
+
+    `output` is [batch, time, heads, value size] in the inputs' type, `last` the memory after the last
+    step in 32 bits. Sizes go up to 128, strides are free (an axis of time before the batch is a
+    transposed view). Gradients reach every floating input; they are the same on every call.
+    """
+    q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, True)
+    if state is not None:
+        state = state.float().contiguous()
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, decay, beta, state)):
+        return _DeltaRule.apply(q, k, v, decay, beta, state, resets, scale)
+    run = torch.ops.cuju_amd.delta_rule if torch.compiler.is_compiling() else _rule_forward
+    output, last, _ = run(q, k, v, decay, beta, state, resets, scale, False)
+    return output, last
+
+
+def delta_rule_step(query, key, value, decay, beta, state, *, resets=None, scale=None):
+    """One step of the gated delta rule, as in acting: returns the output and updates `state` in place.
+
+    As `delta_rule` without the axis of time: `query` and `key` [batch, key heads, key size], `value`
+    [batch, heads, value size], `decay` and `beta` [batch, heads], `resets` [batch]; `state` is a
+    contiguous float32 tensor [batch, heads, key size, value size]. A memory that is reset is not read.
+    It has no gradients: an update learns through `delta_rule`.
+    """
+    q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, False)
+    if state is None or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ArgumentError('expected state as a contiguous float32 tensor, which the step updates')
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, decay, beta, state)):
+        raise ArgumentError('delta_rule_step has no gradients: call it under torch.no_grad(), or call delta_rule')
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if torch.compiler.is_compiling():
+        return torch.ops.cuju_amd.delta_rule_step(q, k, v, decay, beta, state, resets, scale)
+    output = _rule_step(q, k, v, decay, beta, state, resets, scale)
+    torch.autograd.graph.increment_version(state)
+    return output
+
+
+# --------------------------------------------------------------------------------------- group norm
+
+def _norm(x, groups, weight, bias, epsilon, activation, y=None, stats=None, workspace=None, dy=None, dx=None, d_weight=None,
+          d_bias=None) -> bytes:
+    batch, channels = x.shape[0], x.shape[-1]
+    pixels = x.numel() // (batch * channels) if batch else 0
+    return _NORM.pack(TYPES[x.dtype], batch, pixels, channels, groups, activation, epsilon, x.data_ptr(),
+                      _pointer(weight), _pointer(bias), _pointer(y), _pointer(stats), _pointer(workspace),
+                      _pointer(dy), _pointer(dx), _pointer(d_weight), _pointer(d_bias))
+
+
+def _norm_workspace(x, groups):
+    size = load().cuju_group_norm_workspace(_norm(x, groups, None, None, 0.0, 0))
+    return torch.empty(size, dtype=torch.uint8, device=x.device)
+
+
+def _norm_forward(x, weight, bias, groups, epsilon, activation):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+    if x.numel():
+        workspace = _norm_workspace(x, groups)
+        _call('cuju_group_norm_forward', _norm(x, groups, weight, bias, epsilon, activation, y, stats, workspace), x.device)
+    return y, stats
+
+
+def _norm_backward(x, weight, bias, stats, dy, groups, epsilon, activation):
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    d_weight, d_bias = (torch.empty(x.shape[-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    if x.numel():
+        workspace = _norm_workspace(x, groups)
+        _call('cuju_group_norm_backward',
+              _norm(x, groups, weight, bias, epsilon, activation, None, stats, workspace, dy, dx, d_weight, d_bias), x.device)
+    else:
+        d_weight.zero_(), d_bias.zero_()
+    return dx, d_weight, d_bias
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, epsilon, activation):
+        run = torch.ops.cuju_amd.group_norm if torch.compiler.is_compiling() else _norm_forward
+        y, stats = run(x, weight, bias, groups, epsilon, activation)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.options = groups, epsilon, activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        run = torch.ops.cuju_amd.group_norm_backward if torch.compiler.is_compiling() else _norm_backward
+        dx, d_weight, d_bias = run(x, weight, bias, stats, dy.contiguous(), *ctx.options)
+        return dx, d_weight if weight is not None else None, d_bias if bias is not None else None, None, None, None
+
+
+def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='none'):
+    """Group norm with an activation over channels-last maps `x` [batch, ..., channels].
+
+    The channels are cut into `groups` equal runs; each is normalised over its channels and all axes
+    between the batch and the channels, then scaled by `weight` and shifted by `bias` ([channels], held
+    in 32 bits, by default ones and zeros), then passed through `activation`: 'none', 'relu' or
+    'silu'. The output has the type and shape of `x`, contiguous. A NCHW tensor of torch's channels-last
+    memory format is such a map as `x.permute(0, 2, 3, 1)`, without a copy. Gradients reach `x`,
+    `weight` and `bias`; they are the same on every call.
+    """
+    _device('x', x, {'weight': weight, 'bias': bias})
+    if x.dtype not in TYPES:
+        raise ArgumentError(f'expected x of float32, bfloat16 or float16, found {x.dtype}')
+    if x.dim() < 2 or x.shape[-1] < 1:
+        raise ArgumentError(f'expected x of a batch axis and channels, found the shape {tuple(x.shape)}')
+    channels = x.shape[-1]
+    if not isinstance(groups, int) or groups < 1 or channels % groups:
+        raise ArgumentError(f'expected groups that divide the {channels} channels, found {groups}')
+    if activation not in ACTIVATIONS:
+        raise ChoiceError(f"expected the activation 'none', 'relu' or 'silu', found {activation!r}")
+    for name, each in (('weight', weight), ('bias', bias)):
+        if each is not None:
+            _shape(name, each, (channels,))
+            if not each.is_floating_point():
+                raise ArgumentError(f'expected {name} of a floating type, found {each.dtype}')
+    if x.numel() // (x.shape[0] or 1) >= 1 << 31 or x.shape[0] * groups >= 1 << 22:
+        raise ArgumentError(f'expected fewer than 2^22 groups in the batch and 2^31 values in a map, found the shape '
+                            f'{tuple(x.shape)}')
+    x = x.contiguous()
+    weight = weight.float().contiguous() if weight is not None else None
+    bias = bias.float().contiguous() if bias is not None else None
+    options = groups, float(epsilon), ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(each is not None and each.requires_grad for each in (x, weight, bias)):
+        return _GroupNorm.apply(x, weight, bias, *options)
+    run = torch.ops.cuju_amd.group_norm if torch.compiler.is_compiling() else _norm_forward
+    return run(x, weight, bias, *options)[0]
+
+
+# -------------------------------------------------------------------------- operators of torch.compile
+
+_NAMESPACE = torch.library.Library('cuju_amd', 'FRAGMENT')
+_INPUTS = 'Tensor query, Tensor key, Tensor value, Tensor decay, Tensor beta'
+_NAMESPACE.define(f'delta_rule({_INPUTS}, Tensor? state, Tensor? resets, float scale, bool train) -> '
+                  '(Tensor, Tensor, Tensor)')
+_NAMESPACE.define(f'delta_rule_backward({_INPUTS}, Tensor? state, Tensor? resets, float scale, Tensor checkpoints, '
+                  'Tensor d_output, Tensor? d_last) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)')
+_NAMESPACE.define(f'delta_rule_step({_INPUTS}, Tensor(a!) state, Tensor? resets, float scale) -> Tensor')
+_NAMESPACE.define('group_norm(Tensor x, Tensor? weight, Tensor? bias, int groups, float epsilon, int activation) -> '
+                  '(Tensor, Tensor)')
+_NAMESPACE.define('group_norm_backward(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor dy, int groups, '
+                  'float epsilon, int activation) -> (Tensor, Tensor, Tensor)')
+_NAMESPACE.impl('delta_rule', _rule_forward, 'CUDA')
+_NAMESPACE.impl('delta_rule_backward', _rule_backward, 'CUDA')
+_NAMESPACE.impl('delta_rule_step', _rule_step, 'CUDA')
+_NAMESPACE.impl('group_norm', _norm_forward, 'CUDA')
+_NAMESPACE.impl('group_norm_backward', _norm_backward, 'CUDA')
+
+
+@torch.library.register_fake('cuju_amd::delta_rule')
+def _(query, key, value, decay, beta, state, resets, scale, train):
+    batch, time, _, key_size = query.shape
+    heads, value_size = value.shape[2:]
+    kept = max(time - 1, 0) // SEGMENT if train else 0
+    return (value.new_empty(value.shape), decay.new_empty((batch, heads, key_size, value_size)),
+            decay.new_empty((batch, heads, kept, key_size, value_size)))
+
+
+@torch.library.register_fake('cuju_amd::delta_rule_backward')
+def _(query, key, value, decay, beta, state, resets, scale, checkpoints, d_output, d_last):
+    batch, _, _, key_size = query.shape
+    return (*[x.new_empty(x.shape) for x in (query, key, value, decay, beta)],
+            decay.new_empty((batch, value.shape[2], key_size, value.shape[3])))
+
+
+@torch.library.register_fake('cuju_amd::delta_rule_step')
+def _(query, key, value, decay, beta, state, resets, scale):
+    return value.new_empty(value.shape)
+
+
+@torch.library.register_fake('cuju_amd::group_norm')
+def _(x, weight, bias, groups, epsilon, activation):
+    return x.new_empty(x.shape), x.new_empty((x.shape[0], groups, 2), dtype=torch.float32)
+
+
+@torch.library.register_fake('cuju_amd::group_norm_backward')
+def _(x, weight, bias, stats, dy, groups, epsilon, activation):
+    sums = x.new_empty((x.shape[-1],), dtype=torch.float32)
+    return x.new_empty(x.shape), sums, torch.empty_like(sums)

@@ -106,6 +106,13 @@ SIGNATURES = [
     ('cuju_scenario_build_bundle', I, [ctypes.POINTER(ScenarioDescription), ctypes.POINTER(ScenarioDescription),
                                        ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p]),
     ('cuju_debug_libm_device', I, [I, I, ctypes.c_uint, ctypes.c_longlong, P, P, P, P]),
+    # The policy operators take their argument structs as packed bytes (layers.py).
+    ('cuju_delta_rule_step', I, [ctypes.c_char_p, P]),
+    ('cuju_delta_rule_forward', I, [ctypes.c_char_p, P]),
+    ('cuju_delta_rule_backward', I, [ctypes.c_char_p, P]),
+    ('cuju_group_norm_workspace', U64, [ctypes.c_char_p]),
+    ('cuju_group_norm_forward', I, [ctypes.c_char_p, P]),
+    ('cuju_group_norm_backward', I, [ctypes.c_char_p, P]),
 ]
 
 _loaded = {}

@@ -172,6 +172,62 @@ int cuju_scenario_build_bundle(const struct cuju_scenario_description *even, con
 int cuju_debug_libm_device(int kind, int which, unsigned int first, long long count, const void *x, const void *y, void *out,
                            void *stream);
 
+/* The operators of a policy that learns from a batch. None has a counterpart in the reference. They
+   run on `stream` with device memory and wait for nothing; workspaces come from the caller. `type` is
+   the element type: 0 float, 1 bfloat16, 2 IEEE half. 0, or -1 with cuju_last_error(). */
+
+/* The gated delta rule. A head's memory is a matrix S [key_size][value_size] of floats. Step t clears
+   it where `resets` is nonzero, scales it by exp(decay), and writes u = beta (value - S^T key):
+   S += key u^T, output = scale S^T query. Heads h share the query and key head
+   h / (heads / key_heads). Strides are in elements, for [batch][time][head] ([batch][time] for
+   resets), the last axis is contiguous; outputs, memories and gradients are contiguous. Sizes of keys
+   and values are 1 to 128. */
+struct cuju_delta_rule {
+    int type, batch, time, key_heads, heads, key_size, value_size;
+    float scale;
+    const void *query, *key, *value; /* of `type` */
+    const void *decay, *beta;        /* float; decay is the logarithm of the factor */
+    const unsigned char *resets;     /* or null */
+    long long query_strides[3], key_strides[3], value_strides[3], decay_strides[3], beta_strides[3], reset_strides[2];
+    void *state;                     /* [batch][heads][key_size][value_size], or null for zeros; a step updates it */
+    void *output;                    /* of `type`, [batch][time][heads][value_size] */
+    void *last;                      /* the memory after the last step, or null */
+    void *checkpoints;               /* [batch][heads][(time - 1) / 32][key_size][value_size]: the forward pass keeps the
+                                        memory before every 32nd step for the backward pass; null for none */
+    /* Only for the backward pass. */
+    const void *d_output;            /* of `type` */
+    long long d_output_strides[3];
+    const void *d_last;              /* or null for zeros */
+    void *d_query, *d_key, *d_value; /* of `type` */
+    void *d_decay, *d_beta;          /* [batch][time][heads] */
+    void *d_state;                   /* or null */
+    void *workspace;                 /* 2 * batch * time * heads * key_size floats where heads != key_heads */
+};
+/* One step (time 1), the memory updated in place. */
+int cuju_delta_rule_step(const struct cuju_delta_rule *rule, void *stream);
+int cuju_delta_rule_forward(const struct cuju_delta_rule *rule, void *stream);
+int cuju_delta_rule_backward(const struct cuju_delta_rule *rule, void *stream);
+
+/* Group norm with an activation (0 none, 1 relu, 2 silu) over channels-last maps
+   [batch][pixels][channels], contiguous: the channels in `groups` equal runs, each normalised over the
+   pixels and its channels, scaled and shifted by channel. */
+struct cuju_group_norm {
+    int type, batch, pixels, channels, groups, activation;
+    float epsilon;
+    const void *x;
+    const void *weight, *bias;       /* float [channels], or null for ones and zeros */
+    void *y;
+    void *stats;                     /* float [batch][groups][2]: mean and inverse deviation, written forward */
+    void *workspace;                 /* cuju_group_norm_workspace() bytes */
+    /* Only for the backward pass. */
+    const void *dy;
+    void *dx;
+    void *d_weight, *d_bias;         /* float [channels], or null */
+};
+unsigned long long cuju_group_norm_workspace(const struct cuju_group_norm *norm);
+int cuju_group_norm_forward(const struct cuju_group_norm *norm, void *stream);
+int cuju_group_norm_backward(const struct cuju_group_norm *norm, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,9 @@ __device__ __forceinline__ int Opaque(int x) {
     return x;
 }
 
+// What lies in LDS is read again after this rather than kept in registers.
+__device__ __forceinline__ void Forget() { asm volatile("" ::: "memory"); }
+
 // A kernel's only argument, read anew from the arguments' segment: many strides and pointers that are
 // each used once in a long loop would not all fit the scalar registers.
 template <class X>

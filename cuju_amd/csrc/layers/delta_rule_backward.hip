@@ -18,10 +18,11 @@ namespace layers {
 namespace {
 
 // One workgroup takes a head backwards through its steps, a segment of two chunks at a time. A
-// wavefront holds 16 columns of the memory. Of a segment, two wavefronts first build a chunk's
-// triangular matrices each; then the first chunk is played forward from the segment's checkpoint, and
-// the chunks are taken in reverse. The products that contract the columns (S0 dO, S0 dB, dS U) go
-// through LDS, each wavefront taking whole tiles of keys.
+// wavefront holds 16 columns of the memory. The segment's inputs lie in LDS while the next segment's
+// are on their way to registers. Two wavefronts first build a chunk's triangular matrices each; then
+// the first chunk is played forward from the segment's checkpoint, and the chunks are taken in
+// reverse. The products that contract the columns (S0 dO, S0 dB, dS U) go through LDS, each wavefront
+// taking whole tiles of keys.
 template <class T>
 struct BackwardArgs {
     Rule rule;
@@ -31,19 +32,31 @@ struct BackwardArgs {
     bool shared;
 };
 
-constexpr int kMatrixRow = 20, kMatrix = kChunk * kMatrixRow;  // a 16x16 matrix in LDS
+constexpr int kMatrixRow = 16, kMatrix = kChunk * kMatrixRow;  // a 16x16 matrix in LDS
+constexpr int kMostShared = 160 * 1024;
 
 // LDS for keys of up to `KeyTiles` tiles and values of up to `Pairs` pairs of them, in floats.
 template <int KeyTiles, int Pairs, int ElementSize>
 struct BackwardShared {
-    static constexpr int kMemoryRow = Pairs * 32 + 4;  // floats of a row of the memory
-    static constexpr int kRow = Pairs * 32 + 8;        // elements of a step's row of values
+    static constexpr int kWaves = 2 * Pairs;
+    static constexpr int kMemoryRow = Pairs * 32 + 4;     // floats of a row of the memory
+    static constexpr int kRow = Pairs * 32 + 8;           // 16-bit elements of a step's row of pieces
+    static constexpr int kKeyRow = KeyTiles * 16 + 4, kValueRow = Pairs * 32 + 4;  // elements of a step's inputs
     static constexpr int kMatrices = kSegment / kChunk * kMatrix, kPieceRows = kFloatPieces * kChunk * kRow / 2;
+    static constexpr int kMemory1 = KeyTiles * 16 * kMemoryRow;
+    static constexpr int kKeyRows = kSegment * kKeyRow * ElementSize / 4, kValueRows = kSegment * kValueRow * ElementSize / 4;
     static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kCuts = kBetas + kSegment, kInverse = kCuts + 4,
-                         kMixed = kInverse + kMatrices, kProducts = kMixed + kMatrices, kMemory = kProducts + kMatrices,
-                         kU = kMemory + KeyTiles * 16 * kMemoryRow, kB = kU + kPieceRows, kO = kB + kPieceRows,
-                         kTiles = kO + kChunk * kRow * ElementSize / 4, kDots = kTiles + KeyTiles * 256,
-                         kFloats = kDots + 2 * Pairs * 4 * kChunk;
+                         kMixed = kInverse + kMatrices, kProducts = kMixed + kMatrices, kU = kProducts + kMatrices,
+                         kB = kU + kPieceRows, kDots = kB + kPieceRows, kK = kDots + 2 * kWaves * 4 * kChunk, kQ = kK + kKeyRows,
+                         kO = kQ + kKeyRows, kMemory = kO + kValueRows,
+                         // The values are read before any memory is put down.
+                         kV = kMemory;
+    // Both the memory and its gradient where they fit, else one after the other, with the tiles' sums
+    // kept between.
+    static constexpr bool kBoth = (kMemory + 2 * kMemory1) * 4 <= kMostShared;
+    static constexpr int kSecond = kBoth ? kMemory + kMemory1 : kMemory, kTiles = kMemory + kMemory1;
+    static constexpr int kFloats = kMemory + (kBoth ? 2 * kMemory1 : kMemory1 + KeyTiles * 256);
+    static_assert(kValueRows <= kMemory1 + (kBoth ? kMemory1 : 0), "room for the values");
 };
 
 __device__ __forceinline__ F4 RowOrder(const float *matrix, int m, int g) {
@@ -55,22 +68,23 @@ __device__ __forceinline__ F4 ColumnOrder(const float *matrix, int m, int g) {
     for (int r = 0; r < 4; r++) x[r] = matrix[(4 * g + r) * kMatrixRow + m];
     return x;
 }
+
 template <class T, int KeyTiles, int Pairs, bool Whole>
 __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))) void BackwardKernel(BackwardArgs<T> a) {
     using At = BackwardShared<KeyTiles, Pairs, sizeof(T)>;
-    extern __shared__ __align__(16) float shared[];
-    constexpr int P = kPieces<T>;
     using Args = BackwardArgs<T>;
+    extern __shared__ __align__(16) float shared[];
+    constexpr int P = kPieces<T>, kThreads = 128 * Pairs, kWaves = 2 * Pairs;
     const Rule &rule = a.rule;
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    constexpr int ms = At::kMemoryRow, rs = At::kRow;
+    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    constexpr int ms = At::kMemoryRow, rs = At::kRow, ks = At::kKeyRow, vs = At::kValueRow;
     double *reach = reinterpret_cast<double *>(shared + At::kReach);
-    float *betas = shared + At::kBetas, *memory = shared + At::kMemory, *dots = shared + At::kDots;
+    float *betas = shared + At::kBetas, *memory = shared + At::kMemory, *second = shared + At::kSecond;
     unsigned *cutsOf = reinterpret_cast<unsigned *>(shared + At::kCuts);
     // Rows of values by step, [piece][step][column].
     uint16_t *sharedU = reinterpret_cast<uint16_t *>(shared + At::kU), *sharedB = reinterpret_cast<uint16_t *>(shared + At::kB);
-    T *sharedO = reinterpret_cast<T *>(shared + At::kO);
+    T *keys = reinterpret_cast<T *>(shared + At::kK), *queries = reinterpret_cast<T *>(shared + At::kQ);
+    T *values = reinterpret_cast<T *>(shared + At::kV), *outputs = reinterpret_cast<T *>(shared + At::kO);
 
     const unsigned head = Place(blockIdx.x, gridDim.x);
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
@@ -94,46 +108,81 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 if (memories && 16 * t + r < rows && column < dv) s[t][r] = from[(16 * t + r) * stride];
             }
     };
-    // A lane's four elements of each key tile of step m of a chunk.
-    const bool full = Whole && dk == 16 * KeyTiles;
-    const auto loadKeys = [&](const View<const T> &view, int t0, Pack<T, 4>(&x)[KeyTiles]) {
-        const T *p = view.At(b, min(t0 + m, time - 1), kh) + 4 * g;
-        if (full) {
+
+    // A segment's inputs: packs of four elements, thread by thread, on the way from memory to LDS. Past
+    // the end of time the last step is read again, and masked.
+    constexpr int kKeyPacks = (kSegment * KeyTiles * 4 + kThreads - 1) / kThreads, kValuePacks = kSegment * Pairs * 8 / kThreads;
+    Pack<T, 4> nextK[kKeyPacks], nextQ[kKeyPacks], nextV[kValuePacks], nextO[kValuePacks];
+    StepGates nextGate;
+    const auto fetch = [&](int s0) {
+        const Args now = Argument<Args>();
+        int i = threadIdx.x;
 #pragma unroll
-            for (int i = 0; i < KeyTiles; i++) x[i] = *reinterpret_cast<const Pack<T, 4> *>(p + 16 * i);
-        } else {
-            const int size = Opaque(dk) - 4 * g;
+        for (int j = 0; j < kKeyPacks; j++, i += kThreads) {
+            const int t = min(s0 + i / (KeyTiles * 4), time - 1), d = i % (KeyTiles * 4) * 4;
+            const int valid = i < kSegment * KeyTiles * 4 ? dk - d : 0;
+            nextK[j] = Load<4, Whole>(now.key.At(b, t, kh) + d, valid);
+            nextQ[j] = Load<4, Whole>(now.query.At(b, t, kh) + d, valid);
+        }
+        i = threadIdx.x;
 #pragma unroll
-            for (int i = 0; i < KeyTiles; i++) x[i] = Load<4, Whole>(p + 16 * i, size - 16 * i);
+        for (int j = 0; j < kValuePacks; j++, i += kThreads) {
+            const int t = min(s0 + i / (Pairs * 8), time - 1), d = i % (Pairs * 8) * 4;
+            nextV[j] = Load<4, Whole>(now.value.At(b, t, h) + d, dv - d);
+            nextO[j] = Load<4, Whole>(now.dOutput.At(b, t, h) + d, dv - d);
+        }
+        if (wave < kSegment / kChunk) nextGate = LoadGates(now.gates, b, s0 + wave * kChunk + m, time, h);
+    };
+    const auto stage = [&] {
+        int i = threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < kKeyPacks; j++, i += kThreads) {
+            const int to = i / (KeyTiles * 4) * ks + i % (KeyTiles * 4) * 4;
+            if (i < kSegment * KeyTiles * 4) {
+                *reinterpret_cast<Pack<T, 4> *>(keys + to) = nextK[j];
+                *reinterpret_cast<Pack<T, 4> *>(queries + to) = nextQ[j];
+            }
+        }
+        i = threadIdx.x;
+#pragma unroll
+        for (int j = 0; j < kValuePacks; j++, i += kThreads) {
+            const int to = i / (Pairs * 8) * vs + i % (Pairs * 8) * 4;
+            *reinterpret_cast<Pack<T, 4> *>(values + to) = nextV[j];
+            *reinterpret_cast<Pack<T, 4> *>(outputs + to) = nextO[j];
         }
     };
-    const auto loadValues = [&](const View<const T> &view, int t0) {
-        return Load<4, Whole>(view.At(b, min(t0 + m, time - 1), h) + column4, dv - column4);
+    // Step m of chunk c, where it is of this part.
+    const auto keyTile = [&](const T *rows, int c, int t, bool mine) {
+        return Masked(*reinterpret_cast<const Pack<T, 4> *>(rows + (c * kChunk + m) * ks + 16 * t + 4 * g), mine);
     };
-
-    // Columns past the last wavefront's stay zero.
-    for (int i = threadIdx.x; i < kChunk * (2 * Pairs - waves) * 16; i += blockDim.x) {
-        const int row = i % kChunk, to = row * rs + 16 * waves + i / kChunk;
-#pragma unroll
-        for (int p = 0; p < kFloatPieces; p++) sharedU[p * kChunk * rs + to] = sharedB[p * kChunk * rs + to] = 0;
-        sharedO[to] = As<T>(0.f);
-        for (int t = 0; t < KeyTiles; t++) memory[(16 * t + row) * ms + 16 * waves + i / kChunk] = 0;
-    }
+    const auto valueTile = [&](const T *rows, int c, int x, bool mine) {
+        return Masked(*reinterpret_cast<const Pack<T, 4> *>(rows + (c * kChunk + m) * vs + 16 * x + 4 * g), mine);
+    };
 
     F4 dS[KeyTiles];
     loadMemory(rule.d_last, head, dS);
+    if (segments > 0) fetch((segments - 1) * kSegment);
+    int turn = 0;  // which half of `dots`
 
     for (int segment = segments - 1; segment >= 0; segment--) {
         const int s0 = segment * kSegment;
         const int chunks = min(kSegment / kChunk, (time - s0 + kChunk - 1) / kChunk);
+        const auto checkpoint = [&](F4(&s)[KeyTiles]) {
+            const Args now = Argument<Args>();
+            if (segment > 0) loadMemory(now.rule.checkpoints, (long long)head * (segments - 1) + segment - 1, s);
+            else loadMemory(now.rule.state, head, s);
+        };
+        __syncthreads();
+        stage();
+        const StepGates gate = nextGate;
+        F4 start[KeyTiles];
+        checkpoint(start);
+        if (segment > 0) fetch(s0 - kSegment);
         __syncthreads();
         // ---- The chunks' matrices, one wavefront a chunk.
-        for (int c = wave; c < chunks; c += waves) {
-            const int t0 = s0 + c * kChunk, count = min(kChunk, time - t0);
-            const StepGates gate = LoadGates(Argument<Args>().gates, b, t0 + m, time, h);
+        if (wave < chunks) {
+            const int c = wave, count = min(kChunk, time - s0 - c * kChunk);
             const unsigned cuts = (unsigned)(__ballot(gate.reset) & 0xffff);
-            Pack<T, 4> k[KeyTiles], q[KeyTiles];
-            loadKeys(Argument<Args>().key, t0, k), loadKeys(Argument<Args>().query, t0, q);
             if (g == 0) betas[c * kChunk + m] = gate.beta;
             if (lane == 0) cutsOf[c] = cuts;
             for (int low = 0, high; low < count; low = high) {
@@ -147,8 +196,8 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
                 for (int p = 0; p < KeyTiles / 2; p++) {
                     B8 kp[P], qp[P];
-                    Pair<T>(Masked(k[2 * p], mine), Masked(k[2 * p + 1], mine), kp);
-                    Pair<T>(Masked(q[2 * p], mine), Masked(q[2 * p + 1], mine), qp);
+                    Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
+                    Pair<T>(keyTile(queries, c, 2 * p, mine), keyTile(queries, c, 2 * p + 1, mine), qp);
                     kk = Mfma32<P, P>(kp, kp, kk);
                     qk = Mfma32<P, P>(kp, qp, qk);
                 }
@@ -178,27 +227,21 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
         // The values that chunk c writes and their errors, from the memory `s` before it; with `advance`
         // the memory goes on to the next chunk.
         const auto play = [&](int c, bool advance, F4(&s)[KeyTiles], F4 &wrote, F4 &errors) {
-            const int t0 = s0 + c * kChunk, count = min(kChunk, time - t0);
+            const int count = min(kChunk, time - s0 - c * kChunk);
             const unsigned cuts = cutsOf[c];
             wrote = errors = F4{0, 0, 0, 0};
             for (int low = 0, high; low < count; low = high) {
                 const unsigned later = cuts >> (low + 1);
                 high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;
                 const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
-                Pack<T, 4> k[KeyTiles];
-                loadKeys(Argument<Args>().key, t0, k);
                 Four v[P];
-                Split<T>(Masked(loadValues(Argument<Args>().value, t0), mine), v);
-                if (high - low < kChunk) {
-#pragma unroll
-                    for (int t = 0; t < KeyTiles; t++) k[t] = Masked(k[t], mine);
-                }
+                Split<T>(valueTile(values, c, wave, mine), v);
                 F4 seen = {0, 0, 0, 0}, error = Turn<P>(v, eye), written;
                 if (!starts) {
 #pragma unroll
                     for (int p = 0; p < KeyTiles / 2; p++) {
                         B8 kp[P], sp[kFloatPieces];
-                        Pair<T>(k[2 * p], k[2 * p + 1], kp);
+                        Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
                         Pair(s[2 * p], s[2 * p + 1], sp);
                         seen = Mfma32<P, kFloatPieces>(kp, sp, seen);
                     }
@@ -228,8 +271,9 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 const float kept = Exp2(last);
 #pragma unroll
                 for (int t = 0; t < KeyTiles; t++) {
+                    Forget();
                     Four x[P], turned[P];
-                    Split<T>(k[t], x);
+                    Split<T>(keyTile(keys, c, t, mine), x);
                     Turn<P>(x, eye, turned);
                     F4 held = s[t] * kept;
                     if (starts) held = F4{0, 0, 0, 0};
@@ -237,32 +281,25 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 }
             }
         };
-        const auto checkpoint = [&](F4(&s)[KeyTiles]) {
-            const Args now = Argument<Args>();
-            if (segment > 0) loadMemory(now.rule.checkpoints, (long long)head * (segments - 1) + segment - 1, s);
-            else loadMemory(now.rule.state, head, s);
-        };
-        F4 start[KeyTiles], wroteFirst, errorsFirst;
-        checkpoint(start);
-        if (chunks > 1) play(0, true, start, wroteFirst, errorsFirst);
+        F4 wroteFirst, errorsFirst;
+        F4 wroteC, errorC;
+#pragma unroll 1
+        for (int c = 0; c < chunks; c++) {
+            if (c) wroteFirst = wroteC, errorsFirst = errorC;
+            play(c, c + 1 < chunks, start, wroteC, errorC);
+        }
+        __syncthreads();
 
         for (int c = chunks - 1; c >= 0; c--) {
             const int t0 = s0 + c * kChunk;
             const unsigned cuts = cutsOf[c];
-            F4 wroteC, errorC;
-            if (c == 0 && chunks > 1) checkpoint(start), wroteC = wroteFirst, errorC = errorsFirst;
-            else play(c, false, start, wroteC, errorC);
+            if (c + 1 < chunks) checkpoint(start), wroteC = wroteFirst, errorC = errorsFirst;
             for (int high = min(kChunk, time - t0), low; high > 0; high = low) {
                 const unsigned below = cuts & ((1u << high) - 1);
                 low = below ? 31 - __builtin_clz(below) : 0;
                 const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
-                Pack<T, 4> k[KeyTiles], q[KeyTiles];
-                loadKeys(Argument<Args>().key, t0, k), loadKeys(Argument<Args>().query, t0, q);
-                const Pack<T, 4> rawO = Masked(loadValues(Argument<Args>().dOutput, t0), mine);
-                if (high - low < kChunk) {
-#pragma unroll
-                    for (int t = 0; t < KeyTiles; t++) k[t] = Masked(k[t], mine), q[t] = Masked(q[t], mine);
-                }
+                float *dots = shared + At::kDots + turn * kWaves * 4 * kChunk;
+                turn ^= 1;
                 const double G = mine ? reach[c * kChunk + m] : 0.0, last = reach[c * kChunk + high - 1];
                 const float beta = mine ? betas[c * kChunk + m] : 0.f;
                 bool in[4];
@@ -279,16 +316,17 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
 
                 // The gradients of the values written, and of the right side they solve.
                 Four op[P];
-                Split<T>(rawO, op);
+                Split<T>(valueTile(outputs, c, wave, mine), op);
                 const F4 dO = Turn<P>(op, eye);
                 F4 dU = {0, 0, 0, 0};
 #pragma unroll
                 for (int p = 0; p < KeyTiles / 2; p++) {
                     B8 kp[P], sp[kFloatPieces];
-                    Pair<T>(k[2 * p], k[2 * p + 1], kp);
+                    Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
                     Pair(dS[2 * p], dS[2 * p + 1], sp);
                     dU = Mfma32<P, kFloatPieces>(kp, sp, dU);
                 }
+                Forget();
                 F4 dT = ColumnOrder(shared + At::kInverse + c * kMatrix, m, g);
                 F4 dP = ColumnOrder(shared + At::kMixed + c * kMatrix, m, g), written;
 #pragma unroll
@@ -300,43 +338,43 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 }
                 dU = Product(dP, dO, dU);
                 const F4 dB = Product(dT, dU), aB = Product(dU, dT), aU = Product(written, one);
+                Forget();
+                {
+                    Four up[kFloatPieces], bp[kFloatPieces];
+                    Split(aU, up), Split(aB, bp);
+#pragma unroll
+                    for (int p = 0; p < kFloatPieces; p++) {
+                        *reinterpret_cast<Four *>(sharedU + (p * kChunk + m) * rs + column4) = up[p];
+                        *reinterpret_cast<Four *>(sharedB + (p * kChunk + m) * rs + column4) = bp[p];
+                    }
+                }
+                F4 wrong;
+#pragma unroll
+                for (int r = 0; r < 4; r++) wrong[r] = RowSum(in[r] ? dB[r] * errorC[r] : 0.f);
+                if (m == 0) *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kChunk + 4 * g) = wrong;
+                float held = 0;
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        memory[(16 * t + 4 * g + r) * ms + column] = dS[t][r];
+                        if (starts) continue;
+                        if (At::kBoth) second[(16 * t + 4 * g + r) * ms + column] = start[t][r];
+                        held = fmaf(dS[t][r], start[t][r], held);
+                    }
+                held = WaveSum(held);
+                if (lane == 0) dots[(wave * 4 + 3) * kChunk] = held;
                 if (mine) {
                     Pack<T, 4> x;
 #pragma unroll
                     for (int r = 0; r < 4; r++) x.x[r] = As<T>(beta * aB[r]);
-                    Store<4, Whole>(static_cast<T *>(Argument<Args>().rule.d_value) + (((long long)b * time + t0 + m) * rule.heads + h) * dv + column4,
+                    Store<4, Whole>(static_cast<T *>(Argument<Args>().rule.d_value) +
+                                        (((long long)b * time + t0 + m) * rule.heads + h) * dv + column4,
                                     x, dv - column4);
                 }
-                Four up[kFloatPieces], bp[kFloatPieces];
-                Split(aU, up), Split(aB, bp);
-                float held = 0;
-                if (!starts) {
-#pragma unroll
-                    for (int t = 0; t < KeyTiles; t++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) held = fmaf(dS[t][r], start[t][r], held);
-                }
-                held = WaveSum(held);
-                F4 wrong;
-#pragma unroll
-                for (int r = 0; r < 4; r++) wrong[r] = RowSum(in[r] ? dB[r] * errorC[r] : 0.f);
-
-                __syncthreads();
-#pragma unroll
-                for (int p = 0; p < kFloatPieces; p++) {
-                    *reinterpret_cast<Four *>(sharedU + (p * kChunk + m) * rs + column4) = up[p];
-                    *reinterpret_cast<Four *>(sharedB + (p * kChunk + m) * rs + column4) = bp[p];
-                }
-                *reinterpret_cast<Pack<T, 4> *>(sharedO + m * rs + column4) = rawO;
-#pragma unroll
-                for (int t = 0; t < KeyTiles; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + column] = dS[t][r];
-                if (m == 0) *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kChunk + 4 * g) = wrong;
-                if (lane == 0) dots[(wave * 4 + 3) * kChunk] = held;
                 __syncthreads();
 
-                // The matrices' gradients, and dS U for this wavefront's tiles of keys.
+                // The matrices' gradients.
                 const auto rowPieces = [&](const uint16_t *rows, int x, B8(&to)[kFloatPieces]) {
 #pragma unroll
                     for (int p = 0; p < kFloatPieces; p++) {
@@ -344,15 +382,15 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                         to[p] = Eight(*reinterpret_cast<const Four *>(from), *reinterpret_cast<const Four *>(from + 16));
                     }
                 };
-                const auto memoryPieces = [&](int t, int x, B8(&to)[kFloatPieces]) {
-                    const float *from = memory + (16 * t + m) * ms + 32 * x + 4 * g;
+                const auto memoryPieces = [&](const float *from, int t, int x, B8(&to)[kFloatPieces]) {
+                    from += (16 * t + m) * ms + 32 * x + 4 * g;
                     Pair(*reinterpret_cast<const F4 *>(from), *reinterpret_cast<const F4 *>(from + 16), to);
                 };
                 const auto outputPieces = [&](int x, B8(&to)[P]) {
-                    const T *from = sharedO + m * rs + 32 * x + 4 * g;
-                    Pair<T>(*reinterpret_cast<const Pack<T, 4> *>(from), *reinterpret_cast<const Pack<T, 4> *>(from + 16), to);
+                    Pair<T>(valueTile(outputs, c, 2 * x, mine), valueTile(outputs, c, 2 * x + 1, mine), to);
                 };
                 F4 gP = {0, 0, 0, 0}, gA = {0, 0, 0, 0};
+#pragma unroll
                 for (int x = 0; x < Pairs; x++) {
                     B8 uw[kFloatPieces], other[kFloatPieces], out[P];
                     rowPieces(sharedU, x, uw);
@@ -361,17 +399,7 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                     rowPieces(sharedB, x, other);
                     gA = Mfma32<kFloatPieces, kFloatPieces>(uw, other, gA);
                 }
-                for (int t = wave; t < KeyTiles; t += waves) {
-                    F4 sum = {0, 0, 0, 0};
-                    for (int x = 0; x < Pairs; x++) {
-                        B8 uw[kFloatPieces], sp[kFloatPieces];
-                        rowPieces(sharedU, x, uw);
-                        memoryPieces(t, x, sp);
-                        sum = Mfma32<kFloatPieces, kFloatPieces>(uw, sp, sum);
-                    }
-                    // Read back by the same lane.
-                    *reinterpret_cast<F4 *>(shared + At::kTiles + (t * 64 + lane) * 4) = sum;
-                }
+                Forget();
                 const F4 aP = RowOrder(shared + At::kMixed + c * kMatrix, m, g);
                 const F4 aKK = RowOrder(shared + At::kProducts + c * kMatrix, m, g);
                 F4 aM, aN, E;
@@ -390,44 +418,50 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 Four mp[kFloatPieces], mt[kFloatPieces], np[kFloatPieces];
                 Split(aM, mp), Split(Product(aM, one), mt), Split(aN + Product(aN, one), np);
 
-                // S0 dO and S0 dB, with the memory in the gradient's place.
-                if (!starts) {
+                Forget();
+                // This wavefront's tiles of keys: dS U, S0 dO and S0 dB.
+                const auto written1 = [&](int t) {
+                    F4 sum = {0, 0, 0, 0};
+#pragma unroll
+                    for (int x = 0; x < Pairs; x++) {
+                        B8 uw[kFloatPieces], sp[kFloatPieces];
+                        rowPieces(sharedU, x, uw);
+                        memoryPieces(memory, t, x, sp);
+                        sum = Mfma32<kFloatPieces, kFloatPieces>(uw, sp, sum);
+                    }
+                    return sum;
+                };
+                if (!At::kBoth) {
+                    for (int t = wave; t < KeyTiles; t += kWaves)
+                        *reinterpret_cast<F4 *>(shared + At::kTiles + (t * 64 + lane) * 4) = written1(t);
                     __syncthreads();
+                    if (!starts) {
 #pragma unroll
-                    for (int t = 0; t < KeyTiles; t++)
+                        for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + column] = start[t][r];
+                            for (int r = 0; r < 4; r++) second[(16 * t + 4 * g + r) * ms + column] = start[t][r];
+                    }
                     __syncthreads();
                 }
                 F4 f = {0, 0, 0, 0}, e = {0, 0, 0, 0};
-                const float kept = Exp2(last);
-                Four dOp[kFloatPieces], dBp[kFloatPieces];
-                {
-                    F4 x, y;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] = rule.scale * wholeJ[r] * dO[r], y[r] = -betaj[r] * wholeJ[r] * dB[r];
-                    Split(x, dOp), Split(y, dBp);
-                }
-                for (int t = wave; t < KeyTiles; t += waves) {
+#pragma unroll 1
+                for (int t = wave; t < KeyTiles; t += kWaves) {
                     F4 dQ = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                    const F4 dKeys = At::kBoth ? written1(t) : *reinterpret_cast<const F4 *>(shared + At::kTiles + (t * 64 + lane) * 4);
+                    Forget();
                     if (!starts)
+#pragma unroll
                         for (int x = 0; x < Pairs; x++) {
                             B8 sp[kFloatPieces], other[kFloatPieces], out[P];
-                            memoryPieces(t, x, sp);
+                            memoryPieces(second, t, x, sp);
                             outputPieces(x, out);
                             dQ = Mfma32<P, kFloatPieces>(out, sp, dQ);
                             rowPieces(sharedB, x, other);
                             y = Mfma32<kFloatPieces, kFloatPieces>(other, sp, y);
                         }
-                    const Args now = Argument<Args>();
-                    const auto tile = [&](const View<const T> &view) {
-                        const T *p = view.At(b, min(t0 + m, time - 1), kh) + 16 * t + 4 * g;
-                        return Masked(Load<4, Whole>(p, dk - 16 * t - 4 * g), mine);
-                    };
-                    const Pack<T, 4> kt = tile(now.key), qt = tile(now.query);
-                    const F4 dKeys = *reinterpret_cast<const F4 *>(shared + At::kTiles + (t * 64 + lane) * 4);
+                    Forget();
                     Four kx[P], qx[P], kTurned[P], qTurned[P];
-                    Split<T>(kt, kx), Split<T>(qt, qx);
+                    Split<T>(keyTile(keys, c, t, mine), kx), Split<T>(keyTile(queries, c, t, mine), qx);
                     Turn<P>(kx, eye, kTurned), Turn<P>(qx, eye, qTurned);
                     const F4 kf = Turn<P>(kx, eye), qf = Turn<P>(qx, eye);
                     F4 dK;
@@ -443,6 +477,7 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                     dQ = Mfma16(mp, kTurned, dQ);
                     dK = Mfma16(mt, qTurned, dK);
                     dK = Mfma16(np, kTurned, dK);
+                    const Args now = Argument<Args>();
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         if (!in[r] || 16 * t + m >= dk) continue;
@@ -458,6 +493,7 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                         }
                     }
                 }
+                Forget();
                 F4 eSum, fSum;
 #pragma unroll
                 for (int r = 0; r < 4; r++) eSum[r] = RowSum(e[r]), fSum[r] = RowSum(f[r]);
@@ -467,26 +503,35 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
                 }
 
                 // The gradient of the memory before this part.
+                const float kept = Exp2(last);
+                if (starts) {
 #pragma unroll
-                for (int t = 0; t < KeyTiles; t++) {
-                    if (starts) {
-                        dS[t] = F4{0, 0, 0, 0};
-                        continue;
+                    for (int t = 0; t < KeyTiles; t++) dS[t] = F4{0, 0, 0, 0};
+                } else {
+                    Four dOp[kFloatPieces], dBp[kFloatPieces];
+                    F4 x, y;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[r] = rule.scale * wholeJ[r] * dO[r], y[r] = -betaj[r] * wholeJ[r] * dB[r];
+                    Split(x, dOp), Split(y, dBp);
+#pragma unroll
+                    for (int t = 0; t < KeyTiles; t++) {
+                        Forget();
+                        Four x[P], turned[P];
+                        Split<T>(keyTile(queries, c, t, mine), x);
+                        Turn<P>(x, eye, turned);
+                        dS[t] = Mfma16(turned, dOp, dS[t] * kept);
+                        Split<T>(keyTile(keys, c, t, mine), x);
+                        Turn<P>(x, eye, turned);
+                        dS[t] = Mfma16(turned, dBp, dS[t]);
                     }
-                    Four x[P], turned[P];
-                    Split<T>(q[t], x);
-                    Turn<P>(x, eye, turned);
-                    dS[t] = Mfma16(turned, dOp, dS[t] * kept);
-                    Split<T>(k[t], x);
-                    Turn<P>(x, eye, turned);
-                    dS[t] = Mfma16(turned, dBp, dS[t]);
                 }
                 __syncthreads();
 
                 // The gates' gradients, a lane for each step.
                 if (wave == 0) {
                     float eAll = 0, fAll = 0, bAll = 0, heldAll = 0;
-                    for (int w = 0; w < waves; w++) {
+#pragma unroll
+                    for (int w = 0; w < kWaves; w++) {
                         bAll += dots[(w * 4 + 0) * kChunk + m];
                         eAll += dots[(w * 4 + 1) * kChunk + m];
                         fAll += dots[(w * 4 + 2) * kChunk + m];
@@ -539,7 +584,6 @@ __global__ __launch_bounds__(256) void SharedKeysKernel(const float *parts, T *o
 
 template <class T, int KeyTiles>
 bool LaunchBackward(const Rule &r, hipStream_t stream) {
-    const int waves = (r.value_size + 15) / 16;
     const bool shared = r.heads != r.key_heads;
     const long long steps = (long long)r.batch * r.time, each = steps * r.heads * r.key_size;
     float *parts = static_cast<float *>(r.workspace);
@@ -553,19 +597,24 @@ bool LaunchBackward(const Rule &r, hipStream_t stream) {
                       shared ? parts + each : r.d_key,
                       shared};
     const bool whole = a.query.whole && a.key.whole && a.value.whole && a.dOutput.whole && Aligned(4 * sizeof(T), r.d_value);
-    const auto launch = [&](auto kernel, int floats) {
-        const int bytes = floats * sizeof(float);
+    const auto launch = [&](auto wide, auto packed) {
+        constexpr int Pairs = decltype(wide)::value;
+        const auto kernel = BackwardKernel<T, KeyTiles, Pairs, decltype(packed)::value>;
+        constexpr int bytes = BackwardShared<KeyTiles, Pairs, sizeof(T)>::kFloats * sizeof(float);
+        static_assert(bytes <= kMostShared, "the memory of a head fits a compute unit's LDS");
         if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
             hipSuccess)
             return false;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads)), dim3(64 * waves), bytes, stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads)), dim3(128 * Pairs), bytes, stream, a);
         return true;
     };
+    const int pairs = (r.value_size + 31) / 32;
     bool set;
-    if (!whole) set = launch(BackwardKernel<T, KeyTiles, 4, false>, BackwardShared<KeyTiles, 4, sizeof(T)>::kFloats);
-    else if (waves <= 2) set = launch(BackwardKernel<T, KeyTiles, 1, true>, BackwardShared<KeyTiles, 1, sizeof(T)>::kFloats);
-    else if (waves <= 4) set = launch(BackwardKernel<T, KeyTiles, 2, true>, BackwardShared<KeyTiles, 2, sizeof(T)>::kFloats);
-    else set = launch(BackwardKernel<T, KeyTiles, 4, true>, BackwardShared<KeyTiles, 4, sizeof(T)>::kFloats);
+    if (!whole) set = launch(std::integral_constant<int, 4>(), std::false_type());
+    else if (pairs == 1) set = launch(std::integral_constant<int, 1>(), std::true_type());
+    else if (pairs == 2) set = launch(std::integral_constant<int, 2>(), std::true_type());
+    else if (pairs == 3) set = launch(std::integral_constant<int, 3>(), std::true_type());
+    else set = launch(std::integral_constant<int, 4>(), std::true_type());
     if (!set) return false;
     if (shared && steps > 0) {
         const long long count = steps * r.key_heads * r.key_size;

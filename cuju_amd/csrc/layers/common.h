@@ -71,8 +71,23 @@ __device__ __forceinline__ int Opaque(int x) {
     return x;
 }
 
+// A pointer out of an argument struct, known to be to device memory.
+template <class T>
+__device__ __forceinline__ T *Global(T *p) { return (T *)(__attribute__((address_space(1))) T *)(uintptr_t)p; }
+
+// `base` (the same in every lane) moved by a lane's `bytes`: the address stays a scalar pair and one
+// vector register.
+template <class T>
+__device__ __forceinline__ T *Lane(T *base, uint32_t bytes) {
+    using Byte = typename std::conditional<std::is_const<T>::value, const char, char>::type;
+    return Global(reinterpret_cast<T *>(reinterpret_cast<Byte *>(base) + bytes));
+}
+
 // What lies in LDS is read again after this rather than kept in registers.
 __device__ __forceinline__ void Forget() { asm volatile("" ::: "memory"); }
+
+// The same of a lane's own value, so that what follows from it is not kept over a loop.
+__device__ __forceinline__ void Renew(F4 &x) { asm volatile("" : "+v"(x)); }
 
 // A kernel's only argument, read anew from the arguments' segment: many strides and pointers that are
 // each used once in a long loop would not all fit the scalar registers.
@@ -168,7 +183,8 @@ __device__ __forceinline__ F4 Mfma32(const B8 (&a)[A], const B8 (&b)[B], F4 c) {
             if (i + j < 3) c = Mfma32(a[i], b[j], c);
     return c;
 }
-// A product of only 16 contracted indices, four a lane: two pairs of pieces share an instruction.
+// A product of only 16 contracted indices, four a lane: two pairs of pieces share an instruction. (The
+// instruction for 16 indices does not mix with this one: chained on one accumulator they gave wrong sums.)
 template <int A, int B>
 __device__ __forceinline__ F4 Mfma16(const Four (&a)[A], const Four (&b)[B], F4 c) {
     Four left{}, right{};
@@ -181,7 +197,7 @@ __device__ __forceinline__ F4 Mfma16(const Four (&a)[A], const Four (&b)[B], F4 
             if (half) c = Mfma32(Eight(left, a[i]), Eight(right, b[j]), c);
             left = a[i], right = b[j], half = !half;
         }
-    return half ? Mfma32(Eight(left, Four{}), Eight(right, Four{}), c) : c;
+    return half ? Mfma32(Eight(left, left), Eight(right, Four{}), c) : c;
 }
 
 template <int Control>

@@ -22,7 +22,7 @@ struct View {
     T *p;
     long long batch, time, head;
     bool whole;  // packs of four are aligned, and the last axis is made of them
-    __device__ __forceinline__ T *At(int b, int t, int h) const { return p + b * batch + t * time + h * head; }
+    __device__ __forceinline__ T *At(int b, int t, int h) const { return Global(p) + b * batch + t * time + h * head; }
 };
 
 inline bool Aligned(size_t bytes, const void *p) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -48,17 +48,19 @@ inline Gates GatesOf(const Rule &r) {
 }
 
 // A step's gates, one lane of a row of 16 for each step of a chunk; past the end of time a step that
-// keeps everything and writes nothing.
+// keeps everything and writes nothing. What is loaded is looked at only when it is used, so that a load
+// ahead of time waits for nothing.
 struct StepGates {
     float decay, beta;
-    bool reset;
+    unsigned char cleared;
+    __device__ __forceinline__ bool Reset() const { return cleared | (decay < kNothingKept); }
 };
 __device__ __forceinline__ StepGates LoadGates(const Gates &g, int b, int t, int time, int h) {
-    StepGates s{0.f, 0.f, false};
+    StepGates s{0.f, 0.f, 0};
     if (t < time) {
-        s.decay = g.decay[b * g.decayStrides[0] + t * g.decayStrides[1] + h * g.decayStrides[2]];
-        s.beta = g.beta[b * g.betaStrides[0] + t * g.betaStrides[1] + h * g.betaStrides[2]];
-        s.reset = s.decay < kNothingKept || (g.resets && g.resets[b * g.resetStrides[0] + t * g.resetStrides[1]]);
+        s.decay = Global(g.decay)[b * g.decayStrides[0] + t * g.decayStrides[1] + h * g.decayStrides[2]];
+        s.beta = Global(g.beta)[b * g.betaStrides[0] + t * g.betaStrides[1] + h * g.betaStrides[2]];
+        if (g.resets) s.cleared = Global(g.resets)[b * g.resetStrides[0] + t * g.resetStrides[1]];
     }
     return s;
 }
@@ -147,7 +149,7 @@ template <int P>
 __device__ __forceinline__ F4 Turn(const Four (&x)[P], Four eye) {
     F4 sum = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = P - 1; i >= 0; i--) sum = Mfma32(Eight(x[i], Four{}), Eight(eye, Four{}), sum);
+    for (int i = P - 1; i >= 0; i--) sum = Mfma32(Eight(x[i], x[i]), Eight(eye, Four{}), sum);
     return sum;
 }
 // The same piece by piece.
@@ -155,7 +157,7 @@ template <int P>
 __device__ __forceinline__ void Turn(const Four (&x)[P], Four eye, Four (&turned)[P]) {
 #pragma unroll
     for (int i = 0; i < P; i++) {
-        const F4 t = Mfma32(Eight(x[i], Four{}), Eight(eye, Four{}), F4{0, 0, 0, 0});
+        const F4 t = Mfma32(Eight(x[i], x[i]), Eight(eye, Four{}), F4{0, 0, 0, 0});
         const float f[4] = {t[0], t[1], t[2], t[3]};
         Four whole[1];
         Split<1>(f, whole);

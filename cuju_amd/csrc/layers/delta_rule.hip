@@ -39,10 +39,11 @@ __global__ __launch_bounds__(256) void StepKernel(Rule rule, View<const T> query
     const int valid = min(columns - (lane % Lanes) * 4, dv - first);
     float *at = memory + ((long long)head * dk + row0) * dv + first;
     Pack<float, 4> s[kRows];
-    const float kept = gate.reset ? 0.f : expf(gate.decay);
+    const bool cleared = gate.Reset();
+    const float kept = cleared ? 0.f : expf(gate.decay);
     // A memory that is cleared is not read: what it held, infinities among it, is gone.
 #pragma unroll
-    for (int i = 0; i < kRows; i++) s[i] = Load<4, Whole>(at + i * dv, !gate.reset && row0 + i < dk ? valid : 0);
+    for (int i = 0; i < kRows; i++) s[i] = Load<4, Whole>(at + i * dv, !cleared && row0 + i < dk ? valid : 0);
     float seen[4] = {0, 0, 0, 0}, out[4] = {0, 0, 0, 0}, both = 0;
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
     if (time > 0) fetch(0);
     for (int t0 = 0, low = 0, high; t0 < time; low = high) {
         // The part: steps [low, high) of the chunk at t0. The others are masked.
-        const unsigned cuts = (unsigned)(__ballot(next.reset) & 0xffff);
+        const unsigned cuts = (unsigned)(__ballot(next.Reset()) & 0xffff);
         const int count = min(kChunk, time - t0);
         const unsigned later = cuts >> (low + 1);
         high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
         // ---- The chunks' matrices, one wavefront a chunk.
         if (wave < chunks) {
             const int c = wave, count = min(kChunk, time - s0 - c * kChunk);
-            const unsigned cuts = (unsigned)(__ballot(gate.reset) & 0xffff);
+            const unsigned cuts = (unsigned)(__ballot(gate.Reset()) & 0xffff);
             if (g == 0) betas[c * kChunk + m] = gate.beta;
             if (lane == 0) cutsOf[c] = cuts;
             for (int low = 0, high; low < count; low = high) {

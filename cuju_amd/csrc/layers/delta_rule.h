@@ -135,34 +135,42 @@ __device__ __forceinline__ Pack<T, 4> Masked(const Pack<T, 4> &x, bool keep) {
     return __builtin_bit_cast(Pack<T, 4>, r);
 }
 
-// The left columns of the identity as a right operand, for a product that turns row order into column
-// order: exact for a bfloat16.
-__device__ __forceinline__ Four Eye(int m, int g) {
+// The identity as a right operand for the first or the second half of a pair's eight values: a product
+// with it turns that half from row order into column order, exactly.
+struct Eyes {
+    B8 half[2];
+};
+__device__ __forceinline__ Eyes EyesOf(int m, int g) {
     Four eye;
 #pragma unroll
     for (int j = 0; j < 2; j++)
         eye.x[j] = (4 * g + 2 * j == m ? 0x3f80u : 0u) | (4 * g + 2 * j + 1 == m ? 0x3f800000u : 0u);
-    return eye;
+    return Eyes{{Eight(eye, Four{}), Eight(Four{}, eye)}};
 }
-// A matrix's pieces from row into column order, as floats.
+// As floats.
 template <int P>
-__device__ __forceinline__ F4 Turn(const Four (&x)[P], Four eye) {
+__device__ __forceinline__ F4 Turn(const B8 (&x)[P], B8 eye) {
     F4 sum = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = P - 1; i >= 0; i--) sum = Mfma32(Eight(x[i], x[i]), Eight(eye, Four{}), sum);
+    for (int i = P - 1; i >= 0; i--) sum = Mfma32(x[i], eye, sum);
     return sum;
 }
-// The same piece by piece.
+// Piece by piece.
 template <int P>
-__device__ __forceinline__ void Turn(const Four (&x)[P], Four eye, Four (&turned)[P]) {
+__device__ __forceinline__ void Turn(const B8 (&x)[P], B8 eye, Four (&turned)[P]) {
 #pragma unroll
     for (int i = 0; i < P; i++) {
-        const F4 t = Mfma32(Eight(x[i], x[i]), Eight(eye, Four{}), F4{0, 0, 0, 0});
+        const F4 t = Mfma32(x[i], eye, F4{0, 0, 0, 0});
         const float f[4] = {t[0], t[1], t[2], t[3]};
         Four whole[1];
         Split<1>(f, whole);
         turned[i] = whole[0];
     }
+}
+template <int P>
+__device__ __forceinline__ void Eights(const Four (&lo)[P], const Four (&hi)[P], B8 (&x)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; i++) x[i] = Eight(lo[i], hi[i]);
 }
 // The pieces of a lane's eight keys of a pair of tiles.
 template <class T>

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
     };
 
     constexpr int P = kPieces<T>;
-    const Four eye = Eye(m, g);
+    const Eyes eyes = EyesOf(m, g);
 
     if (time > 0) fetch(0);
     for (int t0 = 0, low = 0, high; t0 < time; low = high) {
@@ -246,12 +246,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
             Pair<T>(k[2 * p], k[2 * p + 1], kp), Pair<T>(q[2 * p], q[2 * p + 1], qp);
             kk = Mfma32<P, P>(kp, kp, kk);
             qk = Mfma32<P, P>(kp, qp, qk);
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                Four x[P];
-                Split<T>(k[2 * p + half], x);
-                Turn<P>(x, eye, turned[2 * p + half]);
-            }
+            Turn<P>(kp, eyes.half[0], turned[2 * p]);
+            Turn<P>(kp, eyes.half[1], turned[2 * p + 1]);
 #pragma unroll
             for (int c = 0; c < Tiles; c++) {
                 B8 sp[kFloatPieces];

@@ -17,103 +17,107 @@
 namespace layers {
 namespace {
 
-// One workgroup takes a head backwards through its steps, a segment of two chunks at a time. A
-// wavefront holds 16 columns of the memory. The segment's inputs lie in LDS while the next segment's
-// are on their way to registers. Two wavefronts first build a chunk's triangular matrices each; then
-// the first chunk is played forward from the segment's checkpoint, and the chunks are taken in
-// reverse. The products that contract the columns (S0 dO, S0 dB, dS U) go through LDS, each wavefront
-// taking whole tiles of keys.
+// One workgroup takes 64 columns of a head backwards through its steps, 32 at a time: two tiles of
+// steps, from the memory that the forward pass kept before them. A wavefront holds 16 columns of the
+// memory and of its gradient. The steps' inputs lie in LDS while the next ones are on their way to
+// registers. Between barriers,
+//  - the triangular matrices of the tiles (11, 22) and between them (21), a block to a wavefront;
+//  - U, dU and dB by columns, put down in row order in pieces, with the memory's gradient;
+//  - dP and dA, and from them the matrices the keys' and queries' gradients take, a block to a
+//    wavefront; dS U by tiles of keys, whole tiles to a wavefront;
+//  - with the memory in its gradient's place: S0 dO, S0 dB, and the keys' and queries' gradients.
+// Wider values take several workgroups, whose gradients of the keys, queries and gates a second kernel
+// adds up, as it does for heads that share keys.
 template <class T>
 struct BackwardArgs {
     Rule rule;
     View<const T> query, key, value, dOutput;
     Gates gates;
-    void *dQuery, *dKey;  // of T with the key heads, or of float with the heads where `shared`
-    bool shared;
+    void *dQuery, *dKey;    // of T, or parts of float by head and slice
+    float *dDecay, *dBeta;  // or parts by slice
+    int slices;
+    bool parted;  // whether dQuery and dKey are parts
 };
 
-constexpr int kMatrixRow = 16, kMatrix = kChunk * kMatrixRow;  // a 16x16 matrix in LDS
-constexpr int kMostShared = 160 * 1024;
+constexpr int kSlice = 64;                       // columns of a workgroup
+constexpr int kMatrix = kChunk * kChunk;         // a 16x16 matrix in LDS
+constexpr int kPieceMatrix = kFloatPieces * kMatrix / 2;  // its pieces
+enum Block { kFirst, kSecond, kAcross };         // of two tiles of steps: 11, 22 and 21
 
-// LDS for keys of up to `KeyTiles` tiles and values of up to `Pairs` pairs of them, in floats.
-template <int KeyTiles, int Pairs, int ElementSize>
+// LDS for keys of up to `KeyTiles` tiles and `Waves` wavefronts of 16 columns, in floats.
+template <int KeyTiles, int Waves, int ElementSize>
 struct BackwardShared {
-    static constexpr int kWaves = 2 * Pairs;
-    static constexpr int kMemoryRow = Pairs * 32 + 4;     // floats of a row of the memory
-    static constexpr int kRow = Pairs * 32 + 8;           // 16-bit elements of a step's row of pieces
-    static constexpr int kKeyRow = KeyTiles * 16 + 4, kValueRow = Pairs * 32 + 4;  // elements of a step's inputs
-    static constexpr int kMatrices = kSegment / kChunk * kMatrix, kPieceRows = kFloatPieces * kChunk * kRow / 2;
-    static constexpr int kMemory1 = KeyTiles * 16 * kMemoryRow;
+    static constexpr int kMemoryRow = Waves * 16 + 4;  // floats of a row of the memory
+    static constexpr int kRow = Waves * 16 + 8;        // 16-bit elements of a step's row of pieces
+    static constexpr int kKeyRow = KeyTiles * 16 + 4, kValueRow = Waves * 16 + 4;  // elements of a step's inputs
+    static constexpr int kPieceRows = kFloatPieces * kSegment * kRow / 2;
     static constexpr int kKeyRows = kSegment * kKeyRow * ElementSize / 4, kValueRows = kSegment * kValueRow * ElementSize / 4;
-    static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kCuts = kBetas + kSegment, kInverse = kCuts + 4,
-                         kMixed = kInverse + kMatrices, kProducts = kMixed + kMatrices, kU = kProducts + kMatrices,
-                         kB = kU + kPieceRows, kDots = kB + kPieceRows, kK = kDots + 2 * kWaves * 4 * kChunk, kQ = kK + kKeyRows,
-                         kO = kQ + kKeyRows, kMemory = kO + kValueRows,
-                         // The values are read before any memory is put down.
-                         kV = kMemory;
-    // Both the memory and its gradient where they fit, else one after the other, with the tiles' sums
-    // kept between.
-    static constexpr bool kBoth = (kMemory + 2 * kMemory1) * 4 <= kMostShared;
-    static constexpr int kSecond = kBoth ? kMemory + kMemory1 : kMemory, kTiles = kMemory + kMemory1;
-    static constexpr int kFloats = kMemory + (kBoth ? 2 * kMemory1 : kMemory1 + KeyTiles * 256);
-    static_assert(kValueRows <= kMemory1 + (kBoth ? kMemory1 : 0), "room for the values");
+    static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kWhole = kBetas + kSegment, kAfter = kWhole + kSegment,
+                         kCuts = kAfter + kSegment, kInverse = kCuts + 4, kMixed = kInverse + 2 * kMatrix,
+                         kProducts = kMixed + 3 * kMatrix, kM = kProducts + 3 * kMatrix, kN = kM + 3 * kPieceMatrix,
+                         kSums = kN + 3 * kPieceMatrix, kDots = kSums + 8 * kChunk, kU = kDots + Waves * 4 * kSegment,
+                         kB = kU + kPieceRows, kK = kB + kPieceRows, kQ = kK + kKeyRows, kO = kQ + kKeyRows,
+                         kMemory = kO + kValueRows, kFloats = kMemory + KeyTiles * 16 * kMemoryRow;
 };
 
 __device__ __forceinline__ F4 RowOrder(const float *matrix, int m, int g) {
-    return *reinterpret_cast<const F4 *>(matrix + m * kMatrixRow + 4 * g);
+    return *reinterpret_cast<const F4 *>(matrix + m * kChunk + 4 * g);
 }
 __device__ __forceinline__ F4 ColumnOrder(const float *matrix, int m, int g) {
     F4 x;
 #pragma unroll
-    for (int r = 0; r < 4; r++) x[r] = matrix[(4 * g + r) * kMatrixRow + m];
+    for (int r = 0; r < 4; r++) x[r] = matrix[(4 * g + r) * kChunk + m];
     return x;
 }
 
-template <class T, int KeyTiles, int Pairs, bool Whole>
-__global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))) void BackwardKernel(BackwardArgs<T> a) {
-    using At = BackwardShared<KeyTiles, Pairs, sizeof(T)>;
+template <class T, int KeyTiles, int Waves, bool Whole>
+__global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(2))) void BackwardKernel(BackwardArgs<T> a) {
+    using At = BackwardShared<KeyTiles, Waves, sizeof(T)>;
     using Args = BackwardArgs<T>;
     extern __shared__ __align__(16) float shared[];
-    constexpr int P = kPieces<T>, kThreads = 128 * Pairs, kWaves = 2 * Pairs;
+    constexpr int P = kPieces<T>, kThreads = 64 * Waves, kPairs = Waves / 2;
     const Rule &rule = a.rule;
     const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
     constexpr int ms = At::kMemoryRow, rs = At::kRow, ks = At::kKeyRow, vs = At::kValueRow;
     double *reach = reinterpret_cast<double *>(shared + At::kReach);
-    float *betas = shared + At::kBetas, *memory = shared + At::kMemory, *second = shared + At::kSecond;
+    float *betas = shared + At::kBetas, *wholes = shared + At::kWhole, *afters = shared + At::kAfter;
+    float *memory = shared + At::kMemory, *dots = shared + At::kDots, *sums = shared + At::kSums;
     unsigned *cutsOf = reinterpret_cast<unsigned *>(shared + At::kCuts);
     // Rows of values by step, [piece][step][column].
     uint16_t *sharedU = reinterpret_cast<uint16_t *>(shared + At::kU), *sharedB = reinterpret_cast<uint16_t *>(shared + At::kB);
+    uint16_t *sharedM = reinterpret_cast<uint16_t *>(shared + At::kM), *sharedN = reinterpret_cast<uint16_t *>(shared + At::kN);
     T *keys = reinterpret_cast<T *>(shared + At::kK), *queries = reinterpret_cast<T *>(shared + At::kQ);
-    T *values = reinterpret_cast<T *>(shared + At::kV), *outputs = reinterpret_cast<T *>(shared + At::kO);
+    T *outputs = reinterpret_cast<T *>(shared + At::kO);
 
-    const unsigned head = Place(blockIdx.x, gridDim.x);
+    const unsigned id = Place(blockIdx.x, gridDim.x);
+    const unsigned slice = id % a.slices, head = id / a.slices;
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
     const int dk = rule.key_size, dv = rule.value_size, time = rule.time;
-    const int column = 16 * wave + m;       // the column of a lane in column order
-    const int column4 = 16 * wave + 4 * g;  // its first of four in row order
+    const int base = slice * kSlice;
+    const int column = base + 16 * wave + m;  // a lane's column in column order
+    const int column4 = 16 * wave + 4 * g;    // its first of four in row order, within the slice
     const int segments = (time + kSegment - 1) / kSegment;
-    const Four eye = Eye(m, g);
-    F4 one;
-#pragma unroll
-    for (int r = 0; r < 4; r++) one[r] = m == 4 * g + r ? 1.f : 0.f;
+    const Eyes eyes = EyesOf(m, g);
 
     const auto loadMemory = [&](const void *memories, long long index, F4(&s)[KeyTiles]) {
         const int rows = Opaque(dk) - 4 * g, stride = Opaque(dv);
-        const float *from = static_cast<const float *>(memories) + (index * dk + 4 * g) * stride + column;
+        const float *from = static_cast<const float *>(memories) + index * dk * dv;
+        const uint32_t at = (4 * g * stride + column) * sizeof(float);
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 s[t][r] = 0.f;
-                if (memories && 16 * t + r < rows && column < dv) s[t][r] = from[(16 * t + r) * stride];
+                if (memories && 16 * t + r < rows && column < dv) s[t][r] = *Lane(from + (16 * t + r) * stride, at);
             }
     };
 
-    // A segment's inputs: packs of four elements, thread by thread, on the way from memory to LDS. Past
-    // the end of time the last step is read again, and masked.
-    constexpr int kKeyPacks = (kSegment * KeyTiles * 4 + kThreads - 1) / kThreads, kValuePacks = kSegment * Pairs * 8 / kThreads;
-    Pack<T, 4> nextK[kKeyPacks], nextQ[kKeyPacks], nextV[kValuePacks], nextO[kValuePacks];
-    StepGates nextGate;
+    // The steps' inputs: packs of four elements, thread by thread, on the way from memory to LDS; the
+    // values of a wavefront's own columns in row order. Past the end of time the last step is read again,
+    // and masked.
+    constexpr int kKeyPacks = (kSegment * KeyTiles * 4 + kThreads - 1) / kThreads, kValuePacks = kSegment * Waves * 4 / kThreads;
+    Pack<T, 4> nextK[kKeyPacks], nextQ[kKeyPacks], nextV[2], nextO[kValuePacks];
+    StepGates nextGates[2];
     const auto fetch = [&](int s0) {
         const Args now = Argument<Args>();
         int i = threadIdx.x;
@@ -127,11 +131,15 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
         i = threadIdx.x;
 #pragma unroll
         for (int j = 0; j < kValuePacks; j++, i += kThreads) {
-            const int t = min(s0 + i / (Pairs * 8), time - 1), d = i % (Pairs * 8) * 4;
-            nextV[j] = Load<4, Whole>(now.value.At(b, t, h) + d, dv - d);
+            const int t = min(s0 + i / (Waves * 4), time - 1), d = base + i % (Waves * 4) * 4;
             nextO[j] = Load<4, Whole>(now.dOutput.At(b, t, h) + d, dv - d);
         }
-        if (wave < kSegment / kChunk) nextGate = LoadGates(now.gates, b, s0 + wave * kChunk + m, time, h);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int t = min(s0 + kChunk * j + m, time - 1), d = base + column4;
+            nextV[j] = Load<4, Whole>(now.value.At(b, t, h) + d, dv - d);
+            nextGates[j] = LoadGates(now.gates, b, s0 + kChunk * j + m, time, h);
+        }
     };
     const auto stage = [&] {
         int i = threadIdx.x;
@@ -146,433 +154,519 @@ __global__ __launch_bounds__(128 * Pairs) __attribute__((amdgpu_waves_per_eu(2))
         i = threadIdx.x;
 #pragma unroll
         for (int j = 0; j < kValuePacks; j++, i += kThreads) {
-            const int to = i / (Pairs * 8) * vs + i % (Pairs * 8) * 4;
-            *reinterpret_cast<Pack<T, 4> *>(values + to) = nextV[j];
+            const int to = i / (Waves * 4) * vs + i % (Waves * 4) * 4;
             *reinterpret_cast<Pack<T, 4> *>(outputs + to) = nextO[j];
         }
-    };
-    // Step m of chunk c, where it is of this part.
-    const auto keyTile = [&](const T *rows, int c, int t, bool mine) {
-        return Masked(*reinterpret_cast<const Pack<T, 4> *>(rows + (c * kChunk + m) * ks + 16 * t + 4 * g), mine);
-    };
-    const auto valueTile = [&](const T *rows, int c, int x, bool mine) {
-        return Masked(*reinterpret_cast<const Pack<T, 4> *>(rows + (c * kChunk + m) * vs + 16 * x + 4 * g), mine);
     };
 
     F4 dS[KeyTiles];
     loadMemory(rule.d_last, head, dS);
     if (segments > 0) fetch((segments - 1) * kSegment);
-    int turn = 0;  // which half of `dots`
 
     for (int segment = segments - 1; segment >= 0; segment--) {
-        const int s0 = segment * kSegment;
-        const int chunks = min(kSegment / kChunk, (time - s0 + kChunk - 1) / kChunk);
-        const auto checkpoint = [&](F4(&s)[KeyTiles]) {
-            const Args now = Argument<Args>();
-            if (segment > 0) loadMemory(now.rule.checkpoints, (long long)head * (segments - 1) + segment - 1, s);
-            else loadMemory(now.rule.state, head, s);
-        };
+        const int s0 = segment * kSegment, count = min(kSegment, time - s0);
         __syncthreads();
         stage();
-        const StepGates gate = nextGate;
+        const StepGates gates[2] = {nextGates[0], nextGates[1]};
+        const Pack<T, 4> values[2] = {nextV[0], nextV[1]};
         F4 start[KeyTiles];
-        checkpoint(start);
+        {
+            const Args now = Argument<Args>();
+            if (segment > 0) loadMemory(now.rule.checkpoints, (long long)head * (segments - 1) + segment - 1, start);
+            else loadMemory(now.rule.state, head, start);
+        }
         if (segment > 0) fetch(s0 - kSegment);
+        const unsigned cuts = (unsigned)(__ballot(gates[0].Reset()) & 0xffff) | (unsigned)(__ballot(gates[1].Reset()) & 0xffff) << 16;
         __syncthreads();
-        // ---- The chunks' matrices, one wavefront a chunk.
-        if (wave < chunks) {
-            const int c = wave, count = min(kChunk, time - s0 - c * kChunk);
-            const unsigned cuts = (unsigned)(__ballot(gate.Reset()) & 0xffff);
-            if (g == 0) betas[c * kChunk + m] = gate.beta;
-            if (lane == 0) cutsOf[c] = cuts;
-            for (int low = 0, high; low < count; low = high) {
-                const unsigned later = cuts >> (low + 1);
-                high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;
-                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
-                const double G = RowUpTo(mine && !(starts && m == low) ? gate.decay * kLog2E : 0.0);
-                const float beta = mine ? gate.beta : 0.f;
-                if (mine && g == 0) reach[c * kChunk + m] = G;
+
+        // Parts between resets, last first; the steps of other parts are masked.
+        for (int high = count, low; high > 0; high = low) {
+            const unsigned below = cuts & (high < 32 ? (1u << high) - 1 : ~0u);
+            low = below ? 31 - __builtin_clz(below) : 0;
+            const bool starts = (cuts >> low) & 1;
+            const auto mine = [&](int tile) { return kChunk * tile + m >= low && kChunk * tile + m < high; };
+            const auto in = [&](int tile, int r) { return kChunk * tile + 4 * g + r >= low && kChunk * tile + 4 * g + r < high; };
+            const auto keyPair = [&](const T *rows, int tile, int p, B8(&x)[P]) {
+                const T *from = rows + (kChunk * tile + m) * ks + 32 * p + 4 * g;
+                Pair<T>(Masked(*reinterpret_cast<const Pack<T, 4> *>(from), mine(tile)),
+                        Masked(*reinterpret_cast<const Pack<T, 4> *>(from + 16), mine(tile)), x);
+            };
+            const auto valueTile = [&](const T *rows, int tile, int x) {
+                return Masked(*reinterpret_cast<const Pack<T, 4> *>(rows + (kChunk * tile + m) * vs + 16 * x + 4 * g), mine(tile));
+            };
+
+            // ---- The triangular matrices.
+            double G[2];
+            {
+                const auto kept = [&](int tile) {
+                    return mine(tile) && !(starts && kChunk * tile + m == low) ? gates[tile].decay * kLog2E : 0.0;
+                };
+                G[0] = RowUpTo(kept(0));
+                G[1] = RowUpTo(kept(1)) + __shfl(G[0], 15);
+            }
+            const double last = __shfl(high > kChunk ? G[1] : G[0], (high - 1) & 15);
+            if (wave == 0 && g == 0)
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    const int at = kChunk * tile + m;
+                    reach[at] = mine(tile) ? G[tile] : 0.0;
+                    betas[at] = mine(tile) ? gates[tile].beta : 0.f;
+                    wholes[at] = mine(tile) ? Exp2(G[tile]) : 0.f;
+                    afters[at] = mine(tile) ? Exp2(last - G[tile]) : 0.f;
+                }
+#pragma unroll 1
+            for (int block = wave; block < 3; block += Waves) {
+                const int row = block == kFirst ? 0 : 1, col = block == kSecond ? 1 : 0;
                 F4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
                 for (int p = 0; p < KeyTiles / 2; p++) {
-                    B8 kp[P], qp[P];
-                    Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
-                    Pair<T>(keyTile(queries, c, 2 * p, mine), keyTile(queries, c, 2 * p + 1, mine), qp);
-                    kk = Mfma32<P, P>(kp, kp, kk);
-                    qk = Mfma32<P, P>(kp, qp, qk);
+                    B8 kj[P], ki[P], qi[P];
+                    keyPair(keys, col, p, kj), keyPair(keys, row, p, ki), keyPair(queries, row, p, qi);
+                    kk = Mfma32<P, P>(kj, ki, kk);
+                    qk = Mfma32<P, P>(kj, qi, qk);
                 }
+                const double Gi = row ? G[1] : G[0], Gc = col ? G[1] : G[0];
+                const float beta = mine(row) ? (row ? gates[1].beta : gates[0].beta) : 0.f;
                 F4 aA, dA, aP, aKK;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int j = 4 * g + r;
-                    const double Gj = __shfl(G, j);
+                    const double Gj = __shfl(Gc, j);
                     const float betaj = __shfl(beta, j);
-                    const float d = Exp2(j <= m ? G - Gj : Gj - G);
-                    aP[r] = j <= m ? rule.scale * d * qk[r] : 0.f;
-                    aKK[r] = j < m ? d * kk[r] : 0.f;
+                    const bool later = block == kAcross || j <= m, before = block == kAcross || j < m;
+                    // Either way round, the later step minus the earlier one.
+                    const float d = mine(row) && in(col, r) ? Exp2(later ? Gi - Gj : Gj - Gi) : 0.f;
+                    aP[r] = later ? rule.scale * d * qk[r] : 0.f;
+                    aKK[r] = before ? d * kk[r] : 0.f;
                     aA[r] = beta * aKK[r];
                     dA[r] = m < j ? betaj * d * kk[r] : 0.f;
                 }
-                const F4 aT = UnitLowerInverse<false>(aA, dA, m, g).rows;
-                if (mine) {
-                    const int to = c * kMatrix + m * kMatrixRow + 4 * g;
-                    *reinterpret_cast<F4 *>(shared + At::kInverse + to) = aT;
-                    *reinterpret_cast<F4 *>(shared + At::kMixed + to) = aP;
-                    *reinterpret_cast<F4 *>(shared + At::kProducts + to) = aKK;
-                }
+                const int to = m * kChunk + 4 * g;
+                *reinterpret_cast<F4 *>(shared + At::kMixed + block * kMatrix + to) = aP;
+                *reinterpret_cast<F4 *>(shared + At::kProducts + block * kMatrix + to) = aKK;
+                if (block != kAcross)
+                    *reinterpret_cast<F4 *>(shared + At::kInverse + block * kMatrix + to) = UnitLowerInverse<false>(aA, dA, m, g).rows;
             }
-        }
-        __syncthreads();
+            __syncthreads();
 
-        // The values that chunk c writes and their errors, from the memory `s` before it; with `advance`
-        // the memory goes on to the next chunk.
-        const auto play = [&](int c, bool advance, F4(&s)[KeyTiles], F4 &wrote, F4 &errors) {
-            const int count = min(kChunk, time - s0 - c * kChunk);
-            const unsigned cuts = cutsOf[c];
-            wrote = errors = F4{0, 0, 0, 0};
-            for (int low = 0, high; low < count; low = high) {
-                const unsigned later = cuts >> (low + 1);
-                high = later ? min(count, low + 1 + __builtin_ctz(later)) : count;
-                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
-                Four v[P];
-                Split<T>(valueTile(values, c, wave, mine), v);
-                F4 seen = {0, 0, 0, 0}, error = Turn<P>(v, eye), written;
+            // ---- By columns. First U, what the steps wrote, and its errors, from the memory before.
+            F4 U[2], error[2], dO[2], dB[2], wrong[2];
+            {
+                F4 seen[2];
+                seen[0] = seen[1] = F4{0, 0, 0, 0};
                 if (!starts) {
 #pragma unroll
                     for (int p = 0; p < KeyTiles / 2; p++) {
-                        B8 kp[P], sp[kFloatPieces];
-                        Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
-                        Pair(s[2 * p], s[2 * p + 1], sp);
-                        seen = Mfma32<P, kFloatPieces>(kp, sp, seen);
+                        B8 sp[kFloatPieces];
+                        Pair(start[2 * p], start[2 * p + 1], sp);
+#pragma unroll
+                        for (int tile = 0; tile < 2; tile++) {
+                            B8 kp[P];
+                            keyPair(keys, tile, p, kp);
+                            seen[tile] = Mfma32<P, kFloatPieces>(kp, sp, seen[tile]);
+                        }
                     }
                 }
-                F4 aT = RowOrder(shared + At::kInverse + c * kMatrix, m, g);
-                bool in[4];
-                double Gj[4];
+                B8 v[P], o[P];
+                Pair<T>(Masked(values[0], mine(0)), Masked(values[1], mine(1)), v);
+                Pair<T>(valueTile(outputs, 0, wave), valueTile(outputs, 1, wave), o);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    in[r] = 4 * g + r >= low && 4 * g + r < high;
-                    Gj[r] = in[r] ? reach[c * kChunk + 4 * g + r] : 0.0;
-                    error[r] = fmaf(-Exp2(Gj[r]), seen[r], error[r]);
-                    written[r] = in[r] ? betas[c * kChunk + 4 * g + r] * error[r] : 0.f;
-                    aT[r] = mine && in[r] ? aT[r] : 0.f;
-                }
-                written = Product(aT, written);
-                const double last = reach[c * kChunk + high - 1];
+                for (int tile = 0; tile < 2; tile++) {
+                    const F4 value = Turn<P>(v, eyes.half[tile]);
+                    dO[tile] = Turn<P>(o, eyes.half[tile]);
+                    const F4 whole = *reinterpret_cast<const F4 *>(wholes + kChunk * tile + 4 * g);
+                    const F4 beta = *reinterpret_cast<const F4 *>(betas + kChunk * tile + 4 * g);
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    wrote[r] = in[r] ? written[r] : wrote[r];
-                    errors[r] = in[r] ? error[r] : errors[r];
-                    written[r] *= in[r] ? Exp2(last - Gj[r]) : 0.f;
+                    for (int r = 0; r < 4; r++) error[tile][r] = fmaf(-whole[r], seen[tile][r], value[r]);
+                    U[tile] = beta * error[tile];
                 }
-                if (!advance) continue;
-                Four wp[kFloatPieces];
-                Split(written, wp);
-                const float kept = Exp2(last);
-#pragma unroll
-                for (int t = 0; t < KeyTiles; t++) {
-                    Forget();
-                    Four x[P], turned[P];
-                    Split<T>(keyTile(keys, c, t, mine), x);
-                    Turn<P>(x, eye, turned);
-                    F4 held = s[t] * kept;
-                    if (starts) held = F4{0, 0, 0, 0};
-                    s[t] = Mfma16(turned, wp, held);
-                }
+                U[0] = Product(RowOrder(shared + At::kInverse + kFirst * kMatrix, m, g), U[0]);
+                F4 aA = RowOrder(shared + At::kProducts + kAcross * kMatrix, m, g);
+                aA *= -betas[kChunk + m];
+                U[1] = Product(RowOrder(shared + At::kInverse + kSecond * kMatrix, m, g), Product(aA, U[0], U[1]));
             }
-        };
-        F4 wroteFirst, errorsFirst;
-        F4 wroteC, errorC;
-#pragma unroll 1
-        for (int c = 0; c < chunks; c++) {
-            if (c) wroteFirst = wroteC, errorsFirst = errorC;
-            play(c, c + 1 < chunks, start, wroteC, errorC);
-        }
-        __syncthreads();
-
-        for (int c = chunks - 1; c >= 0; c--) {
-            const int t0 = s0 + c * kChunk;
-            const unsigned cuts = cutsOf[c];
-            if (c + 1 < chunks) checkpoint(start), wroteC = wroteFirst, errorC = errorsFirst;
-            for (int high = min(kChunk, time - t0), low; high > 0; high = low) {
-                const unsigned below = cuts & ((1u << high) - 1);
-                low = below ? 31 - __builtin_clz(below) : 0;
-                const bool starts = (cuts >> low) & 1, mine = m >= low && m < high;
-                float *dots = shared + At::kDots + turn * kWaves * 4 * kChunk;
-                turn ^= 1;
-                const double G = mine ? reach[c * kChunk + m] : 0.0, last = reach[c * kChunk + high - 1];
-                const float beta = mine ? betas[c * kChunk + m] : 0.f;
-                bool in[4];
-                double Gj[4];
-                float betaj[4], afterJ[4], wholeJ[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    in[r] = 4 * g + r >= low && 4 * g + r < high;
-                    Gj[r] = in[r] ? reach[c * kChunk + 4 * g + r] : 0.0;
-                    betaj[r] = in[r] ? betas[c * kChunk + 4 * g + r] : 0.f;
-                    afterJ[r] = in[r] ? Exp2(last - Gj[r]) : 0.f;
-                    wholeJ[r] = in[r] ? Exp2(Gj[r]) : 0.f;
-                }
-
-                // The gradients of the values written, and of the right side they solve.
-                Four op[P];
-                Split<T>(valueTile(outputs, c, wave, mine), op);
-                const F4 dO = Turn<P>(op, eye);
-                F4 dU = {0, 0, 0, 0};
+            // Then dU and dB, from the gradient of the memory after.
+            {
+                F4 dU[2];
+                dU[0] = dU[1] = F4{0, 0, 0, 0};
 #pragma unroll
                 for (int p = 0; p < KeyTiles / 2; p++) {
-                    B8 kp[P], sp[kFloatPieces];
-                    Pair<T>(keyTile(keys, c, 2 * p, mine), keyTile(keys, c, 2 * p + 1, mine), kp);
+                    B8 sp[kFloatPieces];
                     Pair(dS[2 * p], dS[2 * p + 1], sp);
-                    dU = Mfma32<P, kFloatPieces>(kp, sp, dU);
-                }
-                Forget();
-                F4 dT = ColumnOrder(shared + At::kInverse + c * kMatrix, m, g);
-                F4 dP = ColumnOrder(shared + At::kMixed + c * kMatrix, m, g), written;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    dU[r] *= afterJ[r];
-                    dT[r] = in[r] && mine ? dT[r] : 0.f;
-                    dP[r] = in[r] && mine ? dP[r] : 0.f;
-                    written[r] = in[r] ? wroteC[r] : 0.f;
-                }
-                dU = Product(dP, dO, dU);
-                const F4 dB = Product(dT, dU), aB = Product(dU, dT), aU = Product(written, one);
-                Forget();
-                {
-                    Four up[kFloatPieces], bp[kFloatPieces];
-                    Split(aU, up), Split(aB, bp);
-#pragma unroll
-                    for (int p = 0; p < kFloatPieces; p++) {
-                        *reinterpret_cast<Four *>(sharedU + (p * kChunk + m) * rs + column4) = up[p];
-                        *reinterpret_cast<Four *>(sharedB + (p * kChunk + m) * rs + column4) = bp[p];
+                    for (int tile = 0; tile < 2; tile++) {
+                        B8 kp[P];
+                        keyPair(keys, tile, p, kp);
+                        dU[tile] = Mfma32<P, kFloatPieces>(kp, sp, dU[tile]);
                     }
                 }
-                F4 wrong;
-#pragma unroll
-                for (int r = 0; r < 4; r++) wrong[r] = RowSum(in[r] ? dB[r] * errorC[r] : 0.f);
-                if (m == 0) *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kChunk + 4 * g) = wrong;
-                float held = 0;
+                dU[0] *= *reinterpret_cast<const F4 *>(afters + 4 * g);
+                dU[1] *= *reinterpret_cast<const F4 *>(afters + kChunk + 4 * g);
+                const auto mixed = [&](int block) { return ColumnOrder(shared + At::kMixed + block * kMatrix, m, g); };
+                dU[1] = Product(mixed(kSecond), dO[1], dU[1]);
+                dB[1] = Product(ColumnOrder(shared + At::kInverse + kSecond * kMatrix, m, g), dU[1]);
+                dU[0] = Product(mixed(kFirst), dO[0], dU[0]);
+                dU[0] = Product(mixed(kAcross), dO[1], dU[0]);
+                const F4 dA = ColumnOrder(shared + At::kProducts + kAcross * kMatrix, m, g);
+                dU[0] = Product(dA * -*reinterpret_cast<const F4 *>(betas + kChunk + 4 * g), dB[1], dU[0]);
+                dB[0] = Product(ColumnOrder(shared + At::kInverse + kFirst * kMatrix, m, g), dU[0]);
+            }
+            float held = 0;
+            if (!starts) {
 #pragma unroll
                 for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        memory[(16 * t + 4 * g + r) * ms + column] = dS[t][r];
-                        if (starts) continue;
-                        if (At::kBoth) second[(16 * t + 4 * g + r) * ms + column] = start[t][r];
-                        held = fmaf(dS[t][r], start[t][r], held);
-                    }
-                held = WaveSum(held);
-                if (lane == 0) dots[(wave * 4 + 3) * kChunk] = held;
-                if (mine) {
-                    Pack<T, 4> x;
+                    for (int r = 0; r < 4; r++) held = fmaf(dS[t][r], start[t][r], held);
+            }
+            held = WaveSum(held);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) x.x[r] = As<T>(beta * aB[r]);
-                    Store<4, Whole>(static_cast<T *>(Argument<Args>().rule.d_value) +
-                                        (((long long)b * time + t0 + m) * rule.heads + h) * dv + column4,
-                                    x, dv - column4);
+            for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) wrong[tile][r] = RowSum(dB[tile][r] * error[tile][r]);
+            if (m == 0) {
+                *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kSegment + 4 * g) = wrong[0];
+                *reinterpret_cast<F4 *>(dots + (wave * 4 + 0) * kSegment + kChunk + 4 * g) = wrong[1];
+            }
+            if (lane == 0) dots[(wave * 4 + 3) * kSegment] = held;
+            // In row order for the products over columns.
+            {
+                Four lo[kFloatPieces], hi[kFloatPieces];
+                B8 x[kFloatPieces];
+                const auto put = [&](uint16_t *rows) {
+                    Eights<kFloatPieces>(lo, hi, x);
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        Four turned[kFloatPieces];
+                        Turn<kFloatPieces>(x, eyes.half[tile], turned);
+#pragma unroll
+                        for (int i = 0; i < kFloatPieces; i++)
+                            *reinterpret_cast<Four *>(rows + (i * kSegment + kChunk * tile + m) * rs + column4) = turned[i];
+                    }
+                };
+                Split(U[0], lo), Split(U[1], hi);
+                put(sharedU);
+                Split(dB[0], lo), Split(dB[1], hi);
+                put(sharedB);
+                T *to = static_cast<T *>(Argument<Args>().rule.d_value) + (((long long)b * time + s0) * rule.heads + h) * dv + base;
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    const F4 rows = Turn<kFloatPieces>(x, eyes.half[tile]);
+                    Pack<T, 4> v;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) v.x[r] = As<T>(betas[kChunk * tile + m] * rows[r]);
+                    const uint32_t at = ((kChunk * tile + m) * rule.heads * dv + column4) * sizeof(T);
+                    Store<4, Whole>(Lane(to, at), v, mine(tile) ? dv - base - column4 : 0);
                 }
-                __syncthreads();
-
-                // The matrices' gradients.
-                const auto rowPieces = [&](const uint16_t *rows, int x, B8(&to)[kFloatPieces]) {
+            }
 #pragma unroll
-                    for (int p = 0; p < kFloatPieces; p++) {
-                        const uint16_t *from = rows + (p * kChunk + m) * rs + 32 * x + 4 * g;
-                        to[p] = Eight(*reinterpret_cast<const Four *>(from), *reinterpret_cast<const Four *>(from + 16));
-                    }
-                };
-                const auto memoryPieces = [&](const float *from, int t, int x, B8(&to)[kFloatPieces]) {
-                    from += (16 * t + m) * ms + 32 * x + 4 * g;
-                    Pair(*reinterpret_cast<const F4 *>(from), *reinterpret_cast<const F4 *>(from + 16), to);
-                };
-                const auto outputPieces = [&](int x, B8(&to)[P]) {
-                    Pair<T>(valueTile(outputs, c, 2 * x, mine), valueTile(outputs, c, 2 * x + 1, mine), to);
-                };
+            for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + 16 * wave + m] = dS[t][r];
+            __syncthreads();
+
+            const auto rowPieces = [&](const uint16_t *rows, int tile, int x, B8(&to)[kFloatPieces]) {
+#pragma unroll
+                for (int i = 0; i < kFloatPieces; i++) {
+                    const uint16_t *from = rows + (i * kSegment + kChunk * tile + m) * rs + 32 * x + 4 * g;
+                    to[i] = Eight(*reinterpret_cast<const Four *>(from), *reinterpret_cast<const Four *>(from + 16));
+                }
+            };
+            const auto outputPieces = [&](int tile, int x, B8(&to)[P]) {
+                Pair<T>(valueTile(outputs, tile, 2 * x), valueTile(outputs, tile, 2 * x + 1), to);
+            };
+            const auto memoryPieces = [&](int t, int x, B8(&to)[kFloatPieces]) {
+                const float *from = memory + (16 * t + m) * ms + 32 * x + 4 * g;
+                Pair(*reinterpret_cast<const F4 *>(from), *reinterpret_cast<const F4 *>(from + 16), to);
+            };
+            const auto putPieces = [&](uint16_t *pieces, int block, F4 x) {
+                Four p[kFloatPieces];
+                Split(x, p);
+#pragma unroll
+                for (int i = 0; i < kFloatPieces; i++)
+                    *reinterpret_cast<Four *>(pieces + (block * kFloatPieces + i) * kMatrix + m * kChunk + 4 * g) = p[i];
+            };
+            const auto getPieces = [&](const uint16_t *pieces, int block, Four(&p)[kFloatPieces]) {
+#pragma unroll
+                for (int i = 0; i < kFloatPieces; i++)
+                    p[i] = *reinterpret_cast<const Four *>(pieces + (block * kFloatPieces + i) * kMatrix + m * kChunk + 4 * g);
+            };
+            // ---- The matrices' gradients.
+#pragma unroll 1
+            for (int block = wave; block < 3; block += Waves) {
+                const int row = block == kFirst ? 0 : 1, col = block == kSecond ? 1 : 0;
                 F4 gP = {0, 0, 0, 0}, gA = {0, 0, 0, 0};
 #pragma unroll
-                for (int x = 0; x < Pairs; x++) {
-                    B8 uw[kFloatPieces], other[kFloatPieces], out[P];
-                    rowPieces(sharedU, x, uw);
-                    outputPieces(x, out);
+                for (int x = 0; x < kPairs; x++) {
+                    B8 uw[kFloatPieces], bw[kFloatPieces], out[P];
+                    rowPieces(sharedU, col, x, uw), rowPieces(sharedB, row, x, bw), outputPieces(row, x, out);
                     gP = Mfma32<kFloatPieces, P>(uw, out, gP);
-                    rowPieces(sharedB, x, other);
-                    gA = Mfma32<kFloatPieces, kFloatPieces>(uw, other, gA);
+                    gA = Mfma32<kFloatPieces, kFloatPieces>(uw, bw, gA);
                 }
-                Forget();
-                const F4 aP = RowOrder(shared + At::kMixed + c * kMatrix, m, g);
-                const F4 aKK = RowOrder(shared + At::kProducts + c * kMatrix, m, g);
-                F4 aM, aN, E;
+                const F4 aP = RowOrder(shared + At::kMixed + block * kMatrix, m, g);
+                const F4 aKK = RowOrder(shared + At::kProducts + block * kMatrix, m, g);
+                const float beta = betas[kChunk * row + m];
+                const double Gi = row ? G[1] : G[0];
+                F4 M, N, E;
                 float betaSum = 0;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int j = 4 * g + r;
-                    const bool both = mine && in[r];
-                    const float d = both && j <= m ? Exp2(G - Gj[r]) : 0.f;
-                    aM[r] = rule.scale * d * gP[r];
-                    aN[r] = j < m ? -beta * d * gA[r] : 0.f;
-                    const float part = both && j < m ? -gA[r] * aKK[r] : 0.f;
+                    const bool both = mine(row) && in(col, r), later = block == kAcross || j <= m;
+                    const float d = both && later ? Exp2(Gi - reach[kChunk * col + j]) : 0.f;
+                    M[r] = rule.scale * d * gP[r];
+                    N[r] = block == kAcross || j < m ? -beta * d * gA[r] : 0.f;
+                    const float part = both ? -gA[r] * aKK[r] : 0.f;
                     betaSum += part;
-                    E[r] = (both && j <= m ? gP[r] * aP[r] : 0.f) + beta * part;
+                    E[r] = (both ? gP[r] * aP[r] : 0.f) + beta * part;
                 }
-                Four mp[kFloatPieces], mt[kFloatPieces], np[kFloatPieces];
-                Split(aM, mp), Split(Product(aM, one), mt), Split(aN + Product(aN, one), np);
-
-                Forget();
-                // This wavefront's tiles of keys: dS U, S0 dO and S0 dB.
-                const auto written1 = [&](int t) {
-                    F4 sum = {0, 0, 0, 0};
-#pragma unroll
-                    for (int x = 0; x < Pairs; x++) {
-                        B8 uw[kFloatPieces], sp[kFloatPieces];
-                        rowPieces(sharedU, x, uw);
-                        memoryPieces(memory, t, x, sp);
-                        sum = Mfma32<kFloatPieces, kFloatPieces>(uw, sp, sum);
-                    }
-                    return sum;
-                };
-                if (!At::kBoth) {
-                    for (int t = wave; t < KeyTiles; t += kWaves)
-                        *reinterpret_cast<F4 *>(shared + At::kTiles + (t * 64 + lane) * 4) = written1(t);
-                    __syncthreads();
-                    if (!starts) {
-#pragma unroll
-                        for (int t = 0; t < KeyTiles; t++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) second[(16 * t + 4 * g + r) * ms + column] = start[t][r];
-                    }
-                    __syncthreads();
+                putPieces(sharedM, block, M);
+                if (block != kAcross) {
+                    Four lo[kFloatPieces];
+                    B8 x[kFloatPieces];
+                    Split(N, lo);
+                    Eights<kFloatPieces>(lo, lo, x);
+                    N += Turn<kFloatPieces>(x, eyes.half[0]);
                 }
-                F4 f = {0, 0, 0, 0}, e = {0, 0, 0, 0};
-#pragma unroll 1
-                for (int t = wave; t < KeyTiles; t += kWaves) {
-                    F4 dQ = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                    const F4 dKeys = At::kBoth ? written1(t) : *reinterpret_cast<const F4 *>(shared + At::kTiles + (t * 64 + lane) * 4);
-                    Forget();
-                    if (!starts)
+                putPieces(sharedN, block, N);
+                betaSum += __shfl_xor(betaSum, 16);
+                betaSum += __shfl_xor(betaSum, 32);
+                if (g == 0) sums[block * kChunk + m] = betaSum;
+                // What of E crosses each step: from before it to it or after, within the block; and the block
+                // across by rows and by columns.
+                float across = 0;
 #pragma unroll
-                        for (int x = 0; x < Pairs; x++) {
-                            B8 sp[kFloatPieces], other[kFloatPieces], out[P];
-                            memoryPieces(second, t, x, sp);
-                            outputPieces(x, out);
-                            dQ = Mfma32<P, kFloatPieces>(out, sp, dQ);
-                            rowPieces(sharedB, x, other);
-                            y = Mfma32<kFloatPieces, kFloatPieces>(other, sp, y);
+                for (int r = 0; r < 4; r++) {
+                    const float from = block == kAcross ? E[r] : RowFrom(E[r]);
+                    across += block == kAcross || 4 * g + r < m ? from : 0.f;
+                }
+                across += __shfl_xor(across, 16);
+                across += __shfl_xor(across, 32);
+                if (g == 0) sums[(3 + block) * kChunk + m] = across;
+                if (block == kAcross) {
+                    F4 columns;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) columns[r] = RowSum(E[r]);
+                    if (m == 0) *reinterpret_cast<F4 *>(sums + 6 * kChunk + 4 * g) = columns;
+                }
+            }
+            // ---- dS U by tiles of keys, kept in registers until the memory is in dS's place.
+            constexpr int kMine = (KeyTiles + Waves - 1) / Waves;
+            F4 fromLater[kMine][2];
+#pragma unroll
+            for (int i = 0; i < kMine; i++) {
+                const int t = wave + i * Waves;
+                fromLater[i][0] = fromLater[i][1] = F4{0, 0, 0, 0};
+                if (t < KeyTiles) {
+#pragma unroll
+                    for (int x = 0; x < kPairs; x++) {
+                        B8 sp[kFloatPieces];
+                        memoryPieces(t, x, sp);
+#pragma unroll
+                        for (int tile = 0; tile < 2; tile++) {
+                            B8 uw[kFloatPieces];
+                            rowPieces(sharedU, tile, x, uw);
+                            fromLater[i][tile] = Mfma32<kFloatPieces, kFloatPieces>(uw, sp, fromLater[i][tile]);
                         }
-                    Forget();
-                    Four kx[P], qx[P], kTurned[P], qTurned[P];
-                    Split<T>(keyTile(keys, c, t, mine), kx), Split<T>(keyTile(queries, c, t, mine), qx);
-                    Turn<P>(kx, eye, kTurned), Turn<P>(qx, eye, qTurned);
-                    const F4 kf = Turn<P>(kx, eye), qf = Turn<P>(qx, eye);
-                    F4 dK;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        dK[r] = afterJ[r] * dKeys[r];
-                        f[r] = fmaf(dK[r], kf[r], f[r]);
-                        const float fromKey = -betaj[r] * wholeJ[r] * y[r];
-                        dQ[r] *= rule.scale * wholeJ[r];
-                        e[r] = fmaf(qf[r], dQ[r], fmaf(kf[r], fromKey, e[r]));
-                        dK[r] += fromKey;
-                    }
-                    dQ = Mfma16(mp, kTurned, dQ);
-                    dK = Mfma16(mt, qTurned, dK);
-                    dK = Mfma16(np, kTurned, dK);
-                    const Args now = Argument<Args>();
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        if (!in[r] || 16 * t + m >= dk) continue;
-                        const long long row = (long long)b * time + t0 + 4 * g + r;
-                        if (now.shared) {
-                            const long long to = (row * rule.heads + h) * dk + 16 * t + m;
-                            static_cast<float *>(now.dQuery)[to] = dQ[r];
-                            static_cast<float *>(now.dKey)[to] = dK[r];
-                        } else {
-                            const long long to = (row * rule.key_heads + kh) * dk + 16 * t + m;
-                            static_cast<T *>(now.dQuery)[to] = As<T>(dQ[r]);
-                            static_cast<T *>(now.dKey)[to] = As<T>(dK[r]);
-                        }
-                    }
-                }
-                Forget();
-                F4 eSum, fSum;
-#pragma unroll
-                for (int r = 0; r < 4; r++) eSum[r] = RowSum(e[r]), fSum[r] = RowSum(f[r]);
-                if (m == 0) {
-                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 1) * kChunk + 4 * g) = eSum;
-                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 2) * kChunk + 4 * g) = fSum;
-                }
-
-                // The gradient of the memory before this part.
-                const float kept = Exp2(last);
-                if (starts) {
-#pragma unroll
-                    for (int t = 0; t < KeyTiles; t++) dS[t] = F4{0, 0, 0, 0};
-                } else {
-                    Four dOp[kFloatPieces], dBp[kFloatPieces];
-                    F4 x, y;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] = rule.scale * wholeJ[r] * dO[r], y[r] = -betaj[r] * wholeJ[r] * dB[r];
-                    Split(x, dOp), Split(y, dBp);
-#pragma unroll
-                    for (int t = 0; t < KeyTiles; t++) {
-                        Forget();
-                        Four x[P], turned[P];
-                        Split<T>(keyTile(queries, c, t, mine), x);
-                        Turn<P>(x, eye, turned);
-                        dS[t] = Mfma16(turned, dOp, dS[t] * kept);
-                        Split<T>(keyTile(keys, c, t, mine), x);
-                        Turn<P>(x, eye, turned);
-                        dS[t] = Mfma16(turned, dBp, dS[t]);
-                    }
-                }
-                __syncthreads();
-
-                // The gates' gradients, a lane for each step.
-                if (wave == 0) {
-                    float eAll = 0, fAll = 0, bAll = 0, heldAll = 0;
-#pragma unroll
-                    for (int w = 0; w < kWaves; w++) {
-                        bAll += dots[(w * 4 + 0) * kChunk + m];
-                        eAll += dots[(w * 4 + 1) * kChunk + m];
-                        fAll += dots[(w * 4 + 2) * kChunk + m];
-                        heldAll += dots[(w * 4 + 3) * kChunk];
-                    }
-                    float across = 0;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float x = RowFrom(E[r]);
-                        across += 4 * g + r < m ? x : 0.f;
-                    }
-                    across += __shfl_xor(across, 16);
-                    across += __shfl_xor(across, 32);
-                    betaSum += __shfl_xor(betaSum, 16);
-                    betaSum += __shfl_xor(betaSum, 32);
-                    const float through = starts ? 0.f : kept * heldAll;
-                    const float decay = RowFrom(eAll) + across + Dpp<kRowShiftRight + 1>(RowUpTo(fAll)) + through;
-                    if (mine && g == 0) {
-                        const long long to = ((long long)b * time + t0 + m) * rule.heads + h;
-                        const Args now = Argument<Args>();
-                        static_cast<float *>(now.rule.d_decay)[to] = starts && m == low ? 0.f : decay;
-                        static_cast<float *>(now.rule.d_beta)[to] = bAll + betaSum;
                     }
                 }
             }
+            __syncthreads();
+            if (!starts) {
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) memory[(16 * t + 4 * g + r) * ms + 16 * wave + m] = start[t][r];
+            }
+
+            // ---- The gradient of the memory before this part, by columns.
+            const float kept = wholes[high - 1];
+            if (starts) {
+#pragma unroll
+                for (int t = 0; t < KeyTiles; t++) dS[t] = F4{0, 0, 0, 0};
+            } else {
+                B8 op[kFloatPieces], bp[kFloatPieces];
+                {
+                    F4 x[2], y[2];
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        const F4 whole = *reinterpret_cast<const F4 *>(wholes + kChunk * tile + 4 * g);
+                        const F4 beta = *reinterpret_cast<const F4 *>(betas + kChunk * tile + 4 * g);
+                        x[tile] = rule.scale * whole * dO[tile];
+                        y[tile] = -beta * whole * dB[tile];
+                    }
+                    Pair(x[0], x[1], op), Pair(y[0], y[1], bp);
+                }
+#pragma unroll
+                for (int p = 0; p < KeyTiles / 2; p++) {
+                    B8 x0[P], x1[P], y0[P], y1[P];
+                    keyPair(queries, 0, p, x0), keyPair(queries, 1, p, x1);
+                    keyPair(keys, 0, p, y0), keyPair(keys, 1, p, y1);
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        Four lo[P], hi[P];
+                        B8 turned[P];
+                        F4 s = dS[2 * p + half] * kept;
+                        Turn<P>(x0, eyes.half[half], lo), Turn<P>(x1, eyes.half[half], hi);
+                        Eights<P>(lo, hi, turned);
+                        s = Mfma32<P, kFloatPieces>(turned, op, s);
+                        Turn<P>(y0, eyes.half[half], lo), Turn<P>(y1, eyes.half[half], hi);
+                        Eights<P>(lo, hi, turned);
+                        dS[2 * p + half] = Mfma32<P, kFloatPieces>(turned, bp, s);
+                    }
+                }
+            }
+            __syncthreads();
+
+            // ---- The keys' and queries' gradients.
+            F4 e[2], f[2];
+            e[0] = e[1] = f[0] = f[1] = F4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kMine; i++) {
+                const int t = wave + i * Waves;
+                if (t >= KeyTiles) continue;
+                F4 dQ[2], dK[2], y[2];
+                dQ[0] = dQ[1] = y[0] = y[1] = F4{0, 0, 0, 0};
+                if (!starts) {
+#pragma unroll
+                    for (int x = 0; x < kPairs; x++) {
+                        B8 sp[kFloatPieces];
+                        memoryPieces(t, x, sp);
+#pragma unroll
+                        for (int tile = 0; tile < 2; tile++) {
+                            B8 bw[kFloatPieces], out[P];
+                            outputPieces(tile, x, out);
+                            dQ[tile] = Mfma32<P, kFloatPieces>(out, sp, dQ[tile]);
+                            rowPieces(sharedB, tile, x, bw);
+                            y[tile] = Mfma32<kFloatPieces, kFloatPieces>(bw, sp, y[tile]);
+                        }
+                    }
+                }
+                // This tile's keys and queries, both tiles of steps side by side, and in column order.
+                const auto tilePair = [&](const T *rows, B8(&x)[P]) {
+                    const T *from = rows + m * ks + 16 * t + 4 * g;
+                    Pair<T>(Masked(*reinterpret_cast<const Pack<T, 4> *>(from), mine(0)),
+                            Masked(*reinterpret_cast<const Pack<T, 4> *>(from + kChunk * ks), mine(1)), x);
+                };
+                B8 kx[P], qx[P], kAll[P], qAll[P];
+                Four k[2][P], q[2][P];
+                tilePair(keys, kx), tilePair(queries, qx);
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++) {
+                    const F4 whole = *reinterpret_cast<const F4 *>(wholes + kChunk * tile + 4 * g);
+                    const F4 beta = *reinterpret_cast<const F4 *>(betas + kChunk * tile + 4 * g);
+                    const F4 kf = Turn<P>(kx, eyes.half[tile]), qf = Turn<P>(qx, eyes.half[tile]);
+                    Turn<P>(kx, eyes.half[tile], k[tile]), Turn<P>(qx, eyes.half[tile], q[tile]);
+                    dK[tile] = fromLater[i][tile] * *reinterpret_cast<const F4 *>(afters + kChunk * tile + 4 * g);
+                    f[tile] += dK[tile] * kf;
+                    y[tile] *= -beta * whole;
+                    dQ[tile] *= rule.scale * whole;
+                    e[tile] += qf * dQ[tile] + kf * y[tile];
+                    dK[tile] += y[tile];
+                }
+                Eights<P>(k[0], k[1], kAll), Eights<P>(q[0], q[1], qAll);
+                // dq1 = M11 k1, dq2 = M21 k1 + M22 k2; dk1 = M11' q1 + M21' q2 + N11 k1 + N21' k2,
+                // dk2 = M22' q2 + N21 k1 + N22 k2, N11 and N22 with their transposes in them.
+                Four m11[kFloatPieces], m21[kFloatPieces], m22[kFloatPieces];
+                Four lo[kFloatPieces], hi[kFloatPieces];
+                B8 wide[kFloatPieces], turn[kFloatPieces];
+                getPieces(sharedM, kFirst, m11), getPieces(sharedM, kAcross, m21), getPieces(sharedM, kSecond, m22);
+                dQ[0] = Mfma16(m11, k[0], dQ[0]);
+                Eights<kFloatPieces>(m21, m22, wide);
+                dQ[1] = Mfma32<kFloatPieces, P>(wide, kAll, dQ[1]);
+                Eights<kFloatPieces>(m11, m21, turn);
+                Turn<kFloatPieces>(turn, eyes.half[0], lo), Turn<kFloatPieces>(turn, eyes.half[1], hi);
+                Eights<kFloatPieces>(lo, hi, wide);
+                dK[0] = Mfma32<kFloatPieces, P>(wide, qAll, dK[0]);
+                Eights<kFloatPieces>(m22, m22, turn);
+                Turn<kFloatPieces>(turn, eyes.half[0], lo);
+                dK[1] = Mfma16(lo, q[1], dK[1]);
+                getPieces(sharedN, kFirst, m11), getPieces(sharedN, kAcross, m21), getPieces(sharedN, kSecond, m22);
+                Eights<kFloatPieces>(m21, m22, wide);
+                dK[1] = Mfma32<kFloatPieces, P>(wide, kAll, dK[1]);
+                Eights<kFloatPieces>(m21, m21, turn);
+                Turn<kFloatPieces>(turn, eyes.half[0], hi);
+                Eights<kFloatPieces>(m11, hi, wide);
+                dK[0] = Mfma32<kFloatPieces, P>(wide, kAll, dK[0]);
+
+                const Args now = Argument<Args>();
+                const int each = now.parted ? rule.heads * now.slices * dk : rule.key_heads * dk;
+                const long long to = ((long long)b * time + s0) * each + (now.parted ? h * now.slices + slice : kh) * dk + 16 * t;
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if (!in(tile, r) || 16 * t + m >= dk) continue;
+                        const uint32_t at = 4 * g * each + m;
+                        const long long row = to + (kChunk * tile + r) * (long long)each;
+                        if (now.parted) {
+                            *Lane(static_cast<float *>(now.dQuery) + row, at * sizeof(float)) = dQ[tile][r];
+                            *Lane(static_cast<float *>(now.dKey) + row, at * sizeof(float)) = dK[tile][r];
+                        } else {
+                            *Lane(static_cast<T *>(now.dQuery) + row, at * sizeof(T)) = As<T>(dQ[tile][r]);
+                            *Lane(static_cast<T *>(now.dKey) + row, at * sizeof(T)) = As<T>(dK[tile][r]);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int tile = 0; tile < 2; tile++) {
+                F4 eSum, fSum;
+#pragma unroll
+                for (int r = 0; r < 4; r++) eSum[r] = RowSum(e[tile][r]), fSum[r] = RowSum(f[tile][r]);
+                if (m == 0) {
+                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 1) * kSegment + kChunk * tile + 4 * g) = eSum;
+                    *reinterpret_cast<F4 *>(dots + (wave * 4 + 2) * kSegment + kChunk * tile + 4 * g) = fSum;
+                }
+            }
+            __syncthreads();
+
+            // ---- The gates' gradients, a lane for each step.
+            if (wave == Waves - 1) {
+                float eAll[2] = {0, 0}, fAll[2] = {0, 0}, bAll[2] = {0, 0}, heldAll = 0;
+#pragma unroll
+                for (int w = 0; w < Waves; w++) {
+#pragma unroll
+                    for (int tile = 0; tile < 2; tile++) {
+                        bAll[tile] += dots[(w * 4 + 0) * kSegment + kChunk * tile + m];
+                        eAll[tile] += dots[(w * 4 + 1) * kSegment + kChunk * tile + m];
+                        fAll[tile] += dots[(w * 4 + 2) * kSegment + kChunk * tile + m];
+                    }
+                    heldAll += dots[(w * 4 + 3) * kSegment];
+                }
+                const float through = starts ? 0.f : kept * heldAll;
+                const auto before = [](float x) { return Dpp<kRowShiftRight + 1>(RowUpTo(x)); };
+                float decay[2];
+                decay[0] = RowFrom(eAll[0]) + RowSum(eAll[1]) + sums[3 * kChunk + m] + before(sums[6 * kChunk + m]) + before(fAll[0]);
+                decay[1] = RowFrom(eAll[1]) + RowFrom(sums[5 * kChunk + m]) + sums[4 * kChunk + m] + RowSum(fAll[0]) + before(fAll[1]);
+                bAll[0] += sums[m];
+                bAll[1] += sums[kChunk + m] + sums[2 * kChunk + m];
+                const Args now = Argument<Args>();
+#pragma unroll
+                for (int tile = 0; tile < 2; tile++)
+                    if (mine(tile) && g == 0) {
+                        const long long to = (((long long)b * time + s0 + kChunk * tile + m) * rule.heads + h) * now.slices + slice;
+                        Global(now.dDecay)[to] = starts && kChunk * tile + m == low ? 0.f : decay[tile] + through;
+                        Global(now.dBeta)[to] = bAll[tile];
+                    }
+            }
+            // What the next part puts down first (betas, matrices) is still read here only by this wavefront
+            // (sums, dots), which the next barrier waits for.
         }
     }
     if (rule.d_state) {
         const int rows = dk - 4 * g;
-        float *to = static_cast<float *>(rule.d_state) + ((long long)head * dk + 4 * g) * dv + column;
+        float *to = static_cast<float *>(rule.d_state) + (long long)head * dk * dv;
+        const uint32_t at = (4 * g * dv + column) * sizeof(float);
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                if (16 * t + r < rows && column < dv) to[(16 * t + r) * dv] = dS[t][r];
+                if (16 * t + r < rows && column < dv) *Lane(to + (16 * t + r) * dv, at) = dS[t][r];
     }
 }
 
-// The gradients of keys that several heads share: their sum, in the heads' order.
+// Gradients that several heads or slices share: [row][parts][size] summed over the parts, in their order.
 template <class T>
-__global__ __launch_bounds__(256) void SharedKeysKernel(const float *parts, T *out, int group, int size, long long count) {
+__global__ __launch_bounds__(256) void PartsKernel(const float *parts, T *out, int group, int size, long long count) {
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < count; i += gridDim.x * 256ll) {
         const long long row = i / size;
         const float *p = parts + row * group * size + (i - row * size);
@@ -581,49 +675,64 @@ __global__ __launch_bounds__(256) void SharedKeysKernel(const float *parts, T *o
         out[i] = As<T>(sum);
     }
 }
+template <class T>
+void LaunchParts(const float *parts, void *out, int group, int size, long long rows, hipStream_t stream) {
+    const long long count = rows * size;
+    if (count == 0) return;
+    const unsigned blocks = (unsigned)(count < 256ll * 8192 ? (count + 255) / 256 : 8192);
+    hipLaunchKernelGGL(PartsKernel<T>, dim3(blocks), dim3(256), 0, stream, parts, static_cast<T *>(out), group, size, count);
+}
+
+int SlicesOf(const Rule &r) { return (r.value_size + kSlice - 1) / kSlice; }
+// Floats of the parts of the keys' and queries' gradients, and of the gates'; 0 where there are none.
+long long KeyParts(const Rule &r) {
+    const bool parted = r.heads * SlicesOf(r) != r.key_heads;
+    return parted ? (long long)r.batch * r.time * r.heads * SlicesOf(r) * r.key_size : 0;
+}
+long long GateParts(const Rule &r) { return SlicesOf(r) > 1 ? (long long)r.batch * r.time * r.heads * SlicesOf(r) : 0; }
 
 template <class T, int KeyTiles>
 bool LaunchBackward(const Rule &r, hipStream_t stream) {
-    const bool shared = r.heads != r.key_heads;
-    const long long steps = (long long)r.batch * r.time, each = steps * r.heads * r.key_size;
-    float *parts = static_cast<float *>(r.workspace);
+    const int slices = SlicesOf(r);
+    const long long keyParts = KeyParts(r), gateParts = GateParts(r), steps = (long long)r.batch * r.time;
+    float *parts = static_cast<float *>(r.workspace), *gateSums = parts + 2 * keyParts;
     BackwardArgs<T> a{r,
                       ViewOf<const T>(r.query, r.query_strides, r.key_size),
                       ViewOf<const T>(r.key, r.key_strides, r.key_size),
                       ViewOf<const T>(r.value, r.value_strides, r.value_size),
                       ViewOf<const T>(r.d_output, r.d_output_strides, r.value_size),
                       GatesOf(r),
-                      shared ? parts : r.d_query,
-                      shared ? parts + each : r.d_key,
-                      shared};
+                      keyParts ? parts : r.d_query,
+                      keyParts ? parts + keyParts : r.d_key,
+                      gateParts ? gateSums : static_cast<float *>(r.d_decay),
+                      gateParts ? gateSums + gateParts : static_cast<float *>(r.d_beta),
+                      slices,
+                      keyParts != 0};
     const bool whole = a.query.whole && a.key.whole && a.value.whole && a.dOutput.whole && Aligned(4 * sizeof(T), r.d_value);
     const auto launch = [&](auto wide, auto packed) {
-        constexpr int Pairs = decltype(wide)::value;
-        const auto kernel = BackwardKernel<T, KeyTiles, Pairs, decltype(packed)::value>;
-        constexpr int bytes = BackwardShared<KeyTiles, Pairs, sizeof(T)>::kFloats * sizeof(float);
-        static_assert(bytes <= kMostShared, "the memory of a head fits a compute unit's LDS");
+        constexpr int Waves = decltype(wide)::value;
+        const auto kernel = BackwardKernel<T, KeyTiles, Waves, decltype(packed)::value>;
+        constexpr int bytes = BackwardShared<KeyTiles, Waves, sizeof(T)>::kFloats * sizeof(float);
+        static_assert(bytes <= 160 * 1024, "a head's steps fit a compute unit's LDS");
         if (hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
             hipSuccess)
             return false;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads)), dim3(128 * Pairs), bytes, stream, a);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads * slices)), dim3(64 * Waves), bytes, stream, a);
         return true;
     };
-    const int pairs = (r.value_size + 31) / 32;
     bool set;
     if (!whole) set = launch(std::integral_constant<int, 4>(), std::false_type());
-    else if (pairs == 1) set = launch(std::integral_constant<int, 1>(), std::true_type());
-    else if (pairs == 2) set = launch(std::integral_constant<int, 2>(), std::true_type());
-    else if (pairs == 3) set = launch(std::integral_constant<int, 3>(), std::true_type());
+    else if (r.value_size <= 32) set = launch(std::integral_constant<int, 2>(), std::true_type());
     else set = launch(std::integral_constant<int, 4>(), std::true_type());
     if (!set) return false;
-    if (shared && steps > 0) {
-        const long long count = steps * r.key_heads * r.key_size;
-        const unsigned blocks = (unsigned)(count < 256ll * 8192 ? (count + 255) / 256 : 8192);
-        const int group = r.heads / r.key_heads;
-        hipLaunchKernelGGL(SharedKeysKernel<T>, dim3(blocks), dim3(256), 0, stream, parts, static_cast<T *>(r.d_query), group,
-                           r.key_size, count);
-        hipLaunchKernelGGL(SharedKeysKernel<T>, dim3(blocks), dim3(256), 0, stream, parts + each,
-                           static_cast<T *>(r.d_key), group, r.key_size, count);
+    if (keyParts) {
+        const int group = r.heads / r.key_heads * slices;
+        LaunchParts<T>(parts, r.d_query, group, r.key_size, steps * r.key_heads, stream);
+        LaunchParts<T>(parts + keyParts, r.d_key, group, r.key_size, steps * r.key_heads, stream);
+    }
+    if (gateParts) {
+        LaunchParts<float>(gateSums, r.d_decay, slices, 1, steps * r.heads, stream);
+        LaunchParts<float>(gateSums + gateParts, r.d_beta, slices, 1, steps * r.heads, stream);
     }
     return true;
 }
@@ -633,6 +742,11 @@ bool LaunchBackward(const Rule &r, hipStream_t stream) {
 
 using namespace layers;
 
+extern "C" __attribute__((visibility("default"))) unsigned long long cuju_delta_rule_workspace(const struct cuju_delta_rule *rule) {
+    if (!Fits(rule)) return 0;
+    return 2 * (KeyParts(*rule) + GateParts(*rule)) * sizeof(float);
+}
+
 extern "C" __attribute__((visibility("default"))) int cuju_delta_rule_backward(const struct cuju_delta_rule *rule, void *stream) {
     if (!Fits(rule)) return -1;
     const Rule &r = *rule;
@@ -640,7 +754,7 @@ extern "C" __attribute__((visibility("default"))) int cuju_delta_rule_backward(c
     if (r.time > 0 && (!r.query || !r.key || !r.value || !r.decay || !r.beta || !r.d_output || !r.d_query || !r.d_key ||
                        !r.d_value || !r.d_decay || !r.d_beta))
         return Failed("expected inputs and their gradients");
-    if (r.time > 0 && r.heads != r.key_heads && !r.workspace) return Failed("expected a workspace for shared keys");
+    if (KeyParts(r) + GateParts(r) && !r.workspace) return Failed("expected a workspace");
     if (r.time > kSegment && !r.checkpoints) return Failed("expected the forward pass's checkpoints");
     bool set = true;
     ForType(r.type, [&](auto x) {

@@ -140,17 +140,20 @@ def _rule_forward(q, k, v, decay, beta, state, resets, scale, train):
 
 
 def _rule_backward(q, k, v, decay, beta, state, resets, scale, checkpoints, d_output, d_last):
-    batch, time, key_heads, key_size = q.shape
+    batch, _, _, key_size = q.shape
     heads = v.shape[2]
     dense = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v, decay, beta)]
     d_state = torch.empty((batch, heads, key_size, v.shape[3]), dtype=torch.float32, device=v.device)
-    workspace = None
-    if heads != key_heads:
-        workspace = torch.empty(2 * batch * time * heads * key_size, dtype=torch.float32, device=v.device)
     if batch:
-        _call('cuju_delta_rule_backward',
-              _rule(q, k, v, decay, beta, state, resets, scale, checkpoints=checkpoints if checkpoints.numel() else None,
-                    d_output=d_output, d_last=d_last, gradients=(*dense, d_state), workspace=workspace), v.device)
+        def packed(workspace):
+            return _rule(q, k, v, decay, beta, state, resets, scale,
+                         checkpoints=checkpoints if checkpoints.numel() else None, d_output=d_output, d_last=d_last,
+                         gradients=(*dense, d_state), workspace=workspace)
+
+        workspace, size = None, load().cuju_delta_rule_workspace(packed(None))
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=v.device)
+        _call('cuju_delta_rule_backward', packed(workspace), v.device)
     return (*dense, d_state)
 
 

@@ -109,6 +109,7 @@ SIGNATURES = [
     # The policy operators take their argument structs as packed bytes (layers.py).
     ('cuju_delta_rule_step', I, [ctypes.c_char_p, P]),
     ('cuju_delta_rule_forward', I, [ctypes.c_char_p, P]),
+    ('cuju_delta_rule_workspace', U64, [ctypes.c_char_p]),
     ('cuju_delta_rule_backward', I, [ctypes.c_char_p, P]),
     ('cuju_group_norm_workspace', U64, [ctypes.c_char_p]),
     ('cuju_group_norm_forward', I, [ctypes.c_char_p, P]),

@@ -201,11 +201,13 @@ struct cuju_delta_rule {
     void *d_query, *d_key, *d_value; /* of `type` */
     void *d_decay, *d_beta;          /* [batch][time][heads] */
     void *d_state;                   /* or null */
-    void *workspace;                 /* 2 * batch * time * heads * key_size floats where heads != key_heads */
+    void *workspace;                 /* cuju_delta_rule_workspace() bytes */
 };
 /* One step (time 1), the memory updated in place. */
 int cuju_delta_rule_step(const struct cuju_delta_rule *rule, void *stream);
 int cuju_delta_rule_forward(const struct cuju_delta_rule *rule, void *stream);
+/* Bytes of workspace that the backward pass needs, or 0. */
+unsigned long long cuju_delta_rule_workspace(const struct cuju_delta_rule *rule);
 int cuju_delta_rule_backward(const struct cuju_delta_rule *rule, void *stream);
 
 /* Group norm with an activation (0 none, 1 relu, 2 silu) over channels-last maps

@@ -88,6 +88,10 @@ __device__ __forceinline__ void Forget() { asm volatile("" ::: "memory"); }
 
 // The same of a lane's own value, so that what follows from it is not kept over a loop.
 __device__ __forceinline__ void Renew(F4 &x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ int Renewed(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 // A kernel's only argument, read anew from the arguments' segment: many strides and pointers that are
 // each used once in a long loop would not all fit the scalar registers.

@@ -71,13 +71,15 @@ __device__ __forceinline__ F4 ColumnOrder(const float *matrix, int m, int g) {
 }
 
 template <class T, int KeyTiles, int Waves, bool Whole>
-__global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(2))) void BackwardKernel(BackwardArgs<T> a) {
+__global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyTiles > 4 || (sizeof(T) == 4 && Waves < KeyTiles) ? 1 : 2))) void BackwardKernel(BackwardArgs<T> a) {
     using At = BackwardShared<KeyTiles, Waves, sizeof(T)>;
     using Args = BackwardArgs<T>;
     extern __shared__ __align__(16) float shared[];
     constexpr int P = kPieces<T>, kThreads = 64 * Waves, kPairs = Waves / 2;
     const Rule &rule = a.rule;
-    const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    // The lane is read anew in every part: the addresses that follow from it would fill the registers.
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     constexpr int ms = At::kMemoryRow, rs = At::kRow, ks = At::kKeyRow, vs = At::kValueRow;
     double *reach = reinterpret_cast<double *>(shared + At::kReach);
     float *betas = shared + At::kBetas, *wholes = shared + At::kWhole, *afters = shared + At::kAfter;
@@ -94,8 +96,8 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(2)))
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
     const int dk = rule.key_size, dv = rule.value_size, time = rule.time;
     const int base = slice * kSlice;
-    const int column = base + 16 * wave + m;  // a lane's column in column order
-    const int column4 = 16 * wave + 4 * g;    // its first of four in row order, within the slice
+    int column = base + 16 * wave + m;  // a lane's column in column order
+    int column4 = 16 * wave + 4 * g;    // its first of four in row order, within the slice
     const int segments = (time + kSegment - 1) / kSegment;
     const Eyes eyes = EyesOf(m, g);
 
@@ -184,6 +186,9 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(2)))
             const unsigned below = cuts & (high < 32 ? (1u << high) - 1 : ~0u);
             low = below ? 31 - __builtin_clz(below) : 0;
             const bool starts = (cuts >> low) & 1;
+#pragma unroll
+            for (int t = 0; t < KeyTiles; t++) Renew(start[t]);
+            lane = Renewed(lane), m = lane & 15, g = lane >> 4, column4 = 16 * wave + 4 * g;
             const auto mine = [&](int tile) { return kChunk * tile + m >= low && kChunk * tile + m < high; };
             const auto in = [&](int tile, int r) { return kChunk * tile + 4 * g + r >= low && kChunk * tile + 4 * g + r < high; };
             const auto keyPair = [&](const T *rows, int tile, int p, B8(&x)[P]) {

@@ -71,7 +71,32 @@ __device__ __forceinline__ void GroupSums(const float *channels, float *out, con
     __syncthreads();
 }
 
-constexpr int kMostSlab = 512;  // channels of a slab: a wavefront of packs of eight
+// The workgroup's packs: thread by thread, `Packs` rows of threads one after the other. A pack past the
+// map's end is a copy of the first pixel, whose difference from that pixel is zero.
+template <class T, int Vector, int Packs>
+struct Held {
+    Pack<T, Vector> x[Packs];
+    __device__ __forceinline__ void Load(const T *from, const Shape &s, int row, int rows, bool mine) {
+        const T *p = from + (long long)row * s.channels;
+        const long long step = (long long)rows * s.channels;
+#pragma unroll
+        for (int i = 0; i < Packs; i++, p += step) {
+            // Whole rows of threads first, without a comparison of their own.
+            if ((i + 1) * rows <= s.pixels) {
+                if (mine) x[i] = *reinterpret_cast<const Pack<T, Vector> *>(p);
+            } else if (i * rows < s.pixels) {
+                if (mine) x[i] = *reinterpret_cast<const Pack<T, Vector> *>(i * rows + row < s.pixels ? p : from);
+            }
+        }
+    }
+};
+// The packs' body, for each that the map has: body(i, whether this thread's is past the end).
+template <int Packs, class Body>
+__device__ __forceinline__ void ForPacks(const Shape &s, int row, int rows, Body body) {
+#pragma unroll
+    for (int i = 0; i < Packs; i++)
+        if (i * rows < s.pixels) body(i, i * rows + row >= s.pixels);
+}
 
 template <class T, int Vector, int Packs, int Threads>
 __global__ __launch_bounds__(Threads) void ForwardKernel(const T *x, T *y, const float *weight, const float *bias, float *stats,
@@ -84,37 +109,30 @@ __global__ __launch_bounds__(Threads) void ForwardKernel(const T *x, T *y, const
     const bool mine = vector < s.vectors;
     const int channel = slab * s.slabChannels + vector * Vector;
     const long long base = n * s.pixels * s.channels + channel;
-    Pack<T, Vector> v[Packs];
-#pragma unroll
-    for (int i = 0; i < Packs; i++) {
-        const int p = i * rows + row;
-        if (mine && p < s.pixels) v[i] = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
-    }
-    float sum[Vector];
+    Held<T, Vector, Packs> held{};
+    held.Load(x + base, s, row, rows, mine);
+    const float count = 1.f / ((float)s.pixels * s.perGroup);
+    float mean[Vector], sum[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) sum[c] = 0;
+    ForPacks<Packs>(s, row, rows, [&](int i, bool past) {
 #pragma unroll
-    for (int i = 0; i < Packs; i++)
-        if (mine && i * rows + row < s.pixels)
-#pragma unroll
-            for (int c = 0; c < Vector; c++) sum[c] += Float(v[i].x[c]);
+        for (int c = 0; c < Vector; c++) sum[c] += past ? 0.f : Float(held.x[i].x[c]);
+    });
     ChannelSums<Vector>(sum, scratch, channelSums, s);
     GroupSums(channelSums, means, s);
-    const float count = 1.f / ((float)s.pixels * s.perGroup);
-    float mean[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
         mean[c] = mine ? means[(vector * Vector + c) / s.perGroup] * count : 0.f;
         sum[c] = 0;
     }
+    ForPacks<Packs>(s, row, rows, [&](int i, bool past) {
 #pragma unroll
-    for (int i = 0; i < Packs; i++)
-        if (mine && i * rows + row < s.pixels)
-#pragma unroll
-            for (int c = 0; c < Vector; c++) {
-                const float d = Float(v[i].x[c]) - mean[c];
-                sum[c] = fmaf(d, d, sum[c]);
-            }
+        for (int c = 0; c < Vector; c++) {
+            const float d = past ? 0.f : Float(held.x[i].x[c]) - mean[c];
+            sum[c] = fmaf(d, d, sum[c]);
+        }
+    });
     ChannelSums<Vector>(sum, scratch, channelSums, s);
     GroupSums(channelSums, squares, s);
     const int slabGroups = s.slabChannels / s.perGroup;
@@ -124,25 +142,23 @@ __global__ __launch_bounds__(Threads) void ForwardKernel(const T *x, T *y, const
             to[0] = means[i] * count;
             to[1] = 1.f / sqrtf(squares[i] * count + epsilon);
         }
+    if (!mine) return;
     float scale[Vector], shift[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
-        scale[c] = 0, shift[c] = 0;
-        if (!mine) continue;
         scale[c] = 1.f / sqrtf(squares[(vector * Vector + c) / s.perGroup] * count + epsilon);
+        shift[c] = bias ? bias[channel + c] : 0.f;
         if (weight) scale[c] *= weight[channel + c];
-        if (bias) shift[c] = bias[channel + c];
     }
-#pragma unroll
-    for (int i = 0; i < Packs; i++) {
-        const int p = i * rows + row;
-        if (!mine || p >= s.pixels) continue;
+    T *to = y + base + (long long)row * s.channels;
+    const long long step = (long long)rows * s.channels;
+    ForPacks<Packs>(s, row, rows, [&](int i, bool past) {
         Pack<T, Vector> out;
 #pragma unroll
         for (int c = 0; c < Vector; c++)
-            out.x[c] = As<T>(Activate(fmaf(Float(v[i].x[c]) - mean[c], scale[c], shift[c]), activation));
-        *reinterpret_cast<Pack<T, Vector> *>(y + base + (long long)p * s.channels) = out;
-    }
+            out.x[c] = As<T>(Activate(fmaf(Float(held.x[i].x[c]) - mean[c], scale[c], shift[c]), activation));
+        if (!past) *reinterpret_cast<Pack<T, Vector> *>(to + i * step) = out;
+    });
 }
 
 template <class T, int Vector, int Packs, int Threads>
@@ -150,7 +166,7 @@ __global__ __launch_bounds__(Threads) void BackwardKernel(const T *x, const T *d
                                                           const float *bias, const float *stats, float *parts, Shape s,
                                                           int activation) {
     __shared__ float scratch[Threads / 64 * 64 * Vector], biasSums[64 * Vector], weightSums[64 * Vector];
-    __shared__ float channelMeans[64 * Vector], first[64 * Vector], second[64 * Vector];
+    __shared__ float first[64 * Vector], second[64 * Vector];
     const unsigned id = Place(blockIdx.x, gridDim.x);
     const int slab = id % s.slabs;
     const long long n = id / s.slabs;
@@ -158,15 +174,9 @@ __global__ __launch_bounds__(Threads) void BackwardKernel(const T *x, const T *d
     const bool mine = vector < s.vectors;
     const int channel = slab * s.slabChannels + vector * Vector;
     const long long base = n * s.pixels * s.channels + channel;
-    Pack<T, Vector> v[Packs], d[Packs];
-#pragma unroll
-    for (int i = 0; i < Packs; i++) {
-        const int p = i * rows + row;
-        if (mine && p < s.pixels) {
-            v[i] = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
-            d[i] = *reinterpret_cast<const Pack<T, Vector> *>(dy + base + (long long)p * s.channels);
-        }
-    }
+    Held<T, Vector, Packs> v{}, d{};
+    v.Load(x + base, s, row, rows, mine);
+    d.Load(dy + base, s, row, rows, mine);
     float mean[Vector], inverse[Vector], w[Vector], shift[Vector], sumB[Vector], sumW[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
@@ -177,16 +187,15 @@ __global__ __launch_bounds__(Threads) void BackwardKernel(const T *x, const T *d
         if (weight) w[c] = weight[channel + c];
         if (bias) shift[c] = bias[channel + c];
     }
+    ForPacks<Packs>(s, row, rows, [&](int i, bool past) {
 #pragma unroll
-    for (int i = 0; i < Packs; i++)
-        if (mine && i * rows + row < s.pixels)
-#pragma unroll
-            for (int c = 0; c < Vector; c++) {
-                const float xh = (Float(v[i].x[c]) - mean[c]) * inverse[c];
-                const float dz = Float(d[i].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
-                sumB[c] += dz;
-                sumW[c] = fmaf(dz, xh, sumW[c]);
-            }
+        for (int c = 0; c < Vector; c++) {
+            const float xh = (Float(v.x[i].x[c]) - mean[c]) * inverse[c];
+            const float dz = past ? 0.f : Float(d.x[i].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
+            sumB[c] += dz;
+            sumW[c] = fmaf(dz, xh, sumW[c]);
+        }
+    });
     ChannelSums<Vector>(sumB, scratch, biasSums, s);
     ChannelSums<Vector>(sumW, scratch, weightSums, s);
     for (int c = threadIdx.x; c < s.slabChannels; c += Threads) {
@@ -199,26 +208,26 @@ __global__ __launch_bounds__(Threads) void BackwardKernel(const T *x, const T *d
     __syncthreads();
     GroupSums(biasSums, first, s);
     GroupSums(weightSums, second, s);
+    if (!mine) return;
     const float count = 1.f / ((float)s.pixels * s.perGroup);
     float m1[Vector], m2[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
-        m1[c] = mine ? first[(vector * Vector + c) / s.perGroup] * count : 0.f;
-        m2[c] = mine ? second[(vector * Vector + c) / s.perGroup] * count : 0.f;
+        m1[c] = first[(vector * Vector + c) / s.perGroup] * count;
+        m2[c] = second[(vector * Vector + c) / s.perGroup] * count;
     }
-#pragma unroll
-    for (int i = 0; i < Packs; i++) {
-        const int p = i * rows + row;
-        if (!mine || p >= s.pixels) continue;
+    T *to = dx + base + (long long)row * s.channels;
+    const long long step = (long long)rows * s.channels;
+    ForPacks<Packs>(s, row, rows, [&](int i, bool past) {
         Pack<T, Vector> out;
 #pragma unroll
         for (int c = 0; c < Vector; c++) {
-            const float xh = (Float(v[i].x[c]) - mean[c]) * inverse[c];
-            const float dz = Float(d[i].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
+            const float xh = (Float(v.x[i].x[c]) - mean[c]) * inverse[c];
+            const float dz = Float(d.x[i].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
             out.x[c] = As<T>(inverse[c] * (fmaf(w[c], dz, -m1[c]) - xh * m2[c]));
         }
-        *reinterpret_cast<Pack<T, Vector> *>(dx + base + (long long)p * s.channels) = out;
-    }
+        if (!past) *reinterpret_cast<Pack<T, Vector> *>(to + i * step) = out;
+    });
 }
 
 // ------------------------------------------------------------- maps that no workgroup's registers hold
@@ -244,6 +253,21 @@ struct Cut {
     }
 };
 
+// A cut's pixels, four of a thread's at a time, so that their loads are on the way together: load(n, p)
+// for each, then body(n, p).
+constexpr int kAhead = 4;
+template <class Load, class Body>
+__device__ __forceinline__ void ForPixels(const Cut &cut, Load load, Body body) {
+    int p = cut.first;
+    for (; p + (kAhead - 1) * cut.step < cut.end; p += kAhead * cut.step) {
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) load(n, p + n * cut.step);
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) body(n, p + n * cut.step);
+    }
+    for (; p < cut.end; p += cut.step) load(0, p), body(0, p);
+}
+
 // Each channel's sum and sum of squares about its value at the first pixel: [map][cut][2][channels].
 template <class T, int Vector>
 __global__ __launch_bounds__(kSplitThreads) void SumsKernel(const T *x, float *parts, Shape s) {
@@ -253,16 +277,17 @@ __global__ __launch_bounds__(kSplitThreads) void SumsKernel(const T *x, float *p
     float about[Vector], sum[Vector], square[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) about[c] = cut.mine ? Float(at[c]) : 0.f, sum[c] = square[c] = 0;
+    Pack<T, Vector> v[kAhead];
     if (cut.mine)
-        for (int p = cut.first; p < cut.end; p += cut.step) {
-            const auto v = *reinterpret_cast<const Pack<T, Vector> *>(at + (long long)p * s.channels);
+        ForPixels(cut, [&](int n, int p) { v[n] = *reinterpret_cast<const Pack<T, Vector> *>(at + (long long)p * s.channels); },
+                  [&](int n, int) {
 #pragma unroll
-            for (int c = 0; c < Vector; c++) {
-                const float d = Float(v.x[c]) - about[c];
-                sum[c] += d;
-                square[c] = fmaf(d, d, square[c]);
-            }
-        }
+                      for (int c = 0; c < Vector; c++) {
+                          const float d = Float(v[n].x[c]) - about[c];
+                          sum[c] += d;
+                          square[c] = fmaf(d, d, square[c]);
+                      }
+                  });
     Shape slab = s;
     slab.vectors = cut.channels / Vector;
     float *to = parts + (cut.map * gridDim.y + blockIdx.y) * 2 * s.channels + cut.slab;
@@ -272,57 +297,98 @@ __global__ __launch_bounds__(kSplitThreads) void SumsKernel(const T *x, float *p
         __syncthreads();
     }
 }
-// A wavefront a group: its mean and inverse deviation, from the cuts' sums, in 64 bits.
+// A sum of `value(channel, cut)` over a group's channels and all cuts, the same in every lane of a
+// wavefront.
+template <class Value>
+__device__ __forceinline__ double GroupSum(const Shape &s, int group, int cuts, Value value) {
+    double total = 0;
+    for (int i = threadIdx.x & 63; i < s.perGroup * cuts; i += 64) total += value(group * s.perGroup + i % s.perGroup, i / s.perGroup);
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    return total;
+}
+__device__ __forceinline__ double PartOf(const float *parts, const Shape &s, long long n, int cuts, int cut, int k, int c) {
+    return parts[((n * cuts + cut) * 2 + k) * s.channels + c];
+}
+// A group's mean and inverse deviation from the cuts' sums, in 64 bits, by a wavefront.
 template <class T>
-__global__ __launch_bounds__(64) void StatsKernel(const T *x, const float *parts, float *stats, Shape s, int cuts, float epsilon) {
-    const int group = blockIdx.x % s.groups;
-    const long long n = blockIdx.x / s.groups;
-    const auto sumOver = [&](auto value) {
-        double total = 0;
-        for (int i = threadIdx.x; i < s.perGroup; i += 64) total += value(group * s.perGroup + i);
-        for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
-        return total;
-    };
-    const auto part = [&](int k, int c) {
-        double total = 0;
-        for (int i = 0; i < cuts; i++) total += parts[((n * cuts + i) * 2 + k) * s.channels + c];
-        return total;
-    };
+__device__ __forceinline__ float2 StatsOf(const T *x, const float *parts, const Shape &s, long long n, int group, int cuts,
+                                          float epsilon) {
     const T *first = x + n * s.pixels * s.channels;
     const double count = (double)s.pixels * s.perGroup;
-    const double mean = sumOver([&](int c) { return part(0, c) + (double)s.pixels * Float(first[c]); }) / count;
-    const double squares = sumOver([&](int c) {
+    const double mean = GroupSum(s, group, cuts, [&](int c, int cut) {
+                            return PartOf(parts, s, n, cuts, cut, 0, c) + (cut ? 0.0 : (double)s.pixels * Float(first[c]));
+                        }) / count;
+    const double squares = GroupSum(s, group, cuts, [&](int c, int cut) {
         const double off = mean - Float(first[c]);
-        return part(1, c) - 2 * off * part(0, c) + s.pixels * off * off;
+        return PartOf(parts, s, n, cuts, cut, 1, c) - 2 * off * PartOf(parts, s, n, cuts, cut, 0, c) +
+               (cut ? 0.0 : s.pixels * off * off);
     });
-    if (threadIdx.x == 0) {
-        float *to = stats + (n * s.groups + group) * 2;
-        to[0] = (float)mean;
-        to[1] = (float)(1.0 / sqrt(fmax(squares, 0.0) / count + epsilon));
-    }
+    return float2{(float)mean, (float)(1.0 / sqrt(fmax(squares, 0.0) / count + epsilon))};
 }
+// The means of weight dz and of weight dz xh over a group, by a wavefront.
+__device__ __forceinline__ float2 MeansOf(const float *parts, const float *weight, const Shape &s, long long n, int group,
+                                          int cuts) {
+    float2 means;
+    const double count = (double)s.pixels * s.perGroup;
+    for (int k = 0; k < 2; k++) {
+        const double total = GroupSum(s, group, cuts, [&](int c, int cut) {
+            const double sum = PartOf(parts, s, n, cuts, cut, k, c);
+            return weight ? sum * weight[c] : sum;
+        });
+        (k ? means.x : means.y) = (float)(total / count);
+    }
+    return means;
+}
+// Slabs of whole groups, up to this many, find their groups' statistics themselves; others have a
+// kernel of a wavefront a group for it.
+constexpr int kMostGroups = 128;
+template <class T>
+__global__ __launch_bounds__(64) void StatsKernel(const T *x, const float *parts, float2 *stats, Shape s, int cuts, float epsilon) {
+    const float2 found = StatsOf(x, parts, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts, epsilon);
+    if (threadIdx.x == 0) stats[blockIdx.x] = found;
+}
+__global__ __launch_bounds__(64) void MeansKernel(const float *parts, const float *weight, float2 *means, Shape s, int cuts) {
+    const float2 found = MeansOf(parts, weight, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts);
+    if (threadIdx.x == 0) means[blockIdx.x] = found;
+}
+
 template <class T, int Vector>
 __global__ __launch_bounds__(kSplitThreads) void ApplyKernel(const T *x, T *y, const float *weight, const float *bias,
-                                                             const float *stats, Shape s, int activation) {
+                                                             const float *parts, float2 *stats, Shape s, float epsilon,
+                                                             int activation) {
+    __shared__ float2 found[kMostGroups];
     const Cut cut(s, Vector);
-    if (!cut.mine) return;
     const long long n = cut.map, base = n * s.pixels * s.channels + cut.channel;
+    const int firstGroup = cut.slab / s.perGroup;
+    if (parts) {
+        for (int i = threadIdx.x >> 6; i < cut.channels / s.perGroup; i += kSplitThreads / 64) {
+            const float2 each = StatsOf(x, parts, s, n, firstGroup + i, gridDim.y, epsilon);
+            if ((threadIdx.x & 63) == 0) {
+                found[i] = each;
+                if (blockIdx.y == 0) stats[n * s.groups + firstGroup + i] = each;
+            }
+        }
+        __syncthreads();
+    }
+    if (!cut.mine) return;
     float mean[Vector], scale[Vector], shift[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
-        const float *from = stats + (n * s.groups + (cut.channel + c) / s.perGroup) * 2;
-        mean[c] = from[0];
-        scale[c] = from[1] * (weight ? weight[cut.channel + c] : 1.f);
+        const int group = (cut.channel + c) / s.perGroup;
+        const float2 each = parts ? found[group - firstGroup] : stats[n * s.groups + group];
+        mean[c] = each.x;
+        scale[c] = each.y * (weight ? weight[cut.channel + c] : 1.f);
         shift[c] = bias ? bias[cut.channel + c] : 0.f;
     }
-    for (int p = cut.first; p < cut.end; p += cut.step) {
-        const auto v = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
-        Pack<T, Vector> out;
+    Pack<T, Vector> v[kAhead];
+    ForPixels(cut, [&](int n, int p) { v[n] = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels); },
+              [&](int n, int p) {
+                  Pack<T, Vector> out;
 #pragma unroll
-        for (int c = 0; c < Vector; c++)
-            out.x[c] = As<T>(Activate(fmaf(Float(v.x[c]) - mean[c], scale[c], shift[c]), activation));
-        *reinterpret_cast<Pack<T, Vector> *>(y + base + (long long)p * s.channels) = out;
-    }
+                  for (int c = 0; c < Vector; c++)
+                      out.x[c] = As<T>(Activate(fmaf(Float(v[n].x[c]) - mean[c], scale[c], shift[c]), activation));
+                  *reinterpret_cast<Pack<T, Vector> *>(y + base + (long long)p * s.channels) = out;
+              });
 }
 // The gradients' channel sums: [map][cut][2][channels], of dz xh and of dz.
 template <class T, int Vector>
@@ -342,18 +408,21 @@ __global__ __launch_bounds__(kSplitThreads) void GradientSumsKernel(const T *x, 
         if (weight) w[c] = weight[cut.channel + c];
         if (bias) shift[c] = bias[cut.channel + c];
     }
+    Pack<T, Vector> v[kAhead], d[kAhead];
+    const auto load = [&](int n, int p) {
+        v[n] = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
+        d[n] = *reinterpret_cast<const Pack<T, Vector> *>(dy + base + (long long)p * s.channels);
+    };
     if (cut.mine)
-        for (int p = cut.first; p < cut.end; p += cut.step) {
-            const auto v = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
-            const auto d = *reinterpret_cast<const Pack<T, Vector> *>(dy + base + (long long)p * s.channels);
+        ForPixels(cut, load, [&](int n, int) {
 #pragma unroll
             for (int c = 0; c < Vector; c++) {
-                const float xh = (Float(v.x[c]) - mean[c]) * inverse[c];
-                const float dz = Float(d.x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
+                const float xh = (Float(v[n].x[c]) - mean[c]) * inverse[c];
+                const float dz = Float(d[n].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
                 sumB[c] += dz;
                 sumW[c] = fmaf(dz, xh, sumW[c]);
             }
-        }
+        });
     Shape slab = s;
     slab.vectors = cut.channels / Vector;
     float *to = parts + (n * gridDim.y + blockIdx.y) * 2 * s.channels + cut.slab;
@@ -363,67 +432,75 @@ __global__ __launch_bounds__(kSplitThreads) void GradientSumsKernel(const T *x, 
         __syncthreads();
     }
 }
-// A wavefront a group: the means of weight dz and weight dz xh, [map][group][2].
-__global__ __launch_bounds__(64) void GradientMeansKernel(const float *parts, const float *weight, float *means, Shape s,
-                                                          int cuts) {
-    const int group = blockIdx.x % s.groups;
-    const long long n = blockIdx.x / s.groups;
-    for (int k = 0; k < 2; k++) {
-        double total = 0;
-        for (int i = threadIdx.x; i < s.perGroup; i += 64) {
-            const int c = group * s.perGroup + i;
-            double sum = 0;
-            for (int j = 0; j < cuts; j++) sum += parts[((n * cuts + j) * 2 + k) * s.channels + c];
-            total += weight ? sum * weight[c] : sum;
-        }
-        for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
-        if (threadIdx.x == 0) means[(n * s.groups + group) * 2 + k] = (float)(total / ((double)s.pixels * s.perGroup));
-    }
-}
 template <class T, int Vector>
 __global__ __launch_bounds__(kSplitThreads) void GradientKernel(const T *x, const T *dy, T *dx, const float *weight,
-                                                                const float *bias, const float *stats, const float *means,
-                                                                Shape s, int activation) {
+                                                                const float *bias, const float2 *stats, const float *parts,
+                                                                const float2 *means, Shape s, int activation) {
+    __shared__ float2 found[kMostGroups];
     const Cut cut(s, Vector);
-    if (!cut.mine) return;
     const long long n = cut.map, base = n * s.pixels * s.channels + cut.channel;
+    const int firstGroup = cut.slab / s.perGroup;
+    if (parts) {
+        for (int i = threadIdx.x >> 6; i < cut.channels / s.perGroup; i += kSplitThreads / 64) {
+            const float2 each = MeansOf(parts, weight, s, n, firstGroup + i, gridDim.y);
+            if ((threadIdx.x & 63) == 0) found[i] = each;
+        }
+        __syncthreads();
+    }
+    if (!cut.mine) return;
     float mean[Vector], inverse[Vector], w[Vector], shift[Vector], m1[Vector], m2[Vector];
 #pragma unroll
     for (int c = 0; c < Vector; c++) {
-        const long long at = (n * s.groups + (cut.channel + c) / s.perGroup) * 2;
-        mean[c] = stats[at], inverse[c] = stats[at + 1];
-        m2[c] = means[at], m1[c] = means[at + 1];
+        const int group = (cut.channel + c) / s.perGroup;
+        const float2 each = stats[n * s.groups + group];
+        const float2 over = parts ? found[group - firstGroup] : means[n * s.groups + group];
+        mean[c] = each.x, inverse[c] = each.y;
+        m1[c] = over.x, m2[c] = over.y;
         w[c] = weight ? weight[cut.channel + c] : 1.f;
         shift[c] = bias ? bias[cut.channel + c] : 0.f;
     }
-    for (int p = cut.first; p < cut.end; p += cut.step) {
-        const auto v = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
-        const auto d = *reinterpret_cast<const Pack<T, Vector> *>(dy + base + (long long)p * s.channels);
+    Pack<T, Vector> v[kAhead], d[kAhead];
+    const auto load = [&](int n, int p) {
+        v[n] = *reinterpret_cast<const Pack<T, Vector> *>(x + base + (long long)p * s.channels);
+        d[n] = *reinterpret_cast<const Pack<T, Vector> *>(dy + base + (long long)p * s.channels);
+    };
+    ForPixels(cut, load, [&](int n, int p) {
         Pack<T, Vector> out;
 #pragma unroll
         for (int c = 0; c < Vector; c++) {
-            const float xh = (Float(v.x[c]) - mean[c]) * inverse[c];
-            const float dz = Float(d.x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
+            const float xh = (Float(v[n].x[c]) - mean[c]) * inverse[c];
+            const float dz = Float(d[n].x[c]) * Slope(fmaf(w[c], xh, shift[c]), activation);
             out.x[c] = As<T>(inverse[c] * (fmaf(w[c], dz, -m1[c]) - xh * m2[c]));
         }
         *reinterpret_cast<Pack<T, Vector> *>(dx + base + (long long)p * s.channels) = out;
-    }
+    });
 }
 
-// The sums over maps (and cuts) of [rows][2][channels], 64 columns a workgroup of 16 rows at a time.
+// The sums over maps (and cuts) of [rows][2][channels]: 16 columns a workgroup, 64 rows at a time.
 __global__ __launch_bounds__(1024) void ColumnsKernel(const float *parts, float *dWeight, float *dBias, long long rows,
                                                       int channels) {
-    __shared__ float sums[16][64];
-    const int column = blockIdx.x * 64 + (threadIdx.x & 63), slot = threadIdx.x >> 6;
+    __shared__ float sums[64][16];
+    const int column = blockIdx.x * 16 + (threadIdx.x & 15), slot = threadIdx.x >> 4;
     float sum = 0;
-    if (column < 2 * channels)
-        for (long long i = slot; i < rows; i += 16) sum += parts[i * 2 * channels + column];
-    sums[slot][threadIdx.x & 63] = sum;
-    __syncthreads();
+    if (column < 2 * channels) {
+        const float *at = parts + column;
+        long long i = slot;
+        for (; i + 3 * 64 < rows; i += 4 * 64) {
+            float x[4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) x[n] = at[(i + n * 64) * 2 * channels];
+            sum += (x[0] + x[1]) + (x[2] + x[3]);
+        }
+        for (; i < rows; i += 64) sum += at[i * 2 * channels];
+    }
+    sums[slot][threadIdx.x & 15] = sum;
+    for (int half = 32; half > 0; half /= 2) {
+        __syncthreads();
+        if (slot < half) sums[slot][threadIdx.x & 15] += sums[slot + half][threadIdx.x & 15];
+    }
     if (slot == 0 && column < 2 * channels) {
-        for (int i = 1; i < 16; i++) sum += sums[i][threadIdx.x];
         float *to = column < channels ? dWeight : dBias;
-        if (to) to[column < channels ? column : column - channels] = sum;
+        if (to) to[column < channels ? column : column - channels] = sums[0][threadIdx.x];
     }
 }
 
@@ -440,17 +517,27 @@ Shape SlabsOf(const Norm &n, int slabs, int vector) {
     s.lanes = PowerOfTwo(s.vectors);
     return s;
 }
-// The largest pack of elements that the channels and the tensors' alignment allow, in elements.
+// The largest pack of elements that the channels and the tensors' alignment allow, in elements, up to
+// four: with eight, a thread's sums, scales and shifts of as many channels halve the wavefronts on a
+// SIMD (600 bfloat16 maps of 216 KB: the gradients 147 us with eight, 140 with four; 64 maps of 432 KB
+// 55 and 43).
 int VectorOf(const Norm &n) {
     const int size = n.type == 0 ? 4 : 2;
     uintptr_t all = reinterpret_cast<uintptr_t>(n.x) | reinterpret_cast<uintptr_t>(n.y) |
                     reinterpret_cast<uintptr_t>(n.dy) | reinterpret_cast<uintptr_t>(n.dx);
-    int vector = 16 / size;
+    int vector = 4;
     while (vector > 1 && (n.channels % vector || all % (vector * size))) vector /= 2;
     return vector;
 }
 // The first count of slabs (each of whole groups and whole packs) whose pixels fit `packs` packs of
 // each of `threads` threads; 0 if none does.
+//
+// Which maps a workgroup holds (us, held against cut, forward; then the gradients):
+//  - up to 16 KB, 256 threads: 4,000 bfloat16 maps of 16 KB 38 against 47; 63 against 75;
+//  - floats up to 224 KB (112 KB with their gradient) in one or two slabs, 512 threads: 4,000 maps of
+//    108 KB 187 against 269; 325 against 436. In four slabs, 600 maps of 432 KB, 171 against 166.
+//  - 16-bit maps past 16 KB are cut: a pack of four is 8 bytes there, and 4,000 maps of 32 KB took 100
+//    against 68; 149 against 133.
 int SlabsFor(const Norm &n, int vector, int packs, int threads) {
     for (int slabs = 1; slabs <= n.groups; slabs++) {
         if (n.groups % slabs || n.channels / slabs % vector) continue;
@@ -459,28 +546,37 @@ int SlabsFor(const Norm &n, int vector, int packs, int threads) {
     }
     return 0;
 }
-// Maps past the registers: channels in slabs of at most a wavefront of packs, pixels cut so that about
-// 2,048 workgroups run, at least 64 KB each.
+// Other maps: channels in slabs of at most a wavefront of packs, of whole groups where they have it.
 Shape SplitShape(const Norm &n, int vector) {
     Shape s{n.pixels, n.channels, n.groups, n.channels / n.groups, 1, n.channels, 0, 0};
-    s.slabChannels = n.channels < 64 * vector ? n.channels : 64 * vector;
+    if (n.channels > 64 * vector) {
+        int whole = s.perGroup;
+        while (whole % vector) whole += s.perGroup;
+        s.slabChannels = whole <= 64 * vector ? 64 * vector / whole * whole : 64 * vector;
+    }
     s.slabs = (n.channels + s.slabChannels - 1) / s.slabChannels;
     s.vectors = s.slabChannels / vector;
     s.lanes = PowerOfTwo(s.vectors);
     return s;
 }
+bool FindsItself(const Shape &s) { return s.slabChannels % s.perGroup == 0 && s.slabChannels / s.perGroup <= kMostGroups; }
+// Pixels are cut so that about 2,048 workgroups run, with at least 16 KB each.
 int CutsOf(const Norm &n) {
     const long long bytes = (long long)n.pixels * n.channels * (n.type == 0 ? 4 : 2);
-    long long cuts = bytes / 65536;
-    const long long wanted = (2048 + n.batch - 1) / (n.batch > 0 ? n.batch : 1);
-    if (cuts > wanted) cuts = wanted;
-    return (int)(cuts < 1 ? 1 : cuts > 1024 ? 1024 : cuts);
+    long long cuts = n.batch > 0 ? 2048 / n.batch : 1;
+    if (cuts > bytes / 16384) cuts = bytes / 16384;
+    return (int)(cuts < 1 ? 1 : cuts > 64 ? 64 : cuts);
+}
+
+// Packs of `bytes` of a thread's registers.
+template <class T, int Vector>
+constexpr int Packs(int bytes) {
+    return bytes / (Vector * (int)sizeof(T)) < bytes / 8 ? bytes / (Vector * (int)sizeof(T)) : bytes / 8;
 }
 
 template <class Body>
 void ForVector(int vector, Body body) {
     switch (vector) {
-    case 8: body(std::integral_constant<int, 8>()); break;
     case 4: body(std::integral_constant<int, 4>()); break;
     case 2: body(std::integral_constant<int, 2>()); break;
     default: body(std::integral_constant<int, 1>()); break;
@@ -496,22 +592,24 @@ void Forward(const Norm &n, hipStream_t stream) {
     float *stats = static_cast<float *>(n.stats), *work = static_cast<float *>(n.workspace);
     ForVector(vector, [&](auto wide) {
         constexpr int V = decltype(wide)::value;
-        if constexpr (V * sizeof(T) <= 16) {
-            const auto resident = [&](auto kernel, int slabs, int threads) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, y,
-                                   weight, bias, stats, SlabsOf(n, slabs, V), n.epsilon, n.activation);
-            };
-            if (SlabsFor(n, V, 4, 256) == 1) return resident(ForwardKernel<T, V, 4, 256>, 1, 256);
-            if (SlabsFor(n, V, 8, 512) == 1) return resident(ForwardKernel<T, V, 8, 512>, 1, 512);
-            if (const int slabs = SlabsFor(n, V, 14, 1024)) return resident(ForwardKernel<T, V, 14, 1024>, slabs, 1024);
-            const Shape s = SplitShape(n, V);
-            const int cuts = CutsOf(n);
-            const dim3 grid((unsigned)((long long)s.slabs * n.batch), cuts);
-            hipLaunchKernelGGL((SumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, work, s);
-            hipLaunchKernelGGL(StatsKernel<T>, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, x, work, stats, s, cuts, n.epsilon);
-            hipLaunchKernelGGL((ApplyKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, y, weight, bias, stats, s,
-                               n.activation);
-        }
+        const auto resident = [&](auto kernel, int slabs, int threads) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, y,
+                               weight, bias, stats, SlabsOf(n, slabs, V), n.epsilon, n.activation);
+        };
+        if (SlabsFor(n, V, Packs<T, V>(64), 256) == 1) return resident(ForwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
+        if constexpr (sizeof(T) == 4)
+            if (const int slabs = SlabsFor(n, V, Packs<T, V>(224), 512); slabs == 1 || slabs == 2)
+                return resident(ForwardKernel<T, V, Packs<T, V>(224), 512>, slabs, 512);
+        const Shape s = SplitShape(n, V);
+        const int cuts = CutsOf(n);
+        const dim3 grid((unsigned)((long long)s.slabs * n.batch), cuts);
+        hipLaunchKernelGGL((SumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, work, s);
+        float2 *found = reinterpret_cast<float2 *>(stats);
+        if (!FindsItself(s))
+            hipLaunchKernelGGL(StatsKernel<T>, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, x, work,
+                               found, s, cuts, n.epsilon);
+        hipLaunchKernelGGL((ApplyKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, y, weight, bias,
+                           FindsItself(s) ? work : nullptr, found, s, n.epsilon, n.activation);
     });
 }
 
@@ -526,27 +624,29 @@ void Backward(const Norm &n, hipStream_t stream) {
     long long rows = n.batch;
     ForVector(vector, [&](auto wide) {
         constexpr int V = decltype(wide)::value;
-        if constexpr (V * sizeof(T) <= 16) {
-            const auto resident = [&](auto kernel, int slabs, int threads) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, dy, dx,
-                                   weight, bias, stats, parts, SlabsOf(n, slabs, V), n.activation);
-            };
-            if (SlabsFor(n, V, 4, 256) == 1) return resident(BackwardKernel<T, V, 4, 256>, 1, 256);
-            if (const int slabs = SlabsFor(n, V, 14, 512)) return resident(BackwardKernel<T, V, 14, 512>, slabs, 512);
-            const Shape s = SplitShape(n, V);
-            const int cuts = CutsOf(n);
-            rows = (long long)n.batch * cuts;
-            float *means = parts + rows * 2 * n.channels;
-            const dim3 grid((unsigned)((long long)s.slabs * n.batch), cuts);
-            hipLaunchKernelGGL((GradientSumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, weight, bias, stats,
-                               parts, s, n.activation);
-            hipLaunchKernelGGL(GradientMeansKernel, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, parts, weight, means, s, cuts);
-            hipLaunchKernelGGL((GradientKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, dx, weight, bias, stats,
-                               means, s, n.activation);
-        }
+        const auto resident = [&](auto kernel, int slabs, int threads) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, dy, dx,
+                               weight, bias, stats, parts, SlabsOf(n, slabs, V), n.activation);
+        };
+        if (SlabsFor(n, V, Packs<T, V>(64), 256) == 1) return resident(BackwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
+        if constexpr (sizeof(T) == 4)
+            if (const int slabs = SlabsFor(n, V, Packs<T, V>(112), 512); slabs == 1 || slabs == 2)
+                return resident(BackwardKernel<T, V, Packs<T, V>(112), 512>, slabs, 512);
+        const Shape s = SplitShape(n, V);
+        const int cuts = CutsOf(n);
+        rows = (long long)n.batch * cuts;
+        float2 *means = reinterpret_cast<float2 *>(parts + rows * 2 * n.channels);
+        const dim3 grid((unsigned)((long long)s.slabs * n.batch), cuts);
+        hipLaunchKernelGGL((GradientSumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, weight, bias, stats,
+                           parts, s, n.activation);
+        if (!FindsItself(s))
+            hipLaunchKernelGGL(MeansKernel, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, parts,
+                               weight, means, s, cuts);
+        hipLaunchKernelGGL((GradientKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, dx, weight, bias,
+                           reinterpret_cast<const float2 *>(stats), FindsItself(s) ? parts : nullptr, means, s, n.activation);
     });
     if (n.d_weight || n.d_bias)
-        hipLaunchKernelGGL(ColumnsKernel, dim3((2 * n.channels + 63) / 64), dim3(1024), 0, stream, parts,
+        hipLaunchKernelGGL(ColumnsKernel, dim3((2 * n.channels + 15) / 16), dim3(1024), 0, stream, parts,
                            static_cast<float *>(n.d_weight), static_cast<float *>(n.d_bias), rows, n.channels);
 }
 

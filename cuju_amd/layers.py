@@ -15,6 +15,7 @@ type. There is no implementation for another device.
 
 from __future__ import annotations
 
+import functools
 import struct
 
 import torch
@@ -39,8 +40,13 @@ def _pointer(tensor) -> int:
     return 0 if tensor is None else tensor.data_ptr()
 
 
+@functools.lru_cache(maxsize=None)
+def _library():
+    return load()
+
+
 def _call(function, packed: bytes, device: torch.device) -> None:
-    lib = load()
+    lib = _library()
     if device.index == torch.cuda.current_device():
         status = getattr(lib, function)(packed, torch.cuda.current_stream(device).cuda_stream)
     else:
@@ -51,15 +57,16 @@ def _call(function, packed: bytes, device: torch.device) -> None:
 
 
 def _shape(name: str, tensor: torch.Tensor, shape: tuple) -> None:
-    if tuple(tensor.shape) != shape:
+    if tensor.shape != shape:
         raise ArgumentError(f'expected {name} of the shape {shape}, found {tuple(tensor.shape)}')
 
 
 def _device(first: str, tensor: torch.Tensor, others: dict) -> None:
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ArgumentError(f'expected {first} on a HIP device')
+    device = tensor.device
     for name, other in others.items():
-        if other is not None and (not isinstance(other, torch.Tensor) or other.device != tensor.device):
+        if other is not None and (not isinstance(other, torch.Tensor) or other.device != device):
             raise ArgumentError(f'expected {name} on the device of {first}')
 
 
@@ -85,6 +92,13 @@ def _rule(q, k, v, decay, beta, state, resets, scale, output=None, last=None, ch
                       *[_pointer(g) for g in gradients], _pointer(workspace))
 
 
+@functools.lru_cache(maxsize=256)
+def _rule_workspace(kind, batch, time, key_heads, key_size, heads, value_size) -> int:
+    """Bytes of workspace of a backward pass of these sizes."""
+    return _library().cuju_delta_rule_workspace(
+        _RULE.pack(kind, batch, time, key_heads, heads, key_size, value_size, 0.0, *[0] * 39))
+
+
 def _check_rule(query, key, value, decay, beta, state, resets, steps):
     """The checked arguments as the kernels take them; `steps`: whether they have a time axis."""
     axes = 4 if steps else 3
@@ -95,10 +109,10 @@ def _check_rule(query, key, value, decay, beta, state, resets, steps):
         raise ArgumentError(f'expected key and value of {query.dtype}, found {key.dtype} and {value.dtype}')
     if query.dim() != axes or value.dim() != axes:
         raise ArgumentError(f'expected query and value of {axes} axes, found {query.dim()} and {value.dim()}')
-    lead = tuple(query.shape[:axes - 2])
+    lead = query.shape[:axes - 2]
     key_heads, key_size = query.shape[-2:]
     heads, value_size = value.shape[-2:]
-    _shape('key', key, tuple(query.shape))
+    _shape('key', key, query.shape)
     _shape('value', value, (*lead, heads, value_size))
     _shape('decay', decay, (*lead, heads))
     _shape('beta', beta, (*lead, heads))
@@ -129,7 +143,7 @@ def _check_rule(query, key, value, decay, beta, state, resets, steps):
 def _rule_forward(q, k, v, decay, beta, state, resets, scale, train):
     batch, time = q.shape[:2]
     heads, value_size = v.shape[2:]
-    output = torch.empty((batch, time, heads, value_size), dtype=v.dtype, device=v.device)
+    output = v.new_empty((batch, time, heads, value_size))
     last = torch.empty((batch, heads, q.shape[3], value_size), dtype=torch.float32, device=v.device)
     kept = max(time - 1, 0) // SEGMENT if train else 0
     checkpoints = torch.empty((batch, heads, kept, q.shape[3], value_size), dtype=torch.float32, device=v.device)
@@ -142,24 +156,20 @@ def _rule_forward(q, k, v, decay, beta, state, resets, scale, train):
 def _rule_backward(q, k, v, decay, beta, state, resets, scale, checkpoints, d_output, d_last):
     batch, _, _, key_size = q.shape
     heads = v.shape[2]
-    dense = [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v, decay, beta)]
+    dense = [x.new_empty(x.shape) for x in (q, k, v, decay, beta)]
     d_state = torch.empty((batch, heads, key_size, v.shape[3]), dtype=torch.float32, device=v.device)
     if batch:
-        def packed(workspace):
-            return _rule(q, k, v, decay, beta, state, resets, scale,
-                         checkpoints=checkpoints if checkpoints.numel() else None, d_output=d_output, d_last=d_last,
-                         gradients=(*dense, d_state), workspace=workspace)
-
-        workspace, size = None, load().cuju_delta_rule_workspace(packed(None))
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=v.device)
-        _call('cuju_delta_rule_backward', packed(workspace), v.device)
+        size = _rule_workspace(TYPES[q.dtype], *q.shape, *v.shape[2:])
+        workspace = torch.empty(size, dtype=torch.uint8, device=v.device) if size else None
+        _call('cuju_delta_rule_backward',
+              _rule(q, k, v, decay, beta, state, resets, scale, checkpoints=checkpoints if checkpoints.numel() else None,
+                    d_output=d_output, d_last=d_last, gradients=(*dense, d_state), workspace=workspace), v.device)
     return (*dense, d_state)
 
 
 def _rule_step(q, k, v, decay, beta, state, resets, scale):
     batch, heads, value_size = v.shape
-    output = torch.empty((batch, heads, value_size), dtype=v.dtype, device=v.device)
+    output = v.new_empty((batch, heads, value_size))
     if batch:
         sb = resets.stride(0) if resets is not None else 0
         qb, qh = q.stride()[:2]
@@ -260,13 +270,20 @@ def _norm(x, groups, weight, bias, epsilon, activation, y=None, stats=None, work
                       _pointer(dy), _pointer(dx), _pointer(d_weight), _pointer(d_bias))
 
 
+@functools.lru_cache(maxsize=256)
+def _norm_bytes(kind, batch, pixels, channels, groups) -> int:
+    """Bytes of workspace of a pass over maps of these sizes."""
+    return _library().cuju_group_norm_workspace(_NORM.pack(kind, batch, pixels, channels, groups, 0, 0.0, *[0] * 10))
+
+
 def _norm_workspace(x, groups):
-    size = load().cuju_group_norm_workspace(_norm(x, groups, None, None, 0.0, 0))
-    return torch.empty(size, dtype=torch.uint8, device=x.device)
+    batch, channels = x.shape[0], x.shape[-1]
+    return torch.empty(_norm_bytes(TYPES[x.dtype], batch, x.numel() // (batch * channels), channels, groups),
+                       dtype=torch.uint8, device=x.device)
 
 
 def _norm_forward(x, weight, bias, groups, epsilon, activation):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
     if x.numel():
         workspace = _norm_workspace(x, groups)
@@ -275,14 +292,15 @@ def _norm_forward(x, weight, bias, groups, epsilon, activation):
 
 
 def _norm_backward(x, weight, bias, stats, dy, groups, epsilon, activation):
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    d_weight, d_bias = (torch.empty(x.shape[-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    dx = torch.empty_like(x)
+    d_weight, d_bias = torch.empty((2, x.shape[-1]), dtype=torch.float32, device=x.device).unbind()
     if x.numel():
         workspace = _norm_workspace(x, groups)
         _call('cuju_group_norm_backward',
               _norm(x, groups, weight, bias, epsilon, activation, None, stats, workspace, dy, dx, d_weight, d_bias), x.device)
     else:
-        d_weight.zero_(), d_bias.zero_()
+        d_weight.zero_()
+        d_bias.zero_()
     return dx, d_weight, d_bias
 
 

@@ -23,27 +23,30 @@ __global__ __launch_bounds__(256) void StepKernel(Rule rule, View<const T> query
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const unsigned id = blockIdx.x * 4 + wave;
     float *keys = sharedKeys[wave][0], *queries = sharedKeys[wave][1];
-    const bool real = id < waves;
-    const unsigned slice = real ? id % slices : 0, head = real ? id / slices : 0;
+    if (id >= waves) return;
+    const unsigned slice = id % slices, head = id / slices;
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
     const int dk = rule.key_size, dv = rule.value_size;
-#pragma unroll
-    for (int i = lane; i < Keys; i += 64) {
-        keys[i] = i < dk ? Float(key.At(b, 0, kh)[i]) : 0.f;
-        queries[i] = i < dk ? Float(query.At(b, 0, kh)[i]) : 0.f;
-    }
-    __syncthreads();
-    if (!real) return;
+    // All loads start before the first is waited for. A memory that is cleared is loaded too, and
+    // dropped: what it held, infinities among it, is gone.
     const StepGates gate = LoadGates(gates, b, 0, 1, h);
     const int first = slice * columns + (lane % Lanes) * 4, row0 = (lane / Lanes) * kRows;
     const int valid = min(columns - (lane % Lanes) * 4, dv - first);
     float *at = memory + ((long long)head * dk + row0) * dv + first;
     Pack<float, 4> s[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; i++) s[i] = Load<4, Whole>(at + i * dv, row0 + i < dk ? valid : 0);
+    const auto v = Load<4, Whole>(value.At(b, 0, h) + first, valid);
+    const T *key0 = key.At(b, 0, kh), *query0 = query.At(b, 0, kh);
+#pragma unroll
+    for (int i = lane; i < Keys; i += 64) {
+        keys[i] = i < dk ? Float(key0[i]) : 0.f;
+        queries[i] = i < dk ? Float(query0[i]) : 0.f;
+    }
+    // Only this wavefront reads them, and its LDS accesses keep their order.
+    Forget();
     const bool cleared = gate.Reset();
     const float kept = cleared ? 0.f : expf(gate.decay);
-    // A memory that is cleared is not read: what it held, infinities among it, is gone.
-#pragma unroll
-    for (int i = 0; i < kRows; i++) s[i] = Load<4, Whole>(at + i * dv, !cleared && row0 + i < dk ? valid : 0);
     float seen[4] = {0, 0, 0, 0}, out[4] = {0, 0, 0, 0}, both = 0;
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -51,7 +54,7 @@ __global__ __launch_bounds__(256) void StepKernel(Rule rule, View<const T> query
         both = fmaf(k, q, both);
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            s[i].x[c] *= kept;
+            s[i].x[c] = cleared ? 0.f : s[i].x[c] * kept;
             seen[c] = fmaf(k, s[i].x[c], seen[c]);
             out[c] = fmaf(q, s[i].x[c], out[c]);
         }
@@ -65,7 +68,6 @@ __global__ __launch_bounds__(256) void StepKernel(Rule rule, View<const T> query
             out[c] += __shfl_xor(out[c], d);
         }
     }
-    const auto v = Load<4, Whole>(value.At(b, 0, h) + first, valid);
     Pack<T, 4> o;
 #pragma unroll
     for (int c = 0; c < 4; c++) {

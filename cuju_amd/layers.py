@@ -347,9 +347,9 @@ def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='n
             _shape(name, each, (channels,))
             if not each.is_floating_point():
                 raise ArgumentError(f'expected {name} of a floating type, found {each.dtype}')
-    if x.numel() // (x.shape[0] or 1) >= 1 << 31 or x.shape[0] * groups >= 1 << 22:
-        raise ArgumentError(f'expected fewer than 2^22 groups in the batch and 2^31 values in a map, found the shape '
-                            f'{tuple(x.shape)}')
+    if x.numel() // (x.shape[0] or 1) >= 1 << 31 or x.shape[0] * groups >= 1 << 22 or x.shape[0] * channels >= 1 << 30:
+        raise ArgumentError(f'expected fewer than 2^22 groups and 2^30 channels in the batch and 2^31 values in a map, '
+                            f'found the shape {tuple(x.shape)} in {groups} groups')
     x = x.contiguous()
     weight = weight.float().contiguous() if weight is not None else None
     bias = bias.float().contiguous() if bias is not None else None

@@ -170,33 +170,67 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
     Pack<T, Tiles> nextV[4];
     StepGates next;
     const bool full = Whole && dk == 16 * KeyTiles && dv % (16 * Tiles) == 0;
+    // Where the lane reads and writes next: pointers that move on by a chunk, since a lone wavefront's
+    // time is its number of instructions.
+    const long long ahead = kChunk;
+    const T *atK = key.At(b, m, kh) + 4 * g, *atQ = query.At(b, m, kh) + 4 * g, *atV = value.At(b, 4 * g, h) + column;
+    const float *atDecay = gates.decay + b * gates.decayStrides[0] + m * gates.decayStrides[1] + h * gates.decayStrides[2];
+    const float *atBeta = gates.beta + b * gates.betaStrides[0] + m * gates.betaStrides[1] + h * gates.betaStrides[2];
+    T *atOut = static_cast<T *>(rule.output) + (((long long)b * time + 4 * g) * rule.heads + h) * dv + column;
+    const unsigned char *atReset = gates.resets ? gates.resets + b * gates.resetStrides[0] + m * gates.resetStrides[1] : nullptr;
     const auto fetch = [&](int t0) {
-        const int t = min(t0 + m, time - 1);
-        const T *k = key.At(b, t, kh) + 4 * g, *q = query.At(b, t, kh) + 4 * g;
-        const auto v = [&](int r) { return value.At(b, min(t0 + 4 * g + r, time - 1), h) + column; };
-        if (full) {
+        const int left = time - t0;  // steps that are left
+        if (full && left >= kChunk) {
 #pragma unroll
             for (int i = 0; i < KeyTiles; i++) {
-                nextK[i] = *reinterpret_cast<const Pack<T, 4> *>(k + 16 * i);
-                nextQ[i] = *reinterpret_cast<const Pack<T, 4> *>(q + 16 * i);
+                nextK[i] = *reinterpret_cast<const Pack<T, 4> *>(Global(atK) + 16 * i);
+                nextQ[i] = *reinterpret_cast<const Pack<T, 4> *>(Global(atQ) + 16 * i);
             }
+            const T *v = atV;
 #pragma unroll
-            for (int r = 0; r < 4; r++) nextV[r] = *reinterpret_cast<const Pack<T, Tiles> *>(v(r));
+            for (int r = 0; r < 4; r++, v += value.time) nextV[r] = *reinterpret_cast<const Pack<T, Tiles> *>(Global(v));
+            next.decay = *Global(atDecay), next.beta = *Global(atBeta);
+            next.cleared = gates.resets ? *Global(atReset) : 0;
         } else {
-            const int sizes = Opaque(dk) - 4 * g;
+            const int sizes = Opaque(dk) - 4 * g, back = min(0, left - 1 - m);
+            const T *k = Global(atK) + back * key.time, *q = Global(atQ) + back * query.time;
 #pragma unroll
             for (int i = 0; i < KeyTiles; i++) {
                 nextK[i] = Load<4, Whole>(k + 16 * i, sizes - 16 * i);
                 nextQ[i] = Load<4, Whole>(q + 16 * i, sizes - 16 * i);
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) nextV[r] = Load<Tiles, Whole>(v(r), columns);
+            for (int r = 0; r < 4; r++)
+                nextV[r] = Load<Tiles, Whole>(Global(atV) + min(r, left - 1 - 4 * g) * value.time, columns);
+            next = LoadGates(gates, b, t0 + m, time, h);
         }
-        next = LoadGates(gates, b, t0 + m, time, h);
+    };
+    const auto advance = [&] {
+        atK += ahead * key.time, atQ += ahead * query.time, atV += ahead * value.time;
+        atDecay += ahead * gates.decayStrides[1], atBeta += ahead * gates.betaStrides[1];
+        if (gates.resets) atReset += ahead * gates.resetStrides[1];
     };
 
     constexpr int P = kPieces<T>;
     const Eyes eyes = EyesOf(m, g);
+
+    // A part's outputs leave with the next part's loads: the wait for loads, which are answered in the order in
+    // which loads and stores were sent, then finds them gone.
+    Pack<T, Tiles> done[4];
+    int doneLow = 0, doneHigh = 0;
+    const auto put = [&] {
+        T *out = Global(atOut);
+        const int stride = rule.heads * dv;
+        if (full && doneHigh - doneLow == kChunk) {
+#pragma unroll
+            for (int r = 0; r < 4; r++, out += stride) *reinterpret_cast<Pack<T, Tiles> *>(out) = done[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++, out += stride)
+                Store<Tiles, Whole>(out, done[r], 4 * g + r >= doneLow && 4 * g + r < doneHigh ? columns : 0);
+        }
+        if (doneHigh == kChunk) atOut += ahead * stride;
+    };
 
     if (time > 0) fetch(0);
     for (int t0 = 0, low = 0, high; t0 < time; low = high) {
@@ -229,8 +263,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
             for (int r = 0; r < 4; r++)
                 if (4 * g + r < low || 4 * g + r >= high) v[r] = Pack<T, Tiles>{};
         }
-        const int here = t0;
-        if (high == count) t0 += kChunk, high = 0;
+        put();
+        const int end = high;
+        if (high == count) t0 += kChunk, high = 0, advance();
         if (t0 < time) fetch(t0);
 
         __syncthreads();
@@ -289,18 +324,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
             u[c] = Product(aT, u[c]);
             o[c] = Product(aP, u[c], o[c]);
         }
-        T *out = static_cast<T *>(rule.output) + (((long long)b * time + here + 4 * g) * rule.heads + h) * dv + column;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            Pack<T, Tiles> x;
 #pragma unroll
-            for (int c = 0; c < Tiles; c++) x.x[c] = As<T>(o[c][r]);
-            const bool in = 4 * g + r >= low && 4 * g + r < (high ? high : count);
-            Store<Tiles, Whole>(out + (long long)r * rule.heads * dv, x, in ? columns : 0);
+            for (int c = 0; c < Tiles; c++) done[r].x[c] = As<T>(o[c][r]);
             const float after = Exp2(last - Gj[r]);
 #pragma unroll
             for (int c = 0; c < Tiles; c++) u[c][r] *= after;
         }
+        doneLow = low, doneHigh = end;
         const float kept = Exp2(last);
         Four up[Tiles][kFloatPieces];
 #pragma unroll
@@ -310,6 +342,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
 #pragma unroll
             for (int c = 0; c < Tiles; c++) s[t][c] = Mfma16(turned[t], up[c], s[t][c] * kept);
     }
+    put();
     if (rule.last) keep(rule.last, head);
 }
 

@@ -17,8 +17,8 @@
 namespace layers {
 namespace {
 
-// One workgroup takes 64 columns of a head backwards through its steps, 32 at a time: two tiles of
-// steps, from the memory that the forward pass kept before them. A wavefront holds 16 columns of the
+// One workgroup takes a head, or a part of its columns, backwards through its steps, 32 at a time: two
+// tiles of steps, from the memory that the forward pass kept before them. A wavefront holds 16 columns of the
 // memory and of its gradient. The steps' inputs lie in LDS while the next ones are on their way to
 // registers. Between barriers,
 //  - the triangular matrices of the tiles (11, 22) and between them (21), a block to a wavefront;
@@ -39,9 +39,9 @@ struct BackwardArgs {
     bool parted;  // whether dQuery and dKey are parts
 };
 
-constexpr int kSlice = 64;                       // columns of a workgroup
 constexpr int kMatrix = kChunk * kChunk;         // a 16x16 matrix in LDS
 constexpr int kPieceMatrix = kFloatPieces * kMatrix / 2;  // its pieces
+constexpr int kBlock = 2 * kMatrix;  // a block's matrices P and K K^T; the pieces of N take their place
 enum Block { kFirst, kSecond, kAcross };         // of two tiles of steps: 11, 22 and 21
 
 // LDS for keys of up to `KeyTiles` tiles and `Waves` wavefronts of 16 columns, in floats.
@@ -54,8 +54,8 @@ struct BackwardShared {
     static constexpr int kKeyRows = kSegment * kKeyRow * ElementSize / 4, kValueRows = kSegment * kValueRow * ElementSize / 4;
     static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kWhole = kBetas + kSegment, kAfter = kWhole + kSegment,
                          kCuts = kAfter + kSegment, kInverse = kCuts + 4, kMixed = kInverse + 2 * kMatrix,
-                         kProducts = kMixed + 3 * kMatrix, kM = kProducts + 3 * kMatrix, kN = kM + 3 * kPieceMatrix,
-                         kSums = kN + 3 * kPieceMatrix, kDots = kSums + 8 * kChunk, kU = kDots + Waves * 4 * kSegment,
+                         kProducts = kMixed + kMatrix, kM = kMixed + 3 * kBlock, kSums = kM + 3 * kPieceMatrix,
+                         kDots = kSums + 8 * kChunk, kU = kDots + Waves * 4 * kSegment,
                          kB = kU + kPieceRows, kK = kB + kPieceRows, kQ = kK + kKeyRows, kO = kQ + kKeyRows,
                          kMemory = kO + kValueRows, kFloats = kMemory + KeyTiles * 16 * kMemoryRow;
 };
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
     unsigned *cutsOf = reinterpret_cast<unsigned *>(shared + At::kCuts);
     // Rows of values by step, [piece][step][column].
     uint16_t *sharedU = reinterpret_cast<uint16_t *>(shared + At::kU), *sharedB = reinterpret_cast<uint16_t *>(shared + At::kB);
-    uint16_t *sharedM = reinterpret_cast<uint16_t *>(shared + At::kM), *sharedN = reinterpret_cast<uint16_t *>(shared + At::kN);
+    uint16_t *sharedM = reinterpret_cast<uint16_t *>(shared + At::kM), *sharedN = reinterpret_cast<uint16_t *>(shared + At::kMixed);
     T *keys = reinterpret_cast<T *>(shared + At::kK), *queries = reinterpret_cast<T *>(shared + At::kQ);
     T *outputs = reinterpret_cast<T *>(shared + At::kO);
 
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
     const unsigned slice = id % a.slices, head = id / a.slices;
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
     const int dk = rule.key_size, dv = rule.value_size, time = rule.time;
-    const int base = slice * kSlice;
+    const int base = slice * 16 * Waves;
     int column = base + 16 * wave + m;  // a lane's column in column order
     int column4 = 16 * wave + 4 * g;    // its first of four in row order, within the slice
     const int segments = (time + kSegment - 1) / kSegment;
@@ -247,8 +247,8 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                     dA[r] = m < j ? betaj * d * kk[r] : 0.f;
                 }
                 const int to = m * kChunk + 4 * g;
-                *reinterpret_cast<F4 *>(shared + At::kMixed + block * kMatrix + to) = aP;
-                *reinterpret_cast<F4 *>(shared + At::kProducts + block * kMatrix + to) = aKK;
+                *reinterpret_cast<F4 *>(shared + At::kMixed + block * kBlock + to) = aP;
+                *reinterpret_cast<F4 *>(shared + At::kProducts + block * kBlock + to) = aKK;
                 if (block != kAcross)
                     *reinterpret_cast<F4 *>(shared + At::kInverse + block * kMatrix + to) = UnitLowerInverse<false>(aA, dA, m, g).rows;
             }
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                     U[tile] = beta * error[tile];
                 }
                 U[0] = Product(RowOrder(shared + At::kInverse + kFirst * kMatrix, m, g), U[0]);
-                F4 aA = RowOrder(shared + At::kProducts + kAcross * kMatrix, m, g);
+                F4 aA = RowOrder(shared + At::kProducts + kAcross * kBlock, m, g);
                 aA *= -betas[kChunk + m];
                 U[1] = Product(RowOrder(shared + At::kInverse + kSecond * kMatrix, m, g), Product(aA, U[0], U[1]));
             }
@@ -307,12 +307,12 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                 }
                 dU[0] *= *reinterpret_cast<const F4 *>(afters + 4 * g);
                 dU[1] *= *reinterpret_cast<const F4 *>(afters + kChunk + 4 * g);
-                const auto mixed = [&](int block) { return ColumnOrder(shared + At::kMixed + block * kMatrix, m, g); };
+                const auto mixed = [&](int block) { return ColumnOrder(shared + At::kMixed + block * kBlock, m, g); };
                 dU[1] = Product(mixed(kSecond), dO[1], dU[1]);
                 dB[1] = Product(ColumnOrder(shared + At::kInverse + kSecond * kMatrix, m, g), dU[1]);
                 dU[0] = Product(mixed(kFirst), dO[0], dU[0]);
                 dU[0] = Product(mixed(kAcross), dO[1], dU[0]);
-                const F4 dA = ColumnOrder(shared + At::kProducts + kAcross * kMatrix, m, g);
+                const F4 dA = ColumnOrder(shared + At::kProducts + kAcross * kBlock, m, g);
                 dU[0] = Product(dA * -*reinterpret_cast<const F4 *>(betas + kChunk + 4 * g), dB[1], dU[0]);
                 dB[0] = Product(ColumnOrder(shared + At::kInverse + kFirst * kMatrix, m, g), dU[0]);
             }
@@ -383,18 +383,20 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                 const float *from = memory + (16 * t + m) * ms + 32 * x + 4 * g;
                 Pair(*reinterpret_cast<const F4 *>(from), *reinterpret_cast<const F4 *>(from + 16), to);
             };
-            const auto putPieces = [&](uint16_t *pieces, int block, F4 x) {
+            const auto putPieces = [&](uint16_t *pieces, F4 x) {
                 Four p[kFloatPieces];
                 Split(x, p);
 #pragma unroll
                 for (int i = 0; i < kFloatPieces; i++)
-                    *reinterpret_cast<Four *>(pieces + (block * kFloatPieces + i) * kMatrix + m * kChunk + 4 * g) = p[i];
+                    *reinterpret_cast<Four *>(pieces + i * kMatrix + m * kChunk + 4 * g) = p[i];
             };
-            const auto getPieces = [&](const uint16_t *pieces, int block, Four(&p)[kFloatPieces]) {
+            const auto getPieces = [&](const uint16_t *pieces, Four(&p)[kFloatPieces]) {
 #pragma unroll
                 for (int i = 0; i < kFloatPieces; i++)
-                    p[i] = *reinterpret_cast<const Four *>(pieces + (block * kFloatPieces + i) * kMatrix + m * kChunk + 4 * g);
+                    p[i] = *reinterpret_cast<const Four *>(pieces + i * kMatrix + m * kChunk + 4 * g);
             };
+            const auto getM = [&](int block, Four(&p)[kFloatPieces]) { getPieces(sharedM + block * 2 * kPieceMatrix, p); };
+            const auto getN = [&](int block, Four(&p)[kFloatPieces]) { getPieces(sharedN + block * 2 * kBlock, p); };
             // ---- The matrices' gradients.
 #pragma unroll 1
             for (int block = wave; block < 3; block += Waves) {
@@ -407,8 +409,8 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                     gP = Mfma32<kFloatPieces, P>(uw, out, gP);
                     gA = Mfma32<kFloatPieces, kFloatPieces>(uw, bw, gA);
                 }
-                const F4 aP = RowOrder(shared + At::kMixed + block * kMatrix, m, g);
-                const F4 aKK = RowOrder(shared + At::kProducts + block * kMatrix, m, g);
+                const F4 aP = RowOrder(shared + At::kMixed + block * kBlock, m, g);
+                const F4 aKK = RowOrder(shared + At::kProducts + block * kBlock, m, g);
                 const float beta = betas[kChunk * row + m];
                 const double Gi = row ? G[1] : G[0];
                 F4 M, N, E;
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                     betaSum += part;
                     E[r] = (both ? gP[r] * aP[r] : 0.f) + beta * part;
                 }
-                putPieces(sharedM, block, M);
+                putPieces(sharedM + block * 2 * kPieceMatrix, M);
                 if (block != kAcross) {
                     Four lo[kFloatPieces];
                     B8 x[kFloatPieces];
@@ -432,7 +434,8 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                     Eights<kFloatPieces>(lo, lo, x);
                     N += Turn<kFloatPieces>(x, eyes.half[0]);
                 }
-                putPieces(sharedN, block, N);
+                Forget();
+                putPieces(sharedN + block * 2 * kBlock, N);
                 betaSum += __shfl_xor(betaSum, 16);
                 betaSum += __shfl_xor(betaSum, 32);
                 if (g == 0) sums[block * kChunk + m] = betaSum;
@@ -574,7 +577,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                 Four m11[kFloatPieces], m21[kFloatPieces], m22[kFloatPieces];
                 Four lo[kFloatPieces], hi[kFloatPieces];
                 B8 wide[kFloatPieces], turn[kFloatPieces];
-                getPieces(sharedM, kFirst, m11), getPieces(sharedM, kAcross, m21), getPieces(sharedM, kSecond, m22);
+                getM(kFirst, m11), getM(kAcross, m21), getM(kSecond, m22);
                 dQ[0] = Mfma16(m11, k[0], dQ[0]);
                 Eights<kFloatPieces>(m21, m22, wide);
                 dQ[1] = Mfma32<kFloatPieces, P>(wide, kAll, dQ[1]);
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
                 Eights<kFloatPieces>(m22, m22, turn);
                 Turn<kFloatPieces>(turn, eyes.half[0], lo);
                 dK[1] = Mfma16(lo, q[1], dK[1]);
-                getPieces(sharedN, kFirst, m11), getPieces(sharedN, kAcross, m21), getPieces(sharedN, kSecond, m22);
+                getN(kFirst, m11), getN(kAcross, m21), getN(kSecond, m22);
                 Eights<kFloatPieces>(m21, m22, wide);
                 dK[1] = Mfma32<kFloatPieces, P>(wide, kAll, dK[1]);
                 Eights<kFloatPieces>(m21, m21, turn);
@@ -688,7 +691,18 @@ void LaunchParts(const float *parts, void *out, int group, int size, long long r
     hipLaunchKernelGGL(PartsKernel<T>, dim3(blocks), dim3(256), 0, stream, parts, static_cast<T *>(out), group, size, count);
 }
 
-int SlicesOf(const Rule &r) { return (r.value_size + kSlice - 1) / kSlice; }
+// Wavefronts of a workgroup, 16 columns each: all of a head's columns, where LDS holds them. Wide workgroups
+// find the triangular matrices once and leave no parts to add up: 2,048 heads of 64 steps take, with all 128
+// columns against 64 and 64, 400 us against 788 (bfloat16, keys of 128), 302 against 324 (keys of 64), 391
+// against 667 (float32), and with 96 columns 279 against 319. Sixteen heads of 256 steps, which leave most of
+// the chip idle either way, take 170 us against 166. Floats with keys over 96 do not fit.
+int WavesOf(const Rule &r) {
+    if (r.value_size <= 32) return 2;
+    if (r.value_size <= 64) return 4;
+    if (r.value_size <= 96) return 6;
+    return r.type == 0 && r.key_size > 96 ? 4 : 8;
+}
+int SlicesOf(const Rule &r) { return (r.value_size + 16 * WavesOf(r) - 1) / (16 * WavesOf(r)); }
 // Floats of the parts of the keys' and queries' gradients, and of the gates'; 0 where there are none.
 long long KeyParts(const Rule &r) {
     const bool parted = r.heads * SlicesOf(r) != r.key_heads;
@@ -725,10 +739,15 @@ bool LaunchBackward(const Rule &r, hipStream_t stream) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads * slices)), dim3(64 * Waves), bytes, stream, a);
         return true;
     };
-    bool set;
-    if (!whole) set = launch(std::integral_constant<int, 4>(), std::false_type());
-    else if (r.value_size <= 32) set = launch(std::integral_constant<int, 2>(), std::true_type());
-    else set = launch(std::integral_constant<int, 4>(), std::true_type());
+    const auto width = [&](auto packed) {
+        switch (WavesOf(r)) {
+            case 2: return launch(std::integral_constant<int, 2>(), packed);
+            case 4: return launch(std::integral_constant<int, 4>(), packed);
+            case 6: return launch(std::integral_constant<int, 6>(), packed);
+            default: return launch(std::integral_constant<int, (sizeof(T) == 4 && KeyTiles > 6 ? 4 : 8)>(), packed);
+        }
+    };
+    const bool set = whole ? width(std::true_type()) : width(std::false_type());
     if (!set) return false;
     if (keyParts) {
         const int group = r.heads / r.key_heads * slices;

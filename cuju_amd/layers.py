@@ -47,11 +47,13 @@ def _library():
 
 def _call(function, packed: bytes, device: torch.device) -> None:
     lib = _library()
+    # The handle alone: a Stream object around it would be a tenth of a small call's time.
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if device.index == torch.cuda.current_device():
-        status = getattr(lib, function)(packed, torch.cuda.current_stream(device).cuda_stream)
+        status = getattr(lib, function)(packed, stream)
     else:
         with torch.cuda.device(device):
-            status = getattr(lib, function)(packed, torch.cuda.current_stream(device).cuda_stream)
+            status = getattr(lib, function)(packed, stream)
     if status != 0:
         raise from_library(lib.cuju_last_error().decode())
 
@@ -61,13 +63,20 @@ def _shape(name: str, tensor: torch.Tensor, shape: tuple) -> None:
         raise ArgumentError(f'expected {name} of the shape {shape}, found {tuple(tensor.shape)}')
 
 
-def _device(first: str, tensor: torch.Tensor, others: dict) -> None:
+def _device(first: str, tensor: torch.Tensor, names: tuple, others: tuple) -> None:
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ArgumentError(f'expected {first} on a HIP device')
     device = tensor.device
-    for name, other in others.items():
+    for name, other in zip(names, others):
         if other is not None and (not isinstance(other, torch.Tensor) or other.device != device):
             raise ArgumentError(f'expected {name} on the device of {first}')
+
+
+def _gate(name: str, tensor: torch.Tensor) -> torch.Tensor:
+    """`tensor`, of a floating type, in 32 bits."""
+    if not tensor.is_floating_point():
+        raise ArgumentError(f'expected {name} of a floating type, found {tensor.dtype}')
+    return tensor.float()
 
 
 def _flat(tensor: torch.Tensor) -> torch.Tensor:
@@ -99,44 +108,46 @@ def _rule_workspace(kind, batch, time, key_heads, key_size, heads, value_size) -
         _RULE.pack(kind, batch, time, key_heads, heads, key_size, value_size, 0.0, *[0] * 39))
 
 
+_OTHERS = 'key', 'value', 'decay', 'beta', 'state', 'resets'
+
+
 def _check_rule(query, key, value, decay, beta, state, resets, steps):
     """The checked arguments as the kernels take them; `steps`: whether they have a time axis."""
     axes = 4 if steps else 3
-    _device('query', query, {'key': key, 'value': value, 'decay': decay, 'beta': beta, 'state': state, 'resets': resets})
-    if query.dtype not in TYPES:
-        raise ArgumentError(f'expected query of float32, bfloat16 or float16, found {query.dtype}')
-    if key.dtype != query.dtype or value.dtype != query.dtype:
-        raise ArgumentError(f'expected key and value of {query.dtype}, found {key.dtype} and {value.dtype}')
+    _device('query', query, _OTHERS, (key, value, decay, beta, state, resets))
+    dtype = query.dtype
+    if dtype not in TYPES:
+        raise ArgumentError(f'expected query of float32, bfloat16 or float16, found {dtype}')
+    if key.dtype != dtype or value.dtype != dtype:
+        raise ArgumentError(f'expected key and value of {dtype}, found {key.dtype} and {value.dtype}')
     if query.dim() != axes or value.dim() != axes:
         raise ArgumentError(f'expected query and value of {axes} axes, found {query.dim()} and {value.dim()}')
-    lead = query.shape[:axes - 2]
-    key_heads, key_size = query.shape[-2:]
+    shape = query.shape
+    *lead, key_heads, key_size = shape
     heads, value_size = value.shape[-2:]
-    _shape('key', key, query.shape)
+    _shape('key', key, shape)
     _shape('value', value, (*lead, heads, value_size))
-    _shape('decay', decay, (*lead, heads))
-    _shape('beta', beta, (*lead, heads))
+    gates = (*lead, heads)
+    _shape('decay', decay, gates)
+    _shape('beta', beta, gates)
     if key_heads < 1 or heads < 1 or heads % key_heads:
         raise ArgumentError(f'expected heads that are a multiple of the {key_heads} key heads, found {heads}')
     if not 1 <= key_size <= MOST_SIZE or not 1 <= value_size <= MOST_SIZE:
         raise ArgumentError(f'expected key and value sizes from 1 to {MOST_SIZE}, found {key_size} and {value_size}')
     if lead[0] * heads > MOST_HEADS:
         raise ArgumentError(f'expected at most {MOST_HEADS} heads in the batch, found {lead[0] * heads}')
-    for name, gate in (('decay', decay), ('beta', beta)):
-        if not gate.is_floating_point():
-            raise ArgumentError(f'expected {name} of a floating type, found {gate.dtype}')
+    if decay.dtype != torch.float32:
+        decay = _gate('decay', decay)
+    if beta.dtype != torch.float32:
+        beta = _gate('beta', beta)
     if state is not None:
         _shape('state', state, (lead[0], heads, key_size, value_size))
     if resets is not None:
-        _shape('resets', resets, lead)
+        _shape('resets', resets, tuple(lead))
         if resets.dtype == torch.bool:
             resets = resets.view(torch.uint8)
         elif resets.dtype != torch.uint8:
             raise ArgumentError(f'expected resets of bool or uint8, found {resets.dtype}')
-    if decay.dtype != torch.float32:
-        decay = decay.float()
-    if beta.dtype != torch.float32:
-        beta = beta.float()
     return _flat(query), _flat(key), _flat(value), decay, beta, resets
 
 
@@ -249,7 +260,8 @@ def delta_rule_step(query, key, value, decay, beta, state, *, resets=None, scale
     q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, False)
     if state is None or state.dtype != torch.float32 or not state.is_contiguous():
         raise ArgumentError('expected state as a contiguous float32 tensor, which the step updates')
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, decay, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or decay.requires_grad or
+                                    beta.requires_grad or state.requires_grad):
         raise ArgumentError('delta_rule_step has no gradients: call it under torch.no_grad(), or call delta_rule')
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if torch.compiler.is_compiling():
@@ -332,7 +344,7 @@ def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='n
     memory format is such a map as `x.permute(0, 2, 3, 1)`, without a copy. Gradients reach `x`,
     `weight` and `bias`; they are the same on every call.
     """
-    _device('x', x, {'weight': weight, 'bias': bias})
+    _device('x', x, ('weight', 'bias'), (weight, bias))
     if x.dtype not in TYPES:
         raise ArgumentError(f'expected x of float32, bfloat16 or float16, found {x.dtype}')
     if x.dim() < 2 or x.shape[-1] < 1:

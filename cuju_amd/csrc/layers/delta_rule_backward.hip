@@ -254,67 +254,52 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyT
             }
             __syncthreads();
 
-            // ---- By columns. First U, what the steps wrote, and its errors, from the memory before.
+            // ---- By columns: U, what the steps wrote, with its errors, from the memory before, and dU and dB from
+            // the gradient of the memory after. The two chains of products go side by side.
             F4 U[2], error[2], dO[2], dB[2], wrong[2];
             {
-                F4 seen[2];
-                seen[0] = seen[1] = F4{0, 0, 0, 0};
-                if (!starts) {
+                F4 seen[2], dU[2];
+                seen[0] = seen[1] = dU[0] = dU[1] = F4{0, 0, 0, 0};
 #pragma unroll
-                    for (int p = 0; p < KeyTiles / 2; p++) {
-                        B8 sp[kFloatPieces];
+                for (int p = 0; p < KeyTiles / 2; p++) {
+                    B8 kp[2][P], sp[kFloatPieces];
+                    keyPair(keys, 0, p, kp[0]), keyPair(keys, 1, p, kp[1]);
+                    if (!starts) {
                         Pair(start[2 * p], start[2 * p + 1], sp);
-#pragma unroll
-                        for (int tile = 0; tile < 2; tile++) {
-                            B8 kp[P];
-                            keyPair(keys, tile, p, kp);
-                            seen[tile] = Mfma32<P, kFloatPieces>(kp, sp, seen[tile]);
-                        }
+                        seen[0] = Mfma32<P, kFloatPieces>(kp[0], sp, seen[0]);
+                        seen[1] = Mfma32<P, kFloatPieces>(kp[1], sp, seen[1]);
                     }
+                    Pair(dS[2 * p], dS[2 * p + 1], sp);
+                    dU[0] = Mfma32<P, kFloatPieces>(kp[0], sp, dU[0]);
+                    dU[1] = Mfma32<P, kFloatPieces>(kp[1], sp, dU[1]);
                 }
                 B8 v[P], o[P];
                 Pair<T>(Masked(values[0], mine(0)), Masked(values[1], mine(1)), v);
                 Pair<T>(valueTile(outputs, 0, wave), valueTile(outputs, 1, wave), o);
+                F4 beta[2];
 #pragma unroll
                 for (int tile = 0; tile < 2; tile++) {
                     const F4 value = Turn<P>(v, eyes.half[tile]);
                     dO[tile] = Turn<P>(o, eyes.half[tile]);
                     const F4 whole = *reinterpret_cast<const F4 *>(wholes + kChunk * tile + 4 * g);
-                    const F4 beta = *reinterpret_cast<const F4 *>(betas + kChunk * tile + 4 * g);
+                    beta[tile] = *reinterpret_cast<const F4 *>(betas + kChunk * tile + 4 * g);
 #pragma unroll
                     for (int r = 0; r < 4; r++) error[tile][r] = fmaf(-whole[r], seen[tile][r], value[r]);
-                    U[tile] = beta * error[tile];
+                    U[tile] = beta[tile] * error[tile];
+                    dU[tile] *= *reinterpret_cast<const F4 *>(afters + kChunk * tile + 4 * g);
                 }
-                U[0] = Product(RowOrder(shared + At::kInverse + kFirst * kMatrix, m, g), U[0]);
-                F4 aA = RowOrder(shared + At::kProducts + kAcross * kBlock, m, g);
-                aA *= -betas[kChunk + m];
-                U[1] = Product(RowOrder(shared + At::kInverse + kSecond * kMatrix, m, g), Product(aA, U[0], U[1]));
-            }
-            // Then dU and dB, from the gradient of the memory after.
-            {
-                F4 dU[2];
-                dU[0] = dU[1] = F4{0, 0, 0, 0};
-#pragma unroll
-                for (int p = 0; p < KeyTiles / 2; p++) {
-                    B8 sp[kFloatPieces];
-                    Pair(dS[2 * p], dS[2 * p + 1], sp);
-#pragma unroll
-                    for (int tile = 0; tile < 2; tile++) {
-                        B8 kp[P];
-                        keyPair(keys, tile, p, kp);
-                        dU[tile] = Mfma32<P, kFloatPieces>(kp, sp, dU[tile]);
-                    }
-                }
-                dU[0] *= *reinterpret_cast<const F4 *>(afters + 4 * g);
-                dU[1] *= *reinterpret_cast<const F4 *>(afters + kChunk + 4 * g);
                 const auto mixed = [&](int block) { return ColumnOrder(shared + At::kMixed + block * kBlock, m, g); };
+                const auto inverse = [&](int block) { return shared + At::kInverse + block * kMatrix; };
+                const float *across = shared + At::kProducts + kAcross * kBlock;
                 dU[1] = Product(mixed(kSecond), dO[1], dU[1]);
-                dB[1] = Product(ColumnOrder(shared + At::kInverse + kSecond * kMatrix, m, g), dU[1]);
+                U[0] = Product(RowOrder(inverse(kFirst), m, g), U[0]);
                 dU[0] = Product(mixed(kFirst), dO[0], dU[0]);
+                dB[1] = Product(ColumnOrder(inverse(kSecond), m, g), dU[1]);
+                U[1] = Product(RowOrder(across, m, g) * -betas[kChunk + m], U[0], U[1]);
                 dU[0] = Product(mixed(kAcross), dO[1], dU[0]);
-                const F4 dA = ColumnOrder(shared + At::kProducts + kAcross * kBlock, m, g);
-                dU[0] = Product(dA * -*reinterpret_cast<const F4 *>(betas + kChunk + 4 * g), dB[1], dU[0]);
-                dB[0] = Product(ColumnOrder(shared + At::kInverse + kFirst * kMatrix, m, g), dU[0]);
+                U[1] = Product(RowOrder(inverse(kSecond), m, g), U[1]);
+                dU[0] = Product(ColumnOrder(across, m, g) * -beta[1], dB[1], dU[0]);
+                dB[0] = Product(ColumnOrder(inverse(kFirst), m, g), dU[0]);
             }
             float held = 0;
             if (!starts) {

@@ -192,6 +192,8 @@ inline bool Fits(const Rule *r) {
     if (!r || r->type < 0 || r->type > 2) return Failed("expected a delta rule of the type 0, 1 or 2"), false;
     if (r->batch < 0 || r->time < 0 || r->heads < 1 || r->key_heads < 1 || r->heads % r->key_heads)
         return Failed("expected heads that are a multiple of the key heads"), false;
+    // Steps are counted by ints, and a lane's place among the 32 steps of a segment is 32 bits of bytes.
+    if (r->time >= (1 << 30) || r->heads >= (1 << 16)) return Failed("expected fewer than 2^30 steps and 2^16 heads"), false;
     // A grid has fewer than 2^32 threads: at most 512 a head.
     if (r->batch * (long long)r->heads >= (1ll << 23)) return Failed("expected fewer than 2^23 heads in the batch"), false;
     if (r->key_size < 1 || r->key_size > kMaxKey || r->value_size < 1 || r->value_size > kMaxValue)

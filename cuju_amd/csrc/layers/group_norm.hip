@@ -655,10 +655,12 @@ bool Fits(const Norm *n) {
     if (n->activation < kNone || n->activation > kSilu) return Failed("expected an activation from 0 to 2"), false;
     if (n->batch < 0 || n->pixels < 0 || n->channels < 1 || n->groups < 1 || n->channels % n->groups)
         return Failed("expected channels that are a multiple of the groups"), false;
-    // A grid has fewer than 2^32 threads: at most 512 for each of two slabs of a map, 256 for each slab of
-    // a map that is cut, 64 for each group.
-    if ((long long)n->batch * n->groups >= (1ll << 22) || (long long)n->batch * n->channels >= (1ll << 30))
-        return Failed("expected fewer than 2^22 groups and 2^30 channels in the batch"), false;
+    // Places within a map are ints, and a grid has fewer than 2^32 threads: at most 512 for each of two slabs
+    // of a map, 256 for each slab of a map that is cut, 64 for each group, 128 for each channel.
+    if ((long long)n->pixels * n->channels >= (1ll << 30) || n->channels >= (1 << 24))
+        return Failed("expected fewer than 2^30 values and 2^24 channels in a map"), false;
+    if ((long long)n->batch * n->groups >= (1ll << 22) || (long long)n->batch * n->channels >= (1ll << 29))
+        return Failed("expected fewer than 2^22 groups and 2^29 channels in the batch"), false;
     return true;
 }
 

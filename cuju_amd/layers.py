@@ -25,9 +25,10 @@ from .library import load
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2}
-# Key and value sizes, and heads of a batch, that the delta rule's kernels take.
+# Key and value sizes, heads of a sequence and of a batch, and steps, that the delta rule's kernels take.
 MOST_SIZE = 128
-MOST_HEADS = (1 << 23) - 1
+MOST_HEADS, MOST_HEADS_OF_BATCH = (1 << 16) - 1, (1 << 23) - 1
+MOST_STEPS = (1 << 30) - 1
 # Steps between two memories that the forward pass keeps for the backward pass.
 SEGMENT = 32
 
@@ -134,8 +135,9 @@ def _check_rule(query, key, value, decay, beta, state, resets, steps):
         raise ArgumentError(f'expected heads that are a multiple of the {key_heads} key heads, found {heads}')
     if not 1 <= key_size <= MOST_SIZE or not 1 <= value_size <= MOST_SIZE:
         raise ArgumentError(f'expected key and value sizes from 1 to {MOST_SIZE}, found {key_size} and {value_size}')
-    if lead[0] * heads > MOST_HEADS:
-        raise ArgumentError(f'expected at most {MOST_HEADS} heads in the batch, found {lead[0] * heads}')
+    if heads > MOST_HEADS or lead[0] * heads > MOST_HEADS_OF_BATCH or lead[-1] > MOST_STEPS:
+        raise ArgumentError(f'expected at most {MOST_HEADS} heads, {MOST_HEADS_OF_BATCH} in the batch, and {MOST_STEPS} '
+                            f'steps, found the shape {tuple(value.shape)}')
     if decay.dtype != torch.float32:
         decay = _gate('decay', decay)
     if beta.dtype != torch.float32:
@@ -359,9 +361,12 @@ def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='n
             _shape(name, each, (channels,))
             if not each.is_floating_point():
                 raise ArgumentError(f'expected {name} of a floating type, found {each.dtype}')
-    if x.numel() // (x.shape[0] or 1) >= 1 << 31 or x.shape[0] * groups >= 1 << 22 or x.shape[0] * channels >= 1 << 30:
-        raise ArgumentError(f'expected fewer than 2^22 groups and 2^30 channels in the batch and 2^31 values in a map, '
-                            f'found the shape {tuple(x.shape)} in {groups} groups')
+    batch = x.shape[0]
+    if x.numel() // (batch or 1) >= 1 << 30 or channels >= 1 << 24:
+        raise ArgumentError(f'expected fewer than 2^30 values and 2^24 channels in a map, found the shape {tuple(x.shape)}')
+    if batch * groups >= 1 << 22 or batch * channels >= 1 << 29:
+        raise ArgumentError(f'expected fewer than 2^22 groups and 2^29 channels in the batch, found the shape '
+                            f'{tuple(x.shape)} in {groups} groups')
     x = x.contiguous()
     weight = weight.float().contiguous() if weight is not None else None
     bias = bias.float().contiguous() if bias is not None else None

@@ -64,6 +64,25 @@ def test_the_library_refuses_before_any_launch():
     assert lib.cuju_group_norm_workspace(norm(groups=3)) == 0
 
 
+def test_the_library_refuses_what_its_indexes_do_not_reach():
+    from cuju_amd import library
+    lib = library.load(PRODUCT)
+
+    def rule(batch=1, time=1, heads=1):
+        return layers._RULE.pack(0, batch, time, 1, heads, 8, 8, 1.0, *[0] * 39)
+
+    def norm(batch=1, pixels=1, channels=1, groups=1):
+        return layers._NORM.pack(0, batch, pixels, channels, groups, 0, 1e-5, *[0] * 10)
+
+    for call in (lib.cuju_delta_rule_step, lib.cuju_delta_rule_forward, lib.cuju_delta_rule_backward):
+        for bad in (rule(time=1 << 30), rule(heads=1 << 16), rule(batch=1 << 20, heads=8)):
+            assert call(bad, None) == -1 and b'2^' in lib.cuju_last_error()
+    for call in (lib.cuju_group_norm_forward, lib.cuju_group_norm_backward):
+        for bad in (norm(pixels=1 << 20, channels=1 << 10), norm(channels=1 << 24), norm(batch=1 << 22),
+                    norm(batch=1 << 15, channels=1 << 14)):
+            assert call(bad, None) == -1 and b'2^' in lib.cuju_last_error()
+
+
 def test_tensors_of_another_device_are_refused():
     x = torch.zeros(1, 2, 1, 8)
     gate = torch.zeros(1, 2, 1)

@@ -1,8 +1,8 @@
 """A batched Google Research Football step engine for the AMD Instinct MI355X (gfx950).
 
 `BatchEnvironment` steps many matches in one HIP launch and is bit-identical to the reference
-CPU engine for the same seeds and actions. The native library is built in-tree by
-`python -m cuju_amd.build`.
+CPU engine for the same seeds and actions. `cuju_amd.layers` has the operators of a recurrent policy
+that learns from such a batch. The native library is built in-tree by `python -m cuju_amd.build`.
 """
 
 from .environment import (BatchEnvironment, bundled_assets, bundled_scenarios, episode_pickle, memory_estimate,

@@ -26,8 +26,13 @@ namespace {
 //  - dP and dA, and from them the matrices the keys' and queries' gradients take, a block to a
 //    wavefront; dS U by tiles of keys, whole tiles to a wavefront;
 //  - with the memory in its gradient's place: S0 dO, S0 dB, and the keys' and queries' gradients.
-// Wider values take several workgroups, whose gradients of the keys, queries and gates a second kernel
-// adds up, as it does for heads that share keys.
+// Heads that share keys, or whose columns take several workgroups, leave parts of the gradients of the keys,
+// queries and gates that a second kernel adds up, in their order.
+//
+// 16,384 heads of 64 steps, 64 x 64 in bfloat16, 2.0 GB, take 1,172 us. Registers (215 of 256) and LDS hold
+// it at two wavefronts on a SIMD, vector instructions take 42 % of the cycles, a third of them splits into
+// pieces, and the wavefronts wait 43 % of theirs, for LDS between products that need one another and at the
+// barriers.
 template <class T>
 struct BackwardArgs {
     Rule rule;
@@ -39,10 +44,10 @@ struct BackwardArgs {
     bool parted;  // whether dQuery and dKey are parts
 };
 
-constexpr int kMatrix = kChunk * kChunk;         // a 16x16 matrix in LDS
+constexpr int kMatrix = kChunk * kChunk;                  // a 16x16 matrix in LDS
 constexpr int kPieceMatrix = kFloatPieces * kMatrix / 2;  // its pieces
-constexpr int kBlock = 2 * kMatrix;  // a block's matrices P and K K^T; the pieces of N take their place
-enum Block { kFirst, kSecond, kAcross };         // of two tiles of steps: 11, 22 and 21
+constexpr int kBlock = 2 * kMatrix;                       // a block's P and K K^T, and then the pieces of its N
+enum Block { kFirst, kSecond, kAcross };                  // of two tiles of steps: 11, 22 and 21
 
 // LDS for keys of up to `KeyTiles` tiles and `Waves` wavefronts of 16 columns, in floats.
 template <int KeyTiles, int Waves, int ElementSize>
@@ -70,8 +75,14 @@ __device__ __forceinline__ F4 ColumnOrder(const float *matrix, int m, int g) {
     return x;
 }
 
+// Wavefronts that a SIMD has to hold: two, but one where the registers of two would spill (keys over 64, and
+// floats with more tiles of keys than wavefronts) and the workgroup has no more than a wavefront a SIMD.
+template <class T, int KeyTiles, int Waves>
+constexpr int kWavesPerSimd = KeyTiles > 4 || (sizeof(T) == 4 && Waves < KeyTiles) ? 1 : 2;
+
 template <class T, int KeyTiles, int Waves, bool Whole>
-__global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(KeyTiles > 4 || (sizeof(T) == 4 && Waves < KeyTiles) ? 1 : 2))) void BackwardKernel(BackwardArgs<T> a) {
+__global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, KeyTiles, Waves>))) void BackwardKernel(
+    BackwardArgs<T> a) {
     using At = BackwardShared<KeyTiles, Waves, sizeof(T)>;
     using Args = BackwardArgs<T>;
     extern __shared__ __align__(16) float shared[];

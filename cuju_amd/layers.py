@@ -7,8 +7,9 @@
   mini-maps makes, with gradients.
 
 All run on the current stream of their tensors' device, wait for nothing, and can be captured in a
-HIP graph. Under `torch.compile` they are the operators `cuju_amd::delta_rule`,
-`cuju_amd::delta_rule_step` and `cuju_amd::group_norm` with their backward operators. Element types
+HIP graph. Under `torch.compile`, tracers, dispatch modes and function transforms, and for tensors of a
+subclass, they are the operators `cuju_amd::delta_rule`, `cuju_amd::delta_rule_step` and
+`cuju_amd::group_norm` with their backward operators. Element types
 are float32, bfloat16 and float16; sums, statistics and memories are held in 32 bits whatever the
 type. There is no implementation for another device.
 """
@@ -50,13 +51,29 @@ def _call(function, packed: bytes, device: torch.device) -> None:
     lib = _library()
     # The handle alone: a Stream object around it would be a tenth of a small call's time.
     stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         status = getattr(lib, function)(packed, stream)
     else:
         with torch.cuda.device(device):
             status = getattr(lib, function)(packed, stream)
     if status != 0:
         raise from_library(lib.cuju_last_error().decode())
+
+
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
+_compiling = torch.compiler.is_compiling
+_dispatch_modes, _tracing_state = torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+_transform_level = torch._C._functorch.maybe_current_level
+
+
+def _operator(name: str, direct, *tensors):
+    """`direct`, which launches without a way through torch's dispatcher, or the operator that it is
+    registered as where something else has to see the call: a compiler, a tracer, a dispatch mode, a
+    function transform or a subclass of tensors."""
+    if (_compiling() or _dispatch_modes() or _tracing_state() is not None or _transform_level() is not None
+            or not _PLAIN.issuperset(map(type, tensors))):
+        return getattr(torch.ops.cuju_amd, name)
+    return direct
 
 
 def _shape(name: str, tensor: torch.Tensor, shape: tuple) -> None:
@@ -67,10 +84,20 @@ def _shape(name: str, tensor: torch.Tensor, shape: tuple) -> None:
 def _device(first: str, tensor: torch.Tensor, names: tuple, others: tuple) -> None:
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ArgumentError(f'expected {first} on a HIP device')
-    device = tensor.device
-    for name, other in zip(names, others):
-        if other is not None and (not isinstance(other, torch.Tensor) or other.device != device):
+    device, kind = tensor.device, torch.Tensor
+    for other in others:
+        if other is not None and (not isinstance(other, kind) or other.device != device):
+            name = names[[each is other for each in others].index(True)]
             raise ArgumentError(f'expected {name} on the device of {first}')
+
+
+def _learns(*tensors) -> bool:
+    """Whether a call on these tensors has gradients."""
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor is not None and tensor.requires_grad:
+                return True
+    return False
 
 
 def _gate(name: str, tensor: torch.Tensor) -> torch.Tensor:
@@ -195,13 +222,14 @@ def _rule_step(q, k, v, decay, beta, state, resets, scale):
                          q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), beta.data_ptr(), _pointer(resets),
                          qb, 0, qh, kb, 0, kh, vb, 0, vh, db, 0, dh, bb, 0, bh, sb, 0,
                          state.data_ptr(), output.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), v.device)
+    torch.autograd.graph.increment_version(state)
     return output
 
 
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, decay, beta, state, resets, scale):
-        run = torch.ops.cuju_amd.delta_rule if torch.compiler.is_compiling() else _rule_forward
+        run = _operator('delta_rule', _rule_forward, q, k, v, decay, beta, state, resets)
         output, last, checkpoints = run(q, k, v, decay, beta, state, resets, scale, True)
         ctx.save_for_backward(q, k, v, decay, beta, state, resets, checkpoints)
         ctx.scale = scale
@@ -214,7 +242,7 @@ class _DeltaRule(torch.autograd.Function):
         q, k, v, decay, beta, state, resets, checkpoints = ctx.saved_tensors
         d_output = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if d_output is None else _flat(d_output)
         d_last = d_last.contiguous() if d_last is not None else None
-        run = torch.ops.cuju_amd.delta_rule_backward if torch.compiler.is_compiling() else _rule_backward
+        run = _operator('delta_rule_backward', _rule_backward, *ctx.saved_tensors, d_output, d_last)
         *dense, d_state = run(q, k, v, decay, beta, state, resets, ctx.scale, checkpoints, d_output, d_last)
         return (*dense, d_state if state is not None else None, None, None)
 
@@ -244,9 +272,9 @@ def delta_rule(query, key, value, decay, beta, *, state=None, resets=None, scale
     if state is not None:
         state = state.float().contiguous()
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, decay, beta, state)):
+    if _learns(q, k, v, decay, beta, state):
         return _DeltaRule.apply(q, k, v, decay, beta, state, resets, scale)
-    run = torch.ops.cuju_amd.delta_rule if torch.compiler.is_compiling() else _rule_forward
+    run = _operator('delta_rule', _rule_forward, q, k, v, decay, beta, state, resets)
     output, last, _ = run(q, k, v, decay, beta, state, resets, scale, False)
     return output, last
 
@@ -262,15 +290,11 @@ def delta_rule_step(query, key, value, decay, beta, state, *, resets=None, scale
     q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, False)
     if state is None or state.dtype != torch.float32 or not state.is_contiguous():
         raise ArgumentError('expected state as a contiguous float32 tensor, which the step updates')
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or decay.requires_grad or
-                                    beta.requires_grad or state.requires_grad):
+    if _learns(q, k, v, decay, beta, state):
         raise ArgumentError('delta_rule_step has no gradients: call it under torch.no_grad(), or call delta_rule')
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if torch.compiler.is_compiling():
-        return torch.ops.cuju_amd.delta_rule_step(q, k, v, decay, beta, state, resets, scale)
-    output = _rule_step(q, k, v, decay, beta, state, resets, scale)
-    torch.autograd.graph.increment_version(state)
-    return output
+    run = _operator('delta_rule_step', _rule_step, q, k, v, decay, beta, state, resets)
+    return run(q, k, v, decay, beta, state, resets, scale)
 
 
 # --------------------------------------------------------------------------------------- group norm
@@ -321,7 +345,7 @@ def _norm_backward(x, weight, bias, stats, dy, groups, epsilon, activation):
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, epsilon, activation):
-        run = torch.ops.cuju_amd.group_norm if torch.compiler.is_compiling() else _norm_forward
+        run = _operator('group_norm', _norm_forward, x, weight, bias)
         y, stats = run(x, weight, bias, groups, epsilon, activation)
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.options = groups, epsilon, activation
@@ -331,7 +355,7 @@ class _GroupNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        run = torch.ops.cuju_amd.group_norm_backward if torch.compiler.is_compiling() else _norm_backward
+        run = _operator('group_norm_backward', _norm_backward, *ctx.saved_tensors, dy)
         dx, d_weight, d_bias = run(x, weight, bias, stats, dy.contiguous(), *ctx.options)
         return dx, d_weight if weight is not None else None, d_bias if bias is not None else None, None, None, None
 
@@ -371,9 +395,9 @@ def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='n
     weight = weight.float().contiguous() if weight is not None else None
     bias = bias.float().contiguous() if bias is not None else None
     options = groups, float(epsilon), ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(each is not None and each.requires_grad for each in (x, weight, bias)):
+    if _learns(x, weight, bias):
         return _GroupNorm.apply(x, weight, bias, *options)
-    run = torch.ops.cuju_amd.group_norm if torch.compiler.is_compiling() else _norm_forward
+    run = _operator('group_norm', _norm_forward, x, weight, bias)
     return run(x, weight, bias, *options)[0]
 
 

@@ -610,3 +610,106 @@ def test_refusals():
     dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+# ------------------------------------------------- tracers, modes and transforms besides torch.compile
+
+def small_calls():
+    """Calls of each operator as functions of tensors, with tensors for them."""
+    from cuju_amd import layers
+    given = inputs(2, 40, 1, 2, 16, 16, seed=20)
+    names = ('query', 'key', 'value', 'decay', 'beta', 'state')
+    x, weight = torch.randn(2, 5, 8, device='cuda'), torch.rand(8, device='cuda')
+
+    def norm(x, weight):
+        return layers.group_norm(x, 2, weight, activation='silu')
+
+    def rule(q, k, v, decay, beta, state):
+        return layers.delta_rule(q, k, v, decay, beta, state=state)
+
+    def step(q, k, v, decay, beta, state):
+        state = state.clone()
+        return layers.delta_rule_step(q, k, v, decay, beta, state), state
+
+    return [(norm, (x, weight)), (rule, tuple(given[n] for n in names)),
+            (step, (*[given[n][:, 0] for n in names[:5]], given['state']))]
+
+
+def outputs_of(call, tensors):
+    found = call(*tensors)
+    return found if isinstance(found, (tuple, list)) else (found,)
+
+
+def gradients_of(call):
+    def learnt(*tensors):
+        leaves = [x.detach().requires_grad_() for x in tensors]
+        outputs = outputs_of(call, leaves)
+        return torch.autograd.grad(outputs, leaves, [torch.ones_like(y) for y in outputs])
+    return learnt
+
+
+@pytest.mark.parametrize('which', range(3))
+def test_traced_graphs_compute(which):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, tensors = small_calls()[which]
+    other = [x * 0.5 for x in tensors]
+    for each in (call, gradients_of(call)) if which < 2 else (call,):
+        graph = make_fx(lambda *t: each(*t))(*tensors)
+        for found, wanted in zip(outputs_of(graph, other), outputs_of(each, other)):
+            assert torch.equal(found, wanted)
+    traced = torch.jit.trace(call, tensors, check_trace=False)
+    for found, wanted in zip(outputs_of(traced, other), outputs_of(call, other)):
+        assert torch.equal(found, wanted)
+
+
+def test_modes_see_the_gradients():
+    from torch.utils._python_dispatch import TorchDispatchMode
+    names = []
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, function, types, args=(), kwargs=None):
+            names.append(function.name())
+            return function(*args, **(kwargs or {}))
+
+    for call, tensors in small_calls()[:2]:
+        wanted = gradients_of(call)(*tensors)
+        with Seen():
+            found = gradients_of(call)(*tensors)
+        assert all(torch.equal(a, b) for a, b in zip(found, wanted))
+    assert [n for n in names if n.startswith('cuju_amd')] == [
+        'cuju_amd::group_norm', 'cuju_amd::group_norm_backward', 'cuju_amd::delta_rule', 'cuju_amd::delta_rule_backward']
+
+
+def test_transforms():
+    (norm, (x, weight)), (rule, given), _ = small_calls()
+    maps = torch.randn(3, *x.shape, device='cuda')
+    found = torch.func.vmap(norm, (0, None))(maps, weight)
+    assert torch.equal(found, torch.stack([norm(each, weight) for each in maps]))
+    assert torch.equal(torch.func.functionalize(norm)(x, weight), norm(x, weight))
+    assert all(torch.equal(a, b) for a, b in zip(torch.func.functionalize(rule)(*given), rule(*given)))
+    # Gradients of function transforms are not there, and say so.
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: norm(x, weight).sum())(x)
+
+
+def test_compiled_by_the_default_backend():
+    from cuju_amd import layers
+    torch._dynamo.reset()
+    given = inputs(3, 40, 1, 2, 32, 32, seed=21)
+    at = [given[n][:, 0] for n in ('query', 'key', 'value', 'decay', 'beta')]
+    states = [given['state'].clone() for _ in range(2)]
+
+    def act(q, k, v, decay, beta, state):
+        return layers.delta_rule_step(q, k, v, decay, beta, state)
+
+    compiled = torch.compile(act, fullgraph=True)
+    for _ in range(2):
+        assert torch.equal(compiled(*at, states[0]), act(*at, states[1]))
+    assert torch.equal(*states)
+    x, weight = torch.randn(2, 5, 8, device='cuda'), torch.rand(8, device='cuda')
+    norm = torch.compile(lambda x, weight: layers.group_norm(x, 2, weight, activation='silu'), fullgraph=True)
+    found, wanted = ([t.detach().requires_grad_() for t in (x, weight)] for _ in range(2))
+    y, expected = norm(*found), layers.group_norm(wanted[0], 2, wanted[1], activation='silu')
+    assert torch.equal(y, expected)
+    y.backward(torch.ones_like(y)), expected.backward(torch.ones_like(y))
+    assert all(torch.equal(a.grad, b.grad) for a, b in zip(found, wanted))

@@ -136,3 +136,79 @@ def test_the_norms_oracle_is_torchs(activation):
     found = layer_oracle.group_norm(x, 3, weight, bias, activation=activation, dy=dy)
     for name, wanted in zip(('y', 'dx', 'd_weight', 'd_bias'), (y.detach(), *gradients)):
         torch.testing.assert_close(found[name], wanted)
+
+
+# ------------------------------------------------- who else sees a call: modes, tracers and transforms
+
+def fake_inputs(time=3):
+    """Inputs of the delta rule without memory behind them."""
+    lead = (2, time) if time else (2,)
+    query, key = (torch.empty(*lead, 1, 8, device='cuda') for _ in range(2))
+    decay, beta = (torch.empty(*lead, 2, device='cuda') for _ in range(2))
+    return query, key, torch.empty(*lead, 2, 4, device='cuda'), decay, beta, torch.empty(2, 2, 8, 4, device='cuda')
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """Tensors without memory, and a failure instead of a launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def launched(*_):
+        raise AssertionError('launched for tensors without memory')
+
+    monkeypatch.setattr(layers, '_call', launched)
+    return FakeTensorMode()
+
+
+def rule_of(query, key, value, decay, beta, state):
+    return layers.delta_rule(query, key, value, decay, beta, state=state)
+
+
+def norm_of(x, weight):
+    return layers.group_norm(x, 2, weight)
+
+
+def test_tensors_without_memory_are_not_launched_for(fake):
+    with fake:
+        x, weight = torch.empty(2, 3, 8, device='cuda'), torch.empty(8, device='cuda')
+        given, step = fake_inputs(), fake_inputs(time=0)
+        found = (norm_of(x, weight), *rule_of(*given), layers.delta_rule_step(*step))
+        assert [tuple(y.shape) for y in found] == [(2, 3, 8), (2, 3, 2, 4), (2, 2, 8, 4), (2, 2, 4)]
+        weight.requires_grad_()
+        assert norm_of(x, weight).requires_grad
+    # Neither outside of the mode that made them.
+    assert norm_of(x, weight).shape == x.shape and rule_of(*given)[1].shape == (2, 2, 8, 4)
+    assert layers.delta_rule_step(*step).shape == (2, 2, 4)
+
+
+def test_tracers_and_modes_see_the_operators(fake):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, function, types, args=(), kwargs=None):
+            self.names.append(function.name())
+            return function(*args, **(kwargs or {}))
+
+    with fake:
+        x, weight = torch.empty(2, 3, 8, device='cuda'), torch.empty(8, device='cuda')
+        given, step = fake_inputs(), fake_inputs(time=0)
+        for call, tensors, name in ((norm_of, (x, weight), 'group_norm'), (rule_of, given, 'delta_rule'),
+                                    (layers.delta_rule_step, step, 'delta_rule_step')):
+            with Seen() as seen:
+                call(*tensors)
+            assert [n for n in seen.names if n.startswith('cuju_amd')] == [f'cuju_amd::{name}']
+            traced = [node.target.name() for node in make_fx(lambda *t: call(*t))(*tensors).graph.nodes
+                      if node.op == 'call_function' and hasattr(node.target, 'name')]
+            assert [n for n in traced if n.startswith('cuju_amd')] == [f'cuju_amd::{name}']
+
+
+def test_functional_tensors_are_not_launched_for(fake):
+    with fake:
+        x, weight = torch.empty(2, 3, 8, device='cuda'), torch.empty(8, device='cuda')
+        assert torch.func.functionalize(norm_of)(x, weight).shape == x.shape
+        assert torch.func.functionalize(rule_of)(*fake_inputs())[0].shape == (2, 3, 2, 4)

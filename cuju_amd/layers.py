@@ -11,7 +11,8 @@ HIP graph. Under `torch.compile`, tracers, dispatch modes and function transform
 subclass, they are the operators `cuju_amd::delta_rule`, `cuju_amd::delta_rule_step` and
 `cuju_amd::group_norm` with their backward operators. Element types
 are float32, bfloat16 and float16; sums, statistics and memories are held in 32 bits whatever the
-type. There is no implementation for another device.
+type. There is no implementation for another device. Gradients are those of reverse mode, of first
+order; forward-mode derivatives are refused.
 """
 
 from __future__ import annotations
@@ -20,6 +21,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from .errors import ArgumentError, ChoiceError, from_library
 from .library import load
@@ -89,6 +91,9 @@ def _device(first: str, tensor: torch.Tensor, names: tuple, others: tuple) -> No
         if other is not None and (not isinstance(other, kind) or other.device != device):
             name = names[[each is other for each in others].index(True)]
             raise ArgumentError(f'expected {name} on the device of {first}')
+    if forward_ad._current_level >= 0 and any(x is not None and forward_ad.unpack_dual(x).tangent is not None
+                                              for x in (tensor, *others)):
+        raise ArgumentError('there are no forward-mode derivatives: expected tensors without a tangent')
 
 
 def _learns(*tensors) -> bool:

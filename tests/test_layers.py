@@ -212,3 +212,20 @@ def test_functional_tensors_are_not_launched_for(fake):
         x, weight = torch.empty(2, 3, 8, device='cuda'), torch.empty(8, device='cuda')
         assert torch.func.functionalize(norm_of)(x, weight).shape == x.shape
         assert torch.func.functionalize(rule_of)(*fake_inputs())[0].shape == (2, 3, 2, 4)
+
+
+def test_forward_mode_derivatives_are_refused(fake):
+    from torch.autograd import forward_ad
+    with fake:
+        x, weight = torch.empty(2, 3, 8, device='cuda'), torch.empty(8, device='cuda')
+        for call, tensors in ((norm_of, (x, weight)), (rule_of, fake_inputs()),
+                              (layers.delta_rule_step, fake_inputs(time=0))):
+            for which in range(len(tensors)):
+                with forward_ad.dual_level():
+                    call(*tensors)
+                    duals = list(tensors)
+                    duals[which] = forward_ad.make_dual(tensors[which], torch.empty_like(tensors[which]))
+                    with pytest.raises(ArgumentError, match='forward-mode'):
+                        call(*duals)
+        with pytest.raises(ArgumentError, match='forward-mode'):
+            torch.func.jvp(norm_of, (x, weight), (x, weight))

@@ -147,6 +147,8 @@ _OTHERS = 'key', 'value', 'decay', 'beta', 'state', 'resets'
 def _check_rule(query, key, value, decay, beta, state, resets, steps):
     """The checked arguments as the kernels take them; `steps`: whether they have a time axis."""
     axes = 4 if steps else 3
+    if key is None or value is None or decay is None or beta is None:
+        raise ArgumentError('expected a key, value, decay and beta')
     _device('query', query, _OTHERS, (key, value, decay, beta, state, resets))
     dtype = query.dtype
     if dtype not in TYPES:

@@ -229,3 +229,14 @@ def test_forward_mode_derivatives_are_refused(fake):
                         call(*duals)
         with pytest.raises(ArgumentError, match='forward-mode'):
             torch.func.jvp(norm_of, (x, weight), (x, weight))
+
+
+def test_tensors_that_are_missing_are_refused(fake):
+    with fake:
+        for call, tensors in ((layers.delta_rule, fake_inputs()[:5]), (layers.delta_rule_step, fake_inputs(time=0))):
+            for which in range(len(tensors)):
+                for bad in (None, 1.0):
+                    with pytest.raises(ArgumentError):
+                        call(*tensors[:which], bad, *tensors[which + 1:])
+        with pytest.raises(ArgumentError):
+            layers.group_norm(None, 2)

@@ -329,7 +329,8 @@ __device__ __forceinline__ float2 StatsOf(const T *x, const float *parts, const 
         return PartOf(parts, s, n, cuts, cut, 1, c) - 2 * off * PartOf(parts, s, n, cuts, cut, 0, c) +
                (cut ? 0.0 : s.pixels * off * off);
     });
-    return float2{(float)mean, (float)(1.0 / sqrt(fmax(squares, 0.0) / count + epsilon))};
+    // A comparison that keeps a NaN: an infinity leaves its group neither a mean nor a deviation.
+    return float2{(float)mean, (float)(1.0 / sqrt((squares < 0.0 ? 0.0 : squares) / count + epsilon))};
 }
 // The means of weight dz and of weight dz xh over a group, by a wavefront.
 __device__ __forceinline__ float2 MeansOf(const float *parts, const float *weight, const Shape &s, long long n, int group,

@@ -713,3 +713,26 @@ def test_compiled_by_the_default_backend():
     assert torch.equal(y, expected)
     y.backward(torch.ones_like(y)), expected.backward(torch.ones_like(y))
     assert all(torch.equal(a.grad, b.grad) for a, b in zip(found, wanted))
+
+
+# ------------------------------------------------------------------------- group norm: extreme values
+
+@pytest.mark.parametrize('bad', [float('inf'), -float('inf'), float('nan')])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shape', [(2, 6, 6, 16), (2, 150, 150, 16), (1, 40, 40, 700)])
+def test_an_infinity_leaves_its_group_nothing(shape, dtype, bad):
+    # The mean is infinite, so no value has a difference from it: the whole group is NaN, whatever the activation, in
+    # maps that are held, that are cut, and whose groups have a kernel for their statistics.
+    from cuju_amd import layers
+    x, weight, bias, dy = norm_inputs(shape, dtype, 8)
+    each = shape[-1] // 4
+    spoilt = x.clone()
+    spoilt[0, 3, 2, each + 1] = bad
+    for activation in ('none', 'relu', 'silu'):
+        wanted = layers.group_norm(x, 4, weight, bias, activation=activation)
+        found = norm_learn(spoilt, 4, weight, bias, activation, dy)
+        for name, clean in (('y', wanted), ('dx', norm_learn(x, 4, weight, bias, activation, dy)['dx'])):
+            result = found[name].clone()
+            assert bool(torch.isnan(result[0, ..., each:2 * each]).all()), (name, activation)
+            result[0, ..., each:2 * each] = clean[0, ..., each:2 * each]
+            assert torch.equal(result, clean), (name, activation)

@@ -45,8 +45,8 @@ struct Shape {
 
 // Sums over the workgroup's pixels of each thread's channel values `v`, into `out` [channels of the slab].
 // `scratch` holds [wavefronts][channels of the slab].
-template <int Vector>
-__device__ __forceinline__ void ChannelSums(float (&v)[Vector], float *scratch, float *out, const Shape &s) {
+template <int Vector, class Sum>
+__device__ __forceinline__ void ChannelSums(Sum (&v)[Vector], Sum *scratch, Sum *out, const Shape &s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int vector = threadIdx.x & (s.lanes - 1);
     for (int d = s.lanes; d < 64; d *= 2)
@@ -57,7 +57,7 @@ __device__ __forceinline__ void ChannelSums(float (&v)[Vector], float *scratch, 
         for (int i = 0; i < Vector; i++) scratch[wave * s.slabChannels + vector * Vector + i] = v[i];
     __syncthreads();
     for (int c = threadIdx.x; c < s.slabChannels; c += blockDim.x) {
-        float sum = 0;
+        Sum sum = 0;
         for (int w = 0; w < waves; w++) sum += scratch[w * s.slabChannels + c];
         out[c] = sum;
     }
@@ -274,33 +274,46 @@ __device__ __forceinline__ void ForPixels(const Cut &cut, Load load, Body body) 
     for (; p < cut.end; p += cut.step) load(0, p), body(0, p);
 }
 
-// Each channel's sum and sum of squares about its value at the first pixel: [map][cut][2][channels].
+// Pixels of a cut.
+__device__ __forceinline__ int PixelsOf(const Shape &s, int cuts, int cut) {
+    const int each = (s.pixels + cuts - 1) / cuts;
+    return max(0, min(s.pixels, (cut + 1) * each) - cut * each);
+}
+
+// Each channel's mean over a cut, and the squares about it: [map][cut][2][channels]. The sums are in 64 bits, so
+// that the squares lose nothing where values lie far from zero or a few lie far from the rest; the squares about a
+// cut's own mean are then sums of nothing below zero, which 32 bits hold.
 template <class T, int Vector>
 __global__ __launch_bounds__(kSplitThreads) void SumsKernel(const T *x, float *parts, Shape s) {
-    __shared__ float scratch[kSplitThreads * Vector], out[64 * Vector];
+    __shared__ double scratch[kSplitThreads * Vector], sums[64 * Vector], squares[64 * Vector];
     const Cut cut(s, Vector, false);
     const T *at = x + cut.map * s.pixels * s.channels + cut.channel;
-    float about[Vector], sum[Vector], square[Vector];
+    double sum[Vector], square[Vector];
 #pragma unroll
-    for (int c = 0; c < Vector; c++) about[c] = cut.mine ? Float(at[c]) : 0.f, sum[c] = square[c] = 0;
+    for (int c = 0; c < Vector; c++) sum[c] = square[c] = 0;
     Pack<T, Vector> v[kAhead];
     if (cut.mine)
         ForPixels(cut, [&](int n, int p) { v[n] = *reinterpret_cast<const Pack<T, Vector> *>(at + (long long)p * s.channels); },
                   [&](int n, int) {
 #pragma unroll
                       for (int c = 0; c < Vector; c++) {
-                          const float d = Float(v[n].x[c]) - about[c];
+                          const double d = Float(v[n].x[c]);
                           sum[c] += d;
-                          square[c] = fmaf(d, d, square[c]);
+                          square[c] = fma(d, d, square[c]);
                       }
                   });
     Shape slab = s;
     slab.vectors = cut.channels / Vector;
+    slab.slabChannels = cut.channels;
+    ChannelSums<Vector>(sum, scratch, sums, slab);
+    ChannelSums<Vector>(square, scratch, squares, slab);
+    const int count = PixelsOf(s, gridDim.y, blockIdx.y);
     float *to = parts + (cut.map * gridDim.y + blockIdx.y) * 2 * s.channels + cut.slab;
-    for (int k = 0; k < 2; k++) {
-        ChannelSums<Vector>(k ? square : sum, scratch, out, slab);
-        for (int c = threadIdx.x; c < cut.channels; c += kSplitThreads) to[k * s.channels + c] = out[c];
-        __syncthreads();
+    for (int c = threadIdx.x; c < cut.channels; c += kSplitThreads) {
+        const double mean = count ? sums[c] / count : 0.0, about = squares[c] - sums[c] * mean;
+        to[c] = (float)mean;
+        // A comparison that keeps a NaN.
+        to[s.channels + c] = about < 0.0 ? 0.f : (float)about;
     }
 }
 // A sum of `value(channel, cut)` over a group's channels and all cuts, the same in every lane of a
@@ -315,22 +328,18 @@ __device__ __forceinline__ double GroupSum(const Shape &s, int group, int cuts, 
 __device__ __forceinline__ double PartOf(const float *parts, const Shape &s, long long n, int cuts, int cut, int k, int c) {
     return parts[((n * cuts + cut) * 2 + k) * s.channels + c];
 }
-// A group's mean and inverse deviation from the cuts' sums, in 64 bits, by a wavefront.
-template <class T>
-__device__ __forceinline__ float2 StatsOf(const T *x, const float *parts, const Shape &s, long long n, int group, int cuts,
-                                          float epsilon) {
-    const T *first = x + n * s.pixels * s.channels;
+// A group's mean and inverse deviation from the cuts' means and squares, in 64 bits, by a wavefront. An infinity
+// leaves its group neither: the squares are NaN.
+__device__ __forceinline__ float2 StatsOf(const float *parts, const Shape &s, long long n, int group, int cuts, float epsilon) {
     const double count = (double)s.pixels * s.perGroup;
     const double mean = GroupSum(s, group, cuts, [&](int c, int cut) {
-                            return PartOf(parts, s, n, cuts, cut, 0, c) + (cut ? 0.0 : (double)s.pixels * Float(first[c]));
+                            return PixelsOf(s, cuts, cut) * PartOf(parts, s, n, cuts, cut, 0, c);
                         }) / count;
     const double squares = GroupSum(s, group, cuts, [&](int c, int cut) {
-        const double off = mean - Float(first[c]);
-        return PartOf(parts, s, n, cuts, cut, 1, c) - 2 * off * PartOf(parts, s, n, cuts, cut, 0, c) +
-               (cut ? 0.0 : s.pixels * off * off);
+        const double off = PartOf(parts, s, n, cuts, cut, 0, c) - mean;
+        return fma(PixelsOf(s, cuts, cut) * off, off, PartOf(parts, s, n, cuts, cut, 1, c));
     });
-    // A comparison that keeps a NaN: an infinity leaves its group neither a mean nor a deviation.
-    return float2{(float)mean, (float)(1.0 / sqrt((squares < 0.0 ? 0.0 : squares) / count + epsilon))};
+    return float2{(float)mean, (float)(1.0 / sqrt(squares / count + epsilon))};
 }
 // The means of weight dz and of weight dz xh over a group, by a wavefront.
 __device__ __forceinline__ float2 MeansOf(const float *parts, const float *weight, const Shape &s, long long n, int group,
@@ -349,9 +358,8 @@ __device__ __forceinline__ float2 MeansOf(const float *parts, const float *weigh
 // Slabs of whole groups, up to this many, find their groups' statistics themselves; others have a
 // kernel of a wavefront a group for it.
 constexpr int kMostGroups = 128;
-template <class T>
-__global__ __launch_bounds__(64) void StatsKernel(const T *x, const float *parts, float2 *stats, Shape s, int cuts, float epsilon) {
-    const float2 found = StatsOf(x, parts, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts, epsilon);
+__global__ __launch_bounds__(64) void StatsKernel(const float *parts, float2 *stats, Shape s, int cuts, float epsilon) {
+    const float2 found = StatsOf(parts, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts, epsilon);
     if (threadIdx.x == 0) stats[blockIdx.x] = found;
 }
 __global__ __launch_bounds__(64) void MeansKernel(const float *parts, const float *weight, float2 *means, Shape s, int cuts) {
@@ -369,7 +377,7 @@ __global__ __launch_bounds__(kSplitThreads) void ApplyKernel(const T *x, T *y, c
     const int firstGroup = cut.slab / s.perGroup;
     if (parts) {
         for (int i = threadIdx.x >> 6; i < cut.channels / s.perGroup; i += kSplitThreads / 64) {
-            const float2 each = StatsOf(x, parts, s, n, firstGroup + i, gridDim.y, epsilon);
+            const float2 each = StatsOf(parts, s, n, firstGroup + i, gridDim.y, epsilon);
             if ((threadIdx.x & 63) == 0) {
                 found[i] = each;
                 if (blockIdx.y == 0) stats[n * s.groups + firstGroup + i] = each;
@@ -613,7 +621,7 @@ void Forward(const Norm &n, hipStream_t stream) {
         hipLaunchKernelGGL((SumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, work, s);
         float2 *found = reinterpret_cast<float2 *>(stats);
         if (!FindsItself(s))
-            hipLaunchKernelGGL(StatsKernel<T>, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, x, work,
+            hipLaunchKernelGGL(StatsKernel, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, work,
                                found, s, cuts, n.epsilon);
         hipLaunchKernelGGL((ApplyKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, y, weight, bias,
                            FindsItself(s) ? work : nullptr, found, s, n.epsilon, n.activation);

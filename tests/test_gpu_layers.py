@@ -736,3 +736,19 @@ def test_an_infinity_leaves_its_group_nothing(shape, dtype, bad):
             assert bool(torch.isnan(result[0, ..., each:2 * each]).all()), (name, activation)
             result[0, ..., each:2 * each] = clean[0, ..., each:2 * each]
             assert torch.equal(result, clean), (name, activation)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('far', [30.0, 1000.0])
+@pytest.mark.parametrize('shape', [(2, 8, 8, 16), (1, 72, 96, 32), (2, 72, 96, 16), (1, 512, 512, 16), (1, 40, 40, 700)])
+def test_a_pixel_that_stands_out(shape, far, dtype):
+    # A corner many deviations from the rest, in maps that are held and that are cut: as exact as without it, for
+    # squares are taken about a mean.
+    x, weight, bias, dy = norm_inputs(shape, dtype, 9)
+    for at in ((0, 0), (shape[1] - 1, shape[2] // 2)):
+        spoilt = x.clone()
+        spoilt[:, at[0], at[1]] = far
+        found = norm_learn(spoilt, 4, weight, bias, 'silu', dy)
+        exact = exact_norm(spoilt, 4, weight, bias, activation='silu', dy=dy)
+        for name, each in found.items():
+            close(each, exact[name], VALUES if name == 'y' else GRADIENTS, exact['terms'] if name == 'dx' else 0.0)

@@ -358,13 +358,23 @@ __device__ __forceinline__ float2 MeansOf(const float *parts, const float *weigh
 // Slabs of whole groups, up to this many, find their groups' statistics themselves; others have a
 // kernel of a wavefront a group for it.
 constexpr int kMostGroups = 128;
-__global__ __launch_bounds__(64) void StatsKernel(const float *parts, float2 *stats, Shape s, int cuts, float epsilon) {
-    const float2 found = StatsOf(parts, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts, epsilon);
-    if (threadIdx.x == 0) stats[blockIdx.x] = found;
+__global__ __launch_bounds__(64) void StatsKernel(const float *parts, float2 *stats, Shape s, long long count, int cuts, float epsilon) {
+    for (long long i = blockIdx.x; i < count; i += gridDim.x) {
+        const float2 found = StatsOf(parts, s, i / s.groups, i % s.groups, cuts, epsilon);
+        if (threadIdx.x == 0) stats[i] = found;
+    }
 }
-__global__ __launch_bounds__(64) void MeansKernel(const float *parts, const float *weight, float2 *means, Shape s, int cuts) {
-    const float2 found = MeansOf(parts, weight, s, blockIdx.x / s.groups, blockIdx.x % s.groups, cuts);
-    if (threadIdx.x == 0) means[blockIdx.x] = found;
+__global__ __launch_bounds__(64) void MeansKernel(const float *parts, const float *weight, float2 *means, Shape s, long long count,
+                                                  int cuts) {
+    for (long long i = blockIdx.x; i < count; i += gridDim.x) {
+        const float2 found = MeansOf(parts, weight, s, i / s.groups, i % s.groups, cuts);
+        if (threadIdx.x == 0) means[i] = found;
+    }
+}
+// Their grid: a workgroup a group, up to a number far past what the chip holds at once.
+dim3 GroupGrid(const Norm &n) {
+    const long long groups = (long long)n.batch * n.groups;
+    return dim3((unsigned)(groups < (1 << 20) ? groups : 1 << 20));
 }
 
 template <class T, int Vector>
@@ -621,8 +631,8 @@ void Forward(const Norm &n, hipStream_t stream) {
         hipLaunchKernelGGL((SumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, work, s);
         float2 *found = reinterpret_cast<float2 *>(stats);
         if (!FindsItself(s))
-            hipLaunchKernelGGL(StatsKernel, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, work,
-                               found, s, cuts, n.epsilon);
+            hipLaunchKernelGGL(StatsKernel, GroupGrid(n), dim3(64), 0, stream, work, found, s, (long long)n.batch * n.groups,
+                               cuts, n.epsilon);
         hipLaunchKernelGGL((ApplyKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, y, weight, bias,
                            FindsItself(s) ? work : nullptr, found, s, n.epsilon, n.activation);
     });
@@ -655,8 +665,8 @@ void Backward(const Norm &n, hipStream_t stream) {
         hipLaunchKernelGGL((GradientSumsKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, weight, bias, stats,
                            parts, s, n.activation);
         if (!FindsItself(s))
-            hipLaunchKernelGGL(MeansKernel, dim3((unsigned)((long long)n.groups * n.batch)), dim3(64), 0, stream, parts,
-                               weight, means, s, cuts);
+            hipLaunchKernelGGL(MeansKernel, GroupGrid(n), dim3(64), 0, stream, parts, weight, means, s,
+                               (long long)n.batch * n.groups, cuts);
         hipLaunchKernelGGL((GradientKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, dx, weight, bias,
                            reinterpret_cast<const float2 *>(stats), FindsItself(s) ? parts : nullptr, means, s, n.activation);
     });
@@ -671,11 +681,11 @@ bool Fits(const Norm *n) {
     if (n->batch < 0 || n->pixels < 0 || n->channels < 1 || n->groups < 1 || n->channels % n->groups)
         return Failed("expected channels that are a multiple of the groups"), false;
     // Places within a map are ints, and a grid has fewer than 2^32 threads: at most 512 for each of two slabs
-    // of a map, 256 for each slab of a map that is cut, 64 for each group, 128 for each channel.
+    // of a map, 256 for each slab of a map that is cut (of 33 channels and more), 128 for each channel of a map.
     if ((long long)n->pixels * n->channels >= (1ll << 30) || n->channels >= (1 << 24))
         return Failed("expected fewer than 2^30 values and 2^24 channels in a map"), false;
-    if ((long long)n->batch * n->groups >= (1ll << 22) || (long long)n->batch * n->channels >= (1ll << 29))
-        return Failed("expected fewer than 2^22 groups and 2^29 channels in the batch"), false;
+    if (n->batch >= (1 << 22) || (long long)n->batch * n->channels >= (1ll << 29))
+        return Failed("expected fewer than 2^22 maps and 2^29 channels in the batch"), false;
     return true;
 }
 

@@ -395,9 +395,8 @@ def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='n
     batch = x.shape[0]
     if x.numel() // (batch or 1) >= 1 << 30 or channels >= 1 << 24:
         raise ArgumentError(f'expected fewer than 2^30 values and 2^24 channels in a map, found the shape {tuple(x.shape)}')
-    if batch * groups >= 1 << 22 or batch * channels >= 1 << 29:
-        raise ArgumentError(f'expected fewer than 2^22 groups and 2^29 channels in the batch, found the shape '
-                            f'{tuple(x.shape)} in {groups} groups')
+    if batch >= 1 << 22 or batch * channels >= 1 << 29:
+        raise ArgumentError(f'expected fewer than 2^22 maps and 2^29 channels in the batch, found the shape {tuple(x.shape)}')
     x = x.contiguous()
     weight = weight.float().contiguous() if weight is not None else None
     bias = bias.float().contiguous() if bias is not None else None

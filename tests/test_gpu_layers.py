@@ -752,3 +752,26 @@ def test_a_pixel_that_stands_out(shape, far, dtype):
         exact = exact_norm(spoilt, 4, weight, bias, activation='silu', dy=dy)
         for name, each in found.items():
             close(each, exact[name], VALUES if name == 'y' else GRADIENTS, exact['terms'] if name == 'dx' else 0.0)
+
+
+# Maps, pixels, channels and groups: an update's small maps (4,096 matches of 64 steps), acting for 16,384 matches of
+# 11 agents, and maps that are cut and whose many groups have a kernel for their statistics.
+@pytest.mark.parametrize('sizes', [(262144, 3, 64, 16), (180224, 2, 32, 32), (16500, 33, 256, 256)])
+def test_group_norm_of_many_maps_and_groups(sizes):
+    from cuju_amd import layers
+    maps, pixels, channels, groups = sizes
+    x = torch.randn(maps, pixels, channels, device='cuda', dtype=torch.bfloat16)
+    dy = torch.randn(maps, pixels, channels, device='cuda', dtype=torch.bfloat16)
+    weight, bias = torch.rand(channels, device='cuda') + 0.5, torch.randn(channels, device='cuda')
+    found = norm_learn(x, groups, weight, bias, 'silu', dy)
+    # The first, some and the last against the definition, and all against calls of half the maps.
+    some = torch.tensor([0, 1, maps // 3, maps - 2, maps - 1], device='cuda')
+    exact = exact_norm(x[some], groups, weight, bias, activation='silu', dy=dy[some])
+    close(found['y'][some], exact['y'], VALUES)
+    close(found['dx'][some], exact['dx'], GRADIENTS, exact['terms'])
+    half = maps // 2
+    parts = [norm_learn(x[at], groups, weight, bias, 'silu', dy[at]) for at in (slice(0, half), slice(half, None))]
+    assert torch.equal(found['y'], torch.cat([p['y'] for p in parts]))
+    assert torch.equal(found['dx'], torch.cat([p['dx'] for p in parts]))
+    for name in ('d_weight', 'd_bias'):
+        close(found[name], sum(p[name].double() for p in parts).cpu(), GRADIENTS)

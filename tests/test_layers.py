@@ -240,3 +240,13 @@ def test_tensors_that_are_missing_are_refused(fake):
                         call(*tensors[:which], bad, *tensors[which + 1:])
         with pytest.raises(ArgumentError):
             layers.group_norm(None, 2)
+
+
+def test_group_norm_takes_the_maps_of_an_update(fake):
+    # 4,096 matches of 64 steps, acting for 16,384 matches of 11 agents, and the last batch before the refusals.
+    with fake:
+        for maps, channels, groups in ((262144, 64, 16), (180224, 64, 32), ((1 << 22) - 1, 64, 64)):
+            x = torch.empty(maps, 3, channels, device='cuda', dtype=torch.bfloat16)
+            assert layers.group_norm(x, groups).shape == x.shape
+        with pytest.raises(ArgumentError, match='maps'):
+            layers.group_norm(torch.empty(1 << 22, 1, 1, device='cuda'), 1)

@@ -554,8 +554,8 @@ int VectorOf(const Norm &n) {
     while (vector > 1 && (n.channels % vector || all % (vector * size))) vector /= 2;
     return vector;
 }
-// The first count of slabs (each of whole groups and whole packs) whose pixels fit `packs` packs of
-// each of `threads` threads; 0 if none does.
+// The first count of slabs up to `most` (each of whole groups and whole packs) whose pixels fit `packs` packs
+// of each of `threads` threads; 0 if none does.
 //
 // Which maps a workgroup holds (us, held against cut, forward; then the gradients):
 //  - up to 16 KB, 256 threads: 4,000 bfloat16 maps of 16 KB 38 against 47; 63 against 75;
@@ -563,8 +563,8 @@ int VectorOf(const Norm &n) {
 //    108 KB 187 against 269; 325 against 436. In four slabs, 600 maps of 432 KB, 171 against 166.
 //  - 16-bit maps past 16 KB are cut: a pack of four is 8 bytes there, and 4,000 maps of 32 KB took 100
 //    against 68; 149 against 133.
-int SlabsFor(const Norm &n, int vector, int packs, int threads) {
-    for (int slabs = 1; slabs <= n.groups; slabs++) {
+int SlabsFor(const Norm &n, int vector, int packs, int threads, int most) {
+    for (int slabs = 1; slabs <= most; slabs++) {
         if (n.groups % slabs || n.channels / slabs % vector) continue;
         const Shape s = SlabsOf(n, slabs, vector);
         if (s.lanes <= 64 && s.pixels <= (long long)packs * (threads / s.lanes)) return slabs;
@@ -621,9 +621,9 @@ void Forward(const Norm &n, hipStream_t stream) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, y,
                                weight, bias, stats, SlabsOf(n, slabs, V), n.epsilon, n.activation);
         };
-        if (SlabsFor(n, V, Packs<T, V>(64), 256) == 1) return resident(ForwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
+        if (SlabsFor(n, V, Packs<T, V>(64), 256, 1)) return resident(ForwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
         if constexpr (sizeof(T) == 4)
-            if (const int slabs = SlabsFor(n, V, Packs<T, V>(224), 512); slabs == 1 || slabs == 2)
+            if (const int slabs = SlabsFor(n, V, Packs<T, V>(224), 512, 2))
                 return resident(ForwardKernel<T, V, Packs<T, V>(224), 512>, slabs, 512);
         const Shape s = SplitShape(n, V);
         const int cuts = CutsOf(n);
@@ -653,9 +653,9 @@ void Backward(const Norm &n, hipStream_t stream) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, dy, dx,
                                weight, bias, stats, parts, SlabsOf(n, slabs, V), n.activation);
         };
-        if (SlabsFor(n, V, Packs<T, V>(64), 256) == 1) return resident(BackwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
+        if (SlabsFor(n, V, Packs<T, V>(64), 256, 1)) return resident(BackwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
         if constexpr (sizeof(T) == 4)
-            if (const int slabs = SlabsFor(n, V, Packs<T, V>(112), 512); slabs == 1 || slabs == 2)
+            if (const int slabs = SlabsFor(n, V, Packs<T, V>(112), 512, 2))
                 return resident(BackwardKernel<T, V, Packs<T, V>(112), 512>, slabs, 512);
         const Shape s = SplitShape(n, V);
         const int cuts = CutsOf(n);

@@ -202,8 +202,10 @@ __global__ __launch_bounds__(Threads) void BackwardKernel(const T *x, const T *d
     ChannelSums<Vector>(sumW, scratch, weightSums, s);
     for (int c = threadIdx.x; c < s.slabChannels; c += Threads) {
         const int at = slab * s.slabChannels + c;
-        parts[(n * 2 + 0) * s.channels + at] = weightSums[c];
-        parts[(n * 2 + 1) * s.channels + at] = biasSums[c];
+        if (parts) {
+            parts[(n * 2 + 0) * s.channels + at] = weightSums[c];
+            parts[(n * 2 + 1) * s.channels + at] = biasSums[c];
+        }
         const float each = weight ? weight[at] : 1.f;
         biasSums[c] *= each, weightSums[c] *= each;
     }
@@ -646,12 +648,13 @@ void Backward(const Norm &n, hipStream_t stream) {
     const float *weight = static_cast<const float *>(n.weight), *bias = static_cast<const float *>(n.bias);
     const float *stats = static_cast<const float *>(n.stats);
     float *parts = static_cast<float *>(n.workspace);
+    const bool summed = n.d_weight || n.d_bias;
     long long rows = n.batch;
     ForVector(vector, [&](auto wide) {
         constexpr int V = decltype(wide)::value;
         const auto resident = [&](auto kernel, int slabs, int threads) {
             hipLaunchKernelGGL(kernel, dim3((unsigned)((long long)n.batch * slabs)), dim3(threads), 0, stream, x, dy, dx,
-                               weight, bias, stats, parts, SlabsOf(n, slabs, V), n.activation);
+                               weight, bias, stats, summed ? parts : nullptr, SlabsOf(n, slabs, V), n.activation);
         };
         if (SlabsFor(n, V, Packs<T, V>(64), 256, 1)) return resident(BackwardKernel<T, V, Packs<T, V>(64), 256>, 1, 256);
         if constexpr (sizeof(T) == 4)
@@ -670,7 +673,7 @@ void Backward(const Norm &n, hipStream_t stream) {
         hipLaunchKernelGGL((GradientKernel<T, V>), grid, dim3(kSplitThreads), 0, stream, x, dy, dx, weight, bias,
                            reinterpret_cast<const float2 *>(stats), FindsItself(s) ? parts : nullptr, means, s, n.activation);
     });
-    if (n.d_weight || n.d_bias)
+    if (summed)
         hipLaunchKernelGGL(ColumnsKernel, dim3((2 * n.channels + 15) / 16), dim3(1024), 0, stream, parts,
                            static_cast<float *>(n.d_weight), static_cast<float *>(n.d_bias), rows, n.channels);
 }

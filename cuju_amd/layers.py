@@ -336,13 +336,16 @@ def _norm_forward(x, weight, bias, groups, epsilon, activation):
     return y, stats
 
 
-def _norm_backward(x, weight, bias, stats, dy, groups, epsilon, activation):
+def _norm_backward(x, weight, bias, stats, dy, groups, epsilon, activation, of_weight, of_bias):
+    """The gradients of x, weight and bias; those of weight and bias are empty where they are not asked for."""
     dx = torch.empty_like(x)
-    d_weight, d_bias = torch.empty((2, x.shape[-1]), dtype=torch.float32, device=x.device).unbind()
+    d_weight, d_bias = (torch.empty(x.shape[-1] if asked else 0, dtype=torch.float32, device=x.device)
+                        for asked in (of_weight, of_bias))
     if x.numel():
         workspace = _norm_workspace(x, groups)
         _call('cuju_group_norm_backward',
-              _norm(x, groups, weight, bias, epsilon, activation, None, stats, workspace, dy, dx, d_weight, d_bias), x.device)
+              _norm(x, groups, weight, bias, epsilon, activation, None, stats, workspace, dy, dx,
+                    d_weight if of_weight else None, d_bias if of_bias else None), x.device)
     else:
         d_weight.zero_()
         d_bias.zero_()
@@ -363,8 +366,9 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
         run = _operator('group_norm_backward', _norm_backward, *ctx.saved_tensors, dy)
-        dx, d_weight, d_bias = run(x, weight, bias, stats, dy.contiguous(), *ctx.options)
-        return dx, d_weight if weight is not None else None, d_bias if bias is not None else None, None, None, None
+        _, of_weight, of_bias, *_ = ctx.needs_input_grad
+        dx, d_weight, d_bias = run(x, weight, bias, stats, dy.contiguous(), *ctx.options, of_weight, of_bias)
+        return dx, d_weight if of_weight else None, d_bias if of_bias else None, None, None, None
 
 
 def group_norm(x, groups, weight=None, bias=None, *, epsilon=1e-5, activation='none'):
@@ -419,7 +423,7 @@ _NAMESPACE.define(f'delta_rule_step({_INPUTS}, Tensor(a!) state, Tensor? resets,
 _NAMESPACE.define('group_norm(Tensor x, Tensor? weight, Tensor? bias, int groups, float epsilon, int activation) -> '
                   '(Tensor, Tensor)')
 _NAMESPACE.define('group_norm_backward(Tensor x, Tensor? weight, Tensor? bias, Tensor stats, Tensor dy, int groups, '
-                  'float epsilon, int activation) -> (Tensor, Tensor, Tensor)')
+                  'float epsilon, int activation, bool of_weight, bool of_bias) -> (Tensor, Tensor, Tensor)')
 _NAMESPACE.impl('delta_rule', _rule_forward, 'CUDA')
 _NAMESPACE.impl('delta_rule_backward', _rule_backward, 'CUDA')
 _NAMESPACE.impl('delta_rule_step', _rule_step, 'CUDA')
@@ -454,6 +458,6 @@ def _(x, weight, bias, groups, epsilon, activation):
 
 
 @torch.library.register_fake('cuju_amd::group_norm_backward')
-def _(x, weight, bias, stats, dy, groups, epsilon, activation):
-    sums = x.new_empty((x.shape[-1],), dtype=torch.float32)
-    return x.new_empty(x.shape), sums, torch.empty_like(sums)
+def _(x, weight, bias, stats, dy, groups, epsilon, activation, of_weight, of_bias):
+    sums = (x.new_empty((x.shape[-1] if asked else 0,), dtype=torch.float32) for asked in (of_weight, of_bias))
+    return x.new_empty(x.shape), *sums

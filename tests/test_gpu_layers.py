@@ -775,3 +775,20 @@ def test_group_norm_of_many_maps_and_groups(sizes):
     assert torch.equal(found['dx'], torch.cat([p['dx'] for p in parts]))
     for name in ('d_weight', 'd_bias'):
         close(found[name], sum(p[name].double() for p in parts).cpu(), GRADIENTS)
+
+
+@pytest.mark.parametrize('shape', [(3, 8, 8, 16), (2, 72, 96, 16)])
+def test_group_norm_gradients_that_are_asked_for(shape, monkeypatch):
+    from cuju_amd import layers
+    x, weight, bias, dy = norm_inputs(shape, torch.float32, 10)
+    wanted = norm_learn(x, 4, weight, bias, 'silu', dy)
+    given, packed, call = {'dx': x, 'd_weight': weight, 'd_bias': bias}, [], layers._call
+    monkeypatch.setattr(layers, '_call', lambda *a: (packed.append(layers._NORM.unpack(a[1])), call(*a)))
+    for asked in (('dx',), ('dx', 'd_weight'), ('d_bias',), ('d_weight', 'd_bias')):
+        leaves = [t.detach().requires_grad_(name in asked) for name, t in given.items()]
+        y = layers.group_norm(leaves[0], 4, leaves[1], leaves[2], activation='silu')
+        y.backward(dy)
+        for name, leaf in zip(given, leaves):
+            assert torch.equal(leaf.grad, wanted[name]) if name in asked else leaf.grad is None
+        # No sums of channels that nobody wants.
+        assert [bool(p) for p in packed[-1][-2:]] == ['d_weight' in asked, 'd_bias' in asked]

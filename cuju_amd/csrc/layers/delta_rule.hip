@@ -119,15 +119,116 @@ void LaunchStep(const Rule &r, hipStream_t stream) {
 // next, in the same registers; the keys are turned by a product with the identity.
 //
 // A reset within the chunk cuts it: the parts are played one after the other with the other steps'
-// keys, values and gates zero, so nothing of one episode, not even a NaN, meets the next.
+// keys, values and gates zero, so nothing of one episode, not even a NaN, meets the next. Each part costs
+// what a chunk does.
+//
+// The products over a chunk's steps take a later step's NaN or infinity, times a zero, into the outputs before
+// it, all of them at once. A wavefront that finds outputs that are not finite when it is through finds those
+// again, step by step from the definition.
 //
 // Many short sequences are bound by memory: 16,384 heads of 64 steps, 64 x 64 in bfloat16, with the
 // memories kept for the gradients, 1.35 GB, take 326 us, 4.1 TB/s. A wavefront on a SIMD by itself is
 // bound by its own instructions, some 700 a chunk of keys of 128: 44 heads of 3,000 steps, 128 x 128,
 // take 421 us, 2.2 us a chunk.
+template <class T>
+struct ForwardArgs {
+    Rule rule;
+    View<const T> query, key, value;
+    Gates gates;
+    int slices;
+};
+
+// Those outputs of a wavefront's columns that are not finite, one step after the other. From where its columns of the
+// memory hold nothing finite to the end of the episode no output is, and the steps are passed over.
 template <class T, int KeyTiles, int Tiles, bool Whole>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void ForwardKernel(
-    Rule rule, View<const T> query, View<const T> key, View<const T> value, Gates gates, int slices) {
+__device__ __forceinline__ void OutputsByStep() {
+    const ForwardArgs<T> a = Argument<ForwardArgs<T>>();
+    const Rule &rule = a.rule;
+    const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
+    const unsigned id = Place(blockIdx.x, gridDim.x), head = id / a.slices;
+    const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
+    const int dk = rule.key_size, dv = rule.value_size;
+    const int column = id % a.slices * 16 * Tiles + m * Tiles, columns = max(0, min(Tiles, dv - column));
+    float s[KeyTiles][4][Tiles] = {};
+    if (rule.state)
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * t + 4 * g + r;
+                const float *from = static_cast<const float *>(rule.state) + ((long long)head * dk + row) * dv + column;
+                const auto x = Load<Tiles, Whole>(from, row < dk ? columns : 0);
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) s[t][r][c] = x.x[c];
+            }
+    bool lost = false;
+    // What other lanes of the wavefront have put down is read.
+    __threadfence_block();
+#pragma unroll 1
+    for (int step = 0; step < rule.time; step++) {
+        const StepGates gate = LoadGates(a.gates, b, step, rule.time, h);
+        const bool starts = gate.Reset();
+        if (lost && !starts) continue;
+        const float kept = starts ? 0.f : expf(gate.decay);
+        const auto v = Load<Tiles, Whole>(a.value.At(b, step, h) + column, columns);
+        float written[Tiles] = {}, out[Tiles] = {};
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++) {
+            const auto k = Load<4, Whole>(a.key.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) {
+                    s[t][r][c] = starts ? 0.f : kept * s[t][r][c];
+                    written[c] = fmaf(Float(k.x[r]), s[t][r][c], written[c]);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < Tiles; c++) {
+            written[c] += __shfl_xor(written[c], 16);
+            written[c] += __shfl_xor(written[c], 32);
+            written[c] = gate.beta * (Float(v.x[c]) - written[c]);
+        }
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++) {
+            const auto k = Load<4, Whole>(a.key.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+            const auto q = Load<4, Whole>(a.query.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) {
+                    s[t][r][c] = fmaf(Float(k.x[r]), written[c], s[t][r][c]);
+                    out[c] = fmaf(Float(q.x[r]), s[t][r][c], out[c]);
+                }
+        }
+        T *at = static_cast<T *>(rule.output) + (((long long)b * rule.time + step) * rule.heads + h) * dv + column;
+        Pack<T, Tiles> o = Load<Tiles, Whole>(at, columns);
+        bool holds = false;
+#pragma unroll
+        for (int c = 0; c < Tiles; c++) {
+            out[c] += __shfl_xor(out[c], 16);
+            out[c] += __shfl_xor(out[c], 32);
+            if (Float(o.x[c]) * 0.f != 0.f) o.x[c] = As<T>(rule.scale * out[c]);
+            holds |= c < columns && written[c] * 0.f == 0.f;
+        }
+        if (g == 0) Store<Tiles, Whole>(at, o, columns);
+        lost = __ballot(holds) == 0;
+    }
+}
+
+// Wavefronts that a SIMD has to hold: of short keys and narrow pieces more, which they come to with a few registers
+// less (16,000 heads of 32 x 32 in half, 20 steps: 79 us with three, 89 with two).
+template <class T, int KeyTiles, int Tiles>
+constexpr int kForwardWaves = KeyTiles == 2 && Tiles == 1 && kPieces<T> == 1                                ? 4
+                              : KeyTiles == 2 && (Tiles == 1 || (Tiles == 2 && kPieces<T> < kFloatPieces)) ? 3
+                                                                                                            : 2;
+
+template <class T, int KeyTiles, int Tiles, bool Whole>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWaves<T, KeyTiles, Tiles>))) void ForwardKernel(ForwardArgs<T> a) {
+    const Rule &rule = a.rule;
+    const View<const T> &query = a.query, &key = a.key, &value = a.value;
+    const Gates &gates = a.gates;
+    const int slices = a.slices;
     __shared__ double reach[kChunk];
     __shared__ float betas[kChunk];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
@@ -223,11 +324,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
 
     // A part's outputs leave with the next part's loads: the wait for loads, which are answered in the order in
     // which loads and stores were sent, then finds them gone.
-    Pack<T, Tiles> done[4];
+    Pack<T, Tiles> done[4] = {};
     int doneLow = 0, doneHigh = 0;
+    unsigned long long odd = 0;  // lanes with outputs that are not finite
     const auto put = [&] {
         T *out = Global(atOut);
         const int stride = rule.heads * dv;
+        // One row shows it. Looked at here, a part later, it waits for no product.
+#pragma unroll
+        for (int c = 0; c < Tiles; c++) odd |= __ballot(Float(done[0].x[c]) * 0.f != 0.f);
         if (full && doneHigh - doneLow == kChunk) {
 #pragma unroll
             for (int r = 0; r < 4; r++, out += stride) *reinterpret_cast<Pack<T, Tiles> *>(out) = done[r];
@@ -351,6 +456,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2))) void Fo
     }
     put();
     if (rule.last) keep(rule.last, head);
+    if (odd) OutputsByStep<T, KeyTiles, Tiles, Whole>();
 }
 
 template <class T, int KeyTiles>
@@ -362,8 +468,8 @@ void LaunchForward(const Rule &r, hipStream_t stream) {
                        Aligned(16, r.state) && Aligned(16, r.last) && Aligned(16, r.checkpoints);
     const auto launch = [&](auto kernel, int tiles) {
         const int slices = (r.value_size + 16 * tiles - 1) / (16 * tiles);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads * slices)), dim3(64), 0, stream, r, query,
-                           key, value, GatesOf(r), slices);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads * slices)), dim3(64), 0, stream,
+                           ForwardArgs<T>{r, query, key, value, GatesOf(r), slices});
     };
     // Wide pieces repeat less of the keys' work; narrow ones give few heads more wavefronts. The chip
     // has 1,024 SIMDs, and the widest pieces that fill them are the fastest: 64 x 64 in bfloat16, 128 steps,

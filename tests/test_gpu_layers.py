@@ -792,3 +792,60 @@ def test_group_norm_gradients_that_are_asked_for(shape, monkeypatch):
             assert torch.equal(leaf.grad, wanted[name]) if name in asked else leaf.grad is None
         # No sums of channels that nobody wants.
         assert [bool(p) for p in packed[-1][-2:]] == ['d_weight' in asked, 'd_bias' in asked]
+
+
+# --------------------------------------------------------------- delta rule: steps that are not finite
+
+def spoil(x, steps, bad):
+    """`x` with one of its values at the given (sequence, step) places not finite."""
+    x = x.clone()
+    for i, (b, t) in enumerate(steps):
+        at = x[b, t].view(-1)
+        at[(7 * i + 3) % at.numel()] = bad
+    return x
+
+
+# Sequence and step: in a first chunk, in a later one, two in one chunk, in the first and in the last step.
+SPOILT = [(1, 5), (2, 21), (3, 18), (3, 27), (4, 0), (5, 40)]
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+@pytest.mark.parametrize('name', ['query', 'key', 'value', 'decay', 'beta'])
+@pytest.mark.parametrize('heads, key_size, value_size, dtype', [
+    (2, 48, 40, torch.float32), (2, 128, 128, torch.float32), (3, 33, 21, torch.float16), (190, 64, 64, torch.bfloat16),
+    (190, 16, 32, torch.float16)])
+def test_outputs_before_a_step_that_is_not_finite(heads, key_size, value_size, dtype, name, bad):
+    # As in the definition, and in acting: it reaches its own step and the later ones of its episode, no step before.
+    given = inputs(6, 41, 1, heads, key_size, value_size, dtype=dtype, seed=22)
+    given['resets'] = torch.zeros(6, 41, dtype=torch.bool, device='cuda')
+    given['resets'][2, 30] = given['resets'][3, 25] = True
+    given[name] = spoil(given[name], SPOILT, bad)
+    output, last = rule(given)
+    exact = exact_rule(**given)
+    for found, wanted in ((output, exact[0]), (last, exact[1])):
+        finite = torch.isfinite(wanted)
+        assert torch.equal(torch.isfinite(found).cpu(), finite)
+        zero = torch.zeros((), dtype=torch.double)
+        close(torch.where(finite, found.cpu(), zero.to(found.dtype)), torch.where(finite, wanted, zero), VALUES)
+
+
+def test_a_memory_that_is_not_finite_reaches_its_columns():
+    given = inputs(3, 50, 1, 2, 32, 48, seed=23)
+    given['state'][1, 1, 3, 17] = float('nan')
+    given['state'][2] = float('nan')
+    given['resets'] = torch.zeros(3, 50, dtype=torch.bool, device='cuda')
+    given['resets'][2, 44] = True
+    output, last = rule(given)
+    exact = exact_rule(**given)
+    for found, wanted in ((output, exact[0]), (last, exact[1])):
+        finite = torch.isfinite(wanted)
+        assert torch.equal(torch.isfinite(found).cpu(), finite)
+        close(torch.where(finite, found.cpu(), 0.0), torch.where(finite, wanted, 0.0), VALUES)
+
+
+def test_a_sequence_of_nothing_finite_ends():
+    # Long ones are passed over once their memory is lost.
+    given = inputs(8, 2000, 2, 2, 64, 64, dtype=torch.bfloat16, seed=24)
+    given['key'] = torch.full_like(given['key'], float('nan'))
+    output, last = rule(given)
+    assert bool(torch.isnan(output).all()) and bool(torch.isnan(last).all())

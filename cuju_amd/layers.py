@@ -276,7 +276,7 @@ def delta_rule(query, key, value, decay, beta, *, state=None, resets=None, scale
     step in 32 bits. Sizes go up to 128, strides are free (an axis of time before the batch is a
     transposed view). Gradients reach every floating input; they are the same on every call. A NaN or an
     infinity reaches the outputs of its own step and of later ones, as in the definition; in the memory an
-    infinity becomes a NaN.
+    infinity becomes a NaN. It may reach all gradients of its episode, and none of another.
     """
     q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, True)
     if state is not None:

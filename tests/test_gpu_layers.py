@@ -849,3 +849,63 @@ def test_a_sequence_of_nothing_finite_ends():
     given['key'] = torch.full_like(given['key'], float('nan'))
     output, last = rule(given)
     assert bool(torch.isnan(output).all()) and bool(torch.isnan(last).all())
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_a_later_episode_does_not_reach_an_earlier_one(bad):
+    given = inputs(3, 60, 1, 2, 48, 40, seed=25)
+    given['resets'] = torch.zeros(3, 60, dtype=torch.bool, device='cuda')
+    starts = ((0, 32), (1, 21), (2, 37))
+    for b, t in starts:
+        given['resets'][b, t] = True
+    spoilt = {n: x.clone() for n, x in given.items()}
+    for b, t in starts:
+        for name in ('query', 'key', 'value', 'decay', 'beta'):
+            spoilt[name][b, t:] = bad
+    clean, d_output, d_last = learn(given)
+    bad_d_output, bad_d_last = d_output.clone(), torch.full_like(d_last, bad)
+    for b, t in starts:
+        bad_d_output[b, t:] = bad
+    found, _, _ = learn(spoilt, bad_d_output, bad_d_last)
+    for b, t in starts:
+        for name in ('output', 'd_query', 'd_key', 'd_value', 'd_decay', 'd_beta'):
+            assert torch.equal(found[name][b, :t], clean[name][b, :t]), name
+    assert torch.equal(found['d_state'], clean['d_state'])
+
+
+# ------------------------------------------------------- kernels that many heads and other sizes choose
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('key_size, value_size', [(32, 64), (32, 32), (64, 64), (64, 72), (64, 128), (96, 64), (128, 128), (128, 100)])
+def test_gradients_of_many_heads(key_size, value_size, dtype):
+    # Enough heads for the widest pieces of the memory, with last pieces that are not whole, kept memories and resets.
+    # Heads are independent, so some stand for all.
+    given = inputs(1100, 70, 1, 1, key_size, value_size, dtype=dtype, seed=26 + key_size + value_size, episode=25)
+    found, d_output, d_last = learn(given)
+    some = torch.cat([torch.arange(0, 1100, 61), torch.tensor([1023, 1024, 1099])])
+    exact = exact_rule(**{n: x[some.cuda()] for n, x in given.items()}, d_output=d_output[some.cuda()], d_last=d_last[some.cuda()])
+    for name, x in found.items():
+        assert bool(torch.isfinite(x).all()), name
+        close(x[some.cuda()], exact[name], GRADIENTS if name.startswith('d_') else VALUES)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('value_size', [4, 12, 16, 20, 32, 48])
+def test_a_step_of_few_columns(value_size, dtype):
+    from cuju_amd import layers
+    for key_size in (32, 64, 128):
+        given = inputs(9, 1, 1, 2, key_size, value_size, dtype=dtype, seed=27 + key_size + value_size)
+        state = given['state'].clone()
+        output = layers.delta_rule_step(*[given[n].squeeze(1) for n in ('query', 'key', 'value', 'decay', 'beta')], state)
+        exact = exact_rule(**given)
+        close(output, exact[0][:, 0], VALUES)
+        close(state, exact[1], VALUES)
+
+
+@pytest.mark.parametrize('shape, groups', [((2, 26, 26, 64), 8), ((3, 30, 20, 48), 2), ((2, 36, 36, 24), 2)])
+def test_group_norm_of_maps_in_two_slabs(shape, groups):
+    x, weight, bias, dy = norm_inputs(shape, torch.float32, 11)
+    found = norm_learn(x, groups, weight, bias, 'silu', dy)
+    exact = exact_norm(x, groups, weight, bias, activation='silu', dy=dy)
+    for name, each in found.items():
+        close(each, exact[name], GRADIENTS, exact['terms'] if name == 'dx' else 0.0)

@@ -54,7 +54,7 @@ HIP_FLAGS = ['-std=c++17', '-O2', '-fPIC', '-ffp-contract=off', '-fno-fast-math'
 
 # The policy operators (layers/) hold no match: contraction and -O3, and the default scheduler.
 LAYER_SOURCES = ['layers/delta_rule.hip', 'layers/delta_rule_backward.hip', 'layers/group_norm.hip']
-LAYER_FLAGS = ['-std=c++17', '-O3', '-fPIC', '-fvisibility=hidden', '-w', f'--offload-arch={ARCH}',
+LAYER_FLAGS = ['-std=c++17', '-O3', '-fPIC', '-fvisibility=hidden', '-Wall', '-Wextra', '-Werror', f'--offload-arch={ARCH}',
                '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 # The device code is built once per group width (lanes per environment); the first build also

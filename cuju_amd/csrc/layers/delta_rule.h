@@ -70,16 +70,12 @@ __device__ __forceinline__ StepGates LoadGates(const Gates &g, int b, int t, int
 constexpr double kLog2E = 1.4426950408889634;
 __device__ __forceinline__ float Exp2(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// The inverse of I + A for the strictly lower A of a chunk, from A in both orders. Blocks of 4 on the
+// The inverse of I + A for the strictly lower A of a chunk, in row order, from A in both orders. Blocks of 4 on the
 // diagonal are inverted by substitution between the four lanes of a quad (G below); with L the part
 // of A below those blocks, I + A = G^-1 (I + N), N = G L, and N^4 = 0, so that
 // (I + A)^-1 = (I - N)(I + N N) G. Powers of the whole A would cancel in the sixth digit where keys
 // repeat themselves, as they do from one step of a match to the next; the powers of N stay small.
-struct Inverse {
-    F4 rows, columns;  // the inverse in row and in column order
-};
-template <bool Columns>
-__device__ __forceinline__ Inverse UnitLowerInverse(F4 aA, F4 dA, int m, int g) {
+__device__ __forceinline__ F4 UnitLowerInverse(F4 aA, F4 dA, int m, int g) {
     const bool diagonal = g == m / 4;
     F4 aG, dG, dL;
     // Row order: lane m holds row m; row s of a block is final after s steps and is taken off the later ones.
@@ -118,10 +114,7 @@ __device__ __forceinline__ Inverse UnitLowerInverse(F4 aA, F4 dA, int m, int g) 
     aY += one;
     aN = one - aN;
     const F4 dY = Product(aY, dG);
-    Inverse inverse;
-    inverse.rows = Product(dY, aN);
-    if (Columns) inverse.columns = Product(aN, dY);
-    return inverse;
+    return Product(dY, aN);
 }
 
 template <class T>

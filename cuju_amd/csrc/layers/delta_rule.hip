@@ -421,7 +421,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
             aA[r] = j < m ? beta * d * kk[r] : 0.f;
             dA[r] = m < j ? betaj[r] * d * kk[r] : 0.f;
         }
-        const F4 aT = UnitLowerInverse<false>(aA, dA, m, g).rows;
+        const F4 aT = UnitLowerInverse(aA, dA, m, g);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const float whole = Exp2(Gj[r]), asked = -whole * betaj[r], out = rule.scale * whole;

@@ -58,7 +58,7 @@ struct BackwardShared {
     static constexpr int kPieceRows = kFloatPieces * kSegment * kRow / 2;
     static constexpr int kKeyRows = kSegment * kKeyRow * ElementSize / 4, kValueRows = kSegment * kValueRow * ElementSize / 4;
     static constexpr int kReach = 0, kBetas = kReach + 2 * kSegment, kWhole = kBetas + kSegment, kAfter = kWhole + kSegment,
-                         kCuts = kAfter + kSegment, kInverse = kCuts + 4, kMixed = kInverse + 2 * kMatrix,
+                         kInverse = kAfter + kSegment, kMixed = kInverse + 2 * kMatrix,
                          kProducts = kMixed + kMatrix, kM = kMixed + 3 * kBlock, kSums = kM + 3 * kPieceMatrix,
                          kDots = kSums + 8 * kChunk, kU = kDots + Waves * 4 * kSegment,
                          kB = kU + kPieceRows, kK = kB + kPieceRows, kQ = kK + kKeyRows, kO = kQ + kKeyRows,
@@ -95,7 +95,6 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(kWav
     double *reach = reinterpret_cast<double *>(shared + At::kReach);
     float *betas = shared + At::kBetas, *wholes = shared + At::kWhole, *afters = shared + At::kAfter;
     float *memory = shared + At::kMemory, *dots = shared + At::kDots, *sums = shared + At::kSums;
-    unsigned *cutsOf = reinterpret_cast<unsigned *>(shared + At::kCuts);
     // Rows of values by step, [piece][step][column].
     uint16_t *sharedU = reinterpret_cast<uint16_t *>(shared + At::kU), *sharedB = reinterpret_cast<uint16_t *>(shared + At::kB);
     uint16_t *sharedM = reinterpret_cast<uint16_t *>(shared + At::kM), *sharedN = reinterpret_cast<uint16_t *>(shared + At::kMixed);
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(64 * Waves) __attribute__((amdgpu_waves_per_eu(kWav
                 *reinterpret_cast<F4 *>(shared + At::kMixed + block * kBlock + to) = aP;
                 *reinterpret_cast<F4 *>(shared + At::kProducts + block * kBlock + to) = aKK;
                 if (block != kAcross)
-                    *reinterpret_cast<F4 *>(shared + At::kInverse + block * kMatrix + to) = UnitLowerInverse<false>(aA, dA, m, g).rows;
+                    *reinterpret_cast<F4 *>(shared + At::kInverse + block * kMatrix + to) = UnitLowerInverse(aA, dA, m, g);
             }
             __syncthreads();
 

@@ -74,7 +74,7 @@ __device__ __forceinline__ void GroupSums(const float *channels, float *out, con
 }
 
 // The workgroup's packs: thread by thread, `Packs` rows of threads one after the other. A pack past the
-// map's end is a copy of the first pixel, whose difference from that pixel is zero.
+// map's end is a copy of the first pixel, so that all loads are alike; what is made of it is left out.
 template <class T, int Vector, int Packs>
 struct Held {
     Pack<T, Vector> x[Packs];

@@ -249,7 +249,7 @@ class _DeltaRule(torch.autograd.Function):
         q, k, v, decay, beta, state, resets, checkpoints = ctx.saved_tensors
         d_output = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if d_output is None else _flat(d_output)
         d_last = d_last.contiguous() if d_last is not None else None
-        run = _operator('delta_rule_backward', _rule_backward, *ctx.saved_tensors, d_output, d_last)
+        run = _operator('delta_rule_backward', _rule_backward, q, k, v, decay, beta, state, resets, checkpoints, d_output, d_last)
         *dense, d_state = run(q, k, v, decay, beta, state, resets, ctx.scale, checkpoints, d_output, d_last)
         return (*dense, d_state if state is not None else None, None, None)
 
@@ -368,7 +368,7 @@ class _GroupNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        run = _operator('group_norm_backward', _norm_backward, *ctx.saved_tensors, dy)
+        run = _operator('group_norm_backward', _norm_backward, x, weight, bias, stats, dy)
         _, of_weight, of_bias, *_ = ctx.needs_input_grad
         dx, d_weight, d_bias = run(x, weight, bias, stats, dy.contiguous(), *ctx.options, of_weight, of_bias)
         return dx, d_weight if of_weight else None, d_bias if of_bias else None, None, None, None

@@ -909,3 +909,53 @@ def test_group_norm_of_maps_in_two_slabs(shape, groups):
     exact = exact_norm(x, groups, weight, bias, activation='silu', dy=dy)
     for name, each in found.items():
         close(each, exact[name], GRADIENTS, exact['terms'] if name == 'dx' else 0.0)
+
+
+# ---------------------------------------------------------------------- training in a graph, recomputed
+
+def test_gradients_in_a_graph():
+    given = inputs(4, 70, 1, 2, 32, 40, dtype=torch.bfloat16, seed=28, episode=20)
+    x, weight, bias, dy = norm_inputs((3, 72, 96, 16), torch.bfloat16, 12)
+
+    def train():
+        found, d_output, d_last = learn(given, given_d[0], given_d[1])
+        return [*found.values(), *norm_learn(x, 4, weight, bias, 'silu', dy).values()]
+
+    _, *given_d = learn(given)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        found = train()
+    for scale in (1.0, 0.5, -2.0):
+        for each in (*given_d, dy):
+            each.mul_(scale)
+        wanted = train()
+        for each in found:
+            each.fill_(0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(found, wanted))
+
+
+def test_selective_recomputation():
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    seen = []
+
+    def policy(context, operator, *args, **kwargs):
+        if operator.name().startswith('cuju_amd'):
+            seen.append(operator.name())
+            return CheckpointPolicy.MUST_SAVE
+        return CheckpointPolicy.PREFER_RECOMPUTE
+
+    def recomputed(call):
+        return lambda *t: checkpoint(lambda *u: call(*u), *t, use_reentrant=False,
+                                     context_fn=lambda: create_selective_checkpoint_contexts(policy))
+
+    for call, tensors in small_calls()[:2]:
+        found, wanted = (gradients_of(each)(*tensors) for each in (recomputed(call), call))
+        assert all(torch.equal(a, b) for a, b in zip(found, wanted))
+    assert {'cuju_amd::group_norm', 'cuju_amd::delta_rule'} <= set(seen)

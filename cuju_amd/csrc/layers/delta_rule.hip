@@ -123,8 +123,8 @@ void LaunchStep(const Rule &r, hipStream_t stream) {
 // what a chunk does.
 //
 // The products over a chunk's steps take a later step's NaN or infinity, times a zero, into the outputs before
-// it, all of them at once. A wavefront that finds outputs that are not finite when it is through finds those
-// again, step by step from the definition.
+// it. A wavefront that has written values to its memory that are not finite finds the outputs that are not again when
+// it is through, step by step from the definition.
 //
 // Many short sequences are bound by memory: 16,384 heads of 64 steps, 64 x 64 in bfloat16, with the
 // memories kept for the gradients, 1.35 GB, take 326 us, 4.1 TB/s. A wavefront on a SIMD by itself is
@@ -138,51 +138,71 @@ struct ForwardArgs {
     int slices;
 };
 
-// Those outputs of a wavefront's columns that are not finite, one step after the other. From where its columns of the
-// memory hold nothing finite to the end of the episode no output is, and the steps are passed over.
+// Those outputs of a wavefront's columns that are not finite, one step after the other: the chunk at `chunk` is the
+// first that has some for a value written that is not, and where memories are kept the last one before it is
+// the start. From where the columns hold nothing finite to the end of the episode no output is, and steps are passed
+// over. 44 heads of 128 x 128 take 2.3 us a step.
 template <class T, int KeyTiles, int Tiles, bool Whole>
-__device__ __forceinline__ void OutputsByStep() {
+__device__ __forceinline__ void OutputsByStep(int chunk) {
     const ForwardArgs<T> a = Argument<ForwardArgs<T>>();
     const Rule &rule = a.rule;
-    const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
+    // The lane, found anew: the thread's number would take a register all the way here.
+    const int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), m = lane & 15, g = lane >> 4;
     const unsigned id = Place(blockIdx.x, gridDim.x), head = id / a.slices;
     const int h = head % rule.heads, b = head / rule.heads, kh = h / (rule.heads / rule.key_heads);
-    const int dk = rule.key_size, dv = rule.value_size;
+    const int dk = rule.key_size, dv = rule.value_size, time = rule.time;
     const int column = id % a.slices * 16 * Tiles + m * Tiles, columns = max(0, min(Tiles, dv - column));
+    // What other lanes of the wavefront have put down is read.
+    __threadfence_block();
+    const int segment = rule.checkpoints ? chunk / kSegment : 0;
+    const float *memory = static_cast<const float *>(segment ? rule.checkpoints : rule.state);
+    const long long index = segment ? (long long)head * ((time - 1) / kSegment) + segment - 1 : head;
     float s[KeyTiles][4][Tiles] = {};
-    if (rule.state)
+    if (memory)
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * t + 4 * g + r;
-                const float *from = static_cast<const float *>(rule.state) + ((long long)head * dk + row) * dv + column;
-                const auto x = Load<Tiles, Whole>(from, row < dk ? columns : 0);
+                const auto x = Load<Tiles, Whole>(memory + (index * dk + row) * dv + column, row < dk ? columns : 0);
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) s[t][r][c] = x.x[c];
             }
     bool lost = false;
-    // What other lanes of the wavefront have put down is read.
-    __threadfence_block();
 #pragma unroll 1
-    for (int step = 0; step < rule.time; step++) {
-        const StepGates gate = LoadGates(a.gates, b, step, rule.time, h);
-        const bool starts = gate.Reset();
-        if (lost && !starts) continue;
-        const float kept = starts ? 0.f : expf(gate.decay);
+    for (int step = segment * kSegment; step < time; step++) {
+        if (lost) {
+            // To the next start of an episode, 64 steps at a time.
+            const unsigned long long starts = __ballot(LoadGates(a.gates, b, step + lane, time, h).Reset());
+            if (!starts) {
+                step += 63;
+                continue;
+            }
+            step += __builtin_ctzll(starts);
+        }
+        // All loads start before the first is waited for.
+        const StepGates gate = LoadGates(a.gates, b, step, time, h);
+        T *at = static_cast<T *>(rule.output) + (((long long)b * time + step) * rule.heads + h) * dv + column;
+        Pack<T, Tiles> o = Load<Tiles, Whole>(at, columns);
         const auto v = Load<Tiles, Whole>(a.value.At(b, step, h) + column, columns);
-        float written[Tiles] = {}, out[Tiles] = {};
+        Pack<T, 4> k[KeyTiles], q[KeyTiles];
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++) {
-            const auto k = Load<4, Whole>(a.key.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+            k[t] = Load<4, Whole>(a.key.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+            q[t] = Load<4, Whole>(a.query.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+        }
+        const bool starts = gate.Reset();
+        const float kept = starts ? 0.f : expf(gate.decay);
+        float written[Tiles] = {}, out[Tiles] = {};
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
                     s[t][r][c] = starts ? 0.f : kept * s[t][r][c];
-                    written[c] = fmaf(Float(k.x[r]), s[t][r][c], written[c]);
+                    written[c] = fmaf(Float(k[t].x[r]), s[t][r][c], written[c]);
                 }
-        }
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             written[c] += __shfl_xor(written[c], 16);
@@ -190,28 +210,24 @@ __device__ __forceinline__ void OutputsByStep() {
             written[c] = gate.beta * (Float(v.x[c]) - written[c]);
         }
 #pragma unroll
-        for (int t = 0; t < KeyTiles; t++) {
-            const auto k = Load<4, Whole>(a.key.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
-            const auto q = Load<4, Whole>(a.query.At(b, step, kh) + 16 * t + 4 * g, dk - 16 * t - 4 * g);
+        for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
-                    s[t][r][c] = fmaf(Float(k.x[r]), written[c], s[t][r][c]);
-                    out[c] = fmaf(Float(q.x[r]), s[t][r][c], out[c]);
+                    s[t][r][c] = fmaf(Float(k[t].x[r]), written[c], s[t][r][c]);
+                    out[c] = fmaf(Float(q[t].x[r]), s[t][r][c], out[c]);
                 }
-        }
-        T *at = static_cast<T *>(rule.output) + (((long long)b * rule.time + step) * rule.heads + h) * dv + column;
-        Pack<T, Tiles> o = Load<Tiles, Whole>(at, columns);
-        bool holds = false;
+        bool holds = false, found = false;
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             out[c] += __shfl_xor(out[c], 16);
             out[c] += __shfl_xor(out[c], 32);
-            if (Float(o.x[c]) * 0.f != 0.f) o.x[c] = As<T>(rule.scale * out[c]);
+            if (Float(o.x[c]) * 0.f != 0.f) o.x[c] = As<T>(rule.scale * out[c]), found = true;
             holds |= c < columns && written[c] * 0.f == 0.f;
         }
-        if (g == 0) Store<Tiles, Whole>(at, o, columns);
+        // A store where there is nothing to change would hold up the next step's loads.
+        if (found && g == 0) Store<Tiles, Whole>(at, o, columns);
         lost = __ballot(holds) == 0;
     }
 }
@@ -324,15 +340,16 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
 
     // A part's outputs leave with the next part's loads: the wait for loads, which are answered in the order in
     // which loads and stores were sent, then finds them gone.
-    Pack<T, Tiles> done[4] = {};
+    Pack<T, Tiles> done[4];
     int doneLow = 0, doneHigh = 0;
-    unsigned long long odd = 0;  // lanes with outputs that are not finite
+    // Values written: a sum that is not finite where one is not, lanes that had such a one, and the chunk up to which
+    // none had. Looked at a part later, the sum waits for no product.
+    float mark = 0;
+    unsigned long long odd = 0;
+    int clean = 0;
     const auto put = [&] {
         T *out = Global(atOut);
         const int stride = rule.heads * dv;
-        // One row shows it. Looked at here, a part later, it waits for no product.
-#pragma unroll
-        for (int c = 0; c < Tiles; c++) odd |= __ballot(Float(done[0].x[c]) * 0.f != 0.f);
         if (full && doneHigh - doneLow == kChunk) {
 #pragma unroll
             for (int r = 0; r < 4; r++, out += stride) *reinterpret_cast<Pack<T, Tiles> *>(out) = done[r];
@@ -376,6 +393,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
                 if (4 * g + r < low || 4 * g + r >= high) v[r] = Pack<T, Tiles>{};
         }
         put();
+        odd |= __ballot(mark * 0.f != 0.f);
+        if (!odd) clean = t0;
         const int end = high;
         if (high == count) t0 += kChunk, high = 0, advance();
         if (t0 < time) fetch(t0);
@@ -444,6 +463,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
 #pragma unroll
             for (int c = 0; c < Tiles; c++) u[c][r] *= after;
         }
+        mark = 0;
+#pragma unroll
+        for (int c = 0; c < Tiles; c++) mark += (u[c][0] + u[c][1]) + (u[c][2] + u[c][3]);
         doneLow = low, doneHigh = end;
         const float kept = Exp2(last);
         Four up[Tiles][kFloatPieces];
@@ -455,8 +477,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
             for (int c = 0; c < Tiles; c++) s[t][c] = Mfma16(turned[t], up[c], s[t][c] * kept);
     }
     put();
+    odd |= __ballot(mark * 0.f != 0.f);
     if (rule.last) keep(rule.last, head);
-    if (odd) OutputsByStep<T, KeyTiles, Tiles, Whole>();
+    if (odd) OutputsByStep<T, KeyTiles, Tiles, Whole>(clean);
 }
 
 template <class T, int KeyTiles>

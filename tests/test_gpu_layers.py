@@ -829,6 +829,19 @@ def test_outputs_before_a_step_that_is_not_finite(heads, key_size, value_size, d
         close(torch.where(finite, found.cpu(), zero.to(found.dtype)), torch.where(finite, wanted, zero), VALUES)
 
 
+@pytest.mark.parametrize('step', [0, 15, 16, 31, 32, 40, 63, 64, 95, 99])
+def test_outputs_before_a_step_that_is_not_finite_in_training(step):
+    # With the memories kept for the gradients, from which the outputs are found again.
+    given = inputs(3, 100, 1, 2, 48, 40, seed=29)
+    given['value'][1, step, 1, 7] = given['key'][2, step, 0, 3] = float('nan')
+    output, last = rule(given, value=given['value'].clone().requires_grad_())
+    exact = exact_rule(**given)
+    for found, wanted in ((output, exact[0]), (last, exact[1])):
+        found, finite = found.detach().cpu(), torch.isfinite(wanted)
+        assert torch.equal(torch.isfinite(found), finite)
+        close(torch.where(finite, found, 0.0), torch.where(finite, wanted, 0.0), VALUES)
+
+
 def test_a_memory_that_is_not_finite_reaches_its_columns():
     given = inputs(3, 50, 1, 2, 32, 48, seed=23)
     given['state'][1, 1, 3, 17] = float('nan')

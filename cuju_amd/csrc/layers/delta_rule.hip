@@ -127,9 +127,9 @@ void LaunchStep(const Rule &r, hipStream_t stream) {
 // it is through, step by step from the definition.
 //
 // Many short sequences are bound by memory: 16,384 heads of 64 steps, 64 x 64 in bfloat16, with the
-// memories kept for the gradients, 1.35 GB, take 326 us, 4.1 TB/s. A wavefront on a SIMD by itself is
-// bound by its own instructions, some 700 a chunk of keys of 128: 44 heads of 3,000 steps, 128 x 128,
-// take 421 us, 2.2 us a chunk.
+// memories kept for the gradients, 1.35 GB, take 310 us, 4.4 TB/s. A wavefront on a SIMD by itself is
+// bound by its own instructions, some 750 a chunk of keys of 128: 44 heads of 3,000 steps, 128 x 128,
+// take 410 us, 2.2 us a chunk.
 template <class T>
 struct ForwardArgs {
     Rule rule;

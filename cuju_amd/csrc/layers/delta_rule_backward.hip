@@ -29,9 +29,9 @@ namespace {
 // Heads that share keys, or whose columns take several workgroups, leave parts of the gradients of the keys,
 // queries and gates that a second kernel adds up, in their order.
 //
-// 16,384 heads of 64 steps, 64 x 64 in bfloat16, 2.0 GB, take 1,172 us. Registers (215 of 256) and LDS hold
-// it at two wavefronts on a SIMD, vector instructions take 42 % of the cycles, a third of them splits into
-// pieces, and the wavefronts wait 43 % of theirs, for LDS between products that need one another and at the
+// 16,384 heads of 64 steps, 64 x 64 in bfloat16, 2.0 GB, take 1,076 us. Registers (215 of 256) and LDS hold
+// it at two wavefronts on a SIMD, vector instructions take 46 % of the cycles, a third of them splits into
+// pieces, and the wavefronts wait 42 % of theirs, for LDS between products that need one another and at the
 // barriers.
 template <class T>
 struct BackwardArgs {

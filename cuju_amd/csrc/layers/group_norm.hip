@@ -8,8 +8,8 @@
 // All sums are in 32 bits or more. A workgroup that can hold a map (or the channels of some of its
 // groups) in registers reads it once: mean, then the squares about the mean, then the output.
 // Larger maps are read twice, cut over workgroups, with their sums in a workspace between. Both are bound
-// by memory: 600 bfloat16 maps of 432 KB, read twice and written once, 796 MB, take 163 us, 4.9 TB/s; 600
-// of 216 KB 75 us and their gradients, 663 MB, 147 us, 4.5 TB/s.
+// by memory: 600 bfloat16 maps of 432 KB, read twice and written once, 796 MB, take 165 us, 4.8 TB/s; 600
+// of 216 KB 76 us and their gradients, 663 MB, 148 us, 4.5 TB/s.
 #include "../../../include/cuju_amd.h"
 #include "common.h"
 

@@ -136,6 +136,7 @@ struct ForwardArgs {
     View<const T> query, key, value;
     Gates gates;
     int slices;
+    bool inPlace;  // whether the last memory goes where the first one is
 };
 
 // Those outputs of a wavefront's columns that are not finite, one step after the other: the chunk at `chunk` is the
@@ -230,6 +231,17 @@ __device__ __forceinline__ void OutputsByStep(int chunk) {
         if (found && g == 0) Store<Tiles, Whole>(at, o, columns);
         lost = __ballot(holds) == 0;
     }
+    if (a.inPlace)
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * t + 4 * g + r;
+                Pack<float, Tiles> x;
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) x.x[c] = s[t][r][c];
+                Store<Tiles, Whole>(static_cast<float *>(rule.last) + ((long long)head * dk + row) * dv + column, x, row < dk ? columns : 0);
+            }
 }
 
 // Wavefronts that a SIMD has to hold: of short keys and narrow pieces more, which they come to with a few registers
@@ -478,7 +490,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kForwardWave
     }
     put();
     odd |= __ballot(mark * 0.f != 0.f);
-    if (rule.last) keep(rule.last, head);
+    // A last memory in the first one's place leaves that for the steps to be found again from, which end in it too.
+    if (rule.last && !(odd && a.inPlace)) keep(rule.last, head);
     if (odd) OutputsByStep<T, KeyTiles, Tiles, Whole>(clean);
 }
 
@@ -492,7 +505,7 @@ void LaunchForward(const Rule &r, hipStream_t stream) {
     const auto launch = [&](auto kernel, int tiles) {
         const int slices = (r.value_size + 16 * tiles - 1) / (16 * tiles);
         hipLaunchKernelGGL(kernel, dim3((unsigned)(r.batch * (long long)r.heads * slices)), dim3(64), 0, stream,
-                           ForwardArgs<T>{r, query, key, value, GatesOf(r), slices});
+                           ForwardArgs<T>{r, query, key, value, GatesOf(r), slices, r.last && r.last == r.state});
     };
     // Wide pieces repeat less of the keys' work; narrow ones give few heads more wavefronts. The chip
     // has 1,024 SIMDs, and the widest pieces that fill them are the fastest: 64 x 64 in bfloat16, 128 steps,

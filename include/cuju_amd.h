@@ -191,7 +191,7 @@ struct cuju_delta_rule {
     long long query_strides[3], key_strides[3], value_strides[3], decay_strides[3], beta_strides[3], reset_strides[2];
     void *state;                     /* [batch][heads][key_size][value_size], or null for zeros; a step updates it */
     void *output;                    /* of `type`, [batch][time][heads][value_size] */
-    void *last;                      /* the memory after the last step, or null */
+    void *last;                      /* the memory after the last step, or null; may be the forward pass's `state` */
     void *checkpoints;               /* [batch][heads][(time - 1) / 32][key_size][value_size]: the forward pass keeps the
                                         memory before every 32nd step for the backward pass; null for none */
     /* Only for the backward pass. */

@@ -856,6 +856,23 @@ def test_a_memory_that_is_not_finite_reaches_its_columns():
         close(torch.where(finite, found.cpu(), 0.0), torch.where(finite, wanted, 0.0), VALUES)
 
 
+@pytest.mark.parametrize('bad', [0.0, float('nan')])
+def test_a_memory_put_down_where_it_was_taken(bad):
+    # The library takes one buffer for the memory before and after.
+    from cuju_amd import layers
+    given = inputs(3, 50, 1, 2, 32, 48, seed=30)
+    given['value'][1, 21, 0, 5] = bad
+    wanted, last = rule(given)
+    memory, output = given['state'].clone(), torch.empty_like(given['value'])
+    layers._call('cuju_delta_rule_forward',
+                 layers._rule(given['query'], given['key'], given['value'], given['decay'], given['beta'], memory, None,
+                              32 ** -0.5, output, memory), memory.device)
+    assert torch.equal(output.nan_to_num(nan=1e30), wanted.nan_to_num(nan=1e30))
+    # Of the sequence that is played again the memory is that of single steps.
+    assert torch.equal(memory[::2], last[::2]) and torch.equal(torch.isnan(memory[1]), torch.isnan(last[1]))
+    close(memory[1].nan_to_num(nan=0.0), last[1].nan_to_num(nan=0.0).double().cpu(), VALUES)
+
+
 def test_a_sequence_of_nothing_finite_ends():
     # Long ones are passed over once their memory is lost.
     given = inputs(8, 2000, 2, 2, 64, 64, dtype=torch.bfloat16, seed=24)

@@ -1,0 +1,379 @@
+// Norms around a policy's blocks, over rows of up to 8,192 values, and their gradients.
+//
+//   u = block inner, inner = 1 / sqrt(mean(block^2) + epsilon)    (or u = block, without a norm of its own)
+//   b = after act(gate) u
+//   h = x + scale b                                               (or h = b, without a stream)
+//   y = before e, e = h outer, outer = 1 / sqrt(mean(h^2) + epsilon)
+//
+// With dh the gradient of h and dy that of y, means over a row and sums over all rows:
+//   de = before dy,  dh += outer (de - e mean(de e)),  d_before = sum dy e,  dx = dh;
+//   d_scale = sum dh b,  d_after = sum dh scale act(gate) u,  d_gate = dh scale after u act'(gate);
+//   du = dh scale after act(gate),  d_block = inner (du - u mean(du u)).
+//
+// All sums are in 32 bits or more. A row lies in the registers of a part of a wavefront or of a workgroup: every input
+// is read once and every output written once.
+#include "../../../include/cuju_amd.h"
+#include "common.h"
+
+namespace layers {
+namespace {
+
+using Rows = cuju_row_norm;
+enum Activation { kNone, kSigmoid, kSilu };
+constexpr int kMostSize = 8192;
+constexpr int kVectors = 3;  // after, scale and before
+
+__device__ __forceinline__ float Sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+__device__ __forceinline__ float Gate(float z, int activation) {
+    if (activation == kSigmoid) return Sigmoid(z);
+    if (activation == kSilu) return z * Sigmoid(z);
+    return z;
+}
+__device__ __forceinline__ float GateSlope(float z, int activation) {
+    if (activation == kNone) return 1.f;
+    const float s = Sigmoid(z);
+    if (activation == kSigmoid) return s * (1.f - s);
+    return s * fmaf(z, 1.f - s, 1.f);
+}
+
+// A thread's packs of a row: `Lanes` packs side by side, `Packs` such rows of packs after one another. Packs need no
+// alignment but their elements'; the last one may be cut by the row's end.
+template <class T, int Vector>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+    T x[Vector];
+};
+template <class T, int Vector, int Packs, int Lanes>
+struct Held {
+    Loose<T, Vector> x[Packs];
+    __device__ __forceinline__ void Load(const T *row, int lane, int size) {
+#pragma unroll
+        for (int i = 0; i < Packs; i++) {
+            const int at = (i * Lanes + lane) * Vector;
+            if (at + Vector <= size) {
+                x[i] = *reinterpret_cast<const Loose<T, Vector> *>(Global(row) + at);
+            } else {
+#pragma unroll
+                for (int c = 0; c < Vector; c++) x[i].x[c] = at + c < size ? Global(row)[at + c] : As<T>(0.f);
+            }
+        }
+    }
+    __device__ __forceinline__ void Store(T *row, int lane, int size) const {
+#pragma unroll
+        for (int i = 0; i < Packs; i++) {
+            const int at = (i * Lanes + lane) * Vector;
+            if (at + Vector <= size) {
+                *reinterpret_cast<Loose<T, Vector> *>(Global(row) + at) = x[i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < Vector; c++)
+                    if (at + c < size) Global(row)[at + c] = x[i].x[c];
+            }
+        }
+    }
+    __device__ __forceinline__ float At(int i, int c) const { return Float(x[i].x[c]); }
+};
+// A vector of the row's columns, held through all rows.
+template <int Vector, int Packs, int Lanes>
+struct Columns {
+    float x[Packs][Vector];
+    __device__ __forceinline__ Columns(const float *from, float otherwise, int lane, int size) {
+#pragma unroll
+        for (int i = 0; i < Packs; i++)
+#pragma unroll
+            for (int c = 0; c < Vector; c++) {
+                const int at = (i * Lanes + lane) * Vector + c;
+                x[i][c] = from && at < size ? from[at] : otherwise;
+            }
+    }
+};
+
+// The sum over the threads of a row, in each of them. Rows past a wavefront take `scratch`, two halves of a float for
+// each wavefront, used in turn: a wavefront is a sum ahead of another at most.
+template <int Lanes>
+__device__ __forceinline__ float SumOfRow(float x, float *scratch, int &half) {
+    if constexpr (Lanes <= 64) {
+#pragma unroll
+        for (int d = 1; d < Lanes; d *= 2) x += __shfl_xor(x, d);
+    } else {
+        constexpr int kWaves = Lanes / 64;
+        x = WaveSum(x);
+        float *to = scratch + half * kWaves;
+        if ((threadIdx.x & 63) == 0) to[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) x += to[w];
+        half ^= 1;
+    }
+    return x;
+}
+
+template <int Lanes>
+constexpr int kThreads = Lanes <= 64 ? 256 : Lanes;
+
+template <class T>
+__device__ __forceinline__ const T *RowOf(const void *p, const long long *strides, long long row, int inner) {
+    return static_cast<const T *>(p) + row / inner * strides[0] + row % inner * strides[1];
+}
+
+template <class T, int Vector, int Packs, int Lanes, bool Stream>
+__global__ __launch_bounds__(kThreads<Lanes>) void ForwardKernel(Rows n) {
+    __shared__ float scratch[2 * (Lanes <= 64 ? 1 : Lanes / 64)];
+    const int lane = threadIdx.x % Lanes, each = kThreads<Lanes> / Lanes, size = n.size;
+    int half = 0;
+    const Columns<Vector, Packs, Lanes> after(static_cast<const float *>(n.after), 1.f, lane, size);
+    const Columns<Vector, Packs, Lanes> scale(static_cast<const float *>(n.scales), n.scale, lane, size);
+    const Columns<Vector, Packs, Lanes> before(static_cast<const float *>(n.before), 1.f, lane, size);
+    const float count = 1.f / size;
+    for (long long row = (long long)blockIdx.x * each + threadIdx.x / Lanes; row < n.rows; row += (long long)gridDim.x * each) {
+        Held<T, Vector, Packs, Lanes> block, gate{}, x{}, out;
+        block.Load(RowOf<T>(n.block, n.block_strides, row, n.inner), lane, size);
+        if (n.gate) gate.Load(RowOf<T>(n.gate, n.gate_strides, row, n.inner), lane, size);
+        if constexpr (Stream) x.Load(RowOf<T>(n.x, n.x_strides, row, n.inner), lane, size);
+        float inner = 1.f, outer = 1.f;
+        if (n.norm_block) {
+            float sum = 0;
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++) sum = fmaf(block.At(i, c), block.At(i, c), sum);
+            inner = 1.f / sqrtf(fmaf(SumOfRow<Lanes>(sum, scratch, half), count, n.epsilon));
+        }
+        float h[Packs][Vector], sum = 0;
+#pragma unroll
+        for (int i = 0; i < Packs; i++)
+#pragma unroll
+            for (int c = 0; c < Vector; c++) {
+                float b = block.At(i, c) * inner * after.x[i][c];
+                if (n.gate) b *= Gate(gate.At(i, c), n.activation);
+                h[i][c] = Stream ? fmaf(scale.x[i][c], b, x.At(i, c)) : b;
+                // Past the row's end all inputs are zeros, and a gate of zero may not be.
+                if constexpr (Stream) sum = fmaf(h[i][c], h[i][c], sum);
+                out.x[i].x[c] = As<T>(h[i][c]);
+            }
+        out.Store(static_cast<T *>(n.stream) + row * size, lane, size);
+        if constexpr (Stream) {
+            outer = 1.f / sqrtf(fmaf(SumOfRow<Lanes>(sum, scratch, half), count, n.epsilon));
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++) out.x[i].x[c] = As<T>(h[i][c] * outer * before.x[i][c]);
+            out.Store(static_cast<T *>(n.normed) + row * size, lane, size);
+        }
+        if (n.stats && lane == 0) {
+            float *stats = static_cast<float *>(n.stats) + 2 * row;
+            stats[0] = inner, stats[1] = outer;
+        }
+    }
+}
+
+template <class T, int Vector, int Packs, int Lanes, bool Stream>
+__global__ __launch_bounds__(kThreads<Lanes>) void BackwardKernel(Rows n, float *parts) {
+    constexpr int each = kThreads<Lanes> / Lanes;
+    __shared__ float scratch[2 * (Lanes <= 64 ? 1 : Lanes / 64)];
+    const int lane = threadIdx.x % Lanes, size = n.size;
+    int half = 0;
+    const Columns<Vector, Packs, Lanes> after(static_cast<const float *>(n.after), 1.f, lane, size);
+    const Columns<Vector, Packs, Lanes> scale(static_cast<const float *>(n.scales), n.scale, lane, size);
+    const Columns<Vector, Packs, Lanes> before(static_cast<const float *>(n.before), 1.f, lane, size);
+    float sums[kVectors][Packs][Vector] = {};
+    const float count = 1.f / size;
+    for (long long row = (long long)blockIdx.x * each + threadIdx.x / Lanes; row < n.rows; row += (long long)gridDim.x * each) {
+        Held<T, Vector, Packs, Lanes> block, gate{}, x{}, dh{}, dy{}, out;
+        block.Load(RowOf<T>(n.block, n.block_strides, row, n.inner), lane, size);
+        if (n.d_stream) dh.Load(static_cast<const T *>(n.d_stream) + row * size, lane, size);
+        if (n.gate) gate.Load(RowOf<T>(n.gate, n.gate_strides, row, n.inner), lane, size);
+        if constexpr (Stream) {
+            x.Load(RowOf<T>(n.x, n.x_strides, row, n.inner), lane, size);
+            if (n.d_normed) dy.Load(static_cast<const T *>(n.d_normed) + row * size, lane, size);
+        }
+        const float *stats = static_cast<const float *>(n.stats) + 2 * row;
+        const float inner = stats[0], outer = stats[1];
+        float factor[Packs][Vector], u[Packs][Vector], d[Packs][Vector];
+        float sum = 0;
+#pragma unroll
+        for (int i = 0; i < Packs; i++)
+#pragma unroll
+            for (int c = 0; c < Vector; c++) {
+                u[i][c] = block.At(i, c) * inner;
+                factor[i][c] = n.gate ? Gate(gate.At(i, c), n.activation) : 1.f;
+                d[i][c] = dh.At(i, c);
+                if constexpr (Stream) {
+                    const float e = outer * fmaf(scale.x[i][c], after.x[i][c] * factor[i][c] * u[i][c], x.At(i, c));
+                    sums[2][i][c] = fmaf(dy.At(i, c), e, sums[2][i][c]);
+                    sum = fmaf(dy.At(i, c) * before.x[i][c], e, sum);
+                }
+            }
+        if constexpr (Stream) {
+            const float mean = SumOfRow<Lanes>(sum, scratch, half) * count;
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++) {
+                    const float b = after.x[i][c] * factor[i][c] * u[i][c], e = outer * fmaf(scale.x[i][c], b, x.At(i, c));
+                    d[i][c] = fmaf(outer, fmaf(dy.At(i, c), before.x[i][c], -e * mean), d[i][c]);
+                    sums[1][i][c] = fmaf(d[i][c], b, sums[1][i][c]);
+                    out.x[i].x[c] = As<T>(d[i][c]);
+                    d[i][c] *= scale.x[i][c];
+                }
+            if (n.dx) out.Store(static_cast<T *>(n.dx) + row * size, lane, size);
+        }
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < Packs; i++)
+#pragma unroll
+            for (int c = 0; c < Vector; c++) {
+                const float of = d[i][c] * u[i][c];
+                sums[0][i][c] = fmaf(of, factor[i][c], sums[0][i][c]);
+                if (n.gate) out.x[i].x[c] = As<T>(of * after.x[i][c] * GateSlope(gate.At(i, c), n.activation));
+                d[i][c] *= after.x[i][c] * factor[i][c];
+                sum = fmaf(d[i][c], u[i][c], sum);
+            }
+        if (n.d_gate) out.Store(static_cast<T *>(n.d_gate) + row * size, lane, size);
+        const float mean = n.norm_block ? SumOfRow<Lanes>(sum, scratch, half) * count : 0.f;
+#pragma unroll
+        for (int i = 0; i < Packs; i++)
+#pragma unroll
+            for (int c = 0; c < Vector; c++) out.x[i].x[c] = As<T>(inner * fmaf(-u[i][c], mean, d[i][c]));
+        if (n.d_block) out.Store(static_cast<T *>(n.d_block) + row * size, lane, size);
+    }
+    if (!parts) return;
+    // The workgroup's sums over its rows, one vector after the other.
+    __shared__ float shared[each > 1 ? Lanes * Packs * Vector * each : 1];
+    void *const outs[kVectors] = {n.d_after, n.d_scales, n.d_before};
+#pragma unroll
+    for (int v = 0; v < kVectors; v++) {
+        if (!outs[v]) continue;
+        float *to = parts + ((long long)blockIdx.x * kVectors + v) * size;
+        if constexpr (each > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++)
+                    shared[threadIdx.x / Lanes * (Lanes * Packs * Vector) + (i * Lanes + lane) * Vector + c] = sums[v][i][c];
+            __syncthreads();
+            for (int at = threadIdx.x; at < size; at += kThreads<Lanes>) {
+                float sum = 0;
+                for (int r = 0; r < each; r++) sum += shared[r * (Lanes * Packs * Vector) + at];
+                to[at] = sum;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++) {
+                    const int at = (i * Lanes + lane) * Vector + c;
+                    if (at < size) to[at] = sums[v][i][c];
+                }
+        }
+    }
+}
+
+// The sums of all workgroups, always in the same order: 16 columns and 64 threads for each.
+__global__ __launch_bounds__(1024) void PartsKernel(const float *parts, float *after, float *scales, float *before, int size, int blocks) {
+    __shared__ double sums[64][17];
+    const int column = threadIdx.x % 16, slice = threadIdx.x / 16;
+    float *const outs[kVectors] = {after, scales, before};
+    float *out = outs[blockIdx.y];
+    if (!out) return;
+    const int at = blockIdx.x * 16 + column;
+    double sum = 0;
+    if (at < size)
+        for (int r = slice; r < blocks; r += 64) sum += parts[((long long)r * kVectors + blockIdx.y) * size + at];
+    sums[slice][column] = sum;
+    __syncthreads();
+    for (int d = 32; d; d /= 2) {
+        if (slice < d) sums[slice][column] += sums[slice + d][column];
+        __syncthreads();
+    }
+    if (slice == 0 && at < size) out[at] = (float)sums[0][column];
+}
+
+// body(elements of a pack, packs, threads of a row) for rows of `size`.
+template <class T, class Body>
+void ForSize(int size, Body body) {
+    constexpr int V = sizeof(T) == 4 ? 4 : 8;
+    const int packs = (size + V - 1) / V;
+    const auto go = [&](auto packs, auto lanes) { body(std::integral_constant<int, V>(), packs, lanes); };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (packs <= 4) go(One(), std::integral_constant<int, 4>());
+    else if (packs <= 8) go(One(), std::integral_constant<int, 8>());
+    else if (packs <= 16) go(One(), std::integral_constant<int, 16>());
+    else if (packs <= 32) go(One(), std::integral_constant<int, 32>());
+    else if (packs <= 64) go(One(), std::integral_constant<int, 64>());
+    else if (packs <= 128) go(Two(), std::integral_constant<int, 64>());
+    else if (packs <= 256) go(One(), std::integral_constant<int, 256>());
+    else if (packs <= 512) go(Two(), std::integral_constant<int, 256>());
+    else if (packs <= 1024) go(Two(), std::integral_constant<int, 512>());
+    else if constexpr (V == 4) go(std::integral_constant<int, 4>(), std::integral_constant<int, 512>());
+}
+// Workgroups of a launch, which take `each` rows at a time.
+int Blocks(long long rows, int each) {
+    const long long all = (rows + each - 1) / each;
+    return (int)(all < 2048 ? all : 2048);
+}
+
+template <class T>
+void Forward(const Rows &n, hipStream_t stream) {
+    ForSize<T>(n.size, [&](auto vector, auto packs, auto lanes) {
+        constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
+        const dim3 grid(Blocks(n.rows, kThreads<L> / L)), threads(kThreads<L>);
+        if (n.x) hipLaunchKernelGGL((ForwardKernel<T, V, P, L, true>), grid, threads, 0, stream, n);
+        else hipLaunchKernelGGL((ForwardKernel<T, V, P, L, false>), grid, threads, 0, stream, n);
+    });
+}
+template <class T>
+void Backward(const Rows &n, hipStream_t stream) {
+    const bool summed = n.d_after || n.d_scales || n.d_before;
+    float *parts = summed ? static_cast<float *>(n.workspace) : nullptr;
+    int blocks = 0;
+    ForSize<T>(n.size, [&](auto vector, auto packs, auto lanes) {
+        constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
+        blocks = Blocks(n.rows, kThreads<L> / L);
+        if (n.x) hipLaunchKernelGGL((BackwardKernel<T, V, P, L, true>), dim3(blocks), dim3(kThreads<L>), 0, stream, n, parts);
+        else hipLaunchKernelGGL((BackwardKernel<T, V, P, L, false>), dim3(blocks), dim3(kThreads<L>), 0, stream, n, parts);
+    });
+    if (summed)
+        hipLaunchKernelGGL(PartsKernel, dim3((n.size + 15) / 16, kVectors), dim3(1024), 0, stream, parts, static_cast<float *>(n.d_after),
+                           static_cast<float *>(n.d_scales), static_cast<float *>(n.d_before), n.size, blocks);
+}
+
+bool Fits(const Rows *n) {
+    if (!n || n->type < 0 || n->type > 2) return Failed("expected a norm of the type 0, 1 or 2"), false;
+    if (n->activation < kNone || n->activation > kSilu) return Failed("expected an activation from 0 to 2"), false;
+    if (n->rows < 0 || n->inner < 1) return Failed("expected rows"), false;
+    if (n->size < 1 || n->size > kMostSize) return Failed("expected rows of 1 to 8192 values"), false;
+    return true;
+}
+
+}  // namespace
+}  // namespace layers
+
+using namespace layers;
+
+extern "C" __attribute__((visibility("default"))) unsigned long long cuju_row_norm_workspace(const struct cuju_row_norm *norm) {
+    if (!Fits(norm)) return 0;
+    // At least as many workgroups as any launch has.
+    return (unsigned long long)Blocks(norm->rows, 1) * kVectors * norm->size * sizeof(float);
+}
+
+extern "C" __attribute__((visibility("default"))) int cuju_row_norm_forward(const struct cuju_row_norm *norm, void *stream) {
+    if (!Fits(norm)) return -1;
+    const Rows &n = *norm;
+    if (n.rows == 0) return 0;
+    if (!n.block || !n.stream || (n.x && !n.normed)) return Failed("expected rows and their outputs");
+    ForType(n.type, [&](auto x) { Forward<decltype(x)>(n, static_cast<hipStream_t>(stream)); });
+    return Launched("norms of rows");
+}
+
+extern "C" __attribute__((visibility("default"))) int cuju_row_norm_backward(const struct cuju_row_norm *norm, void *stream) {
+    if (!Fits(norm)) return -1;
+    const Rows &n = *norm;
+    if (n.rows == 0) return 0;
+    if (!n.block || !n.stats || (n.d_gate && !n.gate)) return Failed("expected rows, their statistics and a gate for its gradient");
+    if ((n.d_after || n.d_scales || n.d_before) && !n.workspace) return Failed("expected a workspace");
+    ForType(n.type, [&](auto x) { Backward<decltype(x)>(n, static_cast<hipStream_t>(stream)); });
+    return Launched("the gradients of norms of rows");
+}

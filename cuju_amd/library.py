@@ -114,6 +114,16 @@ SIGNATURES = [
     ('cuju_group_norm_workspace', U64, [ctypes.c_char_p]),
     ('cuju_group_norm_forward', I, [ctypes.c_char_p, P]),
     ('cuju_group_norm_backward', I, [ctypes.c_char_p, P]),
+    ('cuju_linear_attention_step', I, [ctypes.c_char_p, P]),
+    ('cuju_linear_attention_forward_workspace', U64, [ctypes.c_char_p]),
+    ('cuju_linear_attention_forward', I, [ctypes.c_char_p, P]),
+    ('cuju_linear_attention_backward_workspace', U64, [ctypes.c_char_p]),
+    ('cuju_linear_attention_backward', I, [ctypes.c_char_p, P]),
+    ('cuju_row_norm_workspace', U64, [ctypes.c_char_p]),
+    ('cuju_row_norm_forward', I, [ctypes.c_char_p, P]),
+    ('cuju_row_norm_backward', I, [ctypes.c_char_p, P]),
+    ('cuju_clip_gradients_workspace', U64, [ctypes.c_char_p]),
+    ('cuju_clip_gradients', I, [ctypes.c_char_p, P]),
 ]
 
 _loaded = {}

@@ -230,6 +230,83 @@ unsigned long long cuju_group_norm_workspace(const struct cuju_group_norm *norm)
 int cuju_group_norm_forward(const struct cuju_group_norm *norm, void *stream);
 int cuju_group_norm_backward(const struct cuju_group_norm *norm, void *stream);
 
+/* Linear attention with decays. A head's memory is a matrix S [key_size][value_size] of floats. Step t
+   clears it where `resets` is nonzero, scales it by exp(decay), and adds the step's product:
+   S += key value^T, output = scale S^T query. Heads, strides, sizes and what is contiguous are as for
+   the delta rule; a decay that is the same at every step has strides of 0. */
+struct cuju_linear_attention {
+    int type, batch, time, key_heads, heads, key_size, value_size;
+    int decay_of_head;               /* whether d_decay is one value for each head, summed over batch and steps */
+    float scale;
+    const void *query, *key, *value; /* of `type` */
+    const void *decay;               /* float, the logarithm of the factor */
+    const unsigned char *resets;     /* or null */
+    long long query_strides[3], key_strides[3], value_strides[3], decay_strides[3], reset_strides[2];
+    void *state;                     /* [batch][heads][key_size][value_size], or null for zeros; a step updates it */
+    void *output;                    /* of `type`, [batch][time][heads][value_size] */
+    void *last;                      /* the memory after the last step, or null */
+    void *checkpoints;               /* [batch][heads][(time - 1) / 128][key_size][value_size]: the forward pass keeps the
+                                        memory before every 128th step for the backward pass; null for none */
+    /* Only for the backward pass. */
+    const void *d_output;            /* of `type` */
+    long long d_output_strides[3];
+    const void *d_last;              /* or null for zeros */
+    void *d_query, *d_key, *d_value; /* of `type` */
+    void *d_decay;                   /* [batch][time][heads] or [heads], or null */
+    void *d_state;                   /* or null */
+    void *workspace;                 /* the pass's bytes of workspace */
+};
+/* One step (time 1), the memory updated in place. */
+int cuju_linear_attention_step(const struct cuju_linear_attention *attention, void *stream);
+/* Bytes of workspace that a pass needs, or 0; it depends on which of `checkpoints` and `d_decay` are null. */
+unsigned long long cuju_linear_attention_forward_workspace(const struct cuju_linear_attention *attention);
+int cuju_linear_attention_forward(const struct cuju_linear_attention *attention, void *stream);
+unsigned long long cuju_linear_attention_backward_workspace(const struct cuju_linear_attention *attention);
+int cuju_linear_attention_backward(const struct cuju_linear_attention *attention, void *stream);
+
+/* Norms around a block, over rows of `size` values (1 to 8192), in two axes [rows / inner][inner] with strides in
+   elements; the values of a row are contiguous, and outputs and gradients are contiguous.
+     b = after act(gate) block / sqrt(mean(block^2) + epsilon)   (without the root where `norm_block` is 0)
+     stream = x + scale b                                        (b where x is null)
+     normed = before stream / sqrt(mean(stream^2) + epsilon)     (only where there is x)
+   Activations: 0 none, 1 sigmoid, 2 silu. */
+struct cuju_row_norm {
+    int type, size, inner, activation, norm_block;
+    float epsilon, scale;            /* `scale` where `scales` is null */
+    long long rows;
+    const void *x, *block, *gate;    /* of `type`; x and gate or null */
+    long long x_strides[2], block_strides[2], gate_strides[2];
+    const void *after, *scales, *before; /* float [size], or null for ones */
+    void *stream, *normed;
+    void *stats;                     /* float [rows][2], written forward unless null: 1 / sqrt(..) of block and stream */
+    /* Only for the backward pass. */
+    const void *d_stream, *d_normed; /* contiguous, or null for zeros */
+    void *dx, *d_block, *d_gate;     /* or null */
+    void *d_after, *d_scales, *d_before; /* float [size], or null */
+    void *workspace;                 /* cuju_row_norm_workspace() bytes, for the sums over rows */
+};
+unsigned long long cuju_row_norm_workspace(const struct cuju_row_norm *norm);
+int cuju_row_norm_forward(const struct cuju_row_norm *norm, void *stream);
+int cuju_row_norm_backward(const struct cuju_row_norm *norm, void *stream);
+
+/* Gradients clipped by their global norm: with n the root of the sum of all squares, in 64 bits, every value is
+   multiplied by min(1, most / (n + epsilon)), in place. The tensors' data must not overlap. `most` of infinity leaves them as
+   they are. */
+struct cuju_gradient {
+    void *data;                      /* device memory */
+    long long size;                  /* values, side by side */
+    long long type;
+};
+struct cuju_gradients {
+    long long count;
+    const struct cuju_gradient *gradients; /* in host memory, read during the call */
+    double most, epsilon;
+    void *norm;                      /* float, on the device */
+    void *workspace;                 /* cuju_clip_gradients_workspace() bytes */
+};
+unsigned long long cuju_clip_gradients_workspace(const struct cuju_gradients *gradients);
+int cuju_clip_gradients(const struct cuju_gradients *gradients, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,24 +18,25 @@
 #include "../../../include/cuju_amd.h"
 #include "steps.h"
 
-#include <array>
-
 namespace layers {
 
 using Attention = cuju_linear_attention;
 constexpr int kSpan = 128;
 
+struct Tensor {
+    const void *p;
+    long long strides[3];  // [batch][time][head]
+    int share;             // heads that share one of its heads
+};
 // One run of the recurrence over all heads.
 struct Run {
-    const void *query, *key, *value, *weight;  // weight: what the outputs' dots are taken with, or null
-    long long queryStrides[3], keyStrides[3], valueStrides[3], weightStrides[3];
-    int queryHeads, keyHeads, valueHeads, weightHeads;  // heads that share one of the tensor's
-    int rows, columns, slices;
+    Tensor query, key, value, weight;  // weight: what the outputs' dots are taken with, or null
+    int rows, columns;
     bool reverse, transposed;  // whether steps go backwards, and memories lie [column][row]
+    bool floats;               // whether the output is float, whatever the type
     float in, out;             // factors of what is written and of what is read
     void *output;
     long long outputStrides[3];
-    bool floats;          // whether the output is float, whatever the type
     const float *first;   // the memory at the run's start, or null for zeros
     const float *starts;  // at the start of its other spans, [head][spans - 1], in the order of time
     float *last;          // the memory at the end of the run, or null (backwards: before the first step)
@@ -45,15 +46,41 @@ struct Run {
     float *crossings;                    // [slice][head][span]
 };
 struct Runs {
-    int time, heads, length, spans, firstSpan, spanCount, units;  // length: steps of a span; units: slices of all runs
+    int time, heads, length, spans, firstSpan, spanCount;  // length: steps of a span
+    int units, slices[3];                                  // slices of all runs and of each
     unsigned firstHead, allHeads;
     const float *decay;
     const unsigned char *resets;
     long long decayStrides[3], resetStrides[2];
+    bool near;       // whether 32 steps of every tensor are within 2^31 bytes
     float *factors;  // [head][spans - 1]: the product of a span's factors, or -1 where an episode starts in it
     Run run[3];
 };
+// A run out of the kernel's arguments, where an index that the compiler does not know would copy them all.
+__device__ __forceinline__ Run RunAt(int which) {
+    using Word = const __attribute__((address_space(4))) uint32_t;
+    Word *p = (Word *)((const __attribute__((address_space(4))) char *)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(Runs, run)) +
+              which * (sizeof(Run) / 4);
+    struct Words {
+        uint32_t x[sizeof(Run) / 4];
+    } words;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Run) / 4); i++) words.x[i] = p[i];
+    return __builtin_bit_cast(Run, words);
+}
+// A tensor's steps of one head, in the order in which a run plays them.
+template <class T>
+struct Line {
+    const T *p;
+    long long step;
+    __device__ __forceinline__ const T *At(int i) const { return p + i * step; }
+};
 
+enum Shape {
+    kLoose,  // sizes and strides that packs of four elements do not fit
+    kWhole,  // that they fit
+    kFull    // and sizes that the tiles fit
+};
 enum Mode {
     kMemory,   // the memory alone, from zeros, at the end of every span that has another behind it
     kOutputs,  // outputs
@@ -69,10 +96,12 @@ struct Step {
     __device__ __forceinline__ bool Steep() const { return !(decay <= 2.f); }
 };
 
-// Wavefronts that a SIMD has to hold.
+// Wavefronts that a SIMD has to hold, and whether the next steps' keys and queries are on their way while the
+// values of these are worked on.
 template <class T, int KeyTiles, int Tiles, Mode mode>
 constexpr int kRunWaves = 2;
-
+template <class T, int KeyTiles, int Tiles>
+constexpr bool kRunsAhead = KeyTiles * (Tiles * 4 + (int)sizeof(T) * 4 + kPieces<T> * 4) <= 112;
 constexpr int kSteps = 2 * kChunk;  // steps that are played together: two tiles of the matrix instruction
 
 // Sums over the products of pieces whose places add up to less than `Most`.
@@ -107,14 +136,93 @@ __device__ __forceinline__ void SplitPair(F4 lo, F4 hi, B8 (&x)[Pieces]) {
     Split<Pieces>(first, a), Split<Pieces>(second, b);
     Eights(a, b, x);
 }
-// Eight elements in memory.
+// Elements as the 32-bit words of memory: an array of 16-bit elements would take a register for each of them.
+template <int N>
+struct Words {
+    uint32_t x[N];
+};
+template <class T, int N>
+constexpr int kWords = N * (int)sizeof(T) < 4 ? 1 : N * (int)sizeof(T) / 4;
 template <class T>
-__device__ __forceinline__ void PiecesOf(const Pack<T, 8> &x, B8 (&piece)[kPieces<T>]) {
-    struct Halves {
-        Pack<T, 4> x[2];
-    };
-    const Halves h = __builtin_bit_cast(Halves, x);
-    Pair<T>(h.x[0], h.x[1], piece);
+__device__ __forceinline__ uint32_t Bits(T x) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
+    else return __builtin_bit_cast(uint16_t, x);
+}
+// N elements from a place aligned to `Aligned` of them, the first `valid` real and the others zero. `Whole`: either all or none.
+template <class T, int N, bool Whole, int Aligned = N>
+__device__ __forceinline__ Words<kWords<T, N>> LoadWords(const T *p, int valid = N) {
+    constexpr int kElements = 4 / sizeof(T);
+    Words<kWords<T, N>> w{};
+    if constexpr (!Whole) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (i < valid) w.x[i / kElements] |= Bits(p[i]) << (16 * (i % kElements));
+    } else if constexpr (N * sizeof(T) < 4) {
+        if (valid > 0) w.x[0] = Bits(*p);
+    } else {
+        struct __attribute__((packed, aligned(Aligned * sizeof(T)))) InMemory {
+            Words<kWords<T, N>> w;
+        };
+        if (valid > 0) w = reinterpret_cast<const InMemory *>(p)->w;
+    }
+    return w;
+}
+// The same at `base`, which all lanes share, and a lane's `place` in bytes. The place is made anew where it is used: an
+// address of a scalar and one register is only found within a block of the program.
+template <class T, int N, bool Whole>
+__device__ __forceinline__ Words<kWords<T, N>> WordsAt(const T *base, int place, int valid) {
+    if constexpr (!Whole) {
+        return LoadWords<T, N, false>(Lane(base, place), valid);
+    } else {
+        Words<kWords<T, N>> w{};
+        if (valid > 0) w = LoadWords<T, N, true>(Lane(base, Renewed(place)));
+        return w;
+    }
+}
+template <int N, bool Whole, class T>
+__device__ __forceinline__ Pack<T, N> LoadAt(const T *base, int place, int valid) {
+    if constexpr (!Whole) {
+        return Load<N, false>(Lane(base, place), valid);
+    } else {
+        Pack<T, N> x{};
+        if (valid > 0) x = Load<N, true>(Lane(base, Renewed(place)), N);
+        return x;
+    }
+}
+template <int N, bool Whole, class T>
+__device__ __forceinline__ void StoreAt(T *base, int place, const Pack<T, N> &x, int valid) {
+    if constexpr (!Whole) Store<N, false>(Lane(base, place), x, valid);
+    else if (valid > 0) Store<N, true>(Lane(base, Renewed(place)), x, N);
+}
+// Element i of such words.
+template <class T, int N>
+__device__ __forceinline__ float ElementOf(const Words<N> &w, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w.x[i]);
+    else if constexpr (std::is_same<T, __hip_bfloat16>::value) return __uint_as_float(i % 2 ? w.x[i / 2] & 0xffff0000u : w.x[i / 2] << 16);
+    else return __half2float(__builtin_bit_cast(__half, (uint16_t)(i % 2 ? w.x[i / 2] >> 16 : w.x[i / 2])));
+}
+// The pieces of a lane's eight neighbouring elements, and of the elements i of four places.
+template <class T, int N>
+__device__ __forceinline__ void PiecesOf(const Words<N> &w, B8 (&piece)[kPieces<T>]) {
+    if constexpr (kPieces<T> == 1) {
+        piece[0] = __builtin_bit_cast(B8, w);
+    } else {
+        F4 half[2];
+#pragma unroll
+        for (int i = 0; i < 8; i++) half[i / 4][i % 4] = ElementOf<T>(w, i);
+        SplitPair<kPieces<T>>(half[0], half[1], piece);
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ void PiecesOf(const Words<N> (&w)[4], int i, Four (&piece)[kPieces<T>]) {
+    if constexpr (kPieces<T> == 1) {
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+            piece[0].x[j] = __builtin_amdgcn_perm(w[2 * j + 1].x[i / 2], w[2 * j].x[i / 2], i % 2 ? 0x07060302 : 0x05040100);
+    } else {
+        const float f[4] = {ElementOf<T>(w[0], i), ElementOf<T>(w[1], i), ElementOf<T>(w[2], i), ElementOf<T>(w[3], i)};
+        Split<kPieces<T>>(f, piece);
+    }
 }
 
 // One wavefront takes 16 * Tiles columns of a head's memory through a span, 32 steps at a time, with the memory in
@@ -129,11 +237,13 @@ __device__ __forceinline__ void PiecesOf(const Pack<T, 8> &x, B8 (&piece)[kPiece
 // A lane holds eight neighbouring rows of a pair of tiles: rows 32 p + 8 g + 4 x + r of the tiles 2 p + x, so that its
 // keys are 16 bytes of memory. Which rows a tile has is free as long as queries, keys and memory agree.
 //
-// The products over a chunk's steps take a NaN or an infinity of a key or value, times a zero, to all of them. A chunk
-// that has one, or factors past e^2, is played step by step.
-template <class T, int KeyTiles, int Tiles, bool Whole, Mode mode>
+// The products over a chunk's steps take a NaN or an infinity of a key or value, times a zero, to all of them. A wavefront
+// that meets one, or a factor past e^2, begins its span again and plays it step by step.
+template <class T, int KeyTiles, int Tiles, Shape shape, Mode mode>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T, KeyTiles, Tiles, mode>))) void RunKernel(Runs a) {
     constexpr int P = kPieces<T>, kPairs = KeyTiles / 2;
+    constexpr bool Whole = shape != kLoose, full = shape == kFull;
+    constexpr bool kAhead = kRunsAhead<T, KeyTiles, Tiles>;
     constexpr int kHeld = mode == kGradient || P == kFloatPieces ? kFloatPieces : 2;
     __shared__ double reach[kSteps];
     __shared__ __align__(16) float wholes[kSteps], afters[kSteps], diagonal[kSteps];
@@ -143,37 +253,36 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
     id /= a.units;
     const int span = a.firstSpan + id % a.spanCount;
     const unsigned head = a.firstHead + id / a.spanCount;
-    while (slice >= a.run[which].slices) slice -= a.run[which++].slices;
-    const Run &run = a.run[which];
+    while (slice >= a.slices[which]) slice -= a.slices[which++];
+    const Run run = RunAt(which);
     const int h = head % a.heads, b = head / a.heads;
-    const int rows = run.rows, columns = run.columns;
+    const int rows = full ? 16 * KeyTiles : run.rows, columns = run.columns;
     const bool reverse = run.reverse;
-    const int column = slice * 16 * Tiles + m * Tiles, mine = max(0, min(Tiles, columns - column));
+    const int column = slice * 16 * Tiles + m * Tiles, firstColumn = column;
+    const int mine = full ? Tiles : max(0, min(Tiles, columns - column)), ownColumns = mine;
     const int begin = span * a.length, count = min(a.length, a.time - begin);
     const long long size = (long long)rows * columns, before = (long long)head * (a.spans - 1);
     const auto rowOf = [&](int t) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1); };
 
     F4 s[KeyTiles][Tiles];
-#pragma unroll
-    for (int t = 0; t < KeyTiles; t++)
-#pragma unroll
-        for (int c = 0; c < Tiles; c++) s[t][c] = F4{0, 0, 0, 0};
     // take(element of the run's memory, element of another) in its place.
     const auto read = [&](const float *memory, auto take) {
+        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), columns = Opaque(run.columns);
+        const int lanes = (run.transposed ? column * rows + 8 * g : 8 * g * columns + column) * 4;
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++) {
-            const int row = rowOf(t);
+            const int row = 32 * (t >> 1) + 4 * (t & 1);
             if (run.transposed) {
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
-                    const auto x = Load<4, Whole>(memory + (long long)(column + c) * rows + row, c < mine ? rows - row : 0);
+                    const auto x = LoadAt<4, Whole>(memory + c * rows + row, lanes, c < mine ? rows - row - 8 * g : 0);
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[t][c][r] = take(s[t][c][r], x.x[r]);
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const auto x = Load<Tiles, Whole>(memory + (long long)(row + r) * columns + column, row + r < rows ? mine : 0);
+                    const auto x = LoadAt<Tiles, Whole>(memory + (row + r) * columns, lanes, row + r + 8 * g < rows ? mine : 0);
 #pragma unroll
                     for (int c = 0; c < Tiles; c++) s[t][c][r] = take(s[t][c][r], x.x[c]);
                 }
@@ -181,35 +290,63 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         }
     };
     const auto write = [&](float *memory) {
+        // What follows from these is not kept over the loop.
+        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), columns = Opaque(run.columns), mine = full ? Tiles : Renewed(ownColumns);
+        const int lanes = (8 * g * columns + Renewed(firstColumn)) * 4;
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = rowOf(t) + r;
+                const int row = 32 * (t >> 1) + 4 * (t & 1) + r;
                 Pack<float, Tiles> x;
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) x.x[c] = s[t][c][r];
-                Store<Tiles, Whole>(memory + (long long)row * columns + column, x, row < rows ? mine : 0);
+                StoreAt<Tiles, Whole>(memory + row * columns, lanes, x, row + 8 * g < rows ? mine : 0);
             }
     };
-    if constexpr (mode != kMemory) {
-        const bool starts = reverse ? span == a.spans - 1 : span == 0;
-        const float *memory = starts ? run.first : run.starts;
-        if (memory)
-            read(memory + (starts ? (long long)head : before + (reverse ? span : span - 1)) * size, [](float, float y) { return y; });
-    }
+    const auto begins = [&] {
+#pragma unroll
+        for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+            for (int c = 0; c < Tiles; c++) s[t][c] = F4{0, 0, 0, 0};
+        if constexpr (mode != kMemory) {
+            const bool starts = reverse ? span == a.spans - 1 : span == 0;
+            const float *memory = starts ? run.first : run.starts;
+            if (memory)
+                read(memory + (starts ? (long long)head : before + (reverse ? span : span - 1)) * size, [](float, float y) { return y; });
+        }
+    };
+    const auto keep = [&](int i) {
+        if constexpr (mode == kOutputs)
+            if (run.kept && i > 0 && i % kSpan == 0)
+                write(run.kept + ((long long)head * ((a.time - 1) / kSpan) + i / kSpan - 1) * size);
+    };
 
-    // The time of the span's step i, and what the memory is scaled by on the way to it: backwards in time that is the
-    // factor of the step that comes after it in time, and none for the first.
-    const auto timeOf = [&](int i) { return reverse ? begin + count - 1 - i : begin + i; };
-    const auto gateAt = [&](int t) {
-        Step step{Global(a.decay)[b * a.decayStrides[0] + t * a.decayStrides[1] + h * a.decayStrides[2]], 0};
-        if (a.resets) step.reset = Global(a.resets)[b * a.resetStrides[0] + t * a.resetStrides[1]];
+    // The tensors' lines of this head, from the span's first step on. What the memory is scaled by on the way to a step is,
+    // backwards in time, the factor of the step that comes after it in time, and nothing for the first.
+    const int opens = reverse ? begin + count - 1 : begin, sign = reverse ? -1 : 1;
+    const auto lineOf = [&](const Tensor &x, auto type) {
+        using Element = decltype(type);
+        return Line<Element>{Global(static_cast<const Element *>(x.p)) + b * x.strides[0] + opens * x.strides[1] + h / x.share * x.strides[2],
+                             sign * x.strides[1]};
+    };
+    const Line<T> keyLine = lineOf(run.key, T()), valueLine = lineOf(run.value, T());
+    const Line<T> queryLine = mode != kMemory ? lineOf(run.query, T()) : Line<T>{};
+    const Line<T> weightLine = mode == kGradient && run.weight.p ? lineOf(run.weight, T()) : Line<T>{};
+    const int late = reverse ? 1 : 0;
+    const Line<float> decayLine{Global(a.decay) + b * a.decayStrides[0] + (opens + late) * a.decayStrides[1] + h * a.decayStrides[2],
+                                sign * a.decayStrides[1]};
+    const Line<unsigned char> resetLine{a.resets ? Global(a.resets) + b * a.resetStrides[0] + (opens + late) * a.resetStrides[1] : nullptr,
+                                        sign * a.resetStrides[1]};
+    const auto gateAt = [&](int i) {
+        Step step{*decayLine.At(i), 0};
+        if (resetLine.p) step.reset = *resetLine.At(i);
         return step;
     };
-    const auto gateOf = [&](int i) {
-        return i < count && (i > 0 || !reverse) ? gateAt(reverse ? timeOf(i) + 1 : timeOf(i)) : Step{0.f, 0};
-    };
+    const Line<char> outputLine{static_cast<const char *>(run.output) + (b * run.outputStrides[0] + opens * run.outputStrides[1] + h * run.outputStrides[2]) *
+                                                                            (run.floats ? 4 : (int)sizeof(T)),
+                                sign * run.outputStrides[1] * (run.floats ? 4 : (int)sizeof(T))};
+    float *const dots = run.dots + ((long long)slice * a.allHeads + head) * a.time + opens;
     const auto scale = [&](Step gate) {
         const bool cleared = gate.Cleared();
         const float kept = cleared ? 0.f : expf(gate.decay);
@@ -220,33 +357,31 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[t][c][r] = cleared ? 0.f : kept * s[t][c][r];
     };
-    const auto at = [&](const void *p, const long long *strides, int heads, int t) {
-        return Global(static_cast<const T *>(p)) + b * strides[0] + t * strides[1] + h / heads * strides[2];
-    };
-    const auto put = [&](int t, const float (&x)[Tiles], int valid) {
-        const long long to = b * run.outputStrides[0] + t * run.outputStrides[1] + h * run.outputStrides[2] + column;
+    // Stores the outputs of the step at `place` in time, counted from the one at `base`.
+    const auto put = [&](const char *base, int place, const float (&x)[Tiles], int valid) {
+        const int step = sign * (int)outputLine.step;
         if (run.floats) {
             Pack<float, Tiles> o;
 #pragma unroll
             for (int c = 0; c < Tiles; c++) o.x[c] = x[c];
-            Store<Tiles, Whole>(Global(static_cast<float *>(run.output)) + to, o, valid);
+            StoreAt<Tiles, Whole>(reinterpret_cast<float *>(const_cast<char *>(base)), place * step + 4 * column, o, valid);
         } else {
             Pack<T, Tiles> o;
 #pragma unroll
             for (int c = 0; c < Tiles; c++) o.x[c] = As<T>(x[c]);
-            Store<Tiles, Whole>(Global(static_cast<T *>(run.output)) + to, o, valid);
+            StoreAt<Tiles, Whole>(reinterpret_cast<T *>(const_cast<char *>(base)), place * step + (int)sizeof(T) * column, o, valid);
         }
     };
 
-    // Steps one after the other.
-    const auto playSteps = [&](int first, int past) {
+    // All steps, one after the other.
+    const auto playSteps = [&] {
+        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), mine = full ? Tiles : Renewed(ownColumns), column = Renewed(firstColumn);
 #pragma unroll 1
-        for (int i = first; i < past; i++) {
-            const int t = timeOf(i);
-            const auto v = Load<Tiles, Whole>(at(run.value, run.valueStrides, run.valueHeads, t) + column, mine);
-            if (i > 0 || !reverse) scale(gateOf(i));
-            const T *key = at(run.key, run.keyStrides, run.keyHeads, t);
-            const T *query = mode == kMemory ? nullptr : at(run.query, run.queryStrides, run.queryHeads, t);
+        for (int i = 0; i < count; i++) {
+            keep(i);
+            const auto v = Load<Tiles, Whole>(valueLine.At(i) + column, mine);
+            if (i >= late) scale(gateAt(i));
+            const T *key = keyLine.At(i), *query = mode == kMemory ? nullptr : queryLine.At(i);
             float strict[Tiles] = {}, own = 0;
 #pragma unroll
             for (int x = 0; x < KeyTiles; x++) {
@@ -269,7 +404,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 own += __shfl_xor(own, 32);
                 Pack<T, Tiles> w{};
                 if constexpr (mode == kGradient)
-                    if (run.weight) w = Load<Tiles, Whole>(at(run.weight, run.weightStrides, run.weightHeads, t) + column, mine);
+                    if (weightLine.p) w = Load<Tiles, Whole>(weightLine.At(i) + column, mine);
                 float dot = 0;
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
@@ -279,61 +414,113 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     if (c < mine) dot = fmaf(strict[c], Float(w.x[c]), dot);
                     strict[c] = fmaf(run.out * run.in * own, Float(v.x[c]), strict[c]);
                 }
-                put(t, strict, g == 0 ? mine : 0);
+                put(outputLine.At(i), 0, strict, g == 0 ? mine : 0);
                 if constexpr (mode == kGradient) {
                     dot = RowSum(dot);
-                    if (run.weight && lane == 0) run.dots[((long long)slice * a.allHeads + head) * a.time + t] = dot;
+                    if (weightLine.p && lane == 0) dots[sign * i] = dot;
                 }
             }
         }
     };
 
     // The inputs of the steps from `first`: of a lane's steps m and 16 + m the keys and queries, of its steps 4 g + r and
-    // 16 + 4 g + r the values. Past the end the last step is read again.
-    Pack<T, 8> nextK[2][kPairs], nextQ[2][kPairs];
-    Pack<T, Tiles> nextV[2][4];
+    // 16 + 4 g + r the values and weights. Past the end the last step is read again. In whole chunks of whole tensors an
+    // address is one that all lanes share and a lane's offset of 32 bits.
+    using RowWords = Words<kWords<T, 8>>;
+    using ColumnWords = Words<kWords<T, Tiles>>;
+    RowWords nextK[2][kPairs], nextQ[2][kPairs];
+    ColumnWords nextV[2][4];
     Step nextGate[2];
-    const auto eight = [&](const T *p, int row) {
-        struct Halves {
-            Pack<T, 4> x[2];
-        } h{Load<4, Whole>(p + row, rows - row), Load<4, Whole>(p + row + 4, rows - row - 4)};
-        return __builtin_bit_cast(Pack<T, 8>, h);
-    };
-    const auto fetchKeys = [&](int first) {
+    // An address is one that all lanes share, that of the chunk's first step in time, and a lane's offset of 32 bits.
+    const auto lowest = [&](const auto &line, int first) { return line.At(first + (reverse ? kSteps - 1 : 0)); };
+    const auto placeOf = [&](int i) { return reverse ? kSteps - 1 - i : i; };
+    const auto keysAt = [&](const Line<T> &line, int first, RowWords(&x)[2][kPairs]) {
+        const T *base = lowest(line, first);
+        const int last = min(kSteps, count - first) - 1, step = sign * (int)line.step;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const int t = timeOf(min(first + 16 * n + m, count - 1));
-            const T *key = at(run.key, run.keyStrides, run.keyHeads, t);
+            const int place = (placeOf(min(16 * n + Renewed(m), last)) * step + 8 * g) * (int)sizeof(T);
+            if constexpr (full) {
+                const uint32_t lanes = Renewed(place);
 #pragma unroll
-            for (int p = 0; p < kPairs; p++) nextK[n][p] = eight(key, rowOf(2 * p));
-            if constexpr (mode != kMemory) {
-                const T *query = at(run.query, run.queryStrides, run.queryHeads, t);
+                for (int q = 0; q < kPairs; q++) x[n][q] = LoadWords<T, 8, true, 4>(Lane(base + 32 * q, lanes));
+            } else {
+                const int left = Opaque(run.rows) - 8 * g;
 #pragma unroll
-                for (int p = 0; p < kPairs; p++) nextQ[n][p] = eight(query, rowOf(2 * p));
+                for (int q = 0; q < kPairs; q++) {
+                    struct Halves {
+                        Words<kWords<T, 4>> x[2];
+                    } half;
+#pragma unroll
+                    for (int i = 0; i < 2; i++) half.x[i] = WordsAt<T, 4, Whole>(base + 32 * q + 4 * i, place, left - 32 * q - 4 * i);
+                    x[n][q] = __builtin_bit_cast(RowWords, half);
+                }
             }
         }
+    };
+    const auto valuesAt = [&](const Line<T> &line, int first, ColumnWords(&x)[2][4]) {
+        const T *base = lowest(line, first);
+        const int last = min(kSteps, count - first) - 1, step = sign * (int)line.step;
+        const int mine = full ? Tiles : Renewed(ownColumns), column = Renewed(firstColumn);
+        if (full && last == kSteps - 1) {
+            const uint32_t lanes = Renewed(((reverse ? 12 - 4 * g : 4 * g) * step + column) * (int)sizeof(T));
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    x[n][r] = LoadWords<T, Tiles, true>(Lane(base + (long long)(reverse ? 19 - 16 * n - r : 16 * n + r) * step, lanes));
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    x[n][r] = WordsAt<T, Tiles, Whole>(base, (placeOf(min(16 * n + 4 * g + r, last)) * step + column) * (int)sizeof(T), mine);
+        }
+    };
+    // Past the end nothing is fetched, and what was fetched before is given up: its registers are free until then.
+    const auto fetchKeys = [&](int first) {
+        if (first >= count) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int q = 0; q < kPairs; q++) nextK[n][q] = nextQ[n][q] = RowWords{};
+            return;
+        }
+        keysAt(keyLine, first, nextK);
+        if constexpr (mode != kMemory) keysAt(queryLine, first, nextQ);
     };
     const auto fetchValues = [&](int first) {
+        if (first >= count) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                nextGate[n] = Step{};
+#pragma unroll
+                for (int r = 0; r < 4; r++) nextV[n][r] = ColumnWords{};
+            }
+            return;
+        }
+        valuesAt(valueLine, first, nextV);
+        const float *decays = lowest(decayLine, first);
+        const unsigned char *resets = resetLine.p ? lowest(resetLine, first) : nullptr;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            nextGate[n] = gateOf(first + 16 * n + m);
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = timeOf(min(first + 16 * n + 4 * g + r, count - 1));
-                nextV[n][r] = Load<Tiles, Whole>(at(run.value, run.valueStrides, run.valueHeads, t) + column, mine);
+            const int i = 16 * n + Renewed(m);
+            nextGate[n] = Step{0.f, 0};
+            if (first + i < count && first + i >= late) {
+                nextGate[n].decay = *Lane(decays, Renewed(placeOf(i) * sign * (int)decayLine.step * 4));
+                if (resets) nextGate[n].reset = *Lane(resets, Renewed(placeOf(i) * sign * (int)resetLine.step));
             }
         }
     };
-
     const Eyes eyes = EyesOf(m, g);
-    const auto ones = __builtin_bit_cast(B8, std::array<uint32_t, 4>{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-    if (count > 0) fetchKeys(0), fetchValues(0);
+    // Steps that are too far apart for 32 bits are played one by one.
+    bool finite = a.near;
+    begins();
+    if (finite) fetchKeys(0), fetchValues(0);
 #pragma unroll 1
-    for (int first = 0; first < count; first += kSteps) {
+    for (int first = 0; first < count && finite; first += kSteps) {
         const int valid = min(kSteps, count - first);
-        if constexpr (mode == kOutputs)
-            if (run.kept && first > 0 && first % kSpan == 0)
-                write(run.kept + ((long long)head * ((a.time - 1) / kSpan) + first / kSpan - 1) * size);
+        keep(first);
 
         // Pieces of the keys and queries; products with the memory, the scores, and the keys' transpose.
         F4 mark = {0, 0, 0, 0}, scores[3], o[2][Tiles];  // scores: of the tiles 00, 10 and 11, in row order
@@ -350,7 +537,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 PiecesOf<T>(nextK[n][p], kp[n]);
-                mark = Mfma32(ones, kp[n][0], mark);
+                mark = Mfma32(eyes.half[0], kp[n][0], mark);
                 Turn<P>(kp[n], eyes.half[0], turned[n][2 * p]);
                 Turn<P>(kp[n], eyes.half[1], turned[n][2 * p + 1]);
             }
@@ -368,42 +555,34 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     for (int n = 0; n < 2; n++) o[n][c] = MfmaMost<kHeld>(qp[n], sp, o[n][c]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        Pack<T, Tiles> v[2][4];
+        ColumnWords v[2][4], w[2][4];
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[n][r] = 16 * n + 4 * g + r < valid ? nextV[n][r] : Pack<T, Tiles>{};
+            for (int r = 0; r < 4; r++) v[n][r] = valid == kSteps || 16 * n + 4 * g + r < valid ? nextV[n][r] : ColumnWords{};
         const Step gate[2] = {nextGate[0], nextGate[1]};
-        Pack<T, Tiles> w[2][4];
-        if constexpr (mode == kGradient)
-            if (run.weight)
+        if constexpr (mode == kGradient) {
+            if (weightLine.p) valuesAt(weightLine, first, w);
+            else
 #pragma unroll
                 for (int n = 0; n < 2; n++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[n][r] = Load<Tiles, Whole>(at(run.weight, run.weightStrides, run.weightHeads,
-                                                        timeOf(min(first + 16 * n + 4 * g + r, count - 1))) + column, mine);
-        if (first + kSteps < count) fetchKeys(first + kSteps), fetchValues(first + kSteps);
-
-        // The values as right operands, [piece].
-        B8 vp[Tiles][P];
+                    for (int r = 0; r < 4; r++) w[n][r] = ColumnWords{};
+        }
+        // A product with anything, zeros too, tells whether a value is not finite.
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             Four half[2][P];
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const Pack<T, 4> x{{v[n][0].x[c], v[n][1].x[c], v[n][2].x[c], v[n][3].x[c]}};
-                Split<T>(x, half[n]);
-            }
-            Eights(half[0], half[1], vp[c]);
-            mark = Mfma32(ones, vp[c][0], mark);
+            for (int n = 0; n < 2; n++) PiecesOf<T>(v[n], c, half[n]);
+            mark = Mfma32(eyes.half[0], Eight(half[0][0], half[1][0]), mark);
         }
         if (__ballot(mark[0] * 0.f != 0.f || gate[0].Steep() || gate[1].Steep())) {
-            playSteps(first, first + valid);
-            continue;
+            finite = false;
+            break;
         }
-
+        __builtin_amdgcn_sched_barrier(0);
         // How the chunk is cut, and the products of its factors.
         const bool cleared[2] = {gate[0].Cleared(), gate[1].Cleared()};
         const unsigned cuts = (unsigned)(__ballot(cleared[0]) & 0xffff) | (unsigned)(__ballot(cleared[1]) & 0xffff) << 16;
@@ -431,77 +610,73 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         __syncthreads();
 
         if constexpr (mode != kMemory) {
-            const float both = run.in * run.out;
-            const bool strict = mode == kGradient;
-            F4 mixed[3];
-#pragma unroll
-            for (int x = 0; x < 3; x++) {
-                const int n = x > 0, j0 = x == 2 ? 16 : 0;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int i = 16 * n + m, j = j0 + 4 * g + r;
-                    const float d = both * Exp2(G[n] - reach[j]);
-                    if (mode == kGradient && x != 1 && i == j) diagonal[i] = both * scores[x][r];
-                    mixed[x][r] = j >= start[n] && (strict ? j < i : j <= i) ? d * scores[x][r] : 0.f;
-                }
-            }
-            Four lower[3][kHeld];
-#pragma unroll
-            for (int x = 0; x < 3; x++) {
-                const float f[4] = {mixed[x][0], mixed[x][1], mixed[x][2], mixed[x][3]};
-                Split<kHeld>(f, lower[x]);
-            }
-            B8 second[kHeld];
-            Eights(lower[1], lower[2], second);
-            __syncthreads();
+            const float factor = run.in * run.out;
+            const char *outputs = lowest(outputLine, first);
 #pragma unroll
             for (int n = 0; n < 2; n++) {
+                // The scores of the tile's steps with those of each tile up to it; for dots without a step's own.
+                Four lower[2][kHeld];
+#pragma unroll
+                for (int x = 0; x <= n; x++) {
+                    float mixed[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int i = 16 * n + m, j = 16 * x + 4 * g + r;
+                        const float score = factor * scores[n + x][r];
+                        if (mode == kGradient && x == n && i == j) diagonal[i] = score;
+                        mixed[r] = j >= start[n] && (mode == kGradient ? j < i : j <= i) ? Exp2(G[n] - reach[j]) * score : 0.f;
+                    }
+                    Split<kHeld>(mixed, lower[x]);
+                }
+                B8 both[kHeld];
+                if (n == 1) Eights(lower[0], lower[1], both);
+                __builtin_amdgcn_sched_barrier(0);
+                __syncthreads();
                 const F4 whole = *reinterpret_cast<const F4 *>(wholes + 16 * n + 4 * g);
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) o[n][c][r] = whole[r] < 0.f ? 0.f : whole[r] * o[n][c][r];
-                    if (n == 1) {
-                        o[n][c] = MfmaMost<kHeld>(second, vp[c], o[n][c]);
+                    Four half[2][P];
+                    PiecesOf<T>(v[0], c, half[0]);
+                    if (n == 0) {
+                        o[n][c] = MfmaHalves<kHeld>(lower[0], half[0], o[n][c]);
                     } else {
-                        Four half[P];
-#pragma unroll
-                        for (int i = 0; i < P; i++) {
-                            struct Both {
-                                Four lo, hi;
-                            };
-                            half[i] = __builtin_bit_cast(Both, vp[c][i]).lo;
-                        }
-                        o[n][c] = MfmaHalves<kHeld>(lower[0], half, o[n][c]);
+                        B8 column[P];
+                        PiecesOf<T>(v[1], c, half[1]);
+                        Eights(half[0], half[1], column);
+                        o[n][c] = MfmaMost<kHeld>(both, column, o[n][c]);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
                 F4 own = {0, 0, 0, 0};
                 if constexpr (mode == kGradient) own = *reinterpret_cast<const F4 *>(diagonal + 16 * n + 4 * g);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int i = 16 * n + 4 * g + r, t = timeOf(first + i);
+                    const int i = 16 * n + 4 * g + r;
                     float x[Tiles], dot = 0;
 #pragma unroll
                     for (int c = 0; c < Tiles; c++) {
                         x[c] = o[n][c][r];
                         if constexpr (mode == kGradient) {
-                            if (c < mine) dot = fmaf(x[c], Float(w[n][r].x[c]), dot);
-                            x[c] = fmaf(own[r], Float(v[n][r].x[c]), x[c]);
+                            if (c < mine) dot = fmaf(x[c], ElementOf<T>(w[n][r], c), dot);
+                            x[c] = fmaf(own[r], ElementOf<T>(v[n][r], c), x[c]);
                         }
                     }
-                    put(t, x, i < valid ? mine : 0);
+                    put(outputs + (long long)(reverse ? 19 - 16 * n - r : 16 * n + r) * sign * outputLine.step, reverse ? 12 - 4 * g : 4 * g, x, i < valid ? mine : 0);
                     if constexpr (mode == kGradient)
-                        if (run.weight) {
+                        if (weightLine.p) {
                             dot = RowSum(dot);
-                            if (m == 0 && i < valid) run.dots[((long long)slice * a.allHeads + head) * a.time + t] = dot;
+                            if (m == 0 && i < valid) *Lane(dots + sign * (first + 16 * n + r + (reverse ? 12 : 0)), Renewed((reverse ? 12 - 4 * g : 4 * g) * 4)) = dot;
                         }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if (kAhead) fetchKeys(first + kSteps);
         }
 
+        __builtin_amdgcn_sched_barrier(0);
+        if (mode == kMemory && kAhead) fetchKeys(first + kSteps);
         const float kept = Exp2(last);
         B8 kt[KeyTiles][P];
 #pragma unroll
@@ -513,7 +688,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             for (int n = 0; n < 2; n++) {
                 const F4 after = *reinterpret_cast<const F4 *>(afters + 16 * n + 4 * g);
 #pragma unroll
-                for (int r = 0; r < 4; r++) x[n][r] = after[r] * Float(v[n][r].x[c]);
+                for (int r = 0; r < 4; r++) x[n][r] = after[r] * ElementOf<T>(v[n][r], c);
             }
             B8 written[kFloatPieces];
             SplitPair<kFloatPieces>(x[0], x[1], written);
@@ -524,18 +699,26 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 for (int r = 0; r < 4; r++) held[r] = cuts ? 0.f : kept * s[t][c][r];
                 s[t][c] = MfmaMost<3>(kt[t], written, held);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        if (!kAhead) fetchKeys(first + kSteps);
+        fetchValues(first + kSteps);
+    }
+
+    if (!finite) {
+        begins();
+        playSteps();
     }
 
     if constexpr (mode == kMemory) {
-        if (reverse && count > 0) scale(gateAt(begin));
+        if (reverse && count > 0) scale(gateAt(count));
         write(run.last + (before + (reverse ? span - 1 : span)) * size);
         if (slice == 0) {
             // The span's factors.
             double sum = 0;
             bool cleared = false;
-            for (int t = begin + lane; t < begin + count; t += 64) {
-                const Step gate = gateAt(t);
+            for (int i = lane; i < count; i += 64) {
+                const Step gate = gateAt(i + late);
                 cleared |= gate.Cleared();
                 sum += gate.decay;
             }
@@ -554,20 +737,17 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 if (lane == 0) run.crossings[((long long)slice * a.allHeads + head) * a.spans + span] = sum;
             }
         if (run.last && span == (reverse ? 0 : a.spans - 1)) {
-            if (reverse && count > 0) scale(gateAt(0));
+            if (reverse && count > 0) scale(gateAt(count));
             write(run.last + (long long)head * size);
         }
     }
 }
 
-// A tensor's place in a run; `heads` share one of its heads.
+// Whether a tensor's packs of four are aligned and none is cut.
 inline bool IsWhole(const void *p, const long long *strides, int size, size_t bytes) {
     return strides[0] % 4 == 0 && strides[1] % 4 == 0 && strides[2] % 4 == 0 && size % 4 == 0 && Aligned(4 * bytes, p);
 }
-inline void Take(const void *&p, long long (&strides)[3], int &heads, const void *from, const long long *fromStrides, int share) {
-    p = from, heads = share;
-    for (int i = 0; i < 3; i++) strides[i] = fromStrides[i];
-}
+inline Tensor TensorOf(const void *p, const long long *strides, int share) { return {p, {strides[0], strides[1], strides[2]}, share}; }
 inline Runs RunsOf(const Attention &a) {
     Runs r{};
     r.time = a.time, r.heads = a.heads, r.length = kSpan, r.spans = a.time > kSpan ? (a.time + kSpan - 1) / kSpan : 1;
@@ -592,17 +772,16 @@ inline bool IsWhole(const Attention &a) {
 
 // The tiles of 16 columns that a wavefront of a launch takes, 0 to 2 as powers of two.
 template <class T>
-int TilesOf(const Runs &runs, int count, int keyTiles, bool whole) {
-    if (!whole) return 1;
+int TilesOf(const Runs &runs, int count, int keyTiles) {
     const int most = kPieces<T> * keyTiles > 12 ? 1 : kPieces<T> * keyTiles > 4 ? 2 : 4;
     for (int tiles = most; tiles > 1; tiles /= 2) {
         long long slices = 0;
-        bool wide = false;
+        bool full = true;
         for (int i = 0; i < count; i++) {
-            slices += (runs.run[i].columns + 16 * tiles - 1) / (16 * tiles);
-            wide |= runs.run[i].columns > 8 * tiles;
+            slices += runs.run[i].columns / (16 * tiles);
+            full &= runs.run[i].rows == 16 * keyTiles && runs.run[i].columns % (16 * tiles) == 0;
         }
-        if (wide && runs.allHeads * slices * runs.spanCount >= 1024) return tiles;
+        if (full && runs.allHeads * slices * runs.spanCount >= 1024) return tiles;
     }
     return 1;
 }
@@ -615,15 +794,28 @@ inline int KeyTilesOf(const Runs &runs, int count) {
 inline void Cut(Runs &runs, int count, int tiles) {
     runs.units = 0;
     for (int i = 0; i < count; i++) {
-        runs.run[i].slices = (runs.run[i].columns + 16 * tiles - 1) / (16 * tiles);
-        runs.units += runs.run[i].slices;
+        runs.slices[i] = (runs.run[i].columns + 16 * tiles - 1) / (16 * tiles);
+        runs.units += runs.slices[i];
     }
+}
+
+inline bool IsNear(const Runs &runs, int count) {
+    const auto near = [](long long stride) { return stride >= 0 && stride < (1 << 24); };
+    if (!near(runs.decayStrides[1]) || !near(runs.resetStrides[1])) return false;
+    for (int i = 0; i < count; i++) {
+        const Run &r = runs.run[i];
+        if (!near(r.query.strides[1]) || !near(r.key.strides[1]) || !near(r.value.strides[1]) || !near(r.weight.strides[1]) ||
+            !near(r.outputStrides[1]))
+            return false;
+    }
+    return true;
 }
 
 template <class T, Mode mode, int KeyTiles>
 void LaunchTiles(Runs &runs, int count, bool whole, hipStream_t stream) {
+    runs.near = IsNear(runs, count);
     constexpr int most = kPieces<T> * KeyTiles > 12 ? 1 : kPieces<T> * KeyTiles > 4 ? 2 : 4;
-    const int tiles = TilesOf<T>(runs, count, KeyTiles, whole);
+    const int tiles = whole ? TilesOf<T>(runs, count, KeyTiles) : 1;
     Cut(runs, count, tiles);
     const auto launch = [&](auto kernel) {
         // A grid has fewer than 2^32 threads.
@@ -634,10 +826,13 @@ void LaunchTiles(Runs &runs, int count, bool whole, hipStream_t stream) {
             hipLaunchKernelGGL(kernel, dim3(heads * blocks), dim3(64), 0, stream, runs);
         }
     };
-    if (!whole) launch(RunKernel<T, KeyTiles, 1, false, mode>);
-    else if (tiles == 4) launch(RunKernel<T, KeyTiles, most >= 4 ? 4 : 1, true, mode>);
-    else if (tiles == 2) launch(RunKernel<T, KeyTiles, most >= 2 ? 2 : 1, true, mode>);
-    else launch(RunKernel<T, KeyTiles, 1, true, mode>);
+    bool full = whole;
+    for (int i = 0; i < count; i++) full &= runs.run[i].rows == 16 * KeyTiles && runs.run[i].columns % (16 * tiles) == 0;
+    if (!whole) launch(RunKernel<T, KeyTiles, 1, kLoose, mode>);
+    else if (!full) launch(RunKernel<T, KeyTiles, 1, kWhole, mode>);
+    else if (tiles == 4) launch(RunKernel<T, KeyTiles, most >= 4 ? 4 : 1, kFull, mode>);
+    else if (tiles == 2) launch(RunKernel<T, KeyTiles, most >= 2 ? 2 : 1, kFull, mode>);
+    else launch(RunKernel<T, KeyTiles, 1, kFull, mode>);
 }
 template <class T, Mode mode>
 void LaunchRuns(Runs &runs, int count, bool whole, hipStream_t stream) {

@@ -110,9 +110,8 @@ void Forward(const Attention &a, hipStream_t stream) {
     Runs runs = RunsOf(a);
     Run &run = runs.run[0];
     const int share = a.heads / a.key_heads;
-    Take(run.query, run.queryStrides, run.queryHeads, a.query, a.query_strides, share);
-    Take(run.key, run.keyStrides, run.keyHeads, a.key, a.key_strides, share);
-    Take(run.value, run.valueStrides, run.valueHeads, a.value, a.value_strides, 1);
+    run.query = TensorOf(a.query, a.query_strides, share), run.key = TensorOf(a.key, a.key_strides, share);
+    run.value = TensorOf(a.value, a.value_strides, 1);
     run.rows = a.key_size, run.columns = a.value_size, run.in = 1, run.out = a.scale;
     run.output = a.output;
     run.outputStrides[0] = (long long)a.time * a.heads * a.value_size, run.outputStrides[1] = (long long)a.heads * a.value_size;

@@ -125,10 +125,8 @@ void Backward(const Attention &a, hipStream_t stream) {
     const int share = a.heads / a.key_heads;
     const long long size = (long long)a.key_size * a.value_size, heads = runs.allHeads, tokens = heads * a.time;
     const bool whole = IsWhole(a);
-    const auto query = [&](Run &r, auto p, auto strides, auto of) { Take(r.*p, r.*strides, r.*of, a.query, a.query_strides, share); };
-    const auto key = [&](Run &r, auto p, auto strides, auto of) { Take(r.*p, r.*strides, r.*of, a.key, a.key_strides, share); };
-    const auto value = [&](Run &r, auto p, auto strides, auto of) { Take(r.*p, r.*strides, r.*of, a.value, a.value_strides, 1); };
-    const auto output = [&](Run &r, auto p, auto strides, auto of) { Take(r.*p, r.*strides, r.*of, a.d_output, a.d_output_strides, 1); };
+    const Tensor query = TensorOf(a.query, a.query_strides, share), key = TensorOf(a.key, a.key_strides, share);
+    const Tensor value = TensorOf(a.value, a.value_strides, 1), output = TensorOf(a.d_output, a.d_output_strides, 1);
     const auto put = [&](Run &r, void *to, bool floats) {
         r.output = to, r.floats = floats;
         r.outputStrides[0] = (long long)a.time * a.heads * r.columns, r.outputStrides[1] = (long long)a.heads * r.columns;
@@ -138,8 +136,7 @@ void Backward(const Attention &a, hipStream_t stream) {
     if (runs.spans > 1) {
         Runs memories = runs;
         Run &r = memories.run[0];
-        query(r, &Run::key, &Run::keyStrides, &Run::keyHeads);
-        output(r, &Run::value, &Run::valueStrides, &Run::valueHeads);
+        r.key = query, r.value = output;
         r.rows = a.key_size, r.columns = a.value_size, r.reverse = true, r.in = a.scale;
         r.last = work + at.memories;
         memories.firstSpan = 1, memories.spanCount = runs.spans - 1, memories.factors = runs.factors = work + at.factors;
@@ -148,25 +145,17 @@ void Backward(const Attention &a, hipStream_t stream) {
     }
 
     Run &dq = runs.run[0], &dk = runs.run[1], &dv = runs.run[2];
-    output(dq, &Run::query, &Run::queryStrides, &Run::queryHeads);
-    value(dq, &Run::key, &Run::keyStrides, &Run::keyHeads);
-    key(dq, &Run::value, &Run::valueStrides, &Run::valueHeads);
-    query(dq, &Run::weight, &Run::weightStrides, &Run::weightHeads);
+    dq.query = output, dq.key = value, dq.value = key, dq.weight = query;
     dq.rows = a.value_size, dq.columns = a.key_size, dq.transposed = true, dq.in = 1, dq.out = a.scale;
     dq.first = static_cast<const float *>(a.state), dq.starts = static_cast<const float *>(a.checkpoints);
     put(dq, share > 1 ? work + at.parts : a.d_query, share > 1);
 
-    value(dk, &Run::query, &Run::queryStrides, &Run::queryHeads);
-    output(dk, &Run::key, &Run::keyStrides, &Run::keyHeads);
-    query(dk, &Run::value, &Run::valueStrides, &Run::valueHeads);
-    key(dk, &Run::weight, &Run::weightStrides, &Run::weightHeads);
+    dk.query = value, dk.key = output, dk.value = query, dk.weight = key;
     dk.rows = a.value_size, dk.columns = a.key_size, dk.reverse = dk.transposed = true, dk.in = a.scale, dk.out = 1;
     dk.first = static_cast<const float *>(a.d_last), dk.starts = work + at.memories;
     put(dk, share > 1 ? work + at.parts + tokens * a.key_size : a.d_key, share > 1);
 
-    key(dv, &Run::query, &Run::queryStrides, &Run::queryHeads);
-    query(dv, &Run::key, &Run::keyStrides, &Run::keyHeads);
-    output(dv, &Run::value, &Run::valueStrides, &Run::valueHeads);
+    dv.query = key, dv.key = query, dv.value = output;
     dv.rows = a.key_size, dv.columns = a.value_size, dv.reverse = true, dv.in = a.scale, dv.out = 1;
     dv.first = static_cast<const float *>(a.d_last), dv.starts = work + at.memories, dv.last = static_cast<float *>(a.d_state);
     put(dv, a.d_value, false);
@@ -176,7 +165,7 @@ void Backward(const Attention &a, hipStream_t stream) {
         dq.dots = work + at.dots, dk.dots = work + at.dots + slices * tokens;
         dq.crossings = work + at.crossings, dq.against = work + at.memories, dq.againstLast = static_cast<const float *>(a.d_last);
         LaunchRuns<T, kGradient>(runs, 3, whole, stream);
-        DecayArgs d{dq.dots, dk.dots, dq.crossings, dq.slices, dk.slices, a.time, a.heads, runs.spans, runs.allHeads, runs.decay,
+        DecayArgs d{dq.dots, dk.dots, dq.crossings, runs.slices[0], runs.slices[1], a.time, a.heads, runs.spans, runs.allHeads, runs.decay,
                     runs.resets, {}, {}, a.decay_of_head ? nullptr : static_cast<float *>(a.d_decay),
                     a.decay_of_head ? reinterpret_cast<double *>(work + at.totals) : nullptr};
         for (int i = 0; i < 3; i++) d.decayStrides[i] = runs.decayStrides[i];

@@ -428,15 +428,16 @@ def test_offsets_past_32_bits():
         found, _, _ = learn({**given, name: view}, d_output, d_last)
         for n in wanted:
             assert torch.equal(found[n], wanted[n]), (name, n)
-    # Two steps of one.
+    # Two steps of one. They are too far apart to be played together, and one after the other their sums are taken in another
+    # order: the bounds of rounding hold, not equality.
     given = inputs(1, 2, 1, 1, 32, 32, dtype=torch.bfloat16, seed=15)
-    wanted, d_output, d_last = learn(given)
+    _, d_output, d_last = learn(given)
+    d = {'d_output': d_output, 'd_last': d_last}
     for name in ('query', 'key', 'value'):
         view = room.as_strided((1, 2, 1, 32), (32, apart, 32, 1))
         view.copy_(given[name])
         found, _, _ = learn({**given, name: view}, d_output, d_last)
-        for n in wanted:
-            assert torch.equal(found[n], wanted[n]), (name, n)
+        all_close(found, exact_attention(**given, **d), attention_terms(**given, **d))
 
 
 def test_calls_repeat_bit_for_bit():

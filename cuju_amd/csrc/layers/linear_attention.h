@@ -56,11 +56,13 @@ struct Runs {
     float *factors;  // [head][spans - 1]: the product of a span's factors, or -1 where an episode starts in it
     Run run[3];
 };
-// A run out of the kernel's arguments, where an index that the compiler does not know would copy them all.
+// A run out of the kernel's arguments, where an index that the compiler does not know would copy them all, read anew
+// at every call: few of its words are needed over the long loop, and all would not fit the scalar registers.
 __device__ __forceinline__ Run RunAt(int which) {
     using Word = const __attribute__((address_space(4))) uint32_t;
     Word *p = (Word *)((const __attribute__((address_space(4))) char *)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(Runs, run)) +
               which * (sizeof(Run) / 4);
+    asm volatile("" : "+s"(p));
     struct Words {
         uint32_t x[sizeof(Run) / 4];
     } words;
@@ -73,6 +75,13 @@ template <class T>
 struct Line {
     const T *p;
     long long step;
+    __device__ __forceinline__ const T *At(int i) const { return p + i * step; }
+};
+// The same within 32 steps, counted in the order of time from the first of them.
+template <class T>
+struct Near {
+    const T *p;
+    int step;
     __device__ __forceinline__ const T *At(int i) const { return p + i * step; }
 };
 
@@ -245,44 +254,43 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
     constexpr bool Whole = shape != kLoose, full = shape == kFull;
     constexpr bool kAhead = kRunsAhead<T, KeyTiles, Tiles>;
     constexpr int kHeld = mode == kGradient || P == kFloatPieces ? kFloatPieces : 2;
-    __shared__ double reach[kSteps];
-    __shared__ __align__(16) float wholes[kSteps], afters[kSteps], diagonal[kSteps];
+    // By step: the factors' sum up to it in two floats, and the factors of what it reads and writes.
+    __shared__ __align__(16) float reach[2][kSteps], wholes[kSteps], afters[kSteps], diagonal[kSteps];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
-    unsigned id = Place(blockIdx.x, gridDim.x);
-    int slice = id % a.units, which = 0;
-    id /= a.units;
-    const int span = a.firstSpan + id % a.spanCount;
-    const unsigned head = a.firstHead + id / a.spanCount;
+    unsigned head = Place(blockIdx.x, gridDim.x);
+    int slice = head % a.units, which = 0;
+    head /= a.units;
+    const int span = a.firstSpan + head % a.spanCount;
+    head = a.firstHead + head / a.spanCount;
     while (slice >= a.slices[which]) slice -= a.slices[which++];
-    const Run run = RunAt(which);
     const int h = head % a.heads, b = head / a.heads;
-    const int rows = full ? 16 * KeyTiles : run.rows, columns = run.columns;
-    const bool reverse = run.reverse;
-    const int column = slice * 16 * Tiles + m * Tiles, firstColumn = column;
-    const int mine = full ? Tiles : max(0, min(Tiles, columns - column)), ownColumns = mine;
     const int begin = span * a.length, count = min(a.length, a.time - begin);
-    const long long size = (long long)rows * columns, before = (long long)head * (a.spans - 1);
-    const auto rowOf = [&](int t) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1); };
+    const bool reverse = RunAt(which).reverse;
+    const int sign = reverse ? -1 : 1, late = reverse ? 1 : 0, opens = reverse ? begin + count - 1 : begin;
+    const int column = slice * 16 * Tiles + m * Tiles;
+    const int ownColumns = full ? Tiles : max(0, min(Tiles, RunAt(which).columns - column));
+    const auto ownRows = [&] { return full ? 16 * KeyTiles : RunAt(which).rows; };
 
     F4 s[KeyTiles][Tiles];
     // take(element of the run's memory, element of another) in its place.
     const auto read = [&](const float *memory, auto take) {
-        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), columns = Opaque(run.columns);
-        const int lanes = (run.transposed ? column * rows + 8 * g : 8 * g * columns + column) * 4;
+        const int rows = ownRows(), columns = RunAt(which).columns;
+        const bool transposed = RunAt(which).transposed;
+        const int lanes = (transposed ? column * rows + 8 * g : 8 * g * columns + column) * 4;
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++) {
             const int row = 32 * (t >> 1) + 4 * (t & 1);
-            if (run.transposed) {
+            if (transposed) {
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
-                    const auto x = LoadAt<4, Whole>(memory + c * rows + row, lanes, c < mine ? rows - row - 8 * g : 0);
+                    const auto x = LoadAt<4, Whole>(memory + c * rows + row, lanes, c < ownColumns ? rows - row - 8 * g : 0);
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[t][c][r] = take(s[t][c][r], x.x[r]);
                 }
             } else {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const auto x = LoadAt<Tiles, Whole>(memory + (row + r) * columns, lanes, row + r + 8 * g < rows ? mine : 0);
+                    const auto x = LoadAt<Tiles, Whole>(memory + (row + r) * columns, lanes, row + r + 8 * g < rows ? ownColumns : 0);
 #pragma unroll
                     for (int c = 0; c < Tiles; c++) s[t][c][r] = take(s[t][c][r], x.x[c]);
                 }
@@ -290,9 +298,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         }
     };
     const auto write = [&](float *memory) {
-        // What follows from these is not kept over the loop.
-        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), columns = Opaque(run.columns), mine = full ? Tiles : Renewed(ownColumns);
-        const int lanes = (8 * g * columns + Renewed(firstColumn)) * 4;
+        const int rows = ownRows(), columns = RunAt(which).columns, mine = full ? Tiles : Renewed(ownColumns);
+        const int lanes = (8 * g * columns + Renewed(column)) * 4;
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
@@ -304,49 +311,63 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 StoreAt<Tiles, Whole>(memory + row * columns, lanes, x, row + 8 * g < rows ? mine : 0);
             }
     };
+    // Places of memories of a head, and of spans, in floats.
+    const auto memoryAt = [&](long long index) {
+        const Run run = RunAt(which);
+        return index * run.rows * run.columns;
+    };
+    const auto between = [&](int index) { return memoryAt((long long)head * (Argument<Runs>().spans - 1) + index); };
     const auto begins = [&] {
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
             for (int c = 0; c < Tiles; c++) s[t][c] = F4{0, 0, 0, 0};
         if constexpr (mode != kMemory) {
-            const bool starts = reverse ? span == a.spans - 1 : span == 0;
-            const float *memory = starts ? run.first : run.starts;
-            if (memory)
-                read(memory + (starts ? (long long)head : before + (reverse ? span : span - 1)) * size, [](float, float y) { return y; });
+            const Run run = RunAt(which);
+            const bool starts = reverse ? span == Argument<Runs>().spans - 1 : span == 0;
+            if (const float *memory = starts ? run.first : run.starts)
+                read(memory + (starts ? memoryAt(head) : between(reverse ? span : span - 1)), [](float, float y) { return y; });
         }
     };
+    const bool keeps = mode == kOutputs && RunAt(which).kept;
     const auto keep = [&](int i) {
-        if constexpr (mode == kOutputs)
-            if (run.kept && i > 0 && i % kSpan == 0)
-                write(run.kept + ((long long)head * ((a.time - 1) / kSpan) + i / kSpan - 1) * size);
+        if (keeps && i > 0 && i % kSpan == 0)
+            write(RunAt(which).kept + memoryAt((long long)head * ((Argument<Runs>().time - 1) / kSpan) + i / kSpan - 1));
     };
 
-    // The tensors' lines of this head, from the span's first step on. What the memory is scaled by on the way to a step is,
+    // A tensor's line of this head, from the span's first step on. What the memory is scaled by on the way to a step is,
     // backwards in time, the factor of the step that comes after it in time, and nothing for the first.
-    const int opens = reverse ? begin + count - 1 : begin, sign = reverse ? -1 : 1;
     const auto lineOf = [&](const Tensor &x, auto type) {
         using Element = decltype(type);
         return Line<Element>{Global(static_cast<const Element *>(x.p)) + b * x.strides[0] + opens * x.strides[1] + h / x.share * x.strides[2],
                              sign * x.strides[1]};
     };
-    const Line<T> keyLine = lineOf(run.key, T()), valueLine = lineOf(run.value, T());
-    const Line<T> queryLine = mode != kMemory ? lineOf(run.query, T()) : Line<T>{};
-    const Line<T> weightLine = mode == kGradient && run.weight.p ? lineOf(run.weight, T()) : Line<T>{};
-    const int late = reverse ? 1 : 0;
-    const Line<float> decayLine{Global(a.decay) + b * a.decayStrides[0] + (opens + late) * a.decayStrides[1] + h * a.decayStrides[2],
-                                sign * a.decayStrides[1]};
-    const Line<unsigned char> resetLine{a.resets ? Global(a.resets) + b * a.resetStrides[0] + (opens + late) * a.resetStrides[1] : nullptr,
-                                        sign * a.resetStrides[1]};
+    const auto decayLine = [&] {
+        const Runs a = Argument<Runs>();
+        return Line<float>{Global(a.decay) + b * a.decayStrides[0] + (opens + late) * a.decayStrides[1] + h * a.decayStrides[2],
+                           sign * a.decayStrides[1]};
+    };
+    const auto resetLine = [&] {
+        const Runs a = Argument<Runs>();
+        return Line<unsigned char>{a.resets ? Global(a.resets) + b * a.resetStrides[0] + (opens + late) * a.resetStrides[1] : nullptr,
+                                   sign * a.resetStrides[1]};
+    };
+    const auto outputLine = [&] {
+        const Run run = RunAt(which);
+        const int bytes = run.floats ? 4 : (int)sizeof(T);
+        const long long first = b * run.outputStrides[0] + opens * run.outputStrides[1] + h * run.outputStrides[2];
+        return Line<char>{static_cast<const char *>(run.output) + first * bytes, sign * run.outputStrides[1] * bytes};
+    };
+    const auto dotsAt = [&] {
+        const Runs a = Argument<Runs>();
+        return RunAt(which).dots + ((long long)slice * a.allHeads + head) * a.time + opens;
+    };
     const auto gateAt = [&](int i) {
-        Step step{*decayLine.At(i), 0};
-        if (resetLine.p) step.reset = *resetLine.At(i);
+        Step step{*decayLine().At(i), 0};
+        const auto resets = resetLine();
+        if (resets.p) step.reset = *resets.At(i);
         return step;
     };
-    const Line<char> outputLine{static_cast<const char *>(run.output) + (b * run.outputStrides[0] + opens * run.outputStrides[1] + h * run.outputStrides[2]) *
-                                                                            (run.floats ? 4 : (int)sizeof(T)),
-                                sign * run.outputStrides[1] * (run.floats ? 4 : (int)sizeof(T))};
-    float *const dots = run.dots + ((long long)slice * a.allHeads + head) * a.time + opens;
     const auto scale = [&](Step gate) {
         const bool cleared = gate.Cleared();
         const float kept = cleared ? 0.f : expf(gate.decay);
@@ -357,35 +378,40 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
                 for (int r = 0; r < 4; r++) s[t][c][r] = cleared ? 0.f : kept * s[t][c][r];
     };
-    // Stores the outputs of the step at `place` in time, counted from the one at `base`.
+    const bool floats = mode != kMemory && RunAt(which).floats, weighs = mode == kGradient && RunAt(which).weight.p;
+    // Stores the outputs of a step at a lane's `place` in bytes.
     const auto put = [&](const char *base, int place, const float (&x)[Tiles], int valid) {
-        const int step = sign * (int)outputLine.step;
-        if (run.floats) {
+        if (floats) {
             Pack<float, Tiles> o;
 #pragma unroll
             for (int c = 0; c < Tiles; c++) o.x[c] = x[c];
-            StoreAt<Tiles, Whole>(reinterpret_cast<float *>(const_cast<char *>(base)), place * step + 4 * column, o, valid);
+            StoreAt<Tiles, Whole>(reinterpret_cast<float *>(const_cast<char *>(base)), place + 4 * column, o, valid);
         } else {
             Pack<T, Tiles> o;
 #pragma unroll
             for (int c = 0; c < Tiles; c++) o.x[c] = As<T>(x[c]);
-            StoreAt<Tiles, Whole>(reinterpret_cast<T *>(const_cast<char *>(base)), place * step + (int)sizeof(T) * column, o, valid);
+            StoreAt<Tiles, Whole>(reinterpret_cast<T *>(const_cast<char *>(base)), place + (int)sizeof(T) * column, o, valid);
         }
     };
 
     // All steps, one after the other.
     const auto playSteps = [&] {
-        const int rows = full ? 16 * KeyTiles : Opaque(run.rows), mine = full ? Tiles : Renewed(ownColumns), column = Renewed(firstColumn);
+        const Run run = RunAt(which);
+        const int rows = ownRows(), mine = ownColumns;
+        const Line<T> keys = lineOf(run.key, T()), values = lineOf(run.value, T());
+        const Line<T> queries = mode != kMemory ? lineOf(run.query, T()) : Line<T>{}, weights = weighs ? lineOf(run.weight, T()) : Line<T>{};
+        const Line<char> outputs = outputLine();
+        float *dots = dotsAt();
 #pragma unroll 1
         for (int i = 0; i < count; i++) {
             keep(i);
-            const auto v = Load<Tiles, Whole>(valueLine.At(i) + column, mine);
+            const auto v = Load<Tiles, Whole>(values.At(i) + column, mine);
             if (i >= late) scale(gateAt(i));
-            const T *key = keyLine.At(i), *query = mode == kMemory ? nullptr : queryLine.At(i);
+            const T *key = keys.At(i), *query = mode == kMemory ? nullptr : queries.At(i);
             float strict[Tiles] = {}, own = 0;
 #pragma unroll
             for (int x = 0; x < KeyTiles; x++) {
-                const int row = rowOf(x);
+                const int row = 32 * (x >> 1) + 8 * g + 4 * (x & 1);
                 const auto k = Load<4, Whole>(key + row, rows - row);
                 Pack<T, 4> q{};
                 if constexpr (mode != kMemory) q = Load<4, Whole>(query + row, rows - row);
@@ -403,8 +429,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 own += __shfl_xor(own, 16);
                 own += __shfl_xor(own, 32);
                 Pack<T, Tiles> w{};
-                if constexpr (mode == kGradient)
-                    if (weightLine.p) w = Load<Tiles, Whole>(weightLine.At(i) + column, mine);
+                if (weighs) w = Load<Tiles, Whole>(weights.At(i) + column, mine);
                 float dot = 0;
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
@@ -414,82 +439,84 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     if (c < mine) dot = fmaf(strict[c], Float(w.x[c]), dot);
                     strict[c] = fmaf(run.out * run.in * own, Float(v.x[c]), strict[c]);
                 }
-                put(outputLine.At(i), 0, strict, g == 0 ? mine : 0);
-                if constexpr (mode == kGradient) {
-                    dot = RowSum(dot);
-                    if (weightLine.p && lane == 0) dots[sign * i] = dot;
-                }
+                put(outputs.At(i), 0, strict, g == 0 ? mine : 0);
+                dot = RowSum(dot);
+                if (weighs && lane == 0) dots[sign * i] = dot;
             }
         }
     };
 
-    // The inputs of the steps from `first`: of a lane's steps m and 16 + m the keys and queries, of its steps 4 g + r and
-    // 16 + 4 g + r the values and weights. Past the end the last step is read again. In whole chunks of whole tensors an
-    // address is one that all lanes share and a lane's offset of 32 bits.
+    // The inputs of the next 32 steps: of a lane's steps m and 16 + m the keys and queries, of its steps 4 g + r and
+    // 16 + 4 g + r the values and weights. Past the end the last step is read again. An address is one that all lanes
+    // share, that of the chunk's first step in time, and a lane's offset of 32 bits.
     using RowWords = Words<kWords<T, 8>>;
     using ColumnWords = Words<kWords<T, Tiles>>;
     RowWords nextK[2][kPairs], nextQ[2][kPairs];
     ColumnWords nextV[2][4];
     Step nextGate[2];
-    // An address is one that all lanes share, that of the chunk's first step in time, and a lane's offset of 32 bits.
-    const auto lowest = [&](const auto &line, int first) { return line.At(first + (reverse ? kSteps - 1 : 0)); };
+    const auto nearOf = [&](const auto &line) {
+        Near<std::remove_const_t<std::remove_pointer_t<decltype(line.p)>>> near{line.p, sign * (int)line.step};
+        if (reverse && near.p) near.p -= (kSteps - 1) * near.step;
+        return near;
+    };
+    const auto advance = [&](auto &near) { near.p += sign * kSteps * near.step; };
+    Near<T> keys{}, queries{}, values{}, weights{};
+    Near<float> decays{};
+    Near<unsigned char> resets{};
+    Near<char> outputs{};
+    const float *dots = nullptr;
     const auto placeOf = [&](int i) { return reverse ? kSteps - 1 - i : i; };
-    const auto keysAt = [&](const Line<T> &line, int first, RowWords(&x)[2][kPairs]) {
-        const T *base = lowest(line, first);
-        const int last = min(kSteps, count - first) - 1, step = sign * (int)line.step;
+    const auto rowsAt = [&](const Near<T> &line, int left, RowWords(&x)[2][kPairs]) {
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const int place = (placeOf(min(16 * n + Renewed(m), last)) * step + 8 * g) * (int)sizeof(T);
+            const int place = (placeOf(min(16 * n + Renewed(m), left - 1)) * line.step + 8 * g) * (int)sizeof(T);
             if constexpr (full) {
                 const uint32_t lanes = Renewed(place);
 #pragma unroll
-                for (int q = 0; q < kPairs; q++) x[n][q] = LoadWords<T, 8, true, 4>(Lane(base + 32 * q, lanes));
+                for (int q = 0; q < kPairs; q++) x[n][q] = LoadWords<T, 8, true, 4>(Lane(line.p + 32 * q, lanes));
             } else {
-                const int left = Opaque(run.rows) - 8 * g;
+                const int rest = ownRows() - 8 * g;
 #pragma unroll
                 for (int q = 0; q < kPairs; q++) {
                     struct Halves {
                         Words<kWords<T, 4>> x[2];
                     } half;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) half.x[i] = WordsAt<T, 4, Whole>(base + 32 * q + 4 * i, place, left - 32 * q - 4 * i);
+                    for (int i = 0; i < 2; i++) half.x[i] = WordsAt<T, 4, Whole>(line.p + 32 * q + 4 * i, place, rest - 32 * q - 4 * i);
                     x[n][q] = __builtin_bit_cast(RowWords, half);
                 }
             }
         }
     };
-    const auto valuesAt = [&](const Line<T> &line, int first, ColumnWords(&x)[2][4]) {
-        const T *base = lowest(line, first);
-        const int last = min(kSteps, count - first) - 1, step = sign * (int)line.step;
-        const int mine = full ? Tiles : Renewed(ownColumns), column = Renewed(firstColumn);
-        if (full && last == kSteps - 1) {
-            const uint32_t lanes = Renewed(((reverse ? 12 - 4 * g : 4 * g) * step + column) * (int)sizeof(T));
+    const auto columnsAt = [&](const Near<T> &line, int left, ColumnWords(&x)[2][4]) {
+        if (full && left >= kSteps) {
+            const uint32_t lanes = Renewed(((reverse ? 12 - 4 * g : 4 * g) * line.step + Renewed(column)) * (int)sizeof(T));
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    x[n][r] = LoadWords<T, Tiles, true>(Lane(base + (long long)(reverse ? 19 - 16 * n - r : 16 * n + r) * step, lanes));
+                for (int r = 0; r < 4; r++) x[n][r] = LoadWords<T, Tiles, true>(Lane(line.At(reverse ? 19 - 16 * n - r : 16 * n + r), lanes));
         } else {
+            const int mine = full ? Tiles : Renewed(ownColumns);
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    x[n][r] = WordsAt<T, Tiles, Whole>(base, (placeOf(min(16 * n + 4 * g + r, last)) * step + column) * (int)sizeof(T), mine);
+                    x[n][r] = WordsAt<T, Tiles, Whole>(line.p, (placeOf(min(16 * n + 4 * g + r, left - 1)) * line.step + Renewed(column)) * (int)sizeof(T), mine);
         }
     };
-    // Past the end nothing is fetched, and what was fetched before is given up: its registers are free until then.
-    const auto fetchKeys = [&](int first) {
-        if (first >= count) {
+    // Where nothing is left nothing is fetched, and what was fetched before is given up: its registers are free until then.
+    const auto fetchRows = [&](int left) {
+        if (left <= 0) {
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int q = 0; q < kPairs; q++) nextK[n][q] = nextQ[n][q] = RowWords{};
             return;
         }
-        keysAt(keyLine, first, nextK);
-        if constexpr (mode != kMemory) keysAt(queryLine, first, nextQ);
+        rowsAt(keys, left, nextK), advance(keys);
+        if constexpr (mode != kMemory) rowsAt(queries, left, nextQ), advance(queries);
     };
-    const auto fetchValues = [&](int first) {
+    const auto fetchColumns = [&](int first) {
         if (first >= count) {
 #pragma unroll
             for (int n = 0; n < 2; n++) {
@@ -499,24 +526,33 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             }
             return;
         }
-        valuesAt(valueLine, first, nextV);
-        const float *decays = lowest(decayLine, first);
-        const unsigned char *resets = resetLine.p ? lowest(resetLine, first) : nullptr;
+        columnsAt(values, count - first, nextV), advance(values);
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const int i = 16 * n + Renewed(m);
             nextGate[n] = Step{0.f, 0};
             if (first + i < count && first + i >= late) {
-                nextGate[n].decay = *Lane(decays, Renewed(placeOf(i) * sign * (int)decayLine.step * 4));
-                if (resets) nextGate[n].reset = *Lane(resets, Renewed(placeOf(i) * sign * (int)resetLine.step));
+                nextGate[n].decay = *Lane(decays.p, Renewed(placeOf(i) * decays.step * 4));
+                if (resets.p) nextGate[n].reset = *Lane(resets.p, Renewed(placeOf(i) * resets.step));
             }
         }
+        advance(decays);
+        if (resets.p) advance(resets);
     };
+
     const Eyes eyes = EyesOf(m, g);
     // Steps that are too far apart for 32 bits are played one by one.
-    bool finite = a.near;
+    bool finite = Argument<Runs>().near;
     begins();
-    if (finite) fetchKeys(0), fetchValues(0);
+    if (finite) {
+        const Run run = RunAt(which);
+        keys = nearOf(lineOf(run.key, T())), values = nearOf(lineOf(run.value, T()));
+        decays = nearOf(decayLine()), resets = nearOf(resetLine());
+        if constexpr (mode != kMemory) queries = nearOf(lineOf(run.query, T())), outputs = nearOf(outputLine());
+        if (weighs) weights = nearOf(lineOf(run.weight, T())), dots = dotsAt() - (reverse ? kSteps - 1 : 0);
+        fetchRows(count), fetchColumns(0);
+    }
+    const float in = RunAt(which).in, out = RunAt(which).out;
 #pragma unroll 1
     for (int first = 0; first < count && finite; first += kSteps) {
         const int valid = min(kSteps, count - first);
@@ -561,20 +597,19 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[n][r] = valid == kSteps || 16 * n + 4 * g + r < valid ? nextV[n][r] : ColumnWords{};
+            for (int r = 0; r < 4; r++) v[n][r] = nextV[n][r], w[n][r] = ColumnWords{};
+        if (valid < kSteps)
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[n][r] = 16 * n + 4 * g + r < valid ? v[n][r] : ColumnWords{};
         const Step gate[2] = {nextGate[0], nextGate[1]};
-        if constexpr (mode == kGradient) {
-            if (weightLine.p) valuesAt(weightLine, first, w);
-            else
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) w[n][r] = ColumnWords{};
-        }
+        if (weighs) columnsAt(weights, valid, w), advance(weights);
         // A product with anything, zeros too, tells whether a value is not finite.
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             Four half[2][P];
+#pragma unroll
             for (int n = 0; n < 2; n++) PiecesOf<T>(v[n], c, half[n]);
             mark = Mfma32(eyes.half[0], Eight(half[0][0], half[1][0]), mark);
         }
@@ -582,137 +617,157 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             finite = false;
             break;
         }
+
         __builtin_amdgcn_sched_barrier(0);
         // How the chunk is cut, and the products of its factors.
         const bool cleared[2] = {gate[0].Cleared(), gate[1].Cleared()};
         const unsigned cuts = (unsigned)(__ballot(cleared[0]) & 0xffff) | (unsigned)(__ballot(cleared[1]) & 0xffff) << 16;
-        double G[2];
-        G[0] = RowUpTo(cleared[0] ? 0.0 : gate[0].decay * kLog2E);
-        G[1] = RowUpTo(cleared[1] ? 0.0 : gate[1].decay * kLog2E) + __shfl(G[0], 15);
-        const double last = __shfl(G[1], 15);
+        float high[2], low[2], kept;
         int start[2];  // where the episode of a lane's steps starts, or -1 before the chunk
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-            const unsigned upTo = cuts & ((2u << (16 * n + m)) - 1);
-            start[n] = upTo ? 31 - __builtin_clz(upTo) : -1;
-        }
-        const int latest = cuts ? 31 - __builtin_clz(cuts) : -1;
-        __syncthreads();
-        if (g == 0) {
+        {
+            double G[2];
+            G[0] = RowUpTo(cleared[0] ? 0.0 : gate[0].decay * kLog2E);
+            G[1] = RowUpTo(cleared[1] ? 0.0 : gate[1].decay * kLog2E) + __shfl(G[0], 15);
+            const double last = __shfl(G[1], 15);
+            const int latest = cuts ? 31 - __builtin_clz(cuts) : -1;
+            kept = Exp2(last);
+            __syncthreads();
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const int i = 16 * n + m;
-                reach[i] = G[n];
-                wholes[i] = start[n] < 0 ? run.out * Exp2(G[n]) : -1.f;
-                afters[i] = i >= latest ? run.in * Exp2(last - G[n]) : 0.f;
+                const unsigned upTo = cuts & ((2u << i) - 1);
+                start[n] = upTo ? 31 - __builtin_clz(upTo) : -1;
+                high[n] = (float)G[n], low[n] = (float)(G[n] - high[n]);
+                if (g == 0) {
+                    reach[0][i] = high[n], reach[1][i] = low[n];
+                    wholes[i] = start[n] < 0 ? out * Exp2(G[n]) : -1.f;
+                    afters[i] = i >= latest ? in * Exp2(last - G[n]) : 0.f;
+                }
             }
+            __syncthreads();
         }
-        __syncthreads();
 
         if constexpr (mode != kMemory) {
-            const float factor = run.in * run.out;
-            const char *outputs = lowest(outputLine, first);
+            const float factor = in * out;
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 // The scores of the tile's steps with those of each tile up to it; for dots without a step's own.
                 Four lower[2][kHeld];
 #pragma unroll
                 for (int x = 0; x <= n; x++) {
+                    const F4 high4 = *reinterpret_cast<const F4 *>(reach[0] + 16 * x + 4 * g);
+                    const F4 low4 = *reinterpret_cast<const F4 *>(reach[1] + 16 * x + 4 * g);
                     float mixed[4];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const int i = 16 * n + m, j = 16 * x + 4 * g + r;
                         const float score = factor * scores[n + x][r];
                         if (mode == kGradient && x == n && i == j) diagonal[i] = score;
-                        mixed[r] = j >= start[n] && (mode == kGradient ? j < i : j <= i) ? Exp2(G[n] - reach[j]) * score : 0.f;
+                        const float d = __builtin_amdgcn_exp2f((high[n] - high4[r]) + (low[n] - low4[r])) * score;
+                        mixed[r] = x < n || (mode == kGradient ? j < i : j <= i) ? d : 0.f;
                     }
+                    if (cuts)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) mixed[r] = 16 * x + 4 * g + r >= start[n] ? mixed[r] : 0.f;
                     Split<kHeld>(mixed, lower[x]);
                 }
                 B8 both[kHeld];
                 if (n == 1) Eights(lower[0], lower[1], both);
                 __builtin_amdgcn_sched_barrier(0);
-                __syncthreads();
                 const F4 whole = *reinterpret_cast<const F4 *>(wholes + 16 * n + 4 * g);
 #pragma unroll
-                for (int c = 0; c < Tiles; c++) {
+                for (int c = 0; c < Tiles; c++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) o[n][c][r] = whole[r] < 0.f ? 0.f : whole[r] * o[n][c][r];
+                    for (int r = 0; r < 4; r++) o[n][c][r] *= whole[r];
+                if (cuts)
+#pragma unroll
+                    for (int c = 0; c < Tiles; c++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++) o[n][c][r] = whole[r] < 0.f ? 0.f : o[n][c][r];
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) {
                     Four half[2][P];
                     PiecesOf<T>(v[0], c, half[0]);
                     if (n == 0) {
                         o[n][c] = MfmaHalves<kHeld>(lower[0], half[0], o[n][c]);
                     } else {
-                        B8 column[P];
+                        B8 both2[P];
                         PiecesOf<T>(v[1], c, half[1]);
-                        Eights(half[0], half[1], column);
-                        o[n][c] = MfmaMost<kHeld>(both, column, o[n][c]);
+                        Eights(half[0], half[1], both2);
+                        o[n][c] = MfmaMost<kHeld>(both, both2, o[n][c]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 F4 own = {0, 0, 0, 0};
-                if constexpr (mode == kGradient) own = *reinterpret_cast<const F4 *>(diagonal + 16 * n + 4 * g);
+                if constexpr (mode == kGradient) {
+                    __syncthreads();
+                    own = *reinterpret_cast<const F4 *>(diagonal + 16 * n + 4 * g);
+                }
+                const int mine = full ? Tiles : Renewed(ownColumns), place = (reverse ? 12 - 4 * g : 4 * g);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int i = 16 * n + 4 * g + r;
+                    const bool real = valid == kSteps || 16 * n + 4 * g + r < valid;
+                    const int later = reverse ? 19 - 16 * n - r : 16 * n + r;
                     float x[Tiles], dot = 0;
 #pragma unroll
                     for (int c = 0; c < Tiles; c++) {
                         x[c] = o[n][c][r];
                         if constexpr (mode == kGradient) {
-                            if (c < mine) dot = fmaf(x[c], ElementOf<T>(w[n][r], c), dot);
+                            if (full || c < mine) dot = fmaf(x[c], ElementOf<T>(w[n][r], c), dot);
                             x[c] = fmaf(own[r], ElementOf<T>(v[n][r], c), x[c]);
                         }
                     }
-                    put(outputs + (long long)(reverse ? 19 - 16 * n - r : 16 * n + r) * sign * outputLine.step, reverse ? 12 - 4 * g : 4 * g, x, i < valid ? mine : 0);
-                    if constexpr (mode == kGradient)
-                        if (weightLine.p) {
-                            dot = RowSum(dot);
-                            if (m == 0 && i < valid) *Lane(dots + sign * (first + 16 * n + r + (reverse ? 12 : 0)), Renewed((reverse ? 12 - 4 * g : 4 * g) * 4)) = dot;
-                        }
+                    put(outputs.At(later), place * outputs.step, x, real ? mine : 0);
+                    if (weighs) {
+                        dot = RowSum(dot);
+                        if (m == 0 && real) *Lane(const_cast<float *>(dots) + later, Renewed(place * 4)) = dot;
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (kAhead) fetchKeys(first + kSteps);
+            advance(outputs);
+            if (weighs) dots += sign * kSteps;
         }
 
-        __builtin_amdgcn_sched_barrier(0);
-        if (mode == kMemory && kAhead) fetchKeys(first + kSteps);
-        const float kept = Exp2(last);
+        if (kAhead) fetchRows(count - first - kSteps);
+        if (cuts)
+#pragma unroll
+            for (int t = 0; t < KeyTiles; t++)
+#pragma unroll
+                for (int c = 0; c < Tiles; c++) s[t][c] = F4{0, 0, 0, 0};
         B8 kt[KeyTiles][P];
 #pragma unroll
         for (int t = 0; t < KeyTiles; t++) Eights(turned[0][t], turned[1][t], kt[t]);
+        F4 after[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) after[n] = *reinterpret_cast<const F4 *>(afters + 16 * n + 4 * g);
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             F4 x[2];
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const F4 after = *reinterpret_cast<const F4 *>(afters + 16 * n + 4 * g);
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) x[n][r] = after[r] * ElementOf<T>(v[n][r], c);
-            }
+                for (int r = 0; r < 4; r++) x[n][r] = after[n][r] * ElementOf<T>(v[n][r], c);
             B8 written[kFloatPieces];
             SplitPair<kFloatPieces>(x[0], x[1], written);
 #pragma unroll
-            for (int t = 0; t < KeyTiles; t++) {
-                F4 held;
-#pragma unroll
-                for (int r = 0; r < 4; r++) held[r] = cuts ? 0.f : kept * s[t][c][r];
-                s[t][c] = MfmaMost<3>(kt[t], written, held);
-            }
+            for (int t = 0; t < KeyTiles; t++) s[t][c] = MfmaMost<3>(kt[t], written, s[t][c] * kept);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (!kAhead) fetchKeys(first + kSteps);
-        fetchValues(first + kSteps);
+        if (!kAhead) fetchRows(count - first - kSteps);
+        fetchColumns(first + kSteps);
     }
-
     if (!finite) {
         begins();
         playSteps();
     }
 
+    const Runs all = Argument<Runs>();
+    const Run run = RunAt(which);
     if constexpr (mode == kMemory) {
         if (reverse && count > 0) scale(gateAt(count));
-        write(run.last + (before + (reverse ? span - 1 : span)) * size);
+        const int place = reverse ? span - 1 : span;
+        write(run.last + between(place));
         if (slice == 0) {
             // The span's factors.
             double sum = 0;
@@ -724,21 +779,21 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             }
             for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
             const float factor = __ballot(cleared) ? -1.f : (float)exp(sum);
-            if (lane == 0) a.factors[before + (reverse ? span - 1 : span)] = factor;
+            if (lane == 0) all.factors[(long long)head * (all.spans - 1) + place] = factor;
         }
     } else {
         if constexpr (mode == kGradient)
             if (run.crossings) {
-                const bool ends = span == a.spans - 1;
-                const float *memory = ends ? run.againstLast : run.against;
+                const bool ends = span == all.spans - 1;
                 float sum = 0;
-                if (memory) read(memory + (ends ? (long long)head : before + span) * size, [&](float x, float y) { return sum = fmaf(x, y, sum), x; });
+                if (const float *memory = ends ? run.againstLast : run.against)
+                    read(memory + (ends ? memoryAt(head) : between(span)), [&](float x, float y) { return sum = fmaf(x, y, sum), x; });
                 sum = WaveSum(sum);
-                if (lane == 0) run.crossings[((long long)slice * a.allHeads + head) * a.spans + span] = sum;
+                if (lane == 0) run.crossings[((long long)slice * all.allHeads + head) * all.spans + span] = sum;
             }
-        if (run.last && span == (reverse ? 0 : a.spans - 1)) {
+        if (run.last && span == (reverse ? 0 : all.spans - 1)) {
             if (reverse && count > 0) scale(gateAt(count));
-            write(run.last + (long long)head * size);
+            write(run.last + memoryAt(head));
         }
     }
 }

@@ -108,7 +108,7 @@ struct Step {
 // Wavefronts that a SIMD has to hold, and whether the next steps' keys and queries are on their way while the
 // values of these are worked on.
 template <class T, int KeyTiles, int Tiles, Mode mode>
-constexpr int kRunWaves = 2;
+constexpr int kRunWaves = mode != kMemory && KeyTiles * kPieces<T> >= 12 ? 1 : 2;
 template <class T, int KeyTiles, int Tiles>
 constexpr bool kRunsAhead = KeyTiles * (Tiles * 4 + (int)sizeof(T) * 4 + kPieces<T> * 4) <= 112;
 constexpr int kSteps = 2 * kChunk;  // steps that are played together: two tiles of the matrix instruction
@@ -175,6 +175,19 @@ __device__ __forceinline__ Words<kWords<T, N>> LoadWords(const T *p, int valid =
         if (valid > 0) w = reinterpret_cast<const InMemory *>(p)->w;
     }
     return w;
+}
+template <class T, int N>
+__device__ __forceinline__ Words<kWords<T, N>> WordsOf(const float (&x)[N]) {
+    Pack<T, N> p;
+#pragma unroll
+    for (int i = 0; i < N; i++) p.x[i] = As<T>(x[i]);
+    if constexpr (N * sizeof(T) < 4) return {{Bits(p.x[0])}};
+    else return __builtin_bit_cast(Words<kWords<T, N>>, p);
+}
+template <class T, int N>
+__device__ __forceinline__ Pack<T, N> PackOf(const Words<kWords<T, N>> &w) {
+    if constexpr (N * sizeof(T) < 4) return __builtin_bit_cast(Pack<T, N>, (uint16_t)w.x[0]);
+    else return __builtin_bit_cast(Pack<T, N>, w);
 }
 // The same at `base`, which all lanes share, and a lane's `place` in bytes. The place is made anew where it is used: an
 // address of a scalar and one register is only found within a block of the program.
@@ -379,19 +392,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 for (int r = 0; r < 4; r++) s[t][c][r] = cleared ? 0.f : kept * s[t][c][r];
     };
     const bool floats = mode != kMemory && RunAt(which).floats, weighs = mode == kGradient && RunAt(which).weight.p;
-    // Stores the outputs of a step at a lane's `place` in bytes.
-    const auto put = [&](const char *base, int place, const float (&x)[Tiles], int valid) {
-        if (floats) {
-            Pack<float, Tiles> o;
+    // Stores the outputs of a step at a lane's `place` in bytes, as floats or as elements.
+    const auto putFloats = [&](const char *base, int place, const float (&x)[Tiles], int valid) {
+        Pack<float, Tiles> o;
 #pragma unroll
-            for (int c = 0; c < Tiles; c++) o.x[c] = x[c];
-            StoreAt<Tiles, Whole>(reinterpret_cast<float *>(const_cast<char *>(base)), place + 4 * column, o, valid);
-        } else {
-            Pack<T, Tiles> o;
-#pragma unroll
-            for (int c = 0; c < Tiles; c++) o.x[c] = As<T>(x[c]);
-            StoreAt<Tiles, Whole>(reinterpret_cast<T *>(const_cast<char *>(base)), place + (int)sizeof(T) * column, o, valid);
-        }
+        for (int c = 0; c < Tiles; c++) o.x[c] = x[c];
+        StoreAt<Tiles, Whole>(reinterpret_cast<float *>(const_cast<char *>(base)), place + 4 * column, o, valid);
+    };
+    const auto put = [&](const char *base, int place, const Words<kWords<T, Tiles>> &x, int valid) {
+        StoreAt<Tiles, Whole>(reinterpret_cast<T *>(const_cast<char *>(base)), place + (int)sizeof(T) * column, PackOf<T, Tiles>(x), valid);
     };
 
     // All steps, one after the other.
@@ -439,7 +448,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     if (c < mine) dot = fmaf(strict[c], Float(w.x[c]), dot);
                     strict[c] = fmaf(run.out * run.in * own, Float(v.x[c]), strict[c]);
                 }
-                put(outputs.At(i), 0, strict, g == 0 ? mine : 0);
+                if (floats) putFloats(outputs.At(i), 0, strict, g == 0 ? mine : 0);
+                else put(outputs.At(i), 0, WordsOf<T>(strict), g == 0 ? mine : 0);
                 dot = RowSum(dot);
                 if (weighs && lane == 0) dots[sign * i] = dot;
             }
@@ -647,6 +657,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             __syncthreads();
         }
 
+        ColumnWords done[2][4];
         if constexpr (mode != kMemory) {
             const float factor = in * out;
 #pragma unroll
@@ -717,7 +728,8 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                             x[c] = fmaf(own[r], ElementOf<T>(v[n][r], c), x[c]);
                         }
                     }
-                    put(outputs.At(later), place * outputs.step, x, real ? mine : 0);
+                    if (!floats) done[n][r] = WordsOf<T>(x);
+                    else putFloats(outputs.At(later), place * outputs.step, x, real ? mine : 0);
                     if (weighs) {
                         dot = RowSum(dot);
                         if (m == 0 && real) *Lane(const_cast<float *>(dots) + later, Renewed(place * 4)) = dot;
@@ -725,7 +737,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            advance(outputs);
             if (weighs) dots += sign * kSteps;
         }
 
@@ -756,6 +767,22 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         }
         if (!kAhead) fetchRows(count - first - kSteps);
         fetchColumns(first + kSteps);
+        // Outputs leave behind the next steps' loads: the wait for loads, which are answered in the order in which loads and
+        // stores were sent, does not wait for them.
+        if constexpr (mode != kMemory) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (!floats) {
+                const int mine = full ? Tiles : Renewed(ownColumns), place = (reverse ? 12 - 4 * g : 4 * g) * outputs.step;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        put(outputs.At(reverse ? 19 - 16 * n - r : 16 * n + r), place, done[n][r],
+                            valid == kSteps || 16 * n + 4 * g + r < valid ? mine : 0);
+            }
+            advance(outputs);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     if (!finite) {
         begins();
@@ -825,10 +852,13 @@ inline bool IsWhole(const Attention &a) {
            (!a.d_output || IsWhole(a.d_output, a.d_output_strides, a.value_size, bytes));
 }
 
-// The tiles of 16 columns that a wavefront of a launch takes, 0 to 2 as powers of two.
+// The most tiles of 16 columns whose memory fits a wavefront's registers beside the rest.
+template <class T, int KeyTiles>
+constexpr int kMostTiles = KeyTiles * kPieces<T> <= 2 ? 4 : KeyTiles * kPieces<T> <= 8 && KeyTiles <= 6 ? 2 : 1;
+// The tiles that a wavefront of a launch takes.
 template <class T>
 int TilesOf(const Runs &runs, int count, int keyTiles) {
-    const int most = kPieces<T> * keyTiles > 12 ? 1 : kPieces<T> * keyTiles > 4 ? 2 : 4;
+    const int most = keyTiles == 2 ? kMostTiles<T, 2> : keyTiles == 4 ? kMostTiles<T, 4> : keyTiles == 6 ? kMostTiles<T, 6> : kMostTiles<T, 8>;
     for (int tiles = most; tiles > 1; tiles /= 2) {
         long long slices = 0;
         bool full = true;
@@ -869,7 +899,7 @@ inline bool IsNear(const Runs &runs, int count) {
 template <class T, Mode mode, int KeyTiles>
 void LaunchTiles(Runs &runs, int count, bool whole, hipStream_t stream) {
     runs.near = IsNear(runs, count);
-    constexpr int most = kPieces<T> * KeyTiles > 12 ? 1 : kPieces<T> * KeyTiles > 4 ? 2 : 4;
+    constexpr int most = kMostTiles<T, KeyTiles>;
     const int tiles = whole ? TilesOf<T>(runs, count, KeyTiles) : 1;
     Cut(runs, count, tiles);
     const auto launch = [&](auto kernel) {

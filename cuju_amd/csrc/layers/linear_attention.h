@@ -138,6 +138,24 @@ __device__ __forceinline__ F4 MfmaHalves(const Four (&a)[A], const Four (&b)[B],
         }
     return half ? Mfma32(Eight(left, left), Eight(right, Four{}), c) : c;
 }
+// The transpose of a lane's first or second four values of eight steps or rows, piece by piece, by a product with the identity: the
+// instruction of 16 contracted indices.
+template <int P>
+__device__ __forceinline__ void TurnHalf(const B8 (&x)[P], int which, Four eye, Four (&turned)[P]) {
+    using S4 = __attribute__((ext_vector_type(4))) short;
+    struct Halves {
+        S4 x[2];
+    };
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        const F4 t = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(Halves, x[i]).x[which], __builtin_bit_cast(S4, eye),
+                                                               F4{0, 0, 0, 0}, 0, 0, 0);
+        const float f[4] = {t[0], t[1], t[2], t[3]};
+        Four whole[1];
+        Split<1>(f, whole);
+        turned[i] = whole[0];
+    }
+}
 template <int Pieces>
 __device__ __forceinline__ void SplitPair(F4 lo, F4 hi, B8 (&x)[Pieces]) {
     const float first[4] = {lo[0], lo[1], lo[2], lo[3]}, second[4] = {hi[0], hi[1], hi[2], hi[3]};
@@ -215,6 +233,14 @@ template <int N, bool Whole, class T>
 __device__ __forceinline__ void StoreAt(T *base, int place, const Pack<T, N> &x, int valid) {
     if constexpr (!Whole) Store<N, false>(Lane(base, place), x, valid);
     else if (valid > 0) Store<N, true>(Lane(base, Renewed(place)), x, N);
+}
+// The words are made here, and not where they are used first, from values that take more registers.
+template <class X>
+__device__ __forceinline__ void Made(X &x) {
+    Words<sizeof(X) / 4> w = __builtin_bit_cast(Words<sizeof(X) / 4>, x);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(X) / 4); i++) asm volatile("" : "+v"(w.x[i]));
+    x = __builtin_bit_cast(X, w);
 }
 // Element i of such words.
 template <class T, int N>
@@ -550,7 +576,10 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         if (resets.p) advance(resets);
     };
 
-    const Eyes eyes = EyesOf(m, g);
+    // The identity as a right operand of four values a lane.
+    Four eye;
+#pragma unroll
+    for (int j = 0; j < 2; j++) eye.x[j] = (4 * g + 2 * j == m ? 0x3f80u : 0u) | (4 * g + 2 * j + 1 == m ? 0x3f800000u : 0u);
     // Steps that are too far apart for 32 bits are played one by one.
     bool finite = Argument<Runs>().near;
     begins();
@@ -570,7 +599,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 
         // Pieces of the keys and queries; products with the memory, the scores, and the keys' transpose.
         F4 mark = {0, 0, 0, 0}, scores[3], o[2][Tiles];  // scores: of the tiles 00, 10 and 11, in row order
-        Four turned[2][KeyTiles][P];
+        B8 turned[KeyTiles][P];
 #pragma unroll
         for (int x = 0; x < 3; x++) scores[x] = F4{0, 0, 0, 0};
 #pragma unroll
@@ -583,9 +612,16 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 PiecesOf<T>(nextK[n][p], kp[n]);
-                mark = Mfma32(eyes.half[0], kp[n][0], mark);
-                Turn<P>(kp[n], eyes.half[0], turned[n][2 * p]);
-                Turn<P>(kp[n], eyes.half[1], turned[n][2 * p + 1]);
+            }
+            mark = Mfma32(kp[0][0], kp[1][0], mark);
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                Four half[2][P];
+#pragma unroll
+                for (int n = 0; n < 2; n++) TurnHalf<P>(kp[n], x, eye, half[n]);
+                Eights(half[0], half[1], turned[2 * p + x]);
+#pragma unroll
+                for (int i = 0; i < P; i++) Made(turned[2 * p + x][i]);
             }
             if constexpr (mode != kMemory) {
 #pragma unroll
@@ -615,15 +651,16 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 for (int r = 0; r < 4; r++) v[n][r] = 16 * n + 4 * g + r < valid ? v[n][r] : ColumnWords{};
         const Step gate[2] = {nextGate[0], nextGate[1]};
         if (weighs) columnsAt(weights, valid, w), advance(weights);
-        // A product with anything, zeros too, tells whether a value is not finite.
+        // Products of keys, and of values, tell whether one is not finite.
 #pragma unroll
         for (int c = 0; c < Tiles; c++) {
             Four half[2][P];
 #pragma unroll
             for (int n = 0; n < 2; n++) PiecesOf<T>(v[n], c, half[n]);
-            mark = Mfma32(eyes.half[0], Eight(half[0][0], half[1][0]), mark);
+            const B8 both = Eight(half[0][0], half[1][0]);
+            mark = Mfma32(both, both, mark);
         }
-        if (__ballot(mark[0] * 0.f != 0.f || gate[0].Steep() || gate[1].Steep())) {
+        if (__ballot(((mark[0] + mark[1]) + (mark[2] + mark[3])) * 0.f != 0.f || gate[0].Steep() || gate[1].Steep())) {
             finite = false;
             break;
         }
@@ -728,8 +765,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                             x[c] = fmaf(own[r], ElementOf<T>(v[n][r], c), x[c]);
                         }
                     }
-                    if (!floats) done[n][r] = WordsOf<T>(x);
-                    else putFloats(outputs.At(later), place * outputs.step, x, real ? mine : 0);
+                    done[n][r] = WordsOf<T>(x);
+                    Made(done[n][r]);
+                    if (floats) putFloats(outputs.At(later), place * outputs.step, x, real ? mine : 0);
                     if (weighs) {
                         dot = RowSum(dot);
                         if (m == 0 && real) *Lane(const_cast<float *>(dots) + later, Renewed(place * 4)) = dot;
@@ -746,9 +784,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             for (int t = 0; t < KeyTiles; t++)
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) s[t][c] = F4{0, 0, 0, 0};
-        B8 kt[KeyTiles][P];
-#pragma unroll
-        for (int t = 0; t < KeyTiles; t++) Eights(turned[0][t], turned[1][t], kt[t]);
         F4 after[2];
 #pragma unroll
         for (int n = 0; n < 2; n++) after[n] = *reinterpret_cast<const F4 *>(afters + 16 * n + 4 * g);
@@ -762,7 +797,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             B8 written[kFloatPieces];
             SplitPair<kFloatPieces>(x[0], x[1], written);
 #pragma unroll
-            for (int t = 0; t < KeyTiles; t++) s[t][c] = MfmaMost<3>(kt[t], written, s[t][c] * kept);
+            for (int t = 0; t < KeyTiles; t++) s[t][c] = MfmaMost<3>(turned[t], written, s[t][c] * kept);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (!kAhead) fetchRows(count - first - kSteps);
@@ -854,7 +889,7 @@ inline bool IsWhole(const Attention &a) {
 
 // The most tiles of 16 columns whose memory fits a wavefront's registers beside the rest.
 template <class T, int KeyTiles>
-constexpr int kMostTiles = KeyTiles * kPieces<T> <= 2 ? 4 : KeyTiles * kPieces<T> <= 8 && KeyTiles <= 6 ? 2 : 1;
+constexpr int kMostTiles = KeyTiles * kPieces<T> <= 4 ? 4 : KeyTiles * kPieces<T> <= 8 ? 2 : 1;
 // The tiles that a wavefront of a launch takes.
 template <class T>
 int TilesOf(const Runs &runs, int count, int keyTiles) {

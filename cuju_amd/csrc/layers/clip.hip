@@ -47,9 +47,10 @@ __device__ __forceinline__ double BlockSum(double x) {
 
 // body(pointer to the first value of a tile, its values) with the tensor's element type, for the tiles of this workgroup.
 template <class Body>
-__device__ __forceinline__ void ForTiles(const Table &table, Body body) {
+__device__ __forceinline__ void ForTiles(const Table &table, bool backwards, Body body) {
     const int tiles = table.tiles[table.count];
-    for (int n = blockIdx.x; n < tiles; n += gridDim.x) {
+    for (int place = blockIdx.x; place < tiles; place += gridDim.x) {
+        const int n = backwards ? tiles - 1 - place : place;
         int low = 0, high = table.count;
         while (high - low > 1) {
             const int middle = (low + high) / 2;
@@ -69,7 +70,7 @@ __device__ __forceinline__ void ForTiles(const Table &table, Body body) {
 
 __global__ __launch_bounds__(kThreads) void SquaresKernel(Table table, double *sums) {
     double sum = 0;
-    ForTiles(table, [&](auto *data, int values) {
+    ForTiles(table, false, [&](auto *data, int values) {
         using T = std::remove_reference_t<decltype(*data)>;
         constexpr int N = 16 / sizeof(T);
         int at = threadIdx.x * N;
@@ -113,7 +114,8 @@ __global__ __launch_bounds__(kThreads) void ClipKernel(Table table, const double
     const float factor = (float)(most / (n + epsilon));
     // A comparison that keeps a NaN.
     if (factor >= 1.f) return;
-    ForTiles(table, [&](auto *data, int values) {
+    // Backwards, from what the first kernel read last and the last-level cache still holds.
+    ForTiles(table, true, [&](auto *data, int values) {
         using T = std::remove_reference_t<decltype(*data)>;
         constexpr int N = 16 / sizeof(T);
         int at = threadIdx.x * N;

@@ -744,7 +744,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                         Eights(half[0], half[1], both2);
                         o[n][c] = MfmaMost<kHeld>(both, both2, o[n][c]);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
                 F4 own = {0, 0, 0, 0};
                 if constexpr (mode == kGradient) {
@@ -798,7 +797,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             SplitPair<kFloatPieces>(x[0], x[1], written);
 #pragma unroll
             for (int t = 0; t < KeyTiles; t++) s[t][c] = MfmaMost<3>(turned[t], written, s[t][c] * kept);
-            __builtin_amdgcn_sched_barrier(0);
         }
         if (!kAhead) fetchRows(count - first - kSteps);
         fetchColumns(first + kSteps);

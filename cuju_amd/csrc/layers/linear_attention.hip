@@ -81,6 +81,7 @@ void LaunchStep(const Attention &a, hipStream_t stream) {
 
 // ------------------------------------------------------------------------------------- many steps
 
+constexpr int kJoined = 8;
 // A thread takes an element of a head's memory through the spans.
 __global__ __launch_bounds__(256) void JoinKernel(const float *first, float *memories, const float *factors, long long size,
                                                   long long elements, int spans, bool reverse) {
@@ -90,11 +91,21 @@ __global__ __launch_bounds__(256) void JoinKernel(const float *first, float *mem
         float memory = first ? first[i] : 0.f;
         float *at = memories + head * (spans - 1) * size + element;
         const float *factor = factors + head * (spans - 1);
-        for (int n = 0; n + 1 < spans; n++) {
-            const int place = reverse ? spans - 2 - n : n;
-            const float own = at[place * size], kept = factor[place];
-            memory = kept < 0.f ? own : fmaf(kept, memory, own);
-            at[place * size] = memory;
+        // Some spans' loads at a time, so that each is not waited for by itself.
+        for (int n = 0; n + 1 < spans; n += kJoined) {
+            float own[kJoined], kept[kJoined];
+#pragma unroll
+            for (int x = 0; x < kJoined; x++)
+                if (n + x + 1 < spans) {
+                    const int place = reverse ? spans - 2 - n - x : n + x;
+                    own[x] = at[place * size], kept[x] = factor[place];
+                }
+#pragma unroll
+            for (int x = 0; x < kJoined; x++)
+                if (n + x + 1 < spans) {
+                    memory = kept[x] < 0.f ? own[x] : fmaf(kept[x], memory, own[x]);
+                    at[(reverse ? spans - 2 - n - x : n + x) * size] = memory;
+                }
         }
     }
 }

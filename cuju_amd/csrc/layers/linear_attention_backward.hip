@@ -17,11 +17,11 @@ struct DecayArgs {
     float *out;      // [batch][time][head], or null
     double *totals;  // [head][span]
 };
-__global__ __launch_bounds__(64) void DecayKernel(DecayArgs a) {
+__global__ __launch_bounds__(256) void DecayKernel(DecayArgs a) {
     static_assert(kSpan == 128, "two steps a lane");
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 63;
     const long long items = (long long)a.allHeads * a.spans;
-    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+    for (long long item = blockIdx.x * 4ll + (threadIdx.x >> 6); item < items; item += gridDim.x * 4ll) {
         const int span = item % a.spans;
         const unsigned head = item / a.spans;
         const int h = head % a.heads, b = head / a.heads, begin = span * kSpan, end = min(begin + kSpan, a.time);
@@ -171,7 +171,7 @@ void Backward(const Attention &a, hipStream_t stream) {
         for (int i = 0; i < 3; i++) d.decayStrides[i] = runs.decayStrides[i];
         for (int i = 0; i < 2; i++) d.resetStrides[i] = runs.resetStrides[i];
         const long long items = heads * runs.spans;
-        hipLaunchKernelGGL(DecayKernel, dim3((unsigned)(items < (1 << 20) ? items : 1 << 20)), dim3(64), 0, stream, d);
+        hipLaunchKernelGGL(DecayKernel, dim3((unsigned)(items < (1 << 22) ? (items + 3) / 4 : 1 << 20)), dim3(256), 0, stream, d);
         if (a.decay_of_head)
             hipLaunchKernelGGL(TotalKernel, dim3(a.heads), dim3(256), 0, stream, d.totals, static_cast<float *>(a.d_decay), a.batch,
                                a.heads, runs.spans);

@@ -37,23 +37,35 @@ __device__ __forceinline__ float GateSlope(float z, int activation) {
 }
 
 // A thread's packs of a row: `Lanes` packs side by side, `Packs` such rows of packs after one another. Packs need no
-// alignment but their elements'; the last one may be cut by the row's end.
-template <class T, int Vector>
-struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    T x[Vector];
-};
+// alignment but their elements'; the last one may be cut by the row's end. They are held as the words of memory, since
+// an array of 16-bit elements would take a register for each.
+template <class T>
+__device__ __forceinline__ uint32_t Bits(T x) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
+    else return __builtin_bit_cast(uint16_t, x);
+}
 template <class T, int Vector, int Packs, int Lanes>
 struct Held {
-    Loose<T, Vector> x[Packs];
+    static constexpr int kElements = 4 / sizeof(T), kWords = Vector / kElements;
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+        uint32_t w[kWords];
+    };
+    uint32_t w[Packs][kWords];
     __device__ __forceinline__ void Load(const T *row, int lane, int size) {
 #pragma unroll
         for (int i = 0; i < Packs; i++) {
             const int at = (i * Lanes + lane) * Vector;
             if (at + Vector <= size) {
-                x[i] = *reinterpret_cast<const Loose<T, Vector> *>(Global(row) + at);
+                const Loose x = *reinterpret_cast<const Loose *>(Global(row) + at);
+#pragma unroll
+                for (int c = 0; c < kWords; c++) w[i][c] = x.w[c];
             } else {
 #pragma unroll
-                for (int c = 0; c < Vector; c++) x[i].x[c] = at + c < size ? Global(row)[at + c] : As<T>(0.f);
+                for (int c = 0; c < kWords; c++) w[i][c] = 0;
+                if (at >= size) continue;
+#pragma unroll
+                for (int c = 0; c < Vector; c++)
+                    if (at + c < size) w[i][c / kElements] |= Bits(Global(row)[at + c]) << (16 * (c % kElements));
             }
         }
     }
@@ -62,21 +74,37 @@ struct Held {
         for (int i = 0; i < Packs; i++) {
             const int at = (i * Lanes + lane) * Vector;
             if (at + Vector <= size) {
-                *reinterpret_cast<Loose<T, Vector> *>(Global(row) + at) = x[i];
-            } else {
+                Loose x;
+#pragma unroll
+                for (int c = 0; c < kWords; c++) x.w[c] = w[i][c];
+                *reinterpret_cast<Loose *>(Global(row) + at) = x;
+            } else if (at < size) {
 #pragma unroll
                 for (int c = 0; c < Vector; c++)
-                    if (at + c < size) Global(row)[at + c] = x[i].x[c];
+                    if (at + c < size) Global(row)[at + c] = As<T>(At(i, c));
             }
         }
     }
-    __device__ __forceinline__ float At(int i, int c) const { return Float(x[i].x[c]); }
+    __device__ __forceinline__ float At(int i, int c) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i][c]);
+        else if constexpr (std::is_same<T, __hip_bfloat16>::value) return __uint_as_float(c % 2 ? w[i][c / 2] & 0xffff0000u : w[i][c / 2] << 16);
+        else return __half2float(__builtin_bit_cast(__half, (uint16_t)(w[i][c / 2] >> (16 * (c % 2)))));
+    }
+    // The elements of a pack, rounded.
+    __device__ __forceinline__ void Set(int i, const float (&x)[Vector]) {
+#pragma unroll
+        for (int c = 0; c < kWords; c++) {
+            w[i][c] = Bits(As<T>(x[c * kElements]));
+            if constexpr (kElements == 2) w[i][c] |= Bits(As<T>(x[c * kElements + 1])) << 16;
+        }
+    }
 };
 // A vector of the row's columns, held through all rows.
 template <int Vector, int Packs, int Lanes>
 struct Columns {
     float x[Packs][Vector];
-    __device__ __forceinline__ Columns(const float *from, float otherwise, int lane, int size) {
+    __device__ __forceinline__ Columns(const void *p, float otherwise, int lane, int size) {
+        const float *from = static_cast<const float *>(p);
 #pragma unroll
         for (int i = 0; i < Packs; i++)
 #pragma unroll
@@ -84,6 +112,29 @@ struct Columns {
                 const int at = (i * Lanes + lane) * Vector + c;
                 x[i][c] = from && at < size ? from[at] : otherwise;
             }
+    }
+    __device__ __forceinline__ float At(int i, int c) const { return x[i][c]; }
+};
+// A thread's sums over its rows, by vector and column: in registers, or in LDS for the largest workgroups, whose threads'
+// registers do not hold them too.
+template <int Vector, int Packs, int Lanes>
+struct Sums {
+    static constexpr bool kShared = Lanes >= 1024;
+    static constexpr int kBytes = kShared ? kVectors * Packs * Vector * Lanes * (int)sizeof(float) : 0;
+    float x[kShared ? 1 : kVectors][kShared ? 1 : Packs][kShared ? 1 : Vector];
+    float *shared;
+    __device__ __forceinline__ float &At(int v, int i, int c) {
+        if constexpr (kShared) return shared[((v * Packs + i) * Vector + c) * Lanes];
+        else return x[v][i][c];
+    }
+    __device__ __forceinline__ void Add(int v, int i, int c, float a, float b) { At(v, i, c) = fmaf(a, b, At(v, i, c)); }
+    __device__ __forceinline__ Sums(float *room) : shared(room + threadIdx.x) {
+#pragma unroll
+        for (int v = 0; v < kVectors; v++)
+#pragma unroll
+            for (int i = 0; i < Packs; i++)
+#pragma unroll
+                for (int c = 0; c < Vector; c++) At(v, i, c) = 0.f;
     }
 };
 
@@ -121,9 +172,9 @@ __global__ __launch_bounds__(kThreads<Lanes>) void ForwardKernel(Rows n) {
     __shared__ float scratch[2 * (Lanes <= 64 ? 1 : Lanes / 64)];
     const int lane = threadIdx.x % Lanes, each = kThreads<Lanes> / Lanes, size = n.size;
     int half = 0;
-    const Columns<Vector, Packs, Lanes> after(static_cast<const float *>(n.after), 1.f, lane, size);
-    const Columns<Vector, Packs, Lanes> scale(static_cast<const float *>(n.scales), n.scale, lane, size);
-    const Columns<Vector, Packs, Lanes> before(static_cast<const float *>(n.before), 1.f, lane, size);
+    const Columns<Vector, Packs, Lanes> after(n.after, 1.f, lane, size);
+    const Columns<Vector, Packs, Lanes> scale(n.scales, n.scale, lane, size);
+    const Columns<Vector, Packs, Lanes> before(n.before, 1.f, lane, size);
     const float count = 1.f / size;
     for (long long row = (long long)blockIdx.x * each + threadIdx.x / Lanes; row < n.rows; row += (long long)gridDim.x * each) {
         Held<T, Vector, Packs, Lanes> block, gate{}, x{}, out;
@@ -144,20 +195,23 @@ __global__ __launch_bounds__(kThreads<Lanes>) void ForwardKernel(Rows n) {
         for (int i = 0; i < Packs; i++)
 #pragma unroll
             for (int c = 0; c < Vector; c++) {
-                float b = block.At(i, c) * inner * after.x[i][c];
+                float b = block.At(i, c) * inner * after.At(i, c);
                 if (n.gate) b *= Gate(gate.At(i, c), n.activation);
-                h[i][c] = Stream ? fmaf(scale.x[i][c], b, x.At(i, c)) : b;
+                h[i][c] = Stream ? fmaf(scale.At(i, c), b, x.At(i, c)) : b;
                 // Past the row's end all inputs are zeros, and a gate of zero may not be.
                 if constexpr (Stream) sum = fmaf(h[i][c], h[i][c], sum);
-                out.x[i].x[c] = As<T>(h[i][c]);
             }
+#pragma unroll
+        for (int i = 0; i < Packs; i++) out.Set(i, h[i]);
         out.Store(static_cast<T *>(n.stream) + row * size, lane, size);
         if constexpr (Stream) {
             outer = 1.f / sqrtf(fmaf(SumOfRow<Lanes>(sum, scratch, half), count, n.epsilon));
 #pragma unroll
-            for (int i = 0; i < Packs; i++)
+            for (int i = 0; i < Packs; i++) {
 #pragma unroll
-                for (int c = 0; c < Vector; c++) out.x[i].x[c] = As<T>(h[i][c] * outer * before.x[i][c]);
+                for (int c = 0; c < Vector; c++) h[i][c] *= outer * before.At(i, c);
+                out.Set(i, h[i]);
+            }
             out.Store(static_cast<T *>(n.normed) + row * size, lane, size);
         }
         if (n.stats && lane == 0) {
@@ -173,10 +227,11 @@ __global__ __launch_bounds__(kThreads<Lanes>) void BackwardKernel(Rows n, float 
     __shared__ float scratch[2 * (Lanes <= 64 ? 1 : Lanes / 64)];
     const int lane = threadIdx.x % Lanes, size = n.size;
     int half = 0;
-    const Columns<Vector, Packs, Lanes> after(static_cast<const float *>(n.after), 1.f, lane, size);
-    const Columns<Vector, Packs, Lanes> scale(static_cast<const float *>(n.scales), n.scale, lane, size);
-    const Columns<Vector, Packs, Lanes> before(static_cast<const float *>(n.before), 1.f, lane, size);
-    float sums[kVectors][Packs][Vector] = {};
+    const Columns<Vector, Packs, Lanes> after(n.after, 1.f, lane, size);
+    const Columns<Vector, Packs, Lanes> scale(n.scales, n.scale, lane, size);
+    const Columns<Vector, Packs, Lanes> before(n.before, 1.f, lane, size);
+    extern __shared__ float room[];
+    Sums<Vector, Packs, Lanes> sums(room);
     const float count = 1.f / size;
     for (long long row = (long long)blockIdx.x * each + threadIdx.x / Lanes; row < n.rows; row += (long long)gridDim.x * each) {
         Held<T, Vector, Packs, Lanes> block, gate{}, x{}, dh{}, dy{}, out;
@@ -189,52 +244,59 @@ __global__ __launch_bounds__(kThreads<Lanes>) void BackwardKernel(Rows n, float 
         }
         const float *stats = static_cast<const float *>(n.stats) + 2 * row;
         const float inner = stats[0], outer = stats[1];
-        float factor[Packs][Vector], u[Packs][Vector], d[Packs][Vector];
+        float factor[Packs][Vector], d[Packs][Vector];
+        const auto unit = [&](int i, int c) { return block.At(i, c) * inner; };
         float sum = 0;
 #pragma unroll
         for (int i = 0; i < Packs; i++)
 #pragma unroll
             for (int c = 0; c < Vector; c++) {
-                u[i][c] = block.At(i, c) * inner;
                 factor[i][c] = n.gate ? Gate(gate.At(i, c), n.activation) : 1.f;
                 d[i][c] = dh.At(i, c);
                 if constexpr (Stream) {
-                    const float e = outer * fmaf(scale.x[i][c], after.x[i][c] * factor[i][c] * u[i][c], x.At(i, c));
-                    sums[2][i][c] = fmaf(dy.At(i, c), e, sums[2][i][c]);
-                    sum = fmaf(dy.At(i, c) * before.x[i][c], e, sum);
+                    const float e = outer * fmaf(scale.At(i, c), after.At(i, c) * factor[i][c] * unit(i, c), x.At(i, c));
+                    sums.Add(2, i, c, dy.At(i, c), e);
+                    sum = fmaf(dy.At(i, c) * before.At(i, c), e, sum);
                 }
             }
         if constexpr (Stream) {
             const float mean = SumOfRow<Lanes>(sum, scratch, half) * count;
 #pragma unroll
-            for (int i = 0; i < Packs; i++)
+            for (int i = 0; i < Packs; i++) {
 #pragma unroll
                 for (int c = 0; c < Vector; c++) {
-                    const float b = after.x[i][c] * factor[i][c] * u[i][c], e = outer * fmaf(scale.x[i][c], b, x.At(i, c));
-                    d[i][c] = fmaf(outer, fmaf(dy.At(i, c), before.x[i][c], -e * mean), d[i][c]);
-                    sums[1][i][c] = fmaf(d[i][c], b, sums[1][i][c]);
-                    out.x[i].x[c] = As<T>(d[i][c]);
-                    d[i][c] *= scale.x[i][c];
+                    const float b = after.At(i, c) * factor[i][c] * unit(i, c), e = outer * fmaf(scale.At(i, c), b, x.At(i, c));
+                    d[i][c] = fmaf(outer, fmaf(dy.At(i, c), before.At(i, c), -e * mean), d[i][c]);
+                    sums.Add(1, i, c, d[i][c], b);
                 }
+                out.Set(i, d[i]);
+#pragma unroll
+                for (int c = 0; c < Vector; c++) d[i][c] *= scale.At(i, c);
+            }
             if (n.dx) out.Store(static_cast<T *>(n.dx) + row * size, lane, size);
         }
         sum = 0;
 #pragma unroll
-        for (int i = 0; i < Packs; i++)
+        for (int i = 0; i < Packs; i++) {
+            float slope[Vector];
 #pragma unroll
             for (int c = 0; c < Vector; c++) {
-                const float of = d[i][c] * u[i][c];
-                sums[0][i][c] = fmaf(of, factor[i][c], sums[0][i][c]);
-                if (n.gate) out.x[i].x[c] = As<T>(of * after.x[i][c] * GateSlope(gate.At(i, c), n.activation));
-                d[i][c] *= after.x[i][c] * factor[i][c];
-                sum = fmaf(d[i][c], u[i][c], sum);
+                const float of = d[i][c] * unit(i, c);
+                sums.Add(0, i, c, of, factor[i][c]);
+                slope[c] = n.gate ? of * after.At(i, c) * GateSlope(gate.At(i, c), n.activation) : 0.f;
+                d[i][c] *= after.At(i, c) * factor[i][c];
+                sum = fmaf(d[i][c], unit(i, c), sum);
             }
+            out.Set(i, slope);
+        }
         if (n.d_gate) out.Store(static_cast<T *>(n.d_gate) + row * size, lane, size);
         const float mean = n.norm_block ? SumOfRow<Lanes>(sum, scratch, half) * count : 0.f;
 #pragma unroll
-        for (int i = 0; i < Packs; i++)
+        for (int i = 0; i < Packs; i++) {
 #pragma unroll
-            for (int c = 0; c < Vector; c++) out.x[i].x[c] = As<T>(inner * fmaf(-u[i][c], mean, d[i][c]));
+            for (int c = 0; c < Vector; c++) d[i][c] = inner * fmaf(-unit(i, c), mean, d[i][c]);
+            out.Set(i, d[i]);
+        }
         if (n.d_block) out.Store(static_cast<T *>(n.d_block) + row * size, lane, size);
     }
     if (!parts) return;
@@ -251,7 +313,7 @@ __global__ __launch_bounds__(kThreads<Lanes>) void BackwardKernel(Rows n, float 
             for (int i = 0; i < Packs; i++)
 #pragma unroll
                 for (int c = 0; c < Vector; c++)
-                    shared[threadIdx.x / Lanes * (Lanes * Packs * Vector) + (i * Lanes + lane) * Vector + c] = sums[v][i][c];
+                    shared[threadIdx.x / Lanes * (Lanes * Packs * Vector) + (i * Lanes + lane) * Vector + c] = sums.At(v, i, c);
             __syncthreads();
             for (int at = threadIdx.x; at < size; at += kThreads<Lanes>) {
                 float sum = 0;
@@ -264,7 +326,7 @@ __global__ __launch_bounds__(kThreads<Lanes>) void BackwardKernel(Rows n, float 
 #pragma unroll
                 for (int c = 0; c < Vector; c++) {
                     const int at = (i * Lanes + lane) * Vector + c;
-                    if (at < size) to[at] = sums[v][i][c];
+                    if (at < size) to[at] = sums.At(v, i, c);
                 }
         }
     }
@@ -279,8 +341,20 @@ __global__ __launch_bounds__(1024) void PartsKernel(const float *parts, float *a
     if (!out) return;
     const int at = blockIdx.x * 16 + column;
     double sum = 0;
-    if (at < size)
-        for (int r = slice; r < blocks; r += 64) sum += parts[((long long)r * kVectors + blockIdx.y) * size + at];
+    if (at < size) {
+        const float *from = parts + (long long)blockIdx.y * size + at;
+        const long long step = (long long)kVectors * size;
+        int r = slice;
+        // Eight loads on the way at a time.
+        for (; r + 7 * 64 < blocks; r += 8 * 64) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = from[(r + i * 64) * step];
+#pragma unroll
+            for (int i = 0; i < 8; i++) sum += x[i];
+        }
+        for (; r < blocks; r += 64) sum += from[r * step];
+    }
     sums[slice][column] = sum;
     __syncthreads();
     for (int d = 32; d; d /= 2) {
@@ -291,23 +365,27 @@ __global__ __launch_bounds__(1024) void PartsKernel(const float *parts, float *a
 }
 
 // body(elements of a pack, packs, threads of a row) for rows of `size`.
-template <class T, class Body>
+template <class T, bool Gradients, class Body>
 void ForSize(int size, Body body) {
-    constexpr int V = sizeof(T) == 4 ? 4 : 8;
+    constexpr int V = 16 / sizeof(T);
+    // One pack a thread: two of eight elements are more than the registers of two wavefronts on a SIMD (bfloat16, 65,536
+    // rows of 1,024: the gradients 266 us on 128 threads, 366 on 64). Past 512 packs that is the largest workgroup, which
+    // the gradients are faster on (8,192 rows of 8,192: 486 against 864 us on 512 threads) and 16-bit outputs slower (204
+    // against 166).
     const int packs = (size + V - 1) / V;
-    const auto go = [&](auto packs, auto lanes) { body(std::integral_constant<int, V>(), packs, lanes); };
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    if (packs <= 4) go(One(), std::integral_constant<int, 4>());
-    else if (packs <= 8) go(One(), std::integral_constant<int, 8>());
-    else if (packs <= 16) go(One(), std::integral_constant<int, 16>());
-    else if (packs <= 32) go(One(), std::integral_constant<int, 32>());
-    else if (packs <= 64) go(One(), std::integral_constant<int, 64>());
-    else if (packs <= 128) go(Two(), std::integral_constant<int, 64>());
-    else if (packs <= 256) go(One(), std::integral_constant<int, 256>());
-    else if (packs <= 512) go(Two(), std::integral_constant<int, 256>());
-    else if (packs <= 1024) go(Two(), std::integral_constant<int, 512>());
-    else if constexpr (V == 4) go(std::integral_constant<int, 4>(), std::integral_constant<int, 512>());
+    const auto go = [&](auto lanes) { body(std::integral_constant<int, V>(), std::integral_constant<int, 1>(), lanes); };
+    if (packs <= 4) go(std::integral_constant<int, 4>());
+    else if (packs <= 8) go(std::integral_constant<int, 8>());
+    else if (packs <= 16) go(std::integral_constant<int, 16>());
+    else if (packs <= 32) go(std::integral_constant<int, 32>());
+    else if (packs <= 64) go(std::integral_constant<int, 64>());
+    else if (packs <= 128) go(std::integral_constant<int, 128>());
+    else if (packs <= 256) go(std::integral_constant<int, 256>());
+    else if (packs <= 512) go(std::integral_constant<int, 512>());
+    else if (packs <= 1024) {
+        if constexpr (Gradients || V == 4) go(std::integral_constant<int, 1024>());
+        else body(std::integral_constant<int, V>(), std::integral_constant<int, 2>(), std::integral_constant<int, 512>());
+    } else if constexpr (V == 4) body(std::integral_constant<int, V>(), std::integral_constant<int, 2>(), std::integral_constant<int, 1024>());
 }
 // Workgroups of a launch, which take `each` rows at a time.
 int Blocks(long long rows, int each) {
@@ -317,7 +395,7 @@ int Blocks(long long rows, int each) {
 
 template <class T>
 void Forward(const Rows &n, hipStream_t stream) {
-    ForSize<T>(n.size, [&](auto vector, auto packs, auto lanes) {
+    ForSize<T, false>(n.size, [&](auto vector, auto packs, auto lanes) {
         constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
         const dim3 grid(Blocks(n.rows, kThreads<L> / L)), threads(kThreads<L>);
         if (n.x) hipLaunchKernelGGL((ForwardKernel<T, V, P, L, true>), grid, threads, 0, stream, n);
@@ -325,19 +403,31 @@ void Forward(const Rows &n, hipStream_t stream) {
     });
 }
 template <class T>
-void Backward(const Rows &n, hipStream_t stream) {
+int Backward(const Rows &n, hipStream_t stream) {
+    bool fits = true;
     const bool summed = n.d_after || n.d_scales || n.d_before;
     float *parts = summed ? static_cast<float *>(n.workspace) : nullptr;
     int blocks = 0;
-    ForSize<T>(n.size, [&](auto vector, auto packs, auto lanes) {
+    ForSize<T, true>(n.size, [&](auto vector, auto packs, auto lanes) {
         constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
         blocks = Blocks(n.rows, kThreads<L> / L);
-        if (n.x) hipLaunchKernelGGL((BackwardKernel<T, V, P, L, true>), dim3(blocks), dim3(kThreads<L>), 0, stream, n, parts);
-        else hipLaunchKernelGGL((BackwardKernel<T, V, P, L, false>), dim3(blocks), dim3(kThreads<L>), 0, stream, n, parts);
+        constexpr int bytes = Sums<V, P, L>::kBytes;
+        const auto launch = [&](auto kernel) {
+            if (bytes && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+                             hipSuccess) {
+                fits = false;
+                return;
+            }
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kThreads<L>), bytes, stream, n, parts);
+        };
+        if (n.x) launch(BackwardKernel<T, V, P, L, true>);
+        else launch(BackwardKernel<T, V, P, L, false>);
     });
+    if (!fits) return Failed("hipFuncSetAttribute: the gradients of norms of rows do not fit the shared memory");
     if (summed)
         hipLaunchKernelGGL(PartsKernel, dim3((n.size + 15) / 16, kVectors), dim3(1024), 0, stream, parts, static_cast<float *>(n.d_after),
                            static_cast<float *>(n.d_scales), static_cast<float *>(n.d_before), n.size, blocks);
+    return Launched("the gradients of norms of rows");
 }
 
 bool Fits(const Rows *n) {
@@ -374,6 +464,7 @@ extern "C" __attribute__((visibility("default"))) int cuju_row_norm_backward(con
     if (n.rows == 0) return 0;
     if (!n.block || !n.stats || (n.d_gate && !n.gate)) return Failed("expected rows, their statistics and a gate for its gradient");
     if ((n.d_after || n.d_scales || n.d_before) && !n.workspace) return Failed("expected a workspace");
-    ForType(n.type, [&](auto x) { Backward<decltype(x)>(n, static_cast<hipStream_t>(stream)); });
-    return Launched("the gradients of norms of rows");
+    int status = -1;
+    ForType(n.type, [&](auto x) { status = Backward<decltype(x)>(n, static_cast<hipStream_t>(stream)); });
+    return status;
 }

@@ -687,7 +687,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 high[n] = (float)G[n], low[n] = (float)(G[n] - high[n]);
                 if (g == 0) {
                     reach[0][i] = high[n], reach[1][i] = low[n];
-                    wholes[i] = start[n] < 0 ? out * Exp2(G[n]) : -1.f;
+                    wholes[i] = out * Exp2(G[n]);
                     afters[i] = i >= latest ? in * Exp2(last - G[n]) : 0.f;
                 }
             }
@@ -731,7 +731,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
                     for (int c = 0; c < Tiles; c++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][c][r] = whole[r] < 0.f ? 0.f : o[n][c][r];
+                        for (int r = 0; r < 4; r++) o[n][c][r] = 16 * n + 4 * g + r >= __builtin_ctz(cuts) ? 0.f : o[n][c][r];
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
                     Four half[2][P];

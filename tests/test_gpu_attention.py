@@ -399,6 +399,20 @@ def test_gates_in_other_types():
         forward_close(scaled, given, decay=decay.float(), state=None, scale=3.0)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('scale', [-0.7, 0.0])
+def test_scales_that_are_not_positive(scale, dtype):
+    from cuju_amd import layers
+    given = inputs(2, 300, 1, 2, 32, 48, dtype=dtype, seed=29, episode=25)
+    leaves = {n: given[n].detach().requires_grad_() for n in NAMES}
+    output, last = layers.linear_attention(*[leaves[n] for n in NAMES[:4]], state=leaves['state'], resets=given['resets'], scale=scale)
+    forward_close((output, last), given, scale=scale)
+    d_output, d_last = torch.randn_like(output), torch.randn_like(last)
+    found = torch.autograd.grad([output, last], list(leaves.values()), [d_output, d_last])
+    d = {'d_output': d_output, 'd_last': d_last, 'scale': scale}
+    all_close({'d_' + n: x for n, x in zip(leaves, found)}, exact_attention(**given, **d), attention_terms(**given, **d))
+
+
 def test_empty_batches_and_times():
     from cuju_amd import layers
     for batch, time in ((0, 5), (3, 0), (0, 0)):

@@ -111,9 +111,11 @@ __global__ __launch_bounds__(kThreads) void NormKernel(const double *sums, int c
 __global__ __launch_bounds__(kThreads) void ClipKernel(Table table, const double *sums, int count, double most, double epsilon, float *norm) {
     const double n = NormOf(sums, count);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    const float factor = (float)(most / (n + epsilon));
+    const double whole = most / (n + epsilon);
     // A comparison that keeps a NaN.
-    if (factor >= 1.f) return;
+    if ((float)whole >= 1.f) return;
+    // A factor that a float has no digits for is taken in two steps.
+    const float factor = whole < 0x1p-100 ? 0x1p-100f : (float)whole, rest = whole < 0x1p-100 ? (float)(whole * 0x1p100) : 1.f;
     // Backwards, from what the first kernel read last and the last-level cache still holds.
     ForTiles(table, true, [&](auto *data, int values) {
         using T = std::remove_reference_t<decltype(*data)>;
@@ -126,13 +128,13 @@ __global__ __launch_bounds__(kThreads) void ClipKernel(Table table, const double
 #pragma unroll
             for (int i = 0; i < kUnroll; i++) {
 #pragma unroll
-                for (int c = 0; c < N; c++) x[i].x[c] = As<T>(Float(x[i].x[c]) * factor);
+                for (int c = 0; c < N; c++) x[i].x[c] = As<T>(Float(x[i].x[c]) * factor * rest);
                 *reinterpret_cast<Loose<T, N> *>(data + at + i * kThreads * N) = x[i];
             }
         }
         for (; at < values; at += kThreads * N)
             for (int c = 0; c < N; c++)
-                if (at + c < values) data[at + c] = As<T>(Float(data[at + c]) * factor);
+                if (at + c < values) data[at + c] = As<T>(Float(data[at + c]) * factor * rest);
     });
 }
 

@@ -113,33 +113,8 @@ template <class T, int KeyTiles, int Tiles>
 constexpr bool kRunsAhead = KeyTiles * (Tiles * 4 + (int)sizeof(T) * 4 + kPieces<T> * 4) <= 112;
 constexpr int kSteps = 2 * kChunk;  // steps that are played together: two tiles of the matrix instruction
 
-// Sums over the products of pieces whose places add up to less than `Most`.
-template <int Most, int A, int B>
-__device__ __forceinline__ F4 MfmaMost(const B8 (&a)[A], const B8 (&b)[B], F4 c) {
-#pragma unroll
-    for (int i = A - 1; i >= 0; i--)
-#pragma unroll
-        for (int j = B - 1; j >= 0; j--)
-            if (i + j < Most) c = Mfma32(a[i], b[j], c);
-    return c;
-}
-// The same of 16 contracted indices, two products to an instruction.
-template <int Most, int A, int B>
-__device__ __forceinline__ F4 MfmaHalves(const Four (&a)[A], const Four (&b)[B], F4 c) {
-    Four left{}, right{};
-    bool half = false;
-#pragma unroll
-    for (int i = A - 1; i >= 0; i--)
-#pragma unroll
-        for (int j = B - 1; j >= 0; j--) {
-            if (i + j >= Most) continue;
-            if (half) c = Mfma32(Eight(left, a[i]), Eight(right, b[j]), c);
-            left = a[i], right = b[j], half = !half;
-        }
-    return half ? Mfma32(Eight(left, left), Eight(right, Four{}), c) : c;
-}
-// The transpose of a lane's first or second four values of eight steps or rows, piece by piece, by a product with the identity: the
-// instruction of 16 contracted indices.
+// The transpose of a lane's first or second four of eight values, piece by piece, by a product with the identity: the
+// instruction of 16 contracted indices, half the time of the one of 32.
 template <int P>
 __device__ __forceinline__ void TurnHalf(const B8 (&x)[P], int which, Four eye, Four (&turned)[P]) {
     using S4 = __attribute__((ext_vector_type(4))) short;
@@ -293,7 +268,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
     constexpr bool Whole = shape != kLoose, full = shape == kFull;
     constexpr bool kAhead = kRunsAhead<T, KeyTiles, Tiles>;
     constexpr int kHeld = mode == kGradient || P == kFloatPieces ? kFloatPieces : 2;
-    // By step: the factors' sum up to it in two floats, and the factors of what it reads and writes.
+    // By step: the factors' sum up to it in two floats, and the factors of what it reads (NaN behind a reset) and writes.
     __shared__ __align__(16) float reach[2][kSteps], wholes[kSteps], afters[kSteps], diagonal[kSteps];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
     unsigned head = Place(blockIdx.x, gridDim.x);
@@ -610,9 +585,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
         for (int p = 0; p < kPairs; p++) {
             B8 kp[2][P], qp[2][P];
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                PiecesOf<T>(nextK[n][p], kp[n]);
-            }
+            for (int n = 0; n < 2; n++) PiecesOf<T>(nextK[n][p], kp[n]);
             mark = Mfma32(kp[0][0], kp[1][0], mark);
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -626,15 +599,15 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             if constexpr (mode != kMemory) {
 #pragma unroll
                 for (int n = 0; n < 2; n++) PiecesOf<T>(nextQ[n][p], qp[n]);
-                scores[0] = MfmaMost<3>(kp[0], qp[0], scores[0]);
-                scores[1] = MfmaMost<3>(kp[0], qp[1], scores[1]);
-                scores[2] = MfmaMost<3>(kp[1], qp[1], scores[2]);
+                scores[0] = Mfma32(kp[0], qp[0], scores[0]);
+                scores[1] = Mfma32(kp[0], qp[1], scores[1]);
+                scores[2] = Mfma32(kp[1], qp[1], scores[2]);
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
                     B8 sp[kHeld];
                     SplitPair<kHeld>(s[2 * p][c], s[2 * p + 1][c], sp);
 #pragma unroll
-                    for (int n = 0; n < 2; n++) o[n][c] = MfmaMost<kHeld>(qp[n], sp, o[n][c]);
+                    for (int n = 0; n < 2; n++) o[n][c] = Mfma32(qp[n], sp, o[n][c], Below<kHeld>());
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -687,7 +660,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 high[n] = (float)G[n], low[n] = (float)(G[n] - high[n]);
                 if (g == 0) {
                     reach[0][i] = high[n], reach[1][i] = low[n];
-                    wholes[i] = out * Exp2(G[n]);
+                    wholes[i] = start[n] < 0 ? out * Exp2(G[n]) : __builtin_nanf("");
                     afters[i] = i >= latest ? in * Exp2(last - G[n]) : 0.f;
                 }
             }
@@ -731,18 +704,18 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
                     for (int c = 0; c < Tiles; c++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][c][r] = 16 * n + 4 * g + r >= __builtin_ctz(cuts) ? 0.f : o[n][c][r];
+                        for (int r = 0; r < 4; r++) o[n][c][r] = whole[r] != whole[r] ? 0.f : o[n][c][r];
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
                     Four half[2][P];
                     PiecesOf<T>(v[0], c, half[0]);
                     if (n == 0) {
-                        o[n][c] = MfmaHalves<kHeld>(lower[0], half[0], o[n][c]);
+                        o[n][c] = Mfma16(lower[0], half[0], o[n][c], Below<kHeld>());
                     } else {
                         B8 both2[P];
                         PiecesOf<T>(v[1], c, half[1]);
                         Eights(half[0], half[1], both2);
-                        o[n][c] = MfmaMost<kHeld>(both, both2, o[n][c]);
+                        o[n][c] = Mfma32(both, both2, o[n][c], Below<kHeld>());
                     }
                 }
                 F4 own = {0, 0, 0, 0};
@@ -796,7 +769,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             B8 written[kFloatPieces];
             SplitPair<kFloatPieces>(x[0], x[1], written);
 #pragma unroll
-            for (int t = 0; t < KeyTiles; t++) s[t][c] = MfmaMost<3>(turned[t], written, s[t][c] * kept);
+            for (int t = 0; t < KeyTiles; t++) s[t][c] = Mfma32(turned[t], written, s[t][c] * kept);
         }
         if (!kAhead) fetchRows(count - first - kSteps);
         fetchColumns(first + kSteps);
@@ -917,13 +890,13 @@ inline void Cut(Runs &runs, int count, int tiles) {
     }
 }
 
-inline bool IsNear(const Runs &runs, int count) {
-    const auto near = [](long long stride) { return stride >= 0 && stride < (1 << 24); };
-    if (!near(runs.decayStrides[1]) || !near(runs.resetStrides[1])) return false;
+inline bool IsNear(const Runs &runs, int count, size_t bytes) {
+    const auto near = [](long long stride, size_t bytes) { return stride >= 0 && stride < (1 << 26) / (long long)bytes; };
+    if (!near(runs.decayStrides[1], sizeof(float)) || !near(runs.resetStrides[1], 1)) return false;
     for (int i = 0; i < count; i++) {
         const Run &r = runs.run[i];
-        if (!near(r.query.strides[1]) || !near(r.key.strides[1]) || !near(r.value.strides[1]) || !near(r.weight.strides[1]) ||
-            !near(r.outputStrides[1]))
+        if (!near(r.query.strides[1], bytes) || !near(r.key.strides[1], bytes) || !near(r.value.strides[1], bytes) ||
+            !near(r.weight.strides[1], bytes) || !near(r.outputStrides[1], r.floats ? sizeof(float) : bytes))
             return false;
     }
     return true;
@@ -931,7 +904,7 @@ inline bool IsNear(const Runs &runs, int count) {
 
 template <class T, Mode mode, int KeyTiles>
 void LaunchTiles(Runs &runs, int count, bool whole, hipStream_t stream) {
-    runs.near = IsNear(runs, count);
+    runs.near = IsNear(runs, count, sizeof(T));
     constexpr int most = kMostTiles<T, KeyTiles>;
     const int tiles = whole ? TilesOf<T>(runs, count, KeyTiles) : 1;
     Cut(runs, count, tiles);

@@ -810,7 +810,8 @@ def clip_gradients(gradients, most, *, epsilon=1e-6):
     summed in 64 bits in an order that is always the same. Every value is multiplied by
     `min(1, most / (norm + epsilon))`; gradients below `most` are not written, and with `most` of infinity none
     are. A norm that is not finite spreads, as in the formula. The values of a tensor have to lie side by side
-    in memory, and no two tensors may share any. The norm is a float32 tensor [] on the device, and nothing waits for it.
+    in memory, and no two tensors may share any. The norm is a float32 tensor [] on the device, and nothing waits for it; one
+    past the range of float32 is returned as infinity, and clips by its value.
     """
     gradients = [gradients] if isinstance(gradients, torch.Tensor) else [each for each in gradients if each is not None]
     if not gradients:

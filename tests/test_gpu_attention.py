@@ -454,6 +454,21 @@ def test_offsets_past_32_bits():
         all_close(found, exact_attention(**given, **d), attention_terms(**given, **d))
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_the_widest_steps_that_are_played_together(dtype):
+    stride = (1 << 26) // dtype.itemsize - 8
+    given = inputs(1, 60, 1, 1, 64, 32, dtype=dtype, seed=30, episode=25)
+    room = torch.empty(60 * stride, dtype=dtype, device='cuda')
+    wanted, d_output, d_last = learn(given)
+    for name in ('query', 'key', 'value'):
+        size = given[name].shape[-1]
+        view = room.as_strided((1, 60, 1, size), (size, stride, size, 1))
+        view.copy_(given[name])
+        found, _, _ = learn({**given, name: view}, d_output, d_last)
+        for n in wanted:
+            assert torch.equal(found[n], wanted[n]), (name, n)
+
+
 def test_calls_repeat_bit_for_bit():
     for fixed in (False, True):
         given = inputs(30, 200, 2, 4, 64, 64, dtype=torch.bfloat16, seed=16, episode=30, fixed=fixed)

@@ -1,7 +1,8 @@
 """Clipped gradients against their definition in 64 bits (tests/block_oracle.py).
 
 The norm is a sum in 64 bits, rounded once to 32: off by at most 2^-24. A clipped value is a product with a factor that is
-rounded once, and is rounded itself: off by 2 x 2^-24 in 32 bits, and by 2^-8 or 2^-11 more in bfloat16 or float16.
+rounded once, and is rounded itself: off by 2 x 2^-24 in 32 bits, and by 2^-8 or 2^-11 more in bfloat16 or float16. (A
+factor below 2^-100 is a power of two, which rounds nothing that is not too small, and a rest that is rounded once.)
 """
 
 import pytest
@@ -29,7 +30,11 @@ def clip_close(gradients, most, **options):
     norm, exact = exact_clip(gradients, most, **options)
     found = clip(gradients, most, **options)
     assert found.shape == () and found.dtype == torch.float32
-    assert abs(float(found) - norm) <= 2.0 ** -24 * norm
+    # Rounded to 32 bits, a norm past their largest number, (2 - 2^-23) 2^127, is an infinity.
+    if norm >= 2.0 ** 128:
+        assert float(found) == float('inf')
+    else:
+        assert abs(float(found) - norm) <= 2.0 ** -24 * norm
     for x, wanted in zip(gradients, exact):
         error, allowed = (x.double() - wanted).abs(), (2.0 ** -23 + ROUNDING[x.dtype]) * wanted.abs()
         # Of numbers too small for all their digits the last digit.
@@ -95,6 +100,12 @@ def test_values_of_all_sizes():
     small = torch.tensor([3e-30, -4e-30], device='cuda')
     assert abs(float(clip([small], 1.0)) - 5e-30) <= 2.0 ** -23 * 5e-30
     clip_close([torch.tensor([6e4, 1.0, 6e-8], device='cuda').half()], 0.5)
+
+
+@pytest.mark.parametrize('most', [1.0, 1e-6, 1e-25])
+def test_factors_below_the_range_of_floats(most):
+    clip_close([torch.full((7,), 3e38, device='cuda'), torch.full((5,), 1e38, dtype=torch.bfloat16, device='cuda'),
+                torch.full((5,), 6e4, dtype=torch.float16, device='cuda')], most)
 
 
 @pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])

@@ -160,11 +160,17 @@ void Backward(const Attention &a, hipStream_t stream) {
     dv.first = static_cast<const float *>(a.d_last), dv.starts = work + at.memories, dv.last = static_cast<float *>(a.d_state);
     put(dv, a.d_value, false);
 
+    // Kernels of full tiles take runs of one number of rows, which those of keys and values of different sizes do not have:
+    // where it makes one of them full, and with enough wavefronts, the values' run has a launch of its own. (bfloat16, 64 steps:
+    // 4,096 heads of 128 x 64 take 274 against 755 us, 512 of 32 x 64 28 against 37; 256 of 48 x 64 33 against 29.)
+    const bool full = a.key_size % 16 == 0 && a.value_size % 16 == 0 && (a.key_size % 32 == 0 || a.value_size % 32 == 0);
+    const bool apart = whole && full && a.key_size != a.value_size &&
+                       heads * runs.spans * ((2 * a.key_size + a.value_size) / 16) >= 11 * 256;
     if (a.d_decay) {
         const long long slices = (a.key_size + 15) / 16;
         dq.dots = work + at.dots, dk.dots = work + at.dots + slices * tokens;
         dq.crossings = work + at.crossings, dq.against = work + at.memories, dq.againstLast = static_cast<const float *>(a.d_last);
-        LaunchRuns<T, kGradient>(runs, 3, whole, stream);
+        LaunchRuns<T, kGradient>(runs, apart ? 2 : 3, whole, stream);
         DecayArgs d{dq.dots, dk.dots, dq.crossings, runs.slices[0], runs.slices[1], a.time, a.heads, runs.spans, runs.allHeads, runs.decay,
                     runs.resets, {}, {}, a.decay_of_head ? nullptr : static_cast<float *>(a.d_decay),
                     a.decay_of_head ? reinterpret_cast<double *>(work + at.totals) : nullptr};
@@ -176,7 +182,11 @@ void Backward(const Attention &a, hipStream_t stream) {
             hipLaunchKernelGGL(TotalKernel, dim3(a.heads), dim3(256), 0, stream, d.totals, static_cast<float *>(a.d_decay), a.batch,
                                a.heads, runs.spans);
     } else {
-        RunOutputs(runs, 3, a.type, whole, stream);
+        RunOutputs(runs, apart ? 2 : 3, a.type, whole, stream);
+    }
+    if (apart) {
+        runs.run[0] = dv;
+        RunOutputs(runs, 1, a.type, whole, stream);
     }
     if (share > 1) {
         const long long count = tokens / share * a.key_size;

@@ -371,7 +371,7 @@ void ForSize(int size, Body body) {
     // One pack a thread: two of eight elements are more than the registers of two wavefronts on a SIMD (bfloat16, 65,536
     // rows of 1,024: the gradients 266 us on 128 threads, 366 on 64). Past 512 packs that is the largest workgroup, which
     // the gradients are faster on (8,192 rows of 8,192: 486 against 864 us on 512 threads) and 16-bit outputs slower (204
-    // against 166).
+    // against 166; both with four times the workgroups of now).
     const int packs = (size + V - 1) / V;
     const auto go = [&](auto lanes) { body(std::integral_constant<int, V>(), std::integral_constant<int, 1>(), lanes); };
     if (packs <= 4) go(std::integral_constant<int, 4>());
@@ -387,17 +387,25 @@ void ForSize(int size, Body body) {
         else body(std::integral_constant<int, V>(), std::integral_constant<int, 2>(), std::integral_constant<int, 512>());
     } else if constexpr (V == 4) body(std::integral_constant<int, V>(), std::integral_constant<int, 2>(), std::integral_constant<int, 1024>());
 }
-// Workgroups of a launch, which take `each` rows at a time.
-int Blocks(long long rows, int each) {
-    const long long all = (rows + each - 1) / each;
-    return (int)(all < 2048 ? all : 2048);
+// Workgroups of a launch of rows of packs of V on L threads. 2^18 threads, four wavefronts a SIMD, read few vectors and leave
+// few sums: bfloat16, 8,192 rows of 8,192: the gradients 274 us, with 2^19 threads 303, with 2^20 367; 16,384 rows of 4,096:
+// 274, 301 and 361. The gradients of rows within a wavefront, whose workgroups leave one sum for all of theirs, and short rows
+// that end within a pack, which wait for their last elements, want more wavefronts: 2^18 and 2^19 threads, 262,144 rows of 256
+// in bfloat16: 261 and 233 us; 262,144 rows of 65 in float32, forward: 121 and 80 us.
+constexpr int kMostBlocks = 1 << 11;
+template <int V, int L, bool Gradients>
+int Blocks(const Rows &n) {
+    constexpr int each = kThreads<L> / L;
+    const long long all = (n.rows + each - 1) / each, most = (L <= 64 && (Gradients || n.size % V) ? 1 << 19 : 1 << 18) / kThreads<L>;
+    static_assert((1 << 19) / 256 <= kMostBlocks && (1 << 18) / 128 <= kMostBlocks, "as many sums as workgroups");
+    return (int)(all < most ? all : most);
 }
 
 template <class T>
 void Forward(const Rows &n, hipStream_t stream) {
     ForSize<T, false>(n.size, [&](auto vector, auto packs, auto lanes) {
         constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
-        const dim3 grid(Blocks(n.rows, kThreads<L> / L)), threads(kThreads<L>);
+        const dim3 grid(Blocks<V, L, false>(n)), threads(kThreads<L>);
         if (n.x) hipLaunchKernelGGL((ForwardKernel<T, V, P, L, true>), grid, threads, 0, stream, n);
         else hipLaunchKernelGGL((ForwardKernel<T, V, P, L, false>), grid, threads, 0, stream, n);
     });
@@ -410,7 +418,7 @@ int Backward(const Rows &n, hipStream_t stream) {
     int blocks = 0;
     ForSize<T, true>(n.size, [&](auto vector, auto packs, auto lanes) {
         constexpr int V = decltype(vector)::value, P = decltype(packs)::value, L = decltype(lanes)::value;
-        blocks = Blocks(n.rows, kThreads<L> / L);
+        blocks = Blocks<V, L, true>(n);
         constexpr int bytes = Sums<V, P, L>::kBytes;
         const auto launch = [&](auto kernel) {
             if (bytes && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
@@ -445,8 +453,8 @@ using namespace layers;
 
 extern "C" __attribute__((visibility("default"))) unsigned long long cuju_row_norm_workspace(const struct cuju_row_norm *norm) {
     if (!Fits(norm)) return 0;
-    // At least as many workgroups as any launch has.
-    return (unsigned long long)Blocks(norm->rows, 1) * kVectors * norm->size * sizeof(float);
+    // At least as many workgroups as any launch has: of a row, or fewer.
+    return (unsigned long long)(norm->rows < kMostBlocks ? norm->rows : kMostBlocks) * kVectors * norm->size * sizeof(float);
 }
 
 extern "C" __attribute__((visibility("default"))) int cuju_row_norm_forward(const struct cuju_row_norm *norm, void *stream) {

@@ -105,12 +105,11 @@ struct Step {
     __device__ __forceinline__ bool Steep() const { return !(decay <= 2.f); }
 };
 
-// Wavefronts that a SIMD has to hold, and whether the next steps' keys and queries are on their way while the
-// values of these are worked on.
+// Wavefronts that a SIMD has to hold: two hide each other's waits, and the largest memories of floats leave registers for
+// one. With one and two, 4,096 heads and 64 steps: float32 64 x 64 forward 230 and 142 us, gradients 659 and 383; float16
+// 128 x 128 598 and 346, 1,498 and 1,168; float32 96 x 96 431 and 552, 1,159 and 1,553.
 template <class T, int KeyTiles, int Tiles, Mode mode>
-constexpr int kRunWaves = mode != kMemory && KeyTiles * kPieces<T> >= 12 ? 1 : 2;
-template <class T, int KeyTiles, int Tiles>
-constexpr bool kRunsAhead = KeyTiles * (Tiles * 4 + (int)sizeof(T) * 4 + kPieces<T> * 4) <= 112;
+constexpr int kRunWaves = mode != kMemory && KeyTiles * kPieces<T> >= 18 ? 1 : 2;
 constexpr int kSteps = 2 * kChunk;  // steps that are played together: two tiles of the matrix instruction
 
 // The transpose of a lane's first or second four of eight values, piece by piece, by a product with the identity: the
@@ -251,6 +250,12 @@ __device__ __forceinline__ void PiecesOf(const Words<N> (&w)[4], int i, Four (&p
 // One wavefront takes 16 * Tiles columns of a head's memory through a span, 32 steps at a time, with the memory in
 // registers. The columns never mix, so the wavefronts of a head share nothing.
 //
+// What bounds it: memory where heads are many and products few: 16,384 heads of 64 x 64 and 64 steps in bfloat16, forward,
+// move 1.07 GB in 250 us, 4.3 TB/s (a copy reaches 4.8), and the three runs of their gradients 1.75 GB in 560 to 585, 3.1 TB/s.
+// There the vector instructions between the products show: two wavefronts a SIMD are all that the registers hold. Few long
+// sequences wait for the chain of chunks: 3,000 steps of 44 heads of 128 x 128 take 39 us for the spans' own memories, 21 to
+// join them and 82 for the outputs.
+//
 // With the steps i, j of a chunk, G_i the product of the factors up to i and D_ij of those from j + 1 to i (0 across an
 // episode's start), O = out (G Q S + in (D o Q K^T) V), and the memory becomes G_C S + K^T (in D_C V). The products
 // are sums of products of bfloat16 pieces (common.h), 32 indices an instruction. A 16-bit output takes the memory and the
@@ -266,7 +271,6 @@ template <class T, int KeyTiles, int Tiles, Shape shape, Mode mode>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T, KeyTiles, Tiles, mode>))) void RunKernel(Runs a) {
     constexpr int P = kPieces<T>, kPairs = KeyTiles / 2;
     constexpr bool Whole = shape != kLoose, full = shape == kFull;
-    constexpr bool kAhead = kRunsAhead<T, KeyTiles, Tiles>;
     constexpr int kHeld = mode == kGradient || P == kFloatPieces ? kFloatPieces : 2;
     // By step: the factors' sum up to it in two floats, and the factors of what it reads (NaN behind a reset) and writes.
     __shared__ __align__(16) float reach[2][kSteps], wholes[kSteps], afters[kSteps], diagonal[kSteps];
@@ -750,7 +754,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
             if (weighs) dots += sign * kSteps;
         }
 
-        if (kAhead) fetchRows(count - first - kSteps);
+        fetchRows(count - first - kSteps);
         if (cuts)
 #pragma unroll
             for (int t = 0; t < KeyTiles; t++)
@@ -771,7 +775,6 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
             for (int t = 0; t < KeyTiles; t++) s[t][c] = Mfma32(turned[t], written, s[t][c] * kept);
         }
-        if (!kAhead) fetchRows(count - first - kSteps);
         fetchColumns(first + kSteps);
         // Outputs leave behind the next steps' loads: the wait for loads, which are answered in the order in which loads and
         // stores were sent, does not wait for them.
@@ -858,10 +861,13 @@ inline bool IsWhole(const Attention &a) {
            (!a.d_output || IsWhole(a.d_output, a.d_output_strides, a.value_size, bytes));
 }
 
-// The most tiles of 16 columns whose memory fits a wavefront's registers beside the rest.
+// The most tiles of 16 columns whose memory fits a wavefront's registers beside the rest: the keys of a chunk are turned once
+// for all of them. With half of them 4,096 heads and 64 steps of bfloat16 64 x 64 take 66 us for 53, gradients 181 for 133;
+// 128 x 128 302 for 225, 713 for 536; float16 96 x 96 217 for 159, 581 for 416. Float32 64 x 64 with two 169 for 140.
 template <class T, int KeyTiles>
-constexpr int kMostTiles = KeyTiles * kPieces<T> <= 4 ? 4 : KeyTiles * kPieces<T> <= 8 ? 2 : 1;
-// The tiles that a wavefront of a launch takes.
+constexpr int kMostTiles = KeyTiles * kPieces<T> <= 4 ? 4 : KeyTiles * kPieces<T> <= (kPieces<T> == kFloatPieces ? 8 : 12) ? 2 : 1;
+// The tiles that a wavefront of a launch takes: as many as leave a wavefront for each of the chip's 1,024 SIMDs. (bfloat16
+// 64 x 64, 64 steps, forward, with one tile and with four: 256 heads 11.3 and 13.4 us, 2,048 heads 43 and 26.)
 template <class T>
 int TilesOf(const Runs &runs, int count, int keyTiles) {
     const int most = keyTiles == 2 ? kMostTiles<T, 2> : keyTiles == 4 ? kMostTiles<T, 4> : keyTiles == 6 ? kMostTiles<T, 6> : kMostTiles<T, 8>;

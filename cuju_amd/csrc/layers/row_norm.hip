@@ -11,7 +11,9 @@
 //   du = dh scale after act(gate),  d_block = inner (du - u mean(du u)).
 //
 // All sums are in 32 bits or more. A row lies in the registers of a part of a wavefront or of a workgroup: every input
-// is read once and every output written once.
+// is read once and every output written once, and memory bounds it. With everything, 262,144 rows of 256 in bfloat16 take
+// 135 us (0.67 GB, 5.0 TB/s) and their gradients 225 to 233 (1.07 GB, 4.7 TB/s; a copy reaches 4.8). Rows of odd sizes and 16-bit
+// rows past 2,048 values reach less: 8,192 rows of 8,192 140 and 274 us (4.8 and 3.9 TB/s), of 8,191 220 and 473.
 #include "../../../include/cuju_amd.h"
 #include "common.h"
 

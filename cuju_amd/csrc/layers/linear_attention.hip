@@ -114,8 +114,8 @@ __global__ __launch_bounds__(256) void JoinKernel(const float *first, float *mem
 
 // Few heads are cut into spans, so that more wavefronts run: the memories at the spans' ends cost more than half of the
 // outputs. Measured in bfloat16 with memories of 64 x 64, cut and whole: 512 tiles and 1,024 steps 47 and 89 us, 256 steps 30
-// and 25; 1,024 tiles 65 and 102; 2,048 tiles 126 and 117. In float32, whose wavefronts have a SIMD to themselves
-// earlier: 512 tiles 130 and 141, 1,024 tiles 236 and 176.
+// and 25; 1,024 tiles 65 and 102; 2,048 tiles 126 and 118. In float32: 512 tiles 92 and
+// 126, 1,024 tiles 167 and 160.
 bool Splits(const Attention &a) {
     const long long heads = (long long)a.batch * a.heads;
     return a.time >= 3 * kSpan && heads * ((a.value_size + 15) / 16) < (a.type == 0 ? 1024 : 2048);

@@ -12,11 +12,12 @@
 * `clip_gradients`: the global norm of an update's gradients, which are clipped by it in place.
 
 All run on the current stream of their tensors' device, wait for nothing, and can be captured in a
-HIP graph. Under `torch.compile`, tracers, dispatch modes and function transforms, and for tensors of a
-subclass, they are operators of torch's namespace `cuju_amd`, of their own names (both norms of rows are
-`cuju_amd::row_norm`) with their backward operators. Element types
-are float32, bfloat16 and float16; sums, statistics and memories are held in 32 bits whatever the
-type. There is no implementation for another device. Gradients are those of reverse mode, of first
+HIP graph; a backward pass only while no eager graph of the same leaves is alive (torch ties a leaf to the
+stream of the first graph that uses it), so let such outputs go first. Under `torch.compile`, tracers,
+dispatch modes and function transforms, and for tensors of a subclass, they are operators of torch's
+namespace `cuju_amd`, of their own names (both norms of rows are `cuju_amd::row_norm`) with their backward
+operators. Element types are float32, bfloat16 and float16; sums, statistics and memories are held in 32
+bits whatever the type. There is no implementation for another device. Gradients are those of reverse mode, of first
 order; forward-mode derivatives are refused.
 """
 

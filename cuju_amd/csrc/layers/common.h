@@ -177,29 +177,27 @@ __device__ __forceinline__ void Split(const Pack<T, 4> &x, Four (&piece)[kPieces
         Split<kPieces<T>>(f, piece);
     }
 }
-// The sum over the pieces' products, largest first in neither order: all i + j below three, or `Most`.
-template <int Most>
-using Below = std::integral_constant<int, Most>;
-template <int A, int B, int Most = 3>
-__device__ __forceinline__ F4 Mfma32(const B8 (&a)[A], const B8 (&b)[B], F4 c, Below<Most> = {}) {
+// The sum over the pieces' products, largest first in neither order: all i + j below three.
+template <int A, int B>
+__device__ __forceinline__ F4 Mfma32(const B8 (&a)[A], const B8 (&b)[B], F4 c) {
 #pragma unroll
     for (int i = A - 1; i >= 0; i--)
 #pragma unroll
         for (int j = B - 1; j >= 0; j--)
-            if (i + j < Most) c = Mfma32(a[i], b[j], c);
+            if (i + j < 3) c = Mfma32(a[i], b[j], c);
     return c;
 }
 // A product of only 16 contracted indices, four a lane: two pairs of pieces share an instruction. (The
 // instruction for 16 indices does not mix with this one: chained on one accumulator they gave wrong sums.)
-template <int A, int B, int Most = 3>
-__device__ __forceinline__ F4 Mfma16(const Four (&a)[A], const Four (&b)[B], F4 c, Below<Most> = {}) {
+template <int A, int B>
+__device__ __forceinline__ F4 Mfma16(const Four (&a)[A], const Four (&b)[B], F4 c) {
     Four left{}, right{};
     bool half = false;
 #pragma unroll
     for (int i = A - 1; i >= 0; i--)
 #pragma unroll
         for (int j = B - 1; j >= 0; j--) {
-            if (i + j >= Most) continue;
+            if (i + j >= 3) continue;
             if (half) c = Mfma32(Eight(left, a[i]), Eight(right, b[j]), c);
             left = a[i], right = b[j], half = !half;
         }

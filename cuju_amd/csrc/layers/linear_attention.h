@@ -258,9 +258,9 @@ __device__ __forceinline__ void PiecesOf(const Words<N> (&w)[4], int i, Four (&p
 //
 // With the steps i, j of a chunk, G_i the product of the factors up to i and D_ij of those from j + 1 to i (0 across an
 // episode's start), O = out (G Q S + in (D o Q K^T) V), and the memory becomes G_C S + K^T (in D_C V). The products
-// are sums of products of bfloat16 pieces (common.h), 32 indices an instruction. A 16-bit output takes the memory and the
-// scores in two pieces, 16 bits: the 2^-16 that is lost of a term is less than the output's rounding by 2^-9 or
-// 2^-12. The memory itself, and outputs whose dots are taken for the decays, keep all three.
+// are sums of products of bfloat16 pieces (common.h), 32 indices an instruction. Memories and scores have all three pieces
+// whatever the type: with two of them, cut off, a term would lose up to 2^-15 of itself, always towards zero, and terms that cancel
+// would leave that of themselves.
 //
 // A lane holds eight neighbouring rows of a pair of tiles: rows 32 p + 8 g + 4 x + r of the tiles 2 p + x, so that its
 // keys are 16 bytes of memory. Which rows a tile has is free as long as queries, keys and memory agree.
@@ -271,7 +271,6 @@ template <class T, int KeyTiles, int Tiles, Shape shape, Mode mode>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T, KeyTiles, Tiles, mode>))) void RunKernel(Runs a) {
     constexpr int P = kPieces<T>, kPairs = KeyTiles / 2;
     constexpr bool Whole = shape != kLoose, full = shape == kFull;
-    constexpr int kHeld = mode == kGradient || P == kFloatPieces ? kFloatPieces : 2;
     // By step: the factors' sum up to it in two floats, and the factors of what it reads (NaN behind a reset) and writes.
     __shared__ __align__(16) float reach[2][kSteps], wholes[kSteps], afters[kSteps], diagonal[kSteps];
     const int lane = threadIdx.x, m = lane & 15, g = lane >> 4;
@@ -608,10 +607,10 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 scores[2] = Mfma32(kp[1], qp[1], scores[2]);
 #pragma unroll
                 for (int c = 0; c < Tiles; c++) {
-                    B8 sp[kHeld];
-                    SplitPair<kHeld>(s[2 * p][c], s[2 * p + 1][c], sp);
+                    B8 sp[kFloatPieces];
+                    SplitPair<kFloatPieces>(s[2 * p][c], s[2 * p + 1][c], sp);
 #pragma unroll
-                    for (int n = 0; n < 2; n++) o[n][c] = Mfma32(qp[n], sp, o[n][c], Below<kHeld>());
+                    for (int n = 0; n < 2; n++) o[n][c] = Mfma32(qp[n], sp, o[n][c]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -677,7 +676,7 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 // The scores of the tile's steps with those of each tile up to it; for dots without a step's own.
-                Four lower[2][kHeld];
+                Four lower[2][kFloatPieces];
 #pragma unroll
                 for (int x = 0; x <= n; x++) {
                     const F4 high4 = *reinterpret_cast<const F4 *>(reach[0] + 16 * x + 4 * g);
@@ -694,9 +693,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     if (cuts)
 #pragma unroll
                         for (int r = 0; r < 4; r++) mixed[r] = 16 * x + 4 * g + r >= start[n] ? mixed[r] : 0.f;
-                    Split<kHeld>(mixed, lower[x]);
+                    Split<kFloatPieces>(mixed, lower[x]);
                 }
-                B8 both[kHeld];
+                B8 both[kFloatPieces];
                 if (n == 1) Eights(lower[0], lower[1], both);
                 __builtin_amdgcn_sched_barrier(0);
                 const F4 whole = *reinterpret_cast<const F4 *>(wholes + 16 * n + 4 * g);
@@ -714,12 +713,12 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                     Four half[2][P];
                     PiecesOf<T>(v[0], c, half[0]);
                     if (n == 0) {
-                        o[n][c] = Mfma16(lower[0], half[0], o[n][c], Below<kHeld>());
+                        o[n][c] = Mfma16(lower[0], half[0], o[n][c]);
                     } else {
                         B8 both2[P];
                         PiecesOf<T>(v[1], c, half[1]);
                         Eights(half[0], half[1], both2);
-                        o[n][c] = Mfma32(both, both2, o[n][c], Below<kHeld>());
+                        o[n][c] = Mfma32(both, both2, o[n][c]);
                     }
                 }
                 F4 own = {0, 0, 0, 0};

@@ -53,7 +53,7 @@ struct Runs {
     const unsigned char *resets;
     long long decayStrides[3], resetStrides[2];
     bool near;       // whether 32 steps of every tensor are within 2^31 bytes
-    float *factors;  // [head][spans - 1]: the product of a span's factors, or -1 where an episode starts in it
+    double *factors;  // [head][spans - 1]: the product of a span's factors, or -1 where an episode starts in it
     Run run[3];
 };
 // A run out of the kernel's arguments, where an index that the compiler does not know would copy them all, read anew
@@ -813,7 +813,9 @@ __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T,
                 sum += gate.decay;
             }
             for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-            const float factor = __ballot(cleared) ? -1.f : (float)exp(sum);
+            // In 64 bits: 128 factors may leave the range of 32 where a memory times them does not. Those that leave 64 leave 32
+            // with the least memory, but not with one of zero.
+            const double factor = __ballot(cleared) ? -1. : exp(sum > 700. && sum < __builtin_inf() ? 700. : sum);
             if (lane == 0) all.factors[(long long)head * (all.spans - 1) + place] = factor;
         }
     } else {

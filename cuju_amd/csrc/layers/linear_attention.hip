@@ -85,17 +85,18 @@ void LaunchStep(const Attention &a, hipStream_t stream) {
 constexpr int kJoined = 8;
 // A thread takes an element of a head's memory through the spans. It waits for memory: eight spans' loads are on their way
 // together (44 heads of 128 x 128 through 24 spans 21 us, 66 MB each way).
-__global__ __launch_bounds__(256) void JoinKernel(const float *first, float *memories, const float *factors, long long size,
+__global__ __launch_bounds__(256) void JoinKernel(const float *first, float *memories, const double *factors, long long size,
                                                   long long elements, int spans, bool reverse) {
     const long long step = (long long)gridDim.x * blockDim.x;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < elements; i += step) {
         const long long head = i / size, element = i % size;
         float memory = first ? first[i] : 0.f;
         float *at = memories + head * (spans - 1) * size + element;
-        const float *factor = factors + head * (spans - 1);
+        const double *factor = factors + head * (spans - 1);
         // Some spans' loads at a time, so that each is not waited for by itself.
         for (int n = 0; n + 1 < spans; n += kJoined) {
-            float own[kJoined], kept[kJoined];
+            float own[kJoined];
+            double kept[kJoined];
 #pragma unroll
             for (int x = 0; x < kJoined; x++)
                 if (n + x + 1 < spans) {
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(256) void JoinKernel(const float *first, float *mem
 #pragma unroll
             for (int x = 0; x < kJoined; x++)
                 if (n + x + 1 < spans) {
-                    memory = kept[x] < 0.f ? own[x] : fmaf(kept[x], memory, own[x]);
+                    memory = kept[x] < 0. ? own[x] : (float)fma(kept[x], (double)memory, (double)own[x]);
                     at[(reverse ? spans - 2 - n - x : n + x) * size] = memory;
                 }
         }
@@ -137,7 +138,7 @@ void Forward(const Attention &a, hipStream_t stream) {
     if (Splits(a)) {
         const long long size = (long long)a.key_size * a.value_size, kept = (long long)runs.allHeads * (runs.spans - 1);
         float *memories = static_cast<float *>(a.checkpoints ? a.checkpoints : a.workspace);
-        runs.factors = a.checkpoints ? static_cast<float *>(a.workspace) : memories + kept * size;
+        runs.factors = static_cast<double *>(a.workspace) + (a.checkpoints ? 0 : (kept * size + 1) / 2);
         run.last = memories, runs.spanCount = runs.spans - 1;
         LaunchRuns<T, kMemory>(runs, 1, whole, stream);
         JoinMemories(runs, run.first, memories, size, false, stream);
@@ -189,7 +190,8 @@ extern "C" __attribute__((visibility("default"))) unsigned long long cuju_linear
     if (!Fits(attention) || !Splits(*attention)) return 0;
     const Attention &a = *attention;
     const unsigned long long kept = (unsigned long long)a.batch * a.heads * ((a.time - 1) / kSpan);
-    return kept * ((a.checkpoints ? 0 : a.key_size * a.value_size) + 1) * sizeof(float);
+    const unsigned long long memories = a.checkpoints ? 0 : (kept * a.key_size * a.value_size + 1) / 2;
+    return (memories + kept) * sizeof(double);
 }
 
 extern "C" __attribute__((visibility("default"))) int cuju_linear_attention_forward(const struct cuju_linear_attention *attention, void *stream) {

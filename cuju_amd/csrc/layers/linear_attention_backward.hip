@@ -109,7 +109,7 @@ Layout LayoutOf(const Attention &a) {
     const auto four = [](long long x) { return (x + 3) / 4 * 4; };
     Layout at{};
     at.factors = four(kept * size);
-    at.dots = at.factors + four(kept);
+    at.dots = at.factors + four(2 * kept);
     at.crossings = at.dots + (a.d_decay ? four(2 * slices * heads * a.time) : 0);
     at.totals = at.crossings + (a.d_decay ? four(slices * heads * runs.spans) : 0);
     at.parts = at.totals + (a.d_decay && a.decay_of_head ? four(2 * heads * runs.spans) : 0);
@@ -139,7 +139,8 @@ void Backward(const Attention &a, hipStream_t stream) {
         r.key = query, r.value = output;
         r.rows = a.key_size, r.columns = a.value_size, r.reverse = true, r.in = a.scale;
         r.last = work + at.memories;
-        memories.firstSpan = 1, memories.spanCount = runs.spans - 1, memories.factors = runs.factors = work + at.factors;
+        memories.firstSpan = 1, memories.spanCount = runs.spans - 1;
+        memories.factors = runs.factors = reinterpret_cast<double *>(work + at.factors);
         RunMemories(memories, a.type, whole, stream);
         JoinMemories(runs, static_cast<const float *>(a.d_last), work + at.memories, size, true, stream);
     }

@@ -254,7 +254,7 @@ struct cuju_linear_attention {
     void *d_query, *d_key, *d_value; /* of `type` */
     void *d_decay;                   /* [batch][time][heads] or [heads], or null */
     void *d_state;                   /* or null */
-    void *workspace;                 /* the pass's bytes of workspace */
+    void *workspace;                 /* the pass's bytes of workspace, at a multiple of 8 */
 };
 /* One step (time 1), the memory updated in place. */
 int cuju_linear_attention_step(const struct cuju_linear_attention *attention, void *stream);

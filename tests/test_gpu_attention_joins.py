@@ -78,3 +78,42 @@ def test_a_factor_that_is_infinite():
     assert not bool(output[:, :130].any()) and not bool(torch.isfinite(output[:, 130:260]).any())
     whole = {n: x[:, 260:] for n, x in given.items() if n != 'state'}
     forward_close((output[:, 260:], last), {**whole, 'state': None})
+
+
+@pytest.mark.parametrize('time, dtype', [(1152, torch.float32), (1153, torch.float32), (1300, torch.bfloat16), (1300, torch.float16),
+                                         (3000, torch.bfloat16)])
+@pytest.mark.parametrize('episode', [0, 700])
+def test_more_spans_than_a_join_takes_at_a_time(episode, time, dtype):
+    # 9 and more joined memories, 8 at a time. An element of the memory, and of its gradient, is a sum of up to 3,000 steps:
+    # sqrt(3000 / 400) of the bounds of 400.
+    given = inputs(2, time, 1, 1, 16, 16, dtype=dtype, seed=time, episode=episode)
+    given['decay'] *= 0.02
+    wider = (time / 400) ** 0.5
+    found = dict(zip(('output', 'last'), attend(given)))
+    exact, terms = dict(zip(('output', 'last'), exact_attention(**given))), attention_terms(**given)
+    for name, x in found.items():
+        close(x, exact[name], wider * bound_of(name), terms[name])
+    found, d_output, d_last = learn(given)
+    d = {'d_output': d_output, 'd_last': d_last}
+    exact, terms = exact_attention(**given, **d), attention_terms(**given, **d)
+    for name, x in found.items():
+        close(x, exact[name], wider * bound_of(name), terms[name])
+
+
+def test_long_sequences_repeat_and_are_captured():
+    given = inputs(2, 1300, 1, 1, 16, 16, dtype=torch.bfloat16, seed=2, episode=700)
+    wanted = attend(given)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(a, b) for a, b in zip(attend(given), wanted))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = attend(given)
+    for scale in (1.0, -0.5, 2.0):
+        given['value'].mul_(scale)
+        wanted = attend(given)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, wanted))

@@ -33,6 +33,19 @@ __device__ __forceinline__ __hip_bfloat16 As<__hip_bfloat16>(float x) { return _
 template <>
 __device__ __forceinline__ __half As<__half>(float x) { return __float2half(x); }
 
+// An element as the low bits of a word, and element i of those of a word of memory.
+template <class T>
+__device__ __forceinline__ uint32_t Bits(T x) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
+    else return __builtin_bit_cast(uint16_t, x);
+}
+template <class T>
+__device__ __forceinline__ float OfWord(uint32_t word, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(word);
+    else if constexpr (std::is_same<T, __hip_bfloat16>::value) return __uint_as_float(i % 2 ? word & 0xffff0000u : word << 16);
+    else return __half2float(__builtin_bit_cast(__half, (uint16_t)(i % 2 ? word >> 16 : word)));
+}
+
 // N neighbouring elements, moved in one access.
 template <class T, int N>
 struct alignas(N * sizeof(T)) Pack {
@@ -128,9 +141,9 @@ __device__ __forceinline__ F4 Product(F4 a, F4 b, F4 c = F4{0, 0, 0, 0}) {
 
 // Products in 32 bits on the 16-bit matrix instruction. A float is the exact sum of three bfloat16
 // values (its leading 8 bits, the next 8, the last 8), a half of two, so a product of two operands is
-// the sum of the instruction's exact products of their pieces, of which those below 2^-24 of it
-// are left out: 3 instructions for a bfloat16 times a float, 5 for a half, 6 for a float, of 32
-// contracted indices and 16 cycles each. The same in the 32-bit instruction takes 8 of 32 cycles. An
+// the sum of the instruction's exact products of their pieces, of which those whose orders add up to
+// three and more are left out (of two floats 2^-24 of it as a rule and 2^-21 at most): 3 instructions
+// for a bfloat16 times a float, 5 for a half, 6 for a float, of 32 contracted indices and 16 cycles each. The same in the 32-bit instruction takes 8 of 32 cycles. An
 // infinity has no such pieces: it comes out as a NaN.
 using B8 = __attribute__((ext_vector_type(8))) __bf16;
 struct Four {  // four bfloat16 values

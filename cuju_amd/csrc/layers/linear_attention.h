@@ -106,9 +106,9 @@ struct Step {
 };
 
 // Wavefronts that a SIMD has to hold: two hide each other's waits, and the largest memories of floats leave registers for
-// one. With one and two, 4,096 heads and 64 steps: float32 64 x 64 forward 230 and 142 us, gradients 659 and 383; float16
-// 128 x 128 598 and 346, 1,498 and 1,168; float32 96 x 96 431 and 552, 1,159 and 1,553.
-template <class T, int KeyTiles, int Tiles, Mode mode>
+// one. With one and two, 4,096 heads and 64 steps: float32 64 x 64 forward 227 and 141 us, gradients 657 and 385; float16
+// 128 x 128 603 and 440, 1,486 and 1,114; float32 96 x 96 425 and 574, 1,160 and 1,533.
+template <class T, int KeyTiles, Mode mode>
 constexpr int kRunWaves = mode != kMemory && KeyTiles * kPieces<T> >= 18 ? 1 : 2;
 constexpr int kSteps = 2 * kChunk;  // steps that are played together: two tiles of the matrix instruction
 
@@ -144,11 +144,6 @@ struct Words {
 };
 template <class T, int N>
 constexpr int kWords = N * (int)sizeof(T) < 4 ? 1 : N * (int)sizeof(T) / 4;
-template <class T>
-__device__ __forceinline__ uint32_t Bits(T x) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
-    else return __builtin_bit_cast(uint16_t, x);
-}
 // N elements from a place aligned to `Aligned` of them, the first `valid` real and the others zero. `Whole`: either all or none.
 template <class T, int N, bool Whole, int Aligned = N>
 __device__ __forceinline__ Words<kWords<T, N>> LoadWords(const T *p, int valid = N) {
@@ -219,9 +214,7 @@ __device__ __forceinline__ void Made(X &x) {
 // Element i of such words.
 template <class T, int N>
 __device__ __forceinline__ float ElementOf(const Words<N> &w, int i) {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w.x[i]);
-    else if constexpr (std::is_same<T, __hip_bfloat16>::value) return __uint_as_float(i % 2 ? w.x[i / 2] & 0xffff0000u : w.x[i / 2] << 16);
-    else return __half2float(__builtin_bit_cast(__half, (uint16_t)(i % 2 ? w.x[i / 2] >> 16 : w.x[i / 2])));
+    return OfWord<T>(w.x[i * (int)sizeof(T) / 4], i);
 }
 // The pieces of a lane's eight neighbouring elements, and of the elements i of four places.
 template <class T, int N>
@@ -251,10 +244,10 @@ __device__ __forceinline__ void PiecesOf(const Words<N> (&w)[4], int i, Four (&p
 // registers. The columns never mix, so the wavefronts of a head share nothing.
 //
 // What bounds it: memory where heads are many and products few: 16,384 heads of 64 x 64 and 64 steps in bfloat16, forward,
-// move 1.07 GB in 250 us, 4.3 TB/s (a copy reaches 4.8), and the three runs of their gradients 1.75 GB in 560 to 585, 3.1 TB/s.
+// move 1.07 GB in 256 us, 4.2 TB/s (a copy reaches 4.8), and the three runs of their gradients 1.75 GB in 590, 3.0 TB/s.
 // There the vector instructions between the products show: two wavefronts a SIMD are all that the registers hold. Few long
-// sequences wait for the chain of chunks: 3,000 steps of 44 heads of 128 x 128 take 39 us for the spans' own memories, 21 to
-// join them and 82 for the outputs.
+// sequences wait for the chain of chunks: 3,000 steps of 44 heads of 128 x 128 take 38 us for the spans' own memories, 21 to
+// join them and 86 for the outputs.
 //
 // With the steps i, j of a chunk, G_i the product of the factors up to i and D_ij of those from j + 1 to i (0 across an
 // episode's start), O = out (G Q S + in (D o Q K^T) V), and the memory becomes G_C S + K^T (in D_C V). The products
@@ -268,7 +261,7 @@ __device__ __forceinline__ void PiecesOf(const Words<N> (&w)[4], int i, Four (&p
 // The products over a chunk's steps take a NaN or an infinity of a key or value, times a zero, to all of them. A wavefront
 // that meets one, or a factor past e^2, begins its span again and plays it step by step.
 template <class T, int KeyTiles, int Tiles, Shape shape, Mode mode>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T, KeyTiles, Tiles, mode>))) void RunKernel(Runs a) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(kRunWaves<T, KeyTiles, mode>))) void RunKernel(Runs a) {
     constexpr int P = kPieces<T>, kPairs = KeyTiles / 2;
     constexpr bool Whole = shape != kLoose, full = shape == kFull;
     // By step: the factors' sum up to it in two floats, and the factors of what it reads (NaN behind a reset) and writes.
@@ -863,12 +856,12 @@ inline bool IsWhole(const Attention &a) {
 }
 
 // The most tiles of 16 columns whose memory fits a wavefront's registers beside the rest: the keys of a chunk are turned once
-// for all of them. With half of them 4,096 heads and 64 steps of bfloat16 64 x 64 take 66 us for 53, gradients 181 for 133;
-// 128 x 128 302 for 225, 713 for 536; float16 96 x 96 217 for 159, 581 for 416. Float32 64 x 64 with two 169 for 140.
+// for all of them. With half of them 4,096 heads and 64 steps of bfloat16 64 x 64 take 68 us for 56, gradients 186 for 137;
+// 128 x 128 310 for 232, 719 for 543; float16 96 x 96 223 for 165, 590 for 429. Float32 64 x 64 with two 169 for 141.
 template <class T, int KeyTiles>
 constexpr int kMostTiles = KeyTiles * kPieces<T> <= 4 ? 4 : KeyTiles * kPieces<T> <= (kPieces<T> == kFloatPieces ? 8 : 12) ? 2 : 1;
 // The tiles that a wavefront of a launch takes: as many as leave a wavefront for each of the chip's 1,024 SIMDs. (bfloat16
-// 64 x 64, 64 steps, forward, with one tile and with four: 256 heads 11.3 and 13.4 us, 2,048 heads 43 and 26.)
+// 64 x 64, 64 steps, forward, with one tile and with four: 256 heads 11.1 and 12.6 us, 2,048 heads 38 and 24.)
 template <class T>
 int TilesOf(const Runs &runs, int count, int keyTiles) {
     const int most = keyTiles == 2 ? kMostTiles<T, 2> : keyTiles == 4 ? kMostTiles<T, 4> : keyTiles == 6 ? kMostTiles<T, 6> : kMostTiles<T, 8>;

@@ -114,9 +114,11 @@ __global__ __launch_bounds__(256) void JoinKernel(const float *first, float *mem
 }
 
 // Few heads are cut into spans, so that more wavefronts run: the memories at the spans' ends cost more than half of the
-// outputs. Measured in bfloat16 with memories of 64 x 64, cut and whole: 512 tiles and 1,024 steps 47 and 89 us, 256 steps 30
-// and 25; 1,024 tiles 65 and 102; 2,048 tiles 126 and 118. In float32: 512 tiles 92 and
-// 126, 1,024 tiles 167 and 160.
+// outputs. Cut and whole, with square memories of 16, 32, 64 and 128 and 1,024 steps, in us: bfloat16 of 1,024 tiles 85 and 102, 64
+// and 93, 71 and 108, 126 and 148, of 2,048 159 and 126, 115 and 106, 134 and 130, 248 and 164; float32 of 512 tiles 72 and 119,
+// 52 and 105, 95 and 128, 210 and 213, of 1,024 132 and 127, 94 and 128, 169 and 161, 390 and 275. 384 steps gain less: 43
+// and 45 in bfloat16 of 1,024 tiles of 64. The largest memories would take half the limit: 384 steps of 128 in float16 of
+// 1,024 tiles 106 and 90, in float32 of 512 97 and 86.
 bool Splits(const Attention &a) {
     const long long heads = (long long)a.batch * a.heads;
     return a.time >= 3 * kSpan && heads * ((a.value_size + 15) / 16) < (a.type == 0 ? 1024 : 2048);

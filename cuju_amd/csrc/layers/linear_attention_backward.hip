@@ -421,8 +421,11 @@ void Backward(const Attention &a, hipStream_t stream) {
     put(dv, a.d_value, false);
 
     // A launch has one number of rows, in tiles of 32, and kernels of full tiles take no other. Where keys and values differ in
-    // it, or one of them fills its tiles alone, and with enough wavefronts, the values' run has a launch of its own. (bfloat16, 64
-    // steps: 4,096 heads of 128 x 64 take 274 against 755 us, 512 of 32 x 64 28 against 37; 256 of 48 x 64 33 against 29.)
+    // it, or one of them fills its tiles alone, and with enough wavefronts, the values' run has a launch of its own. Enough
+    // are 11 of 16 columns for each of the 256 compute units, where the two cross: apart and together, 64 steps, of 1,408, 2,816 and
+    // 8,192 wavefronts in all, in us: bfloat16 128 x 64 39 and 34, 40 and 50, 54 and 96; 32 x 64 28 and 26, 34 and 33, 53 and 65;
+    // float16 64 x 128 41 and 41, 52 and 63, 103 and 121; float32 32 x 128 39 and 48, 49 and 70, 106 and 176. Sizes like 48 x 80 in
+    // 16 bits (95 and 83 of 8,192) and 48 x 64 in 32 (96 and 84) would be better off together.
     const bool full = a.key_size % 16 == 0 && a.value_size % 16 == 0 && (a.key_size % 32 == 0 || a.value_size % 32 == 0);
     const bool apart = a.key_size != a.value_size && ((whole && full) || (a.key_size + 31) / 32 != (a.value_size + 31) / 32) &&
                        heads * runs.spans * ((2 * a.key_size + a.value_size) / 16) >= 11 * 256;

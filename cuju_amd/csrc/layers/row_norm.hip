@@ -56,11 +56,6 @@ __device__ __forceinline__ float GateSlope(float z, int activation) {
 // A thread's packs of a row: `Lanes` packs side by side, `Packs` such rows of packs after one another. Packs need no
 // alignment but their elements'; the last one may be cut by the row's end. They are held as the words of memory, since
 // an array of 16-bit elements would take a register for each.
-template <class T>
-__device__ __forceinline__ uint32_t Bits(T x) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
-    else return __builtin_bit_cast(uint16_t, x);
-}
 template <class T, int Vector, int Packs, int Lanes>
 struct Held {
     static constexpr int kElements = 4 / sizeof(T), kWords = Vector / kElements;
@@ -102,11 +97,7 @@ struct Held {
             }
         }
     }
-    __device__ __forceinline__ float At(int i, int c) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i][c]);
-        else if constexpr (std::is_same<T, __hip_bfloat16>::value) return __uint_as_float(c % 2 ? w[i][c / 2] & 0xffff0000u : w[i][c / 2] << 16);
-        else return __half2float(__builtin_bit_cast(__half, (uint16_t)(w[i][c / 2] >> (16 * (c % 2)))));
-    }
+    __device__ __forceinline__ float At(int i, int c) const { return OfWord<T>(w[i][c / kElements], c); }
     // The elements of a pack, rounded.
     __device__ __forceinline__ void Set(int i, const float (&x)[Vector]) {
 #pragma unroll

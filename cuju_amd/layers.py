@@ -310,7 +310,8 @@ def delta_rule_step(query, key, value, decay, beta, state, *, resets=None, scale
 
     As `delta_rule` without the axis of time: `query` and `key` [batch, key heads, key size], `value`
     [batch, heads, value size], `decay` and `beta` [batch, heads], `resets` [batch]; `state` is a
-    contiguous float32 tensor [batch, heads, key size, value size]. A memory that is reset is not read.
+    contiguous float32 tensor [batch, heads, key size, value size]. It is read whether it is reset or not, but
+    what a memory that is reset held does not matter, infinities and NaN included.
     It has no gradients: an update learns through `delta_rule`.
     """
     q, k, v, decay, beta, resets = _check_rule(query, key, value, decay, beta, state, resets, False)
@@ -456,7 +457,8 @@ def linear_attention(query, key, value, decay, *, state=None, resets=None, scale
     * `query`, `key`: [batch, time, key heads, key size]; `value`: [batch, time, heads, value size], all
       of one type. Head h reads the key head `h // (heads / key heads)`.
     * `decay` (the logarithm of the factor, so at most 0 in use; -inf keeps nothing): [batch, time,
-      heads], or [heads] for one that is the same at every step, of any floating type, held in 32 bits.
+      heads], or [heads] for one that is the same at every step, of any floating type, held in 32 bits. From 89 on the
+      factor leaves the range of 32 bits, and a memory of zeros times it is no number.
     * `state`: [batch, heads, key size, value size], in 32 bits.
     * `resets`: [batch, time], bool or uint8: true where an episode starts. Nothing before such a step,
       not even an infinity, reaches its outputs, the later ones or their gradients.
@@ -464,7 +466,11 @@ def linear_attention(query, key, value, decay, *, state=None, resets=None, scale
 
     `output` is [batch, time, heads, value size] in the inputs' type, `last` the memory after the last
     step in 32 bits. Sizes go up to 128, strides are free (an axis of time before the batch is a
-    transposed view). Gradients reach every floating input; they are the same on every call. A NaN or an
+    transposed view). Gradients reach every floating input; they are the same on every call. Memories, scores and sums
+    have 32 bits whatever the type, also where an output or a gradient is rounded to 16. The gradient of a log decay is
+    found from the products of queries and keys with their gradients at the same 128 steps, and is some 2^-24 of
+    those off; where one of the 128 has a log decay below -4, all of them are sums of their own and as much of those off.
+    Such steps cost more: about as much as the rest of the backward pass where every 128 have one. A NaN or an
     infinity reaches the outputs of its own step and of later ones, as in the definition; in the memory an
     infinity may become a NaN. It may reach all gradients of its episode, and none of another.
     """
@@ -484,7 +490,8 @@ def linear_attention_step(query, key, value, decay, state, *, resets=None, scale
 
     As `linear_attention` without the axis of time: `query` and `key` [batch, key heads, key size],
     `value` [batch, heads, value size], `decay` [batch, heads] or [heads], `resets` [batch]; `state` is a
-    contiguous float32 tensor [batch, heads, key size, value size]. A memory that is reset is not read.
+    contiguous float32 tensor [batch, heads, key size, value size]. It is read whether it is reset or not, but
+    what a memory that is reset held does not matter, infinities and NaN included.
     It has no gradients: an update learns through `linear_attention`.
     """
     q, k, v, decay, resets = _check_attention(query, key, value, decay, state, resets, False)

@@ -94,24 +94,28 @@ __device__ __forceinline__ double BlockSum(double x, double (&sums)[4]) {
     __syncthreads();
     return (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
-// A lane's eight elements of each pair of tiles of a step's row, zeros past its end.
+// A lane's eight elements of each pair of tiles of a step's row, zeros past its end; 16 bytes at once, for the lines of the cache
+// that a load touches (by eight bytes the kernel below takes 675 us for 518).
 template <class T, int kPairs, bool Whole>
 struct Row {
-    struct Halves {
-        Words<kWords<T, 4>> x[2];
-    } pair[kPairs];
+    Words<kWords<T, 8>> pair[kPairs];
     __device__ __forceinline__ void Load(const T *row, int g, int size) {
 #pragma unroll
-        for (int p = 0; p < kPairs; p++)
+        for (int p = 0; p < kPairs; p++) {
+            const int at = 32 * p + 8 * g;
+            if (Whole && sizeof(T) == 2 && at + 8 <= size) {
+                pair[p] = LoadWords<T, 8, true, 4>(row + at);
+            } else {
+                struct Halves {
+                    Words<kWords<T, 4>> x[2];
+                } half;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int at = 32 * p + 8 * g + 4 * i;
-                pair[p].x[i] = LoadWords<T, 4, Whole>(row + at, size - at);
+                for (int i = 0; i < 2; i++) half.x[i] = LoadWords<T, 4, Whole>(row + at + 4 * i, size - at - 4 * i);
+                pair[p] = __builtin_bit_cast(Words<kWords<T, 8>>, half);
             }
+        }
     }
-    __device__ __forceinline__ void Pieces(int p, B8 (&piece)[kPieces<T>]) const {
-        PiecesOf<T>(__builtin_bit_cast(Words<kWords<T, 8>>, pair[p]), piece);
-    }
+    __device__ __forceinline__ void Pieces(int p, B8 (&piece)[kPieces<T>]) const { PiecesOf<T>(pair[p], piece); }
 };
 
 // The gradients of the decays of spans with sharp steps, as sums of what passes each step: no difference of large sums. Of an
@@ -119,8 +123,8 @@ struct Row {
 // span (ii) scale q_i S do_i F_i, of the gradient D of the memory behind it (iii) k_j D v_j F_j, and of both (iv) <S, D> F, where F
 // are the products of the factors in between. A step that is cleared ends all of them. The products are of pieces (common.h). A tile
 // of 16 x 16 pairs is summed by row and by column, for the steps within its later and its earlier steps, and whole, for
-// those between. Vector instructions bound it: 16,384 heads of 64 x 64 and 64 steps in bfloat16, each with a sharp step, take
-// 660 to 680 us, and 5 where none has one.
+// those between. 16,384 heads of 64 x 64 and 64 steps in bfloat16, each with a sharp step, take 500 to 520 us, and 5 where none has
+// one. Wavefronts wait for loads for 72 % of their cycles: a load of steps' rows touches 16 lines of the cache, one after the other.
 struct SharpArgs {
     DecayArgs decays;
     Tensor query, key, value, output;  // output: its gradient
@@ -227,19 +231,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kSharpWaves
                 if (g == 0) columns[late][early][m] = column;
             }
         }
-        // (ii) and (iii): a step's row times a memory, times its answer. A wavefront takes 16 columns of the memory.
-        const auto pass = [&](const Line<T> &left, const float *memory, const Line<T> &right, float (&out)[kTiles][kSpan]) {
+        // (ii) and (iii): a step's row times a memory, times its answer. A wavefront takes 16 columns of the memory. (iv): their
+        // products with those of another.
+        double both = 0;
+        const auto pass = [&](const Line<T> &left, const float *memory, const Line<T> &right, const float *other, float (&out)[kTiles][kSpan]) {
             for (int first = wave * kChunk; first < s.columns; first += 4 * kChunk) {
                 const int column = min(first + m, s.columns - 1);
                 B8 held[kPairs][kFloatPieces];
 #pragma unroll
                 for (int p = 0; p < kPairs; p++) {
-                    F4 x[2];
+                    F4 x[2], y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
                     for (int r = 0; r < 8; r++) {
                         const int row = 32 * p + 8 * g + r;
                         x[r / 4][r % 4] = row < s.rows ? memory[row * s.columns + column] : 0.f;
+                        if (other) y[r / 4][r % 4] = row < s.rows && first + m < s.columns ? other[row * s.columns + column] : 0.f;
                     }
+                    if (other)
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (first + m < s.columns) both += (double)x[r / 4][r % 4] * y[r / 4][r % 4];
                     SplitPair<kFloatPieces>(x[0], x[1], held[p]);
                 }
                 for (int tile = 0; tile < tiles; tile++) {
@@ -262,12 +273,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kSharpWaves
                 }
             }
         };
-        if (start) pass(queries, start, outputs, parts[0]);
-        if (end) pass(keys, end, values, parts[1]);
-        // (iv)
-        double both = 0;
-        if (episodes == 0 && start && end)
-            for (int x = t; x < size; x += 256) both += (double)start[x] * end[x];
+        if (start) pass(queries, start, outputs, nullptr, parts[0]);
+        if (end) pass(keys, end, values, episodes == 0 ? start : nullptr, parts[1]);
         both = BlockSum(both, sums);
 
         // Everything within the steps' own tiles, 16 threads each: what later steps read, and what earlier steps wrote.

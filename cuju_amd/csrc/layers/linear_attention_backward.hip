@@ -4,8 +4,9 @@
 namespace layers {
 namespace {
 
-// A step whose log decay is below this passes on so little that differences of the dots around it would not hold its gradient:
-// they are 2^-24 of the dots off, 2^-18 of what passes a step of e^-4.
+// A step whose log decay is below this passes on so little that differences of the dots around it would not hold its gradient.
+// Beside steps that forget nothing, in 64 x 64, the gradient at a decay of -0.5 is 3e-6 of its terms' 2-norm off, of -2 9e-6, of
+// -3.99 5e-5; what SharpKernel finds is 7e-7 off at any.
 constexpr float kSharp = -4.f;
 // One wavefront takes a span of a head: two steps a lane. Backwards from the product of the memory at the span's end
 // and its gradient, each step adds q.dq - k.dk without its own product to the gradient of the step after it,

@@ -468,8 +468,8 @@ def linear_attention(query, key, value, decay, *, state=None, resets=None, scale
     step in 32 bits. Sizes go up to 128, strides are free (an axis of time before the batch is a
     transposed view). Gradients reach every floating input; they are the same on every call. Memories, scores and sums
     have 32 bits whatever the type, also where an output or a gradient is rounded to 16. The gradient of a log decay is
-    found from the products of queries and keys with their gradients at the same 128 steps, and is some 2^-24 of
-    those off; where one of the 128 has a log decay below -4, all of them are sums of their own and as much of those off.
+    found from the products of queries and keys with their gradients at the same 128 steps, and is some times 2^-24 of
+    those off; where one of the 128 has a log decay below -4, each is a sum of its own and as much of that off.
     Such steps cost more: about as much as the rest of the backward pass where every 128 have one. A NaN or an
     infinity reaches the outputs of its own step and of later ones, as in the definition; in the memory an
     infinity may become a NaN. It may reach all gradients of its episode, and none of another.

@@ -35,7 +35,7 @@ def test_workspaces_of_joined_spans(time, key_size, value_size):
 
 def test_rows_that_lie_in_no_two_axes():
     x = torch.zeros(4, 3, 5, 8)
-    # Rows 8 apart within, 40 and then 120 apart: three strides, whichever axis is of one.
+    # Five rows 8 apart, four times 120 apart, before an axis of one row: two strides where there is room for one.
     moved = x[:, :1].transpose(1, 2)
     assert moved.shape == (4, 5, 1, 8) and layers._row_strides(moved) is None
     for each in (moved, x.transpose(0, 2), x[:, ::2], x[:, :2]):
